@@ -109,6 +109,20 @@ def lib():
                                       ctypes.POINTER(ctypes.c_int)]
         L.zk_kzg_commit.argtypes = [vp, vp, vp, ctypes.c_size_t, vp, vp]
         L.zk_kzg_open.argtypes = [vp, vp, vp, ctypes.c_size_t, vp, vp, vp, vp]
+        sz, ci = ctypes.c_size_t, ctypes.c_int
+        L.zk_i8_matmul.argtypes = [vp, vp, sz, vp, vp, sz, vp, vp, sz, sz, sz, ci, vp, ci, sz, vp]
+        L.zk_i8_quantize.argtypes = [vp, vp, ci, sz, sz, sz, vp, sz, vp, vp]
+        L.zk_i8_linear_work.argtypes = [sz, sz]
+        L.zk_i8_linear_work.restype = sz
+        L.zk_i8_linear.argtypes = [vp, vp, ci, sz, vp, sz, vp, vp, sz, sz, sz, ci, vp, ci, sz, vp, sz, vp]
+        L.zk_i8_matmul_experts.argtypes = [vp, vp, sz, vp, sz, vp, sz, vp, vp, vp, ci, vp, ci, sz, sz, sz, ci, vp, ci,
+                                           sz, vp]
+        L.zk_experts_sort_work.argtypes = [sz, ci]
+        L.zk_experts_sort_work.restype = sz
+        L.zk_experts_sort.argtypes = [vp, vp, sz, ci, vp, vp, vp, vp, sz, vp]
+        L.zk_experts_gather.argtypes = [vp, vp, ci, sz, sz, vp, sz, sz, ci, vp, sz, vp]
+        L.zk_experts_combine.argtypes = [vp, vp, ci, sz, sz, vp, vp, sz, sz, ci, vp, sz, vp]
+        L.zk_experts_combine_grad.argtypes = [vp, vp, sz, vp, sz, ci, sz, vp, vp, vp, sz, sz, ci, vp, sz, vp, vp]
         L.zk_poseidon_permute.argtypes = [vp]
         L.zk_poseidon_hash2.argtypes = [vp, vp, vp]
         L.zk_poseidon_commit.argtypes = [vp, ctypes.c_size_t, ctypes.c_uint64, vp]
@@ -128,6 +142,26 @@ def lib():
         L.zk_statement_meta_json.argtypes = [vp, ctypes.c_uint64, ctypes.c_char_p, ctypes.c_size_t, sp]
         _lib = L
     return _lib
+
+
+# zk_type: element types of the 8-bit layers and the experts' rows
+F32, F16, BF16, I32 = range(4)
+# hipStreamLegacy: what a torch program's default stream (handle 0) is called
+# here, where no stream means the context's own
+LEGACY_STREAM = 1
+
+
+def _dev(b):
+    """Address of device memory: a DeviceBuffer (or what has .ptr), a torch
+    tensor, or None."""
+    if b is None:
+        return None
+    p = getattr(b, "ptr", None)
+    return b.data_ptr() if p is None else p
+
+
+def _nbytes(b):
+    return 0 if b is None else b.nbytes
 
 
 def _np_ptr(a):
@@ -331,6 +365,77 @@ class Context:
 
     def g2_generator_mul(self, d_scalars, n, d_out):
         self._check(lib().zk_g2_generator_mul(self.h, vp(d_scalars.ptr), n, vp(d_out.ptr), None), "g2_generator_mul")
+
+    # ---- 8-bit integer layers and routed experts
+    # Device arguments are DeviceBuffers or torch tensors; row strides (in
+    # elements) default to the rows' length; stream None is the context's own.
+    def i8_matmul(self, x, w, rows, n_out, n_in, y, y_type=I32, x_scale=None, w_scale=None, bias=None, relu=False,
+                  ld_x=None, ld_w=None, ld_y=None, stream=None):
+        """y = x w^T over int8 (zk_i8_matmul): the int32 sums, or scaled."""
+        self._check(lib().zk_i8_matmul(self.h, _dev(x), n_in if ld_x is None else ld_x, _dev(x_scale), _dev(w),
+                                       n_in if ld_w is None else ld_w, _dev(w_scale), _dev(bias), rows, n_out, n_in,
+                                       relu, _dev(y), y_type, n_out if ld_y is None else ld_y, stream),
+                    "zk_i8_matmul")
+
+    def i8_quantize(self, x, x_type, rows, cols, q, scale, ld_x=None, ld_q=None, stream=None):
+        """Rows of x to int8 with a scale each (zk_i8_quantize)."""
+        self._check(lib().zk_i8_quantize(self.h, _dev(x), x_type, cols if ld_x is None else ld_x, rows, cols,
+                                         _dev(q), cols if ld_q is None else ld_q, _dev(scale), stream),
+                    "zk_i8_quantize")
+
+    @staticmethod
+    def i8_linear_work(rows, n_in):
+        return lib().zk_i8_linear_work(rows, n_in)
+
+    def i8_linear(self, x, x_type, w, w_scale, rows, n_out, n_in, y, y_type, work, bias=None, relu=False, ld_x=None,
+                  ld_w=None, ld_y=None, stream=None):
+        """Quantizes x's rows and multiplies (zk_i8_linear); work:
+        i8_linear_work(rows, n_in) bytes."""
+        self._check(lib().zk_i8_linear(self.h, _dev(x), x_type, n_in if ld_x is None else ld_x, _dev(w),
+                                       n_in if ld_w is None else ld_w, _dev(w_scale), _dev(bias), rows, n_out, n_in,
+                                       relu, _dev(y), y_type, n_out if ld_y is None else ld_y, _dev(work),
+                                       _nbytes(work), stream), "zk_i8_linear")
+
+    def i8_matmul_experts(self, x, w, offsets, rows, experts, n_out, n_in, y, y_type=I32, x_scale=None, w_scale=None,
+                          bias=None, relu=False, order=None, slots=1, tokens=None, ld_x=None, ld_w=None, ld_y=None,
+                          stream=None):
+        """i8_matmul with each expert's weights for its rows (zk_i8_matmul_experts)."""
+        self._check(lib().zk_i8_matmul_experts(
+            self.h, _dev(x), n_in if ld_x is None else ld_x, _dev(x_scale), rows if tokens is None else tokens,
+            _dev(w), n_in if ld_w is None else ld_w, _dev(w_scale), _dev(bias), _dev(offsets), experts, _dev(order),
+            slots, rows, n_out, n_in, relu, _dev(y), y_type, n_out if ld_y is None else ld_y, stream),
+            "zk_i8_matmul_experts")
+
+    @staticmethod
+    def experts_sort_work(pairs, experts):
+        return lib().zk_experts_sort_work(pairs, experts)
+
+    def experts_sort(self, expert, pairs, experts, offsets, order, place, work=None, stream=None):
+        """Pairs sorted by expert (zk_experts_sort); work: experts_sort_work bytes."""
+        self._check(lib().zk_experts_sort(self.h, _dev(expert), pairs, experts, _dev(offsets), _dev(order),
+                                          _dev(place), _dev(work), _nbytes(work), stream), "zk_experts_sort")
+
+    def experts_gather(self, x, rows_type, cols, order, rows, tokens, slots, out, ld_x=None, ld_out=None,
+                       stream=None):
+        """Tokens' rows in the sorted order (zk_experts_gather)."""
+        self._check(lib().zk_experts_gather(self.h, _dev(x), rows_type, cols if ld_x is None else ld_x, cols,
+                                            _dev(order), rows, tokens, slots, _dev(out),
+                                            cols if ld_out is None else ld_out, stream), "zk_experts_gather")
+
+    def experts_combine(self, y, rows_type, cols, place, rows, tokens, slots, out, weight=None, ld_y=None,
+                        ld_out=None, stream=None):
+        """Rows put back and summed with their weights (zk_experts_combine)."""
+        self._check(lib().zk_experts_combine(self.h, _dev(y), rows_type, cols if ld_y is None else ld_y, cols,
+                                             _dev(place), _dev(weight), rows, tokens, slots, _dev(out),
+                                             cols if ld_out is None else ld_out, stream), "zk_experts_combine")
+
+    def experts_combine_grad(self, grad, y, rows_type, cols, order, place, weight, rows, tokens, slots, grad_y,
+                             grad_weight=None, ld_grad=None, ld_y=None, ld_grad_y=None, stream=None):
+        """Gradients of experts_combine (zk_experts_combine_grad)."""
+        self._check(lib().zk_experts_combine_grad(
+            self.h, _dev(grad), cols if ld_grad is None else ld_grad, _dev(y), cols if ld_y is None else ld_y,
+            rows_type, cols, _dev(order), _dev(place), _dev(weight), rows, tokens, slots, _dev(grad_y),
+            cols if ld_grad_y is None else ld_grad_y, _dev(grad_weight), stream), "zk_experts_combine_grad")
 
     # ---- Groth16
     def r1cs(self, num_constraints, num_variables, num_public, A, B, C):

@@ -254,6 +254,94 @@ int zk_wtns_write(const char* path, const void* w_mont, size_t m);
 int zk_synthetic_r1cs(int num_constraints, int num_public, int num_inputs, uint64_t seed, zk_sparse_entry* A,
                       size_t* nA, zk_sparse_entry* B, size_t* nB, zk_sparse_entry* C, size_t* nC, void* w_mont);
 
+/* ---- 8-bit integer layers -------------------------------------------------
+ * No counterpart in the reference, whose GPU layers work on field elements
+ * (src/nn/layers.cu:37-190).  The linear layer of a quantized model (LINEAR of
+ * the statement producer below: weights n_out x n_in, row major) over whole
+ * batches, in the integers a statement proves, and with the scales that tie
+ * them to the real-valued model.
+ *
+ * zk_i8_matmul: acc[t][n] = sum_k x[t][k] w[n][k] (int8, exact in int32;
+ * n_in <= 131071), then
+ *   y_type ZK_I32: y = acc (no scales, no bias);
+ *   else           y = float(acc) * (x_scale[t] * w_scale[n]) + bias[n],
+ * in 32-bit floats, rounded once to y_type; relu != 0 replaces what is below
+ * zero by zero (a NaN stays).  d_x_scale (rows), d_w_scale and d_bias (n_out)
+ * may be NULL (1, 1 and 0).  ld_* are row strides in elements, at least the
+ * row's length; rows of x and w may start at any byte.
+ * zk_i8_quantize: scale[t] = max_k |x[t][k]| / 127, q[t][k] = the integer
+ * nearest to 127 x[t][k] / max_k |x[t][k]| (ties to even).  A row of zeros
+ * has scale 0 and zeros; a row that holds an infinity or a NaN has scale NaN
+ * and zeros, so that what is made of it is NaN.
+ * zk_i8_linear: zk_i8_quantize of x's rows, then zk_i8_matmul with their
+ * scales.  d_work: zk_i8_linear_work(rows, n_in) bytes (0: sizes out of
+ * range), 16-byte aligned, free again when the call's work on the stream is
+ * done.
+ * zk_i8_matmul_experts: rows offsets[e] .. offsets[e+1] of y (see
+ * zk_experts_sort) use expert e's weights, d_w + e * n_out * ld_w, w_scale and
+ * bias + e * n_out; row p takes row order[p] / slots of x (tokens rows) and
+ * its scale, or row p itself when d_order is NULL.  Rows that belong to no
+ * expert, or whose order names no token, become zeros.  offsets[0] is 0 and
+ * the offsets do not fall.
+ * None of these allocates, waits or uses memory of the context, so calls on
+ * different streams do not touch each other.  y may not overlap an input.
+ * stream may be hipStreamLegacy (the default stream of a program that does
+ * not name one). */
+enum zk_type { ZK_F32 = 0, ZK_F16 = 1, ZK_BF16 = 2, ZK_I32 = 3 };
+enum { ZK_MAX_EXPERTS = 1024, ZK_MAX_EXPERT_ROWS = 1 << 22 };
+
+int zk_i8_matmul(zk_context* ctx, const int8_t* d_x, size_t ld_x, const float* d_x_scale, const int8_t* d_w,
+                 size_t ld_w, const float* d_w_scale, const float* d_bias, size_t rows, size_t n_out, size_t n_in,
+                 int relu, void* d_y, int y_type, size_t ld_y, void* stream);
+int zk_i8_quantize(zk_context* ctx, const void* d_x, int x_type, size_t ld_x, size_t rows, size_t cols, int8_t* d_q,
+                   size_t ld_q, float* d_scale, void* stream);
+size_t zk_i8_linear_work(size_t rows, size_t n_in);
+int zk_i8_linear(zk_context* ctx, const void* d_x, int x_type, size_t ld_x, const int8_t* d_w, size_t ld_w,
+                 const float* d_w_scale, const float* d_bias, size_t rows, size_t n_out, size_t n_in, int relu,
+                 void* d_y, int y_type, size_t ld_y, void* d_work, size_t work_bytes, void* stream);
+int zk_i8_matmul_experts(zk_context* ctx, const int8_t* d_x, size_t ld_x, const float* d_x_scale, size_t tokens,
+                         const int8_t* d_w, size_t ld_w, const float* d_w_scale, const float* d_bias,
+                         const int32_t* d_offsets, int experts, const int32_t* d_order, int slots, size_t rows,
+                         size_t n_out, size_t n_in, int relu, void* d_y, int y_type, size_t ld_y, void* stream);
+
+/* ---- routed experts ---------------------------------------------------------
+ * No counterpart in the reference, whose routing ends with each sample's class
+ * and flag (src/prover/statement_v2.cuh:243-266).  Samples ("tokens") sorted by
+ * the expert that a route names and put back with the routes' weights.  A pair
+ * i = token * slots + j is a token's j-th route.
+ *
+ * zk_experts_sort: stable counting sort of the pairs by expert (1 to 1024
+ * experts, at most 2^22 pairs).  offsets[e] (experts + 1 words) = pairs with an
+ * expert below e; order[p] = the pair at position p; place[i] = the pair's
+ * position.  A pair whose expert is outside [0, experts) is dropped: place[i] =
+ * -1, and order[p] = -1 from offsets[experts] on.  d_work:
+ * zk_experts_sort_work(pairs, experts) bytes (0: none needed, may be NULL).
+ * zk_experts_gather: out[p] = x[order[p] / slots], zeros where order[p] is -1.
+ * Its gradient is zk_experts_combine of the rows' gradients without weights.
+ * zk_experts_combine: out[t] = sum_j weight[t][j] * y[place[t][j]] over the
+ * pairs that have a place, summed in 32-bit floats in the order of j, rounded
+ * once; d_weight NULL: 1.  Tokens with no place become zeros.
+ * zk_experts_combine_grad: for the gradient g of that sum,
+ *   grad_y[place[t][j]] = weight[t][j] * g[t], zeros where order is -1;
+ *   grad_weight[t][j] = sum_c g[t][c] * y[place[t][j]][c], 0 for dropped pairs.
+ * d_grad_weight may be NULL (then d_y may be, too).  place and order are those
+ * of one zk_experts_sort, rows <= tokens * slots.
+ * type: that of all rows (ZK_F32, ZK_F16, ZK_BF16); ld_* row strides in
+ * elements.  Results do not depend on the order of execution.  Indexes outside
+ * their range are taken as -1. */
+size_t zk_experts_sort_work(size_t pairs, int experts);
+int zk_experts_sort(zk_context* ctx, const int32_t* d_expert, size_t pairs, int experts, int32_t* d_offsets,
+                    int32_t* d_order, int32_t* d_place, void* d_work, size_t work_bytes, void* stream);
+int zk_experts_gather(zk_context* ctx, const void* d_x, int type, size_t ld_x, size_t cols, const int32_t* d_order,
+                      size_t rows, size_t tokens, int slots, void* d_out, size_t ld_out, void* stream);
+int zk_experts_combine(zk_context* ctx, const void* d_y, int type, size_t ld_y, size_t cols, const int32_t* d_place,
+                       const float* d_weight, size_t rows, size_t tokens, int slots, void* d_out, size_t ld_out,
+                       void* stream);
+int zk_experts_combine_grad(zk_context* ctx, const void* d_grad, size_t ld_grad, const void* d_y, size_t ld_y,
+                            int type, size_t cols, const int32_t* d_order, const int32_t* d_place,
+                            const float* d_weight, size_t rows, size_t tokens, int slots, void* d_grad_y,
+                            size_t ld_grad_y, float* d_grad_weight, void* stream);
+
 /* ---- pairing and verification (host code, no device needed) -------------
  * zk_pairing replaces bn254::pairing (src/curve/pairing.cuh:198-282): the
  * reduced optimal ate pairing e(P, Q).  P: 64 bytes x, y; Q: 128 bytes x.c0,
