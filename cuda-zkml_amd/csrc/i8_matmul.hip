@@ -8,6 +8,8 @@
 // A product of two int8 is at most 2^14, so acc is exact for n_in <= 131071.
 // The grouped form takes its weights by expert: rows offsets[e] to
 // offsets[e+1] of y use w[e].
+#include <type_traits>
+
 #include "zk_internal.hpp"
 
 namespace zk {
@@ -16,6 +18,7 @@ typedef int v4i __attribute__((ext_vector_type(4)));
 typedef int v16i __attribute__((ext_vector_type(16)));
 
 constexpr size_t I8_MAX_IN = 131071;
+constexpr size_t I8_MAX_TILES = (size_t)1 << 22;  // blocks of one launch (its threads stay below 2^32)
 
 // What every kernel of this file is given.
 struct I8Args {
@@ -74,94 +77,596 @@ __device__ __forceinline__ int64_t source_row(const I8Args& a, uint32_t p) {
   return t < a.tokens ? (int64_t)t : -1;
 }
 
-template <class T, bool GROUPED>
-__global__ __launch_bounds__(256) void k_i8_tile(I8Args a) {
-  constexpr int B = 64, LD = 80;
-  __shared__ __align__(16) int8_t X[B * LD], W[B * LD];
-  const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const uint32_t n0 = blockIdx.x * B;
-  uint32_t r0 = blockIdx.y * B, r1 = a.rows, e = 0;
-  if (GROUPED) {
-    // the tile's expert: tiles are counted expert by expert, the rows that
-    // belong to none last
-    uint32_t tile = blockIdx.y;
-    bool found = false;
-    for (; e < a.experts; e++) {
-      const uint32_t lo = offset_of(a, e), hi = offset_of(a, e + 1);
-      const uint32_t n = hi > lo ? (hi - lo + B - 1) / B : 0;
-      if (tile < n) {
-        r0 = lo + tile * B;
-        r1 = hi;
-        found = true;
-        break;
-      }
-      tile -= n;
+// Tile (tt, tn) of block b.  Blocks b, b + 8, b + 16, ... share an XCD and its
+// L2: each XCD gets one run of the tiles, and a run goes over 8 token tiles
+// before it takes the next channel tile, so that the 32 blocks an XCD holds at
+// a time read about 8 + 4 tiles of rows between them.
+__device__ __forceinline__ bool tile_of_block(uint32_t b, uint32_t tiles_t, uint32_t tiles_n, uint32_t& tt,
+                                              uint32_t& tn) {
+  constexpr uint32_t G = 8;
+  const uint32_t total = tiles_t * tiles_n, per = (total + 7) / 8;
+  const uint32_t t = (b & 7) * per + (b >> 3);
+  if (t >= total) return false;
+  const uint32_t group = t / (G * tiles_n), at = t % (G * tiles_n);
+  const uint32_t size = tiles_t - group * G < G ? tiles_t - group * G : G;
+  tt = group * G + at % size;
+  tn = at / size;
+  return true;
+}
+
+// Rows [r0, r1) and expert of row tile tt of the grouped form: tiles are
+// counted expert by expert, those of the rows without an expert (e = experts)
+// last.  The whole wave takes part; the answer is the same in every lane.
+__device__ __forceinline__ void expert_tile(const I8Args& a, uint32_t tt, uint32_t bt, uint32_t& r0, uint32_t& r1,
+                                            uint32_t& e) {
+  const uint32_t lane = threadIdx.x & 63;
+  uint32_t run = 0;
+  for (uint32_t e0 = 0; e0 < a.experts; e0 += 64) {
+    const uint32_t me = e0 + lane;
+    uint32_t lo = 0, hi = 0;
+    if (me < a.experts) lo = offset_of(a, me), hi = offset_of(a, me + 1);
+    const uint32_t n = hi > lo ? (hi - lo + bt - 1) / bt : 0;
+    uint32_t s = n;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const uint32_t o = __shfl_up(s, d);
+      if (lane >= (uint32_t)d) s += o;
     }
-    if (!found) {
-      r0 = offset_of(a, a.experts) + tile * B;
-      r1 = a.rows;
+    const uint64_t past = __ballot(run + s > tt);
+    if (past) {
+      const int l = __ffsll((unsigned long long)past) - 1;
+      const uint32_t first = run + __shfl(s, l) - __shfl(n, l);
+      e = e0 + l;
+      r0 = __shfl(lo, l) + (tt - first) * bt;
+      r1 = __shfl(hi, l);
+      return;
+    }
+    run += __shfl(s, 63);
+  }
+  e = a.experts;
+  const uint64_t r = (uint64_t)offset_of(a, a.experts) + (uint64_t)(tt - run) * bt;
+  r1 = a.rows;
+  r0 = r < r1 ? (uint32_t)r : r1;
+}
+
+// What rows are padded with: a lane that has no bytes to load takes these.
+__device__ const v4i zeros16 = {0, 0, 0, 0};
+
+// ------------------------------------------------------------ tiles in LDS
+// A block computes BT tokens x BN channels, its WT x WN waves a grid of
+// FT x FN squares of 32 x 32 each (D rows are channels, so that a lane holds
+// four neighbouring channels of one token).  Steps of 128 bytes of k, a whole
+// cache line of each row, pass through LDS.
+
+// 16 bytes a lane from `p` to LDS at `at` + 16 * lane (`at` the same in the
+// whole wave).  Only wait_loads() waits for it: to the compiler's own counting
+// it is unknown, which makes the compiler's waits longer, never shorter.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"  // m0 is named so that nothing of the compiler's is kept in it
+__device__ __forceinline__ void load_to_lds(const int8_t* p, uint32_t at) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(at), "v"(p) : "m0");
+}
+#pragma clang diagnostic pop
+// Until at most N of the wave's loads are under way.
+template <int N>
+__device__ __forceinline__ void wait_loads() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+__device__ __forceinline__ void meet() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+// ---- what a tile's sums become
+// The tile's scales and biases: a thread holds a few of them from the start,
+// so that they are there when the sums are, and puts them into LDS after the
+// last step: sx[BT], sw[BN], bias[BN] and, in the grouped form, has[BT] (does
+// the row have a token?).
+template <bool GROUPED, uint32_t BT, uint32_t BN, uint32_t THREADS>
+struct Factors {
+  static constexpr uint32_t ALL = BT + 2 * BN + (GROUPED ? BT : 0), N = (ALL + THREADS - 1) / THREADS;
+  float v[N];
+  __device__ __forceinline__ void load(const I8Args& a, uint32_t r0, uint32_t r1, uint32_t n0, uint32_t e) {
+    const bool none = GROUPED && e >= a.experts;
+    const size_t ch = none ? 0 : (size_t)e * a.n_out;
+#pragma unroll
+    for (uint32_t i = 0; i < N; i++) {
+      const uint32_t k = threadIdx.x + i * THREADS;
+      v[i] = 0.0f;
+      if (k < BT || k >= BT + 2 * BN) {
+        const uint32_t t = r0 + (k < BT ? k : k - BT - 2 * BN);
+        int64_t s = -1;
+        if (t < r1 && !none) s = GROUPED ? source_row(a, t) : (int64_t)t;
+        v[i] = s < 0 ? 0.0f : k < BT && a.sx ? a.sx[s] : 1.0f;
+      } else {
+        const bool second = k >= BT + BN;
+        const uint32_t n = n0 + k - BT - (second ? BN : 0);
+        const float* from = second ? a.bias : a.sw;
+        v[i] = from ? (n < a.n_out ? from[ch + n] : 0.0f) : second ? 0.0f : 1.0f;
+      }
     }
   }
+  __device__ __forceinline__ void store(float* to) const {
+#pragma unroll
+    for (uint32_t i = 0; i < N; i++) {
+      const uint32_t k = threadIdx.x + i * THREADS;
+      if (k < ALL) to[k] = v[i];
+    }
+  }
+};
+
+// Writes a wave's FN x FT squares: through LDS of its own, 32 tokens at a time,
+// so that a row's results leave in 16-byte pieces side by side (8-byte pieces
+// of 32 rows at once took 12 us for a tile of 256 x 256).
+// f: the block's factors; t0, c0: the wave's first token and channel in the tile.
+template <class T, bool GROUPED, uint32_t BT, uint32_t BN, int FT, int FN>
+__device__ __forceinline__ void put_results(const I8Args& a, const v16i (&acc)[FN][FT], const float* f, int8_t* own,
+                                            uint32_t r0, uint32_t r1, uint32_t n0, uint32_t t0, uint32_t c0) {
+  constexpr uint32_t E = 16 / sizeof(T), PIECES = FN * 32 / E, ROWS = 64 / PIECES;  // of one 16-byte store
+  constexpr uint32_t LD = FN * 32 * sizeof(T) + 16;
+  const uint32_t lane = threadIdx.x & 63, fr = lane & 31, hi = lane >> 5;
+  const float *sw = f + BT + c0, *bias = sw + BN, *has = f + BT + 2 * BN;
+#pragma unroll
+  for (int j = 0; j < FT; j++) {
+    const float sx = f[t0 + j * 32 + fr];
+    const bool zero = GROUPED && has[t0 + j * 32 + fr] == 0.0f;
+#pragma unroll
+    for (int i = 0; i < FN; i++)
+#pragma unroll
+      for (int q = 0; q < 4; q++) {
+        T v[4];
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+          const uint32_t c = i * 32 + 8 * q + 4 * hi + k;
+          v[k] = zero ? (T)0 : finish<T>(acc[i][j][4 * q + k], sx * sw[c], bias[c], a.relu);
+        }
+        __builtin_memcpy(own + fr * LD + (i * 32 + 8 * q + 4 * hi) * sizeof(T), v, sizeof(v));
+      }
+    wait_lds();  // one wave's LDS accesses are in order; this keeps the compiler to it
+#pragma unroll
+    for (uint32_t s = 0; s < 32; s += ROWS) {
+      const uint32_t row = s + lane / PIECES, c = lane % PIECES * E;
+      const uint32_t t = r0 + t0 + j * 32 + row, n = n0 + c0 + c;
+      if (t < r1 && n < a.n_out) {
+        const int8_t* from = own + row * LD + c * sizeof(T);
+        T* y = (T*)a.y + (size_t)t * a.ld_y + n;
+        if (n + E <= a.n_out) {
+          v4i v = *(const v4i*)from;
+          __builtin_memcpy(y, &v, 16);
+        } else {
+          for (uint32_t k = 0; k < a.n_out - n; k++) y[k] = ((const T*)from)[k];
+        }
+      }
+    }
+    wait_lds();
+  }
+}
+
+template <class T, bool GROUPED, int WT, int WN, int FT, int FN>
+__global__ __launch_bounds__(64 * WT * WN) void k_i8_ring(I8Args a, uint32_t tiles_t, uint32_t tiles_n) {
+  constexpr uint32_t WAVES = WT * WN, BT = WT * FT * 32, BN = WN * FN * 32, BK = 128;
+  static_assert(BT == BN, "the ring's slots hold either side's tile");
+  constexpr uint32_t SLOT = BT * BK, PER = BT / 8 / WAVES;  // 8-row pieces of 1 KB that a wave fills
+  constexpr int HALF = PER / 2;
+  constexpr uint32_t OWN = 32 * (FN * 32 * sizeof(T) + 16);  // a wave's part of LDS for its results
+  __shared__ __align__(16) int8_t lds[5 * SLOT];
+  auto swz = [](uint32_t row) { return (row >> 1) & 7u; };
+  const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  uint32_t tt, tn;
+  if (!tile_of_block(blockIdx.x, tiles_t, tiles_n, tt, tn)) return;
+  const uint32_t n0 = tn * BN;
+  uint32_t r0 = tt * BT, r1 = a.rows, e = 0;
+  if (GROUPED) expert_tile(a, tt, BT, r0, r1, e);
   if (r0 >= r1) return;
   const bool none = GROUPED && e >= a.experts;
-  const int8_t* w = a.w + (size_t)e * a.n_out * a.ld_w;
-  // a thread moves 16 bytes of one row of each tile
-  const uint32_t lr = tid >> 2, lk = (tid & 3) * 16;
-  int64_t xr = -1;
-  if (r0 + lr < r1 && !none) xr = GROUPED ? source_row(a, r0 + lr) : (int64_t)(r0 + lr);
-  const bool wr = n0 + lr < a.n_out && !none;
-  v16i acc = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
-  const uint32_t wn = (wave & 1) * 32, wt = (wave >> 1) * 32;
-  for (uint32_t k = 0; k < a.n_in && !none; k += 64) {
-    const v4i zero = {0, 0, 0, 0};
-    const v4i xv = xr >= 0 ? load16(a.x + (size_t)xr * a.ld_x, k + lk, a.n_in) : zero;
-    const v4i wv = wr ? load16(w + (size_t)(n0 + lr) * a.ld_w, k + lk, a.n_in) : zero;
-    *(v4i*)&X[lr * LD + lk] = xv;
-    *(v4i*)&W[lr * LD + lk] = wv;
-    __syncthreads();
+  const int8_t* w = a.w + (none ? 0 : (size_t)e * a.n_out * a.ld_w);
+  Factors<GROUPED, BT, BN, 64 * WAVES> factors;
+  factors.load(a, r0, r1, n0, e);
+  const int8_t *xp[PER], *wp[PER];
+  auto chunk = [&](uint32_t piece) { return ((lane & 7) ^ swz(piece * 8 + (lane >> 3))) * 16; };
 #pragma unroll
-    for (int s = 0; s < 2; s++) {
-      const uint32_t o = s * 32 + (lane >> 5) * 16;
-      const v4i fw = *(const v4i*)&W[(wn + (lane & 31)) * LD + o];
-      const v4i fx = *(const v4i*)&X[(wt + (lane & 31)) * LD + o];
-      acc = __builtin_amdgcn_mfma_i32_32x32x32_i8(fw, fx, acc, 0, 0, 0);
+  for (uint32_t i = 0; i < PER; i++) {
+    const uint32_t row = (wave * PER + i) * 8 + (lane >> 3);
+    const uint32_t r = r0 + row < r1 ? r0 + row : r1 - 1;
+    int64_t s = GROUPED ? source_row(a, r) : (int64_t)r;
+    if (s < 0) s = 0;
+    xp[i] = a.x + (size_t)s * a.ld_x + chunk(wave * PER + i);
+    const uint32_t n = n0 + row < a.n_out ? n0 + row : a.n_out - 1;
+    wp[i] = w + (size_t)n * a.ld_w + chunk(wave * PER + i);
+  }
+  const uint32_t base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) int8_t*)lds + wave * PER * 1024;
+  const uint32_t full = none ? 0 : a.n_in / BK, tail = none ? 0 : a.n_in % BK;
+  const uint32_t steps = full + (tail ? 1 : 0);
+  // piece i of one side's tile of `step` into ring slot `slot`
+  auto fill = [&](const int8_t*& p, uint32_t i, uint32_t step, uint32_t slot) {
+    const uint32_t at = base + slot * SLOT + i * 1024;
+    if (step < full) load_to_lds(p, at);
+    else if (step < steps) load_to_lds(chunk(wave * PER + i) < tail ? p : (const int8_t*)&zeros16, at);
+    p += BK;
+  };
+  const uint32_t wave_t = wave % WT, wave_n = wave / WT;
+  const uint32_t fr = lane & 31;
+  const int8_t* fx = lds + (wave_t * FT * 32 + fr) * BK;
+  const int8_t* fw = lds + (wave_n * FN * 32 + fr) * BK;
+  uint32_t ch[4];
+#pragma unroll
+  for (uint32_t s = 0; s < 4; s++) ch[s] = ((2 * s + (lane >> 5)) ^ swz(fr)) * 16;
+  v16i acc[FN][FT] = {};
+  v4i wf[2][FN], xf[2][FT];
+  auto read = [&](int set, int r, uint32_t xs, uint32_t ws, uint32_t s) {
+    if (r < FN) wf[set][r] = *(const v4i*)(fw + ws * SLOT + r * 32 * BK + ch[s]);
+    else xf[set][r - FN] = *(const v4i*)(fx + xs * SLOT + (r - FN) * 32 * BK + ch[s]);
+  };
+  if (steps) {
+#pragma unroll
+    for (uint32_t i = 0; i < PER; i++) fill(xp[i], i, 0, 0);
+#pragma unroll
+    for (uint32_t i = 0; i < PER; i++) fill(wp[i], i, 0, 1);
+#pragma unroll
+    for (uint32_t i = 0; i < PER; i++) fill(xp[i], i, 1, 2);
+#pragma unroll
+    for (uint32_t i = 0; i < PER; i++) fill(wp[i], i, 1, 3);
+#pragma unroll
+    for (uint32_t i = 0; i < PER; i++) fill(xp[i], i, 2, 4);
+    if (steps > 2) wait_loads<3 * PER>();
+    else wait_loads<0>();
+    meet();
+    uint32_t xs = 0;  // slot of this step's x
+    auto up = [](uint32_t slot, uint32_t by) { return slot + by < 5 ? slot + by : slot + by - 5; };
+#pragma unroll
+    for (int r = 0; r < FN + FT; r++) read(0, r, 0, 1, 0);
+    // One step.  LONG: it is not the first, and all that it fills lies in full steps.
+    auto run = [&](auto is_long, uint32_t step) {
+      constexpr bool LONG = decltype(is_long)::value;
+      constexpr int M = FN * FT, R = FN + FT, SPREAD = M >= 4 ? M * 3 / 4 : M;
+      const uint32_t x0 = xs, w0 = up(xs, 1), x1 = up(xs, 2), w1 = up(xs, 3), x2 = up(xs, 4);
+      auto put = [&](const int8_t*& p, uint32_t i, uint32_t of, uint32_t slot) {
+        if constexpr (LONG) {
+          load_to_lds(p, base + slot * SLOT + i * 1024);
+          p += BK;
+        } else {
+          fill(p, i, of, slot);
+        }
+      };
+#pragma unroll
+      for (int s = 0; s < 4; s++) {
+        if (s == 3) {
+          // the next step's tiles are in, and everybody has read this one's
+          if (LONG || step + 2 < steps) wait_loads<PER>();
+          else wait_loads<0>();
+          wait_lds();
+          meet();
+        }
+#pragma unroll
+        for (int m = 0; m < M; m++) {
+#pragma unroll
+          for (int r = m * R / SPREAD; r < (m + 1) * R / SPREAD && r < R; r++) {
+            if (s < 3) read((s + 1) & 1, r, x0, w0, s + 1);
+            else if (LONG || step + 1 < steps) read(0, r, x1, w1, 0);
+          }
+          acc[m / FT][m % FT] =
+              __builtin_amdgcn_mfma_i32_32x32x32_i8(wf[s & 1][m / FT], xf[s & 1][m % FT], acc[m / FT][m % FT], 0, 0, 0);
+#pragma unroll
+          for (int d = 0; d < HALF; d++)
+            if (d * M / HALF == m) {
+              if (s == 3) put(wp[d], d, step + 2, x0);
+              if (LONG || step) {
+                if (s == 0) put(wp[HALF + d], HALF + d, step + 1, w1);
+                if (s == 1) put(xp[d], d, step + 2, x2);
+                if (s == 2) put(xp[HALF + d], HALF + d, step + 2, x2);
+              }
+            }
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+      xs = x1;
+    };
+    uint32_t step = 0;
+    run(std::false_type(), step++);
+    for (; step + 2 < full; step++) run(std::true_type(), step);
+    for (; step < steps; step++) run(std::false_type(), step);
+  }
+  // the last step ended with everybody past its reads: the ring is free
+  float* f = (float*)(lds + WAVES * OWN);
+  factors.store(f);
+  wait_lds();
+  meet();
+  put_results<T, GROUPED, BT, BN, FT, FN>(a, acc, f, lds + wave * OWN, r0, r1, n0, wave_t * FT * 32, wave_n * FN * 32);
+}
+
+// The same tiles where a row may start at any byte, or end inside a chunk: the
+// steps pass through registers (masked), loaded a step ahead and stored before
+// the stage's turn.
+template <class T, bool GROUPED, int WT, int WN, int FT, int FN>
+__global__ __launch_bounds__(64 * WT * WN) void k_i8_odd(I8Args a, uint32_t tiles_t, uint32_t tiles_n) {
+  constexpr uint32_t WAVES = WT * WN, BT = WT * FT * 32, BN = WN * FN * 32, BK = 128;
+  constexpr uint32_t XB = BT * BK, STAGE = XB + BN * BK, XR = BT / 8 / WAVES, WR = BN / 8 / WAVES;
+  constexpr uint32_t OWN = 32 * (FN * 32 * sizeof(T) + 16);
+  static_assert(WAVES * OWN + 4 * (2 * BT + 2 * BN) <= 2 * STAGE, "the results' LDS is the stages'");
+  __shared__ __align__(16) int8_t lds[2 * STAGE];
+  auto swz = [](uint32_t row) { return (row >> 1) & 7u; };
+  const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  uint32_t tt, tn;
+  if (!tile_of_block(blockIdx.x, tiles_t, tiles_n, tt, tn)) return;
+  const uint32_t n0 = tn * BN;
+  uint32_t r0 = tt * BT, r1 = a.rows, e = 0;
+  if (GROUPED) expert_tile(a, tt, BT, r0, r1, e);
+  if (r0 >= r1) return;
+  const bool none = GROUPED && e >= a.experts;
+  const int8_t* w = a.w + (none ? 0 : (size_t)e * a.n_out * a.ld_w);
+  Factors<GROUPED, BT, BN, 64 * WAVES> factors;
+  factors.load(a, r0, r1, n0, e);
+  const int8_t *xp[XR], *wp[WR];
+#pragma unroll
+  for (uint32_t i = 0; i < XR; i++) {
+    const uint32_t row = (wave * XR + i) * 8 + (lane >> 3);
+    const uint32_t r = r0 + row < r1 ? r0 + row : r1 - 1;
+    int64_t s = GROUPED ? source_row(a, r) : (int64_t)r;
+    if (s < 0) s = 0;
+    xp[i] = a.x + (size_t)s * a.ld_x;
+  }
+#pragma unroll
+  for (uint32_t i = 0; i < WR; i++) {
+    const uint32_t row = (wave * WR + i) * 8 + (lane >> 3);
+    const uint32_t n = n0 + row < a.n_out ? n0 + row : a.n_out - 1;
+    wp[i] = w + (size_t)n * a.ld_w;
+  }
+  const uint32_t steps = none ? 0 : (a.n_in + BK - 1) / BK;
+  v4i held[XR + WR];
+  auto chunk = [&](uint32_t piece) { return ((lane & 7) ^ swz(piece * 8 + (lane >> 3))) * 16; };
+  auto take = [&](uint32_t step) {
+#pragma unroll
+    for (uint32_t i = 0; i < XR; i++) held[i] = load16(xp[i], step * BK + chunk(wave * XR + i), a.n_in);
+#pragma unroll
+    for (uint32_t i = 0; i < WR; i++) held[XR + i] = load16(wp[i], step * BK + chunk(wave * WR + i), a.n_in);
+  };
+  auto store = [&](uint32_t stage) {
+    int8_t* at = lds + stage * STAGE + lane * 16;
+#pragma unroll
+    for (uint32_t i = 0; i < XR; i++) *(v4i*)(at + (wave * XR + i) * 1024) = held[i];
+#pragma unroll
+    for (uint32_t i = 0; i < WR; i++) *(v4i*)(at + XB + (wave * WR + i) * 1024) = held[XR + i];
+  };
+  const uint32_t wave_t = wave % WT, wave_n = wave / WT;
+  const uint32_t fr = lane & 31;
+  const int8_t* fx = lds + (wave_t * FT * 32 + fr) * BK;
+  const int8_t* fw = lds + XB + (wave_n * FN * 32 + fr) * BK;
+  uint32_t ch[4];
+#pragma unroll
+  for (uint32_t s = 0; s < 4; s++) ch[s] = ((2 * s + (lane >> 5)) ^ swz(fr)) * 16;
+  v16i acc[FN][FT] = {};
+  v4i wf[2][FN], xf[2][FT];
+  auto read = [&](int set, uint32_t stage, uint32_t s) {
+#pragma unroll
+    for (int j = 0; j < FN; j++) wf[set][j] = *(const v4i*)(fw + stage * STAGE + j * 32 * BK + ch[s]);
+#pragma unroll
+    for (int j = 0; j < FT; j++) xf[set][j] = *(const v4i*)(fx + stage * STAGE + j * 32 * BK + ch[s]);
+  };
+  if (steps) {
+    take(0);
+    store(0);
+    if (steps > 1) take(1);
+    wait_lds();
+    meet();
+    read(0, 0, 0);
+    for (uint32_t step = 0; step < steps; step++) {
+      const uint32_t stage = step & 1;
+#pragma unroll
+      for (uint32_t s = 0; s < 4; s++) {
+        if (s < 3) {
+          read((s + 1) & 1, stage, s + 1);
+        } else {
+          // once all have read this stage and filled the next, it may be filled again
+          if (step + 1 < steps) store(stage ^ 1);
+          wait_lds();
+          meet();
+          if (step + 2 < steps) take(step + 2);
+          if (step + 1 < steps) read(0, stage ^ 1, 0);
+        }
+#pragma unroll
+        for (int i = 0; i < FN; i++)
+#pragma unroll
+          for (int j = 0; j < FT; j++)
+            acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(wf[s & 1][i], xf[s & 1][j], acc[i][j], 0, 0, 0);
+      }
     }
-    __syncthreads();
   }
-  const uint32_t t = r0 + wt + (lane & 31);
-  if (t >= r1) return;
-  int64_t src = GROUPED ? (none ? -1 : source_row(a, t)) : (int64_t)t;
-  const float sx = src >= 0 && a.sx ? a.sx[src] : 1.0f;
-  const size_t ch = (size_t)e * a.n_out;
+  // the last step ended with everybody past its reads: the ring is free
+  float* f = (float*)(lds + WAVES * OWN);
+  factors.store(f);
+  wait_lds();
+  meet();
+  put_results<T, GROUPED, BT, BN, FT, FN>(a, acc, f, lds + wave * OWN, r0, r1, n0, wave_t * FT * 32, wave_n * FN * 32);
+}
+
+// ------------------------------------------------------------ few rows on one side
+// Few tokens (decoding) or few channels (scoring): one side is read once from
+// HBM and each block needs little of the other, so fragments come straight from
+// global memory.  A block has 16 FT tokens x 16 FN channels; its KW waves split
+// k between them in steps of 128 bytes (a cache line of every row: lane r + 16 c
+// takes bytes 32 c to 32 c + 31 of row r, which gives both sides the same order
+// of k) and add up their sums in LDS.
+template <class T, bool GROUPED, int FT, int FN, int KW>
+__global__ __launch_bounds__(64 * KW) void k_i8_direct(I8Args a, uint32_t tiles_t, uint32_t tiles_n) {
+  constexpr uint32_t BT = 16 * FT, BN = 16 * FN, BK = 128;
+  constexpr int U = FT + FN <= 2 ? 4 : 2;  // steps whose loads are under way together
+  __shared__ __align__(16) v4i sums[KW > 1 ? KW : 1][FN * FT][64];
+  const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  uint32_t tt, tn;
+  if (!tile_of_block(blockIdx.x, tiles_t, tiles_n, tt, tn)) return;
+  const uint32_t n0 = tn * BN;
+  uint32_t r0 = tt * BT, r1 = a.rows, e = 0;
+  if (GROUPED) expert_tile(a, tt, BT, r0, r1, e);
+  if (r0 >= r1) return;
+  const bool none = GROUPED && e >= a.experts;
+  const int8_t* w = a.w + (none ? 0 : (size_t)e * a.n_out * a.ld_w);
+  const uint32_t fr = lane & 15, c = lane >> 4;
+  const int8_t *xp[FT], *wp[FN];
+  int64_t src[FT];
 #pragma unroll
-  for (int i = 0; i < 16; i++) {
-    const uint32_t n = n0 + wn + 8 * (i >> 2) + 4 * (lane >> 5) + (i & 3);
-    if (n >= a.n_out) continue;
-    T v = (T)0;
-    if (!GROUPED || src >= 0)
-      v = finish<T>(acc[i], sx * (a.sw ? a.sw[ch + n] : 1.0f), a.bias ? a.bias[ch + n] : 0.0f, a.relu);
-    ((T*)a.y)[(size_t)t * a.ld_y + n] = v;
+  for (int j = 0; j < FT; j++) {
+    const uint32_t t = r0 + j * 16 + fr, r = t < r1 ? t : r1 - 1;
+    const int64_t s = GROUPED ? source_row(a, r) : (int64_t)r;
+    src[j] = none ? -1 : s;
+    xp[j] = a.x + (size_t)(s < 0 ? 0 : s) * a.ld_x;
+  }
+#pragma unroll
+  for (int i = 0; i < FN; i++) {
+    const uint32_t n = n0 + i * 16 + fr;
+    wp[i] = w + (size_t)(n < a.n_out ? n : a.n_out - 1) * a.ld_w;
+  }
+  v4i acc[FN][FT] = {};
+  const uint32_t steps = none ? 0 : (a.n_in + BK - 1) / BK, full = none ? 0 : a.n_in / BK;
+  uint32_t step = wave;
+  v4i xf[U][FT][2], wf[U][FN][2];
+  auto multiply = [&](int u) {
+#pragma unroll
+    for (int h = 0; h < 2; h++)
+#pragma unroll
+      for (int i = 0; i < FN; i++)
+#pragma unroll
+        for (int j = 0; j < FT; j++)
+          acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[u][i][h], xf[u][j][h], acc[i][j], 0, 0, 0);
+  };
+  for (; step + (U - 1) * KW < full; step += U * KW) {
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      const uint32_t k = (step + u * KW) * BK + c * 32;
+#pragma unroll
+      for (int i = 0; i < FN; i++) __builtin_memcpy(wf[u][i], wp[i] + k, 32);
+#pragma unroll
+      for (int j = 0; j < FT; j++) __builtin_memcpy(xf[u][j], xp[j] + k, 32);
+    }
+#pragma unroll
+    for (int u = 0; u < U; u++) multiply(u);
+  }
+  // the rest, all loads together again: whole steps, and the row's end masked
+  if (step < steps) {
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      const uint32_t k = (step + u * KW) * BK + c * 32;
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+#pragma unroll
+        for (int i = 0; i < FN; i++) wf[u][i][h] = load16(wp[i], k + 16 * h, a.n_in);
+#pragma unroll
+        for (int j = 0; j < FT; j++) xf[u][j][h] = load16(xp[j], k + 16 * h, a.n_in);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; u++) multiply(u);
+  }
+  // ---- results: lane r + 16 q holds channels 4 q to 4 q + 3 of token r
+  auto put = [&](int i, int j, const v4i& sum) {
+    const uint32_t t = r0 + j * 16 + fr, n = n0 + i * 16 + 4 * c;
+    if (t >= r1 || n >= a.n_out) return;
+    const bool zero = GROUPED && src[j] < 0;
+    const float sx = a.sx && !zero ? a.sx[src[j]] : 1.0f;
+    const size_t ch = (none ? 0 : (size_t)e * a.n_out) + n;
+    T v[4];
+#pragma unroll
+    for (uint32_t k = 0; k < 4; k++) {
+      const bool in = n + k < a.n_out;
+      const float sw = a.sw && in ? a.sw[ch + k] : 1.0f, b = a.bias && in ? a.bias[ch + k] : 0.0f;
+      v[k] = zero ? (T)0 : finish<T>(sum[k], sx * sw, b, a.relu);
+    }
+    T* y = (T*)a.y + (size_t)t * a.ld_y + n;
+    if (n + 4 <= a.n_out) {
+      __builtin_memcpy(y, v, sizeof(v));
+    } else {
+      for (uint32_t k = 0; k < a.n_out - n; k++) y[k] = v[k];
+    }
+  };
+  if constexpr (KW == 1) {
+#pragma unroll
+    for (int i = 0; i < FN; i++)
+#pragma unroll
+      for (int j = 0; j < FT; j++) put(i, j, acc[i][j]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < FN; i++)
+#pragma unroll
+      for (int j = 0; j < FT; j++) sums[wave][i * FT + j][lane] = acc[i][j];
+    __syncthreads();
+    // wave k adds up square k
+#pragma unroll
+    for (int sq = 0; sq < FN * FT; sq++) {
+      if ((uint32_t)sq % KW != wave) continue;
+      v4i sum = sums[0][sq][lane];
+#pragma unroll
+      for (int k = 1; k < KW; k++) sum += sums[k][sq][lane];
+      put(sq / FT, sq % FT, sum);
+    }
   }
 }
 
-template <class T>
-static int launch_tile(zk_context* ctx, const I8Args& a, bool grouped, hipStream_t st) {
-  const size_t by = grouped ? (size_t)(a.rows + 63) / 64 + (a.experts < a.rows ? a.experts : a.rows) + 1
-                            : ((size_t)a.rows + 63) / 64;
-  const dim3 grid(cdiv(a.n_out, 64), (uint32_t)by);
-  if (grouped)
-    ZK_LAUNCH(ctx, st, "i8_matmul_experts", (k_i8_tile<T, true>), grid, dim3(256), 0, a);
-  else
-    ZK_LAUNCH(ctx, st, "i8_matmul", (k_i8_tile<T, false>), grid, dim3(256), 0, a);
-  return ZK_OK;
+// ------------------------------------------------------------ which kernel
+// Estimated time of a product in ns: a tile's own part (its first loads and its
+// results) and its steps, of which each of the 256 CUs has ceil(tiles / 256) to do.
+struct TileCost {
+  uint32_t size, own, step;
+};
+static uint64_t tile_cost(const TileCost& c, uint64_t rows, uint64_t spare_tiles, uint64_t n_out, uint64_t n_in) {
+  const uint64_t tiles = (rows / c.size + (rows % c.size != 0) + spare_tiles) * ((n_out + c.size - 1) / c.size);
+  return (tiles + 255) / 256 * ((n_in + 127) / 128) * c.step + c.own;
 }
 
-static int i8_dispatch(zk_context* ctx, const I8Args& a, int type, bool grouped, hipStream_t st) {
+template <class T, bool GROUPED>
+static int launch_product(zk_context* ctx, const I8Args& a, hipStream_t st) {
+  const char* name = GROUPED ? "i8_matmul_experts" : "i8_matmul";
+  // row tiles of the grouped form: one more than whole ones for each group
+  const uint32_t groups = GROUPED ? (a.experts + 1 < a.rows ? a.experts + 1 : a.rows) : 0;
+  auto go = [&](auto kernel, uint32_t bt, uint32_t bn, uint32_t threads) -> int {
+    const uint32_t tiles_t = GROUPED ? a.rows / bt + groups : cdiv(a.rows, bt), tiles_n = cdiv(a.n_out, bn);
+    const size_t tiles = (size_t)tiles_t * tiles_n;
+    if (tiles > I8_MAX_TILES) return ctx->fail(ZK_ERR_SIZE, "i8 experts: rows and n_out make too many tiles");
+    const dim3 grid(cdiv(tiles, 8) * 8);
+    ZK_LAUNCH(ctx, st, name, kernel, grid, dim3(threads), 0, a, tiles_t, tiles_n);
+    return ZK_OK;
+  };
+  const uint32_t per = GROUPED ? (a.rows + a.experts - 1) / a.experts : a.rows;  // rows of an average expert
+  if (per <= 64) {
+    if (per <= 16) return go(k_i8_direct<T, GROUPED, 1, 1, 8>, 16, 16, 512);
+    if (per <= 32) return go(k_i8_direct<T, GROUPED, 2, 1, 8>, 32, 16, 512);
+    return go(k_i8_direct<T, GROUPED, 4, 1, 8>, 64, 16, 512);
+  }
+  if (!GROUPED && a.n_out <= 64) {
+    if (a.n_in <= 256) {
+      if (a.n_out <= 16) return go(k_i8_direct<T, GROUPED, 4, 1, 1>, 64, 16, 64);
+      return go(k_i8_direct<T, GROUPED, 4, 2, 1>, 64, 32, 64);
+    }
+    if (a.n_out <= 16) return go(k_i8_direct<T, GROUPED, 1, 1, 8>, 16, 16, 512);
+    if (a.n_out <= 32) return go(k_i8_direct<T, GROUPED, 1, 2, 8>, 16, 32, 512);
+    return go(k_i8_direct<T, GROUPED, 1, 4, 8>, 16, 64, 512);
+  }
+  const TileCost even[3] = {{64, 2500, 230}, {128, 5000, 530}, {256, 9000, 1600}};
+  const TileCost odd[2] = {{64, 2500, 280}, {128, 5000, 700}};
+  const bool whole = ((uintptr_t)a.x | (uintptr_t)a.w | a.ld_x | a.ld_w | a.n_in) % 16 == 0;
+  uint32_t best = 64;
+  uint64_t least = ~0ull;
+  for (int i = 0; i < (whole ? 3 : 2); i++) {
+    const TileCost& c = whole ? even[i] : odd[i];
+    const uint64_t t = tile_cost(c, a.rows, groups / 2, a.n_out, a.n_in);
+    if (t < least) least = t, best = c.size;
+  }
+  if (!whole) {
+    if (best == 64) return go(k_i8_odd<T, GROUPED, 2, 2, 1, 1>, 64, 64, 256);
+    return go(k_i8_odd<T, GROUPED, 2, 2, 2, 2>, 128, 128, 256);
+  }
+  if (best == 64) return go(k_i8_ring<T, GROUPED, 2, 2, 1, 1>, 64, 64, 256);
+  if (best == 128) return go(k_i8_ring<T, GROUPED, 2, 2, 2, 2>, 128, 128, 256);
+  return go(k_i8_ring<T, GROUPED, 2, 4, 4, 2>, 256, 256, 512);
+}
+
+template <bool GROUPED>
+static int i8_dispatch(zk_context* ctx, const I8Args& a, int type, hipStream_t st) {
   switch (type) {
-    case ZK_I32: return launch_tile<int>(ctx, a, grouped, st);
-    case ZK_F32: return launch_tile<float>(ctx, a, grouped, st);
-    case ZK_F16: return launch_tile<_Float16>(ctx, a, grouped, st);
-    default: return launch_tile<__bf16>(ctx, a, grouped, st);
+    case ZK_I32: return launch_product<int, GROUPED>(ctx, a, st);
+    case ZK_F32: return launch_product<float, GROUPED>(ctx, a, st);
+    case ZK_F16: return launch_product<_Float16, GROUPED>(ctx, a, st);
+    default: return launch_product<__bf16, GROUPED>(ctx, a, st);
   }
 }
 
@@ -237,6 +742,7 @@ static int check_product(zk_context* ctx, const I8Args& a, size_t rows, size_t n
     return ctx->fail(ZK_ERR_INVALID, "i8 product: integer sums take no scales and no bias");
   if (n_in > I8_MAX_IN) return ctx->fail(ZK_ERR_SIZE, "i8 product: n_in above 131071 can pass 32 bits");
   if (rows > 0x7fffffffu || n_out > 0x7fffffffu) return ctx->fail(ZK_ERR_SIZE, "i8 product: sizes above 2^31 - 1");
+  if (n_out > 16 * I8_MAX_TILES) return ctx->fail(ZK_ERR_SIZE, "i8 product: n_out above 2^26");
   if (a.ld_x < n_in || a.ld_w < n_in || a.ld_y < n_out)
     return ctx->fail(ZK_ERR_INVALID, "i8 product: a row stride below the row's length");
   if (rows && n_out && (!a.y || (n_in && (!a.x || !a.w))))
@@ -276,15 +782,15 @@ static int matmul_impl(zk_context* ctx, const int8_t* x, size_t ld_x, const floa
   ZK_TRY(check_product(ctx, a, rows, n_out, n_in, type));
   if (!rows || !n_out) return ZK_OK;
   a.n_out = (uint32_t)n_out, a.n_in = (uint32_t)n_in, a.relu = relu != 0;
-  // a launch has at most 65535 row tiles
-  const size_t most = (size_t)65535 * 64;
+  // rows in runs of at most I8_MAX_TILES tiles of 16 x 16
+  const size_t most = I8_MAX_TILES / ((n_out + 15) / 16) * 16;
   for (size_t r = 0; r < rows; r += most) {
     I8Args b = a;
     b.rows = (uint32_t)(rows - r < most ? rows - r : most);
     b.x = x ? x + r * ld_x : x;
     b.sx = sx ? sx + r : sx;
     b.y = (uint8_t*)y + r * ld_y * type_bytes(type);
-    ZK_TRY(i8_dispatch(ctx, b, type, false, st));
+    ZK_TRY(i8_dispatch<false>(ctx, b, type, st));
   }
   return ZK_OK;
 }
@@ -371,7 +877,7 @@ int zk_i8_matmul_experts(zk_context* ctx, const int8_t* d_x, size_t ld_x, const 
     a.rows = (uint32_t)rows, a.n_out = (uint32_t)n_out, a.n_in = (uint32_t)n_in, a.relu = relu != 0;
     a.offsets = d_offsets, a.order = d_order, a.experts = (uint32_t)experts, a.slots = (uint32_t)slots;
     a.tokens = (uint32_t)tokens;
-    return i8_dispatch(ctx, a, y_type, true, ctx->s(stream));
+    return i8_dispatch<true>(ctx, a, y_type, ctx->s(stream));
   });
 }
 
