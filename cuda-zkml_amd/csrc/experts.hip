@@ -10,6 +10,7 @@
 // A pair whose expert is outside [0, experts) is dropped: place -1, and order
 // holds -1 behind the last sorted pair.  No result depends on the order in
 // which blocks or atomics run.
+#include "rows.hpp"
 #include "zk_internal.hpp"
 
 namespace zk {
@@ -143,42 +144,6 @@ __global__ __launch_bounds__(SORT_THREADS) void k_sort_place(const int32_t* __re
 }
 
 // ------------------------------------------------------------ rows
-// Rows move 16 bytes a lane at any address (gfx950 loads and stores 16 bytes
-// from any address); a row's last, shorter piece is taken 16 bytes back from
-// its end, so that two lanes may write the same values there.  Rows under 16
-// bytes go element by element.
-template <class T>
-struct Vec {
-  static constexpr uint32_t N = 16 / sizeof(T);
-  T v[N];
-};
-
-template <class T>
-__device__ __forceinline__ Vec<T> row_load(const T* p, uint32_t left) {
-  Vec<T> r;
-  if (left >= Vec<T>::N) {
-    __builtin_memcpy(&r, p, 16);
-  } else {
-    for (uint32_t i = 0; i < Vec<T>::N; i++) r.v[i] = i < left ? p[i] : (T)0.0f;
-  }
-  return r;
-}
-template <class T>
-__device__ __forceinline__ void row_store(T* p, uint32_t left, const Vec<T>& r) {
-  if (left >= Vec<T>::N) {
-    __builtin_memcpy(p, &r, 16);
-  } else {
-    for (uint32_t i = 0; i < Vec<T>::N; i++)
-      if (i < left) p[i] = r.v[i];
-  }
-}
-// First element of a row's c-th piece and the elements from there on.
-template <class T>
-__device__ __forceinline__ uint32_t piece(uint32_t c, uint32_t cols) {
-  const uint32_t at = c * Vec<T>::N;
-  return at + Vec<T>::N <= cols || cols < Vec<T>::N ? at : cols - Vec<T>::N;
-}
-
 // out[p] = x[order[p] / slots], zeros where order[p] names no token.
 template <class T>
 __global__ __launch_bounds__(256) void k_gather(const T* __restrict__ x, size_t ld_x,
@@ -188,7 +153,7 @@ __global__ __launch_bounds__(256) void k_gather(const T* __restrict__ x, size_t 
   if (p >= rows) return;
   const int o = order[p];
   const uint32_t t = o < 0 ? tokens : (uint32_t)o / slots;
-  const uint32_t pieces = (cols + Vec<T>::N - 1) / Vec<T>::N;
+  const uint32_t pieces = pieces_of<T>(cols);
   for (uint32_t c = threadIdx.x; c < pieces; c += 256) {
     const uint32_t at = piece<T>(c, cols);
     Vec<T> v = {};
@@ -204,7 +169,7 @@ __global__ __launch_bounds__(256) void k_combine(const T* __restrict__ y, size_t
                                                  uint32_t rows, uint32_t slots, uint32_t cols, T* __restrict__ out,
                                                  size_t ld_out) {
   const uint32_t t = blockIdx.x;
-  const uint32_t pieces = (cols + Vec<T>::N - 1) / Vec<T>::N;
+  const uint32_t pieces = pieces_of<T>(cols);
   for (uint32_t c = threadIdx.x; c < pieces; c += 256) {
     const uint32_t at = piece<T>(c, cols);
     float s[Vec<T>::N] = {};
@@ -232,7 +197,7 @@ __global__ __launch_bounds__(256) void k_combine_grad(const T* __restrict__ g, s
                                                       float* __restrict__ dw) {
   __shared__ float part[4];
   const uint32_t t = blockIdx.x, tid = threadIdx.x;
-  const uint32_t pieces = (cols + Vec<T>::N - 1) / Vec<T>::N;
+  const uint32_t pieces = pieces_of<T>(cols);
   for (uint32_t j = 0; j < slots; j++) {
     const size_t i = (size_t)t * slots + j;
     if (i < rows && order[i] < 0) {
@@ -269,9 +234,6 @@ __global__ __launch_bounds__(256) void k_combine_grad(const T* __restrict__ g, s
 }
 
 // ------------------------------------------------------------ arguments
-static size_t type_bytes(int type) { return type == ZK_F32 ? 4 : 2; }
-static bool aligned(const void* p, size_t n) { return (uintptr_t)p % n == 0; }
-
 static int check_experts(zk_context* ctx, size_t pairs, int experts) {
   if (experts < 1 || experts > ZK_MAX_EXPERTS) return ctx->fail(ZK_ERR_SIZE, "experts: between 1 and 1024 experts");
   if (pairs > ZK_MAX_EXPERT_ROWS) return ctx->fail(ZK_ERR_SIZE, "experts: more than 2^22 pairs");
@@ -279,7 +241,7 @@ static int check_experts(zk_context* ctx, size_t pairs, int experts) {
 }
 
 static int check_rows(zk_context* ctx, int type, size_t rows, size_t tokens, int slots, size_t cols) {
-  if (type != ZK_F32 && type != ZK_F16 && type != ZK_BF16)
+  if (!float_type(type))
     return ctx->fail(ZK_ERR_INVALID, "experts: rows are f32, f16 or bf16");
   if (slots < 1) return ctx->fail(ZK_ERR_INVALID, "experts: slots is at least 1");
   if (rows > ZK_MAX_EXPERT_ROWS || tokens > ZK_MAX_EXPERT_ROWS || tokens * (size_t)slots > ZK_MAX_EXPERT_ROWS)
@@ -299,14 +261,6 @@ static int check_words(zk_context* ctx, const void* p, bool may_be_null) {
   if (!p && !may_be_null) return ctx->fail(ZK_ERR_INVALID, "experts: null pointer");
   if (!aligned(p, 4)) return ctx->fail(ZK_ERR_INVALID, "experts: a pointer is not aligned to its type");
   return ZK_OK;
-}
-
-// Calls f with a value of the rows' type.
-template <class Fn>
-static int by_type(int type, Fn&& f) {
-  if (type == ZK_F32) return f(0.0f);
-  if (type == ZK_F16) return f((_Float16)0.0f);
-  return f((__bf16)0.0f);
 }
 
 }  // namespace zk

@@ -10,6 +10,7 @@
 // offsets[e+1] of y use w[e].
 #include <type_traits>
 
+#include "rows.hpp"
 #include "zk_internal.hpp"
 
 namespace zk {
@@ -37,17 +38,27 @@ struct I8Args {
   uint32_t experts, slots, tokens;
 };
 
-// 16 bytes of a row from byte k on, zeros from n_in on.  The row's address may
-// be odd: gfx950 loads 16 bytes from any address.
-__device__ __forceinline__ v4i load16(const int8_t* __restrict__ row, uint32_t k, uint32_t n_in) {
-  v4i v = {0, 0, 0, 0};
-  if (k + 16 <= n_in) {
-    __builtin_memcpy(&v, row + k, 16);
-  } else if (k < n_in) {
-    uint32_t b[4] = {0, 0, 0, 0};
-    for (uint32_t i = 0; i < n_in - k; i++) b[i / 4] |= (uint32_t)(uint8_t)row[k + i] << (8 * (i % 4));
-    v = v4i{(int)b[0], (int)b[1], (int)b[2], (int)b[3]};
-  }
+// Where a lane takes the 16 bytes of k from byte k on, for rows of n_in >= 16
+// bytes: a chunk that passes the rows' end is the last 16 bytes of both x's and
+// w's rows, with the bytes before k masked off x.  The same order of k on both
+// sides is all that a sum needs, and no byte outside a row is read.
+struct Chunk {
+  uint32_t at;
+  v4i mask;
+};
+__device__ __forceinline__ Chunk last_chunk(uint32_t k, uint32_t n_in) {
+  Chunk c;
+  c.at = k < n_in - 16 ? k : n_in - 16;
+  const uint32_t skip = k - c.at;
+#pragma unroll
+  for (uint32_t d = 0; d < 4; d++)
+    c.mask[d] = skip <= 4 * d ? -1 : skip >= 4 * d + 4 ? 0 : (int)(~0u << (8 * (skip - 4 * d)));
+  return c;
+}
+// 16 bytes from any address: gfx950 loads them whatever its alignment.
+__device__ __forceinline__ v4i load16(const int8_t* p) {
+  v4i v;
+  __builtin_memcpy(&v, p, 16);
   return v;
 }
 
@@ -417,10 +428,21 @@ __global__ __launch_bounds__(64 * WT * WN) void k_i8_odd(I8Args a, uint32_t tile
   v4i held[XR + WR];
   auto chunk = [&](uint32_t piece) { return ((lane & 7) ^ swz(piece * 8 + (lane >> 3))) * 16; };
   auto take = [&](uint32_t step) {
+    if ((step + 1) * BK <= a.n_in) {
 #pragma unroll
-    for (uint32_t i = 0; i < XR; i++) held[i] = load16(xp[i], step * BK + chunk(wave * XR + i), a.n_in);
+      for (uint32_t i = 0; i < XR; i++) held[i] = load16(xp[i] + step * BK + chunk(wave * XR + i));
 #pragma unroll
-    for (uint32_t i = 0; i < WR; i++) held[XR + i] = load16(wp[i], step * BK + chunk(wave * WR + i), a.n_in);
+      for (uint32_t i = 0; i < WR; i++) held[XR + i] = load16(wp[i] + step * BK + chunk(wave * WR + i));
+    } else {
+#pragma unroll
+      for (uint32_t i = 0; i < XR; i++) {
+        const Chunk c = last_chunk(step * BK + chunk(wave * XR + i), a.n_in);
+        held[i] = load16(xp[i] + c.at) & c.mask;
+      }
+#pragma unroll
+      for (uint32_t i = 0; i < WR; i++)
+        held[XR + i] = load16(wp[i] + last_chunk(step * BK + chunk(wave * WR + i), a.n_in).at);
+    }
   };
   auto store = [&](uint32_t stage) {
     int8_t* at = lds + stage * STAGE + lane * 16;
@@ -481,18 +503,17 @@ __global__ __launch_bounds__(64 * WT * WN) void k_i8_odd(I8Args a, uint32_t tile
   put_results<T, GROUPED, BT, BN, FT, FN>(a, acc, f, lds + wave * OWN, r0, r1, n0, wave_t * FT * 32, wave_n * FN * 32);
 }
 
-// ------------------------------------------------------------ few rows on one side
-// Few tokens (decoding) or few channels (scoring): one side is read once from
-// HBM and each block needs little of the other, so fragments come straight from
-// global memory.  A block has 16 FT tokens x 16 FN channels; its KW waves split
-// k between them in steps of 128 bytes (a cache line of every row: lane r + 16 c
-// takes bytes 32 c to 32 c + 31 of row r, which gives both sides the same order
-// of k) and add up their sums in LDS.
+// ------------------------------------------------------------ few rows
+// Few tokens (decoding), or a small layer: w is read once and a block needs
+// little of x, so fragments come straight from global memory.  A block has
+// 16 FT tokens x 16 FN channels; its KW waves split k between them in steps of
+// 128 bytes (a cache line of every row) and add up their sums in LDS.  Bound by
+// what the L2 hands over: 16 (FT + FN) rows a block, 9.3 TB/s over the chip.
 template <class T, bool GROUPED, int FT, int FN, int KW>
 __global__ __launch_bounds__(64 * KW) void k_i8_direct(I8Args a, uint32_t tiles_t, uint32_t tiles_n) {
   constexpr uint32_t BT = 16 * FT, BN = 16 * FN, BK = 128;
   constexpr int U = FT + FN <= 2 ? 4 : 2;  // steps whose loads are under way together
-  __shared__ __align__(16) v4i sums[KW > 1 ? KW : 1][FN * FT][64];
+  __shared__ __align__(16) v4i sums[KW][FN * FT][64];
   const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   uint32_t tt, tn;
   if (!tile_of_block(blockIdx.x, tiles_t, tiles_n, tt, tn)) return;
@@ -533,30 +554,38 @@ __global__ __launch_bounds__(64 * KW) void k_i8_direct(I8Args a, uint32_t tiles_
   for (; step + (U - 1) * KW < full; step += U * KW) {
 #pragma unroll
     for (int u = 0; u < U; u++) {
-      const uint32_t k = (step + u * KW) * BK + c * 32;
-#pragma unroll
-      for (int i = 0; i < FN; i++) __builtin_memcpy(wf[u][i], wp[i] + k, 32);
-#pragma unroll
-      for (int j = 0; j < FT; j++) __builtin_memcpy(xf[u][j], xp[j] + k, 32);
-    }
-#pragma unroll
-    for (int u = 0; u < U; u++) multiply(u);
-  }
-  // the rest, all loads together again: whole steps, and the row's end masked
-  if (step < steps) {
-#pragma unroll
-    for (int u = 0; u < U; u++) {
-      const uint32_t k = (step + u * KW) * BK + c * 32;
+      const uint32_t k = (step + u * KW) * BK + c * 16;
 #pragma unroll
       for (int h = 0; h < 2; h++) {
 #pragma unroll
-        for (int i = 0; i < FN; i++) wf[u][i][h] = load16(wp[i], k + 16 * h, a.n_in);
+        for (int i = 0; i < FN; i++) wf[u][i][h] = load16(wp[i] + k + 64 * h);
 #pragma unroll
-        for (int j = 0; j < FT; j++) xf[u][j][h] = load16(xp[j], k + 16 * h, a.n_in);
+        for (int j = 0; j < FT; j++) xf[u][j][h] = load16(xp[j] + k + 64 * h);
       }
     }
 #pragma unroll
     for (int u = 0; u < U; u++) multiply(u);
+  }
+  // the rest, all loads together again
+  if (step < steps) {
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      if (step + u * KW >= steps) break;
+      const uint32_t k = (step + u * KW) * BK + c * 16;
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        const Chunk part = last_chunk(k + 64 * h, a.n_in);
+#pragma unroll
+        for (int i = 0; i < FN; i++) wf[u][i][h] = load16(wp[i] + part.at);
+#pragma unroll
+        for (int j = 0; j < FT; j++) xf[u][j][h] = load16(xp[j] + part.at) & part.mask;
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      if (step + u * KW >= steps) break;
+      multiply(u);
+    }
   }
   // ---- results: lane r + 16 q holds channels 4 q to 4 q + 3 of token r
   auto put = [&](int i, int j, const v4i& sum) {
@@ -579,85 +608,115 @@ __global__ __launch_bounds__(64 * KW) void k_i8_direct(I8Args a, uint32_t tiles_
       for (uint32_t k = 0; k < a.n_out - n; k++) y[k] = v[k];
     }
   };
-  if constexpr (KW == 1) {
 #pragma unroll
-    for (int i = 0; i < FN; i++)
+  for (int i = 0; i < FN; i++)
 #pragma unroll
-      for (int j = 0; j < FT; j++) put(i, j, acc[i][j]);
-  } else {
+    for (int j = 0; j < FT; j++) sums[wave][i * FT + j][lane] = acc[i][j];
+  __syncthreads();
+  // wave k adds up square k
 #pragma unroll
-    for (int i = 0; i < FN; i++)
+  for (int sq = 0; sq < FN * FT; sq++) {
+    if ((uint32_t)sq % KW != wave) continue;
+    v4i sum = sums[0][sq][lane];
 #pragma unroll
-      for (int j = 0; j < FT; j++) sums[wave][i * FT + j][lane] = acc[i][j];
-    __syncthreads();
-    // wave k adds up square k
-#pragma unroll
-    for (int sq = 0; sq < FN * FT; sq++) {
-      if ((uint32_t)sq % KW != wave) continue;
-      v4i sum = sums[0][sq][lane];
-#pragma unroll
-      for (int k = 1; k < KW; k++) sum += sums[k][sq][lane];
-      put(sq / FT, sq % FT, sum);
+    for (int k = 1; k < KW; k++) sum += sums[k][sq][lane];
+    put(sq / FT, sq % FT, sum);
+  }
+}
+
+// ------------------------------------------------------------ rows under 16 bytes
+// A thread takes one result at a time: its sum has 15 terms at the most.
+template <class T, bool GROUPED>
+__global__ __launch_bounds__(256) void k_i8_short(I8Args a) {
+  const uint64_t all = (uint64_t)a.rows * a.n_out, stride = (uint64_t)gridDim.x * 256;
+  for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += stride) {
+    const uint32_t p = (uint32_t)(i / a.n_out), n = (uint32_t)(i % a.n_out);
+    int64_t s = p;
+    size_t ch = n;
+    if (GROUPED) {
+      uint32_t e = 0, hi = a.experts;  // the last expert whose rows begin at p or before, with p among them
+      while (e < hi) {
+        const uint32_t mid = (e + hi) / 2;
+        if (offset_of(a, mid + 1) <= p) e = mid + 1;
+        else hi = mid;
+      }
+      s = e < a.experts ? source_row(a, p) : -1;
+      ch += (size_t)e * a.n_out;
     }
+    T v = (T)0;
+    if (s >= 0) {
+      int acc = 0;
+      for (uint32_t k = 0; k < a.n_in; k++) acc += (int)a.x[(size_t)s * a.ld_x + k] * (int)a.w[ch * a.ld_w + k];
+      v = finish<T>(acc, (a.sx ? a.sx[s] : 1.0f) * (a.sw ? a.sw[ch] : 1.0f), a.bias ? a.bias[ch] : 0.0f, a.relu);
+    }
+    ((T*)a.y)[(size_t)p * a.ld_y + n] = v;
   }
 }
 
 // ------------------------------------------------------------ which kernel
-// Estimated time of a product in ns: a tile's own part (its first loads and its
-// results) and its steps, of which each of the 256 CUs has ceil(tiles / 256) to do.
+// A tile's time in ns: its own part (first loads, results) and its steps of 128
+// bytes of k, of which a CU has ceil(tiles / 256) tiles to do.  Measured on rows
+// that are multiples of 16 bytes (`odd`: on others).
 struct TileCost {
-  uint32_t size, own, step;
+  uint32_t bt, bn, own, step, odd_own, odd_step;
 };
-static uint64_t tile_cost(const TileCost& c, uint64_t rows, uint64_t spare_tiles, uint64_t n_out, uint64_t n_in) {
-  const uint64_t tiles = (rows / c.size + (rows % c.size != 0) + spare_tiles) * ((n_out + c.size - 1) / c.size);
-  return (tiles + 255) / 256 * ((n_in + 127) / 128) * c.step + c.own;
+constexpr TileCost TILE_COST[] = {
+    {16, 16, 600, 114, 600, 170},     {32, 16, 600, 171, 600, 260},     {16, 32, 600, 171, 600, 260},
+    {32, 32, 600, 228, 600, 340},     {64, 64, 1700, 230, 2000, 280},   {128, 128, 4500, 530, 4500, 700},
+    {256, 256, 8500, 1600, 0, 0},
+};
+
+// The kernel with the least estimated time: few rows are split over small tiles
+// that read straight from memory, many go through the tiles that read each row
+// fewest times.
+static int choose_tile(const I8Args& a, bool grouped, bool odd) {
+  const uint64_t groups = grouped ? (a.experts < a.rows ? a.experts : a.rows) : 0;
+  const uint64_t steps = (a.n_in + 127) / 128;
+  int best = 0;
+  uint64_t least = ~0ull;
+  for (int i = 0; i < (int)(sizeof(TILE_COST) / sizeof(TILE_COST[0])); i++) {
+    const TileCost& c = TILE_COST[i];
+    if (odd && !c.odd_step) continue;
+    // an expert's last row tile is half full, or it has only one
+    uint64_t tt = cdiv(a.rows, c.bt);
+    if (grouped && (tt += groups / 2) < groups) tt = groups;
+    const uint64_t rounds = (tt * cdiv(a.n_out, c.bn) + 255) / 256;
+    const uint64_t t = (odd ? c.odd_own : c.own) + rounds * steps * (odd ? c.odd_step : c.step);
+    if (t < least) least = t, best = i;
+  }
+  return best;
 }
 
 template <class T, bool GROUPED>
 static int launch_product(zk_context* ctx, const I8Args& a, hipStream_t st) {
   const char* name = GROUPED ? "i8_matmul_experts" : "i8_matmul";
-  // row tiles of the grouped form: one more than whole ones for each group
-  const uint32_t groups = GROUPED ? (a.experts + 1 < a.rows ? a.experts + 1 : a.rows) : 0;
-  auto go = [&](auto kernel, uint32_t bt, uint32_t bn, uint32_t threads) -> int {
-    const uint32_t tiles_t = GROUPED ? a.rows / bt + groups : cdiv(a.rows, bt), tiles_n = cdiv(a.n_out, bn);
+  if (a.n_in < 16) {
+    const size_t blocks = ((size_t)a.rows * a.n_out + 255) / 256;
+    ZK_LAUNCH(ctx, st, name, (k_i8_short<T, GROUPED>), dim3(blocks < 65536 ? (uint32_t)blocks : 65536), dim3(256), 0, a);
+    return ZK_OK;
+  }
+  const bool odd = ((uintptr_t)a.x | (uintptr_t)a.w | a.ld_x | a.ld_w | a.n_in) % 16 != 0;
+  const int c = choose_tile(a, GROUPED, odd);
+  auto go = [&](auto kernel, uint32_t threads) -> int {
+    // row tiles of the grouped form: whole ones, and a part of one for each
+    // expert and for the rows without an expert
+    const uint32_t bt = TILE_COST[c].bt, groups = a.experts + 1 < a.rows ? a.experts + 1 : a.rows;
+    const uint32_t tiles_t = GROUPED ? a.rows / bt + groups : cdiv(a.rows, bt);
+    const uint32_t tiles_n = cdiv(a.n_out, TILE_COST[c].bn);
     const size_t tiles = (size_t)tiles_t * tiles_n;
     if (tiles > I8_MAX_TILES) return ctx->fail(ZK_ERR_SIZE, "i8 experts: rows and n_out make too many tiles");
-    const dim3 grid(cdiv(tiles, 8) * 8);
-    ZK_LAUNCH(ctx, st, name, kernel, grid, dim3(threads), 0, a, tiles_t, tiles_n);
+    ZK_LAUNCH(ctx, st, name, kernel, dim3(cdiv(tiles, 8) * 8), dim3(threads), 0, a, tiles_t, tiles_n);
     return ZK_OK;
   };
-  const uint32_t per = GROUPED ? (a.rows + a.experts - 1) / a.experts : a.rows;  // rows of an average expert
-  if (per <= 64) {
-    if (per <= 16) return go(k_i8_direct<T, GROUPED, 1, 1, 8>, 16, 16, 512);
-    if (per <= 32) return go(k_i8_direct<T, GROUPED, 2, 1, 8>, 32, 16, 512);
-    return go(k_i8_direct<T, GROUPED, 4, 1, 8>, 64, 16, 512);
+  switch (c) {
+    case 0: return go(k_i8_direct<T, GROUPED, 1, 1, 8>, 512);
+    case 1: return go(k_i8_direct<T, GROUPED, 2, 1, 8>, 512);
+    case 2: return go(k_i8_direct<T, GROUPED, 1, 2, 8>, 512);
+    case 3: return go(k_i8_direct<T, GROUPED, 2, 2, 8>, 512);
+    case 4: return odd ? go(k_i8_odd<T, GROUPED, 2, 2, 1, 1>, 256) : go(k_i8_ring<T, GROUPED, 2, 2, 1, 1>, 256);
+    case 5: return odd ? go(k_i8_odd<T, GROUPED, 2, 2, 2, 2>, 256) : go(k_i8_ring<T, GROUPED, 2, 2, 2, 2>, 256);
+    default: return go(k_i8_ring<T, GROUPED, 2, 4, 4, 2>, 512);
   }
-  if (!GROUPED && a.n_out <= 64) {
-    if (a.n_in <= 256) {
-      if (a.n_out <= 16) return go(k_i8_direct<T, GROUPED, 4, 1, 1>, 64, 16, 64);
-      return go(k_i8_direct<T, GROUPED, 4, 2, 1>, 64, 32, 64);
-    }
-    if (a.n_out <= 16) return go(k_i8_direct<T, GROUPED, 1, 1, 8>, 16, 16, 512);
-    if (a.n_out <= 32) return go(k_i8_direct<T, GROUPED, 1, 2, 8>, 16, 32, 512);
-    return go(k_i8_direct<T, GROUPED, 1, 4, 8>, 16, 64, 512);
-  }
-  const TileCost even[3] = {{64, 2500, 230}, {128, 5000, 530}, {256, 9000, 1600}};
-  const TileCost odd[2] = {{64, 2500, 280}, {128, 5000, 700}};
-  const bool whole = ((uintptr_t)a.x | (uintptr_t)a.w | a.ld_x | a.ld_w | a.n_in) % 16 == 0;
-  uint32_t best = 64;
-  uint64_t least = ~0ull;
-  for (int i = 0; i < (whole ? 3 : 2); i++) {
-    const TileCost& c = whole ? even[i] : odd[i];
-    const uint64_t t = tile_cost(c, a.rows, groups / 2, a.n_out, a.n_in);
-    if (t < least) least = t, best = c.size;
-  }
-  if (!whole) {
-    if (best == 64) return go(k_i8_odd<T, GROUPED, 2, 2, 1, 1>, 64, 64, 256);
-    return go(k_i8_odd<T, GROUPED, 2, 2, 2, 2>, 128, 128, 256);
-  }
-  if (best == 64) return go(k_i8_ring<T, GROUPED, 2, 2, 1, 1>, 64, 64, 256);
-  if (best == 128) return go(k_i8_ring<T, GROUPED, 2, 2, 2, 2>, 128, 128, 256);
-  return go(k_i8_ring<T, GROUPED, 2, 4, 4, 2>, 256, 256, 512);
 }
 
 template <bool GROUPED>
@@ -677,64 +736,135 @@ static int i8_dispatch(zk_context* ctx, const I8Args& a, int type, hipStream_t s
 // multiplied by a power of two, so that neither 127 x nor the quotient leaves
 // the type.  A row of zeros gives s = 0 and zeros; a row with an infinity or a
 // NaN gives s = NaN and zeros, so that its products show it.
-template <class T>
-__global__ __launch_bounds__(256) void k_i8_quantize(const T* __restrict__ x, size_t ld_x, uint32_t cols,
-                                                     int8_t* __restrict__ q, size_t ld_q,
-                                                     float* __restrict__ scale) {
-  __shared__ float part[4];
-  const uint32_t tid = threadIdx.x;
-  const T* row = x + (size_t)blockIdx.x * ld_x;
-  int8_t* out = q + (size_t)blockIdx.x * ld_q;
-  // magnitudes as integers: their order is the floats', NaN above infinity
-  uint32_t m = 0;
-  for (uint32_t i = tid; i < cols; i += 256) {
-    const uint32_t u = __float_as_uint((float)row[i]) & 0x7fffffffu;
-    m = u > m ? u : m;
+struct RowScale {
+  float s;     // the row's scale
+  float c, a;  // q = rint(127 (x c) / a); a = 0: all zeros
+};
+
+// From the largest magnitude's bits (as integers magnitudes are in the floats'
+// order, NaN above infinity).
+__device__ __forceinline__ RowScale row_scale(uint32_t m) {
+  const float a = __uint_as_float(m);
+  RowScale r = {a / 127.0f, 1.0f, 0.0f};
+  if (m >= 0x7f800000u) {
+    r.s = __uint_as_float(0x7fc00000u);
+  } else if (m) {
+    r.c = a >= 0x1p64f ? 0x1p-32f : a < 0x1p-64f ? 0x1p64f : 1.0f;
+    r.a = a * r.c;
   }
-  for (int d = 32; d; d >>= 1) {
-    const uint32_t o = __shfl_xor((int)m, d);
-    m = o > m ? o : m;
-  }
-  if ((tid & 63) == 0) part[tid >> 6] = __uint_as_float(m);
-  __syncthreads();
-  for (int i = 0; i < 4; i++) {
-    const uint32_t o = __float_as_uint(part[i]);
-    m = o > m ? o : m;
-  }
-  const bool finite = m < 0x7f800000u;
-  float a = __uint_as_float(m);
-  if (tid == 0) scale[blockIdx.x] = finite ? a / 127.0f : __uint_as_float(0x7fc00000u);
-  const float c = a >= 0x1p64f ? 0x1p-32f : a < 0x1p-64f ? 0x1p64f : 1.0f;
-  a *= c;
-  for (uint32_t i = tid; i < cols; i += 256) {
-    const float f = (float)row[i] * c;
-    out[i] = finite && m ? (int8_t)rintf(f * 127.0f / a) : (int8_t)0;
-  }
+  return r;
 }
 
 template <class T>
-static int launch_quantize(zk_context* ctx, const void* x, size_t ld_x, size_t rows, size_t cols, int8_t* q,
-                           size_t ld_q, float* scale, hipStream_t st) {
-  ZK_LAUNCH(ctx, st, "i8_quantize", k_i8_quantize<T>, dim3((uint32_t)rows), dim3(256), 0, (const T*)x, ld_x,
-            (uint32_t)cols, q, ld_q, scale);
-  return ZK_OK;
+__device__ __forceinline__ uint32_t magnitude(T x) {
+  return __float_as_uint((float)x) & 0x7fffffffu;
+}
+
+template <class T>
+__device__ __forceinline__ void quantize_piece(const Vec<T>& x, const RowScale& r, int8_t* q) {
+#pragma unroll
+  for (uint32_t i = 0; i < Vec<T>::N; i++)
+    q[i] = r.a != 0.0f ? (int8_t)rintf((float)x.v[i] * r.c * 127.0f / r.a) : (int8_t)0;
+}
+
+// THREADS threads a row, ROWS rows a block.  A thread keeps its first HELD
+// pieces of 16 bytes from the pass for the maximum to the pass that divides.
+template <class T, int THREADS, int ROWS>
+__global__ __launch_bounds__(THREADS* ROWS) void k_i8_quantize(const T* __restrict__ x, size_t ld_x, uint32_t rows,
+                                                               uint32_t cols, int8_t* __restrict__ q, size_t ld_q,
+                                                               float* __restrict__ scale) {
+  constexpr int HELD = 4;
+  constexpr int WAVES = THREADS / 64;
+  __shared__ uint32_t part[ROWS * WAVES];
+  const uint32_t tid = threadIdx.x % THREADS, sub = threadIdx.x / THREADS;
+  const uint32_t r = blockIdx.x * ROWS + sub;
+  const bool on = r < rows;
+  const T* row = x + (size_t)(on ? r : rows - 1) * ld_x;
+  int8_t* out = q + (size_t)(on ? r : rows - 1) * ld_q;
+  const uint32_t pieces = pieces_of<T>(cols);
+  Vec<T> held[HELD];
+  uint32_t m = 0;
+  auto look = [&](const Vec<T>& v) {
+#pragma unroll
+    for (uint32_t i = 0; i < Vec<T>::N; i++) {
+      const uint32_t u = magnitude(v.v[i]);
+      m = u > m ? u : m;
+    }
+  };
+#pragma unroll
+  for (int h = 0; h < HELD; h++) {
+    const uint32_t c = tid + h * THREADS;
+    held[h] = Vec<T>{};
+    if (c < pieces) held[h] = row_load(row + piece<T>(c, cols), cols - piece<T>(c, cols));
+  }
+#pragma unroll
+  for (int h = 0; h < HELD; h++) look(held[h]);
+  for (uint32_t c = tid + HELD * THREADS; c < pieces; c += THREADS)
+    look(row_load(row + piece<T>(c, cols), cols - piece<T>(c, cols)));
+#pragma unroll
+  for (int d = 32; d; d >>= 1) {
+    const uint32_t o = (uint32_t)__shfl_xor((int)m, d);
+    m = o > m ? o : m;
+  }
+  if (WAVES > 1) {
+    if ((tid & 63) == 0) part[sub * WAVES + (tid >> 6)] = m;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < WAVES; i++) {
+      const uint32_t o = part[sub * WAVES + i];
+      m = o > m ? o : m;
+    }
+  }
+  if (!on) return;
+  const RowScale rs = row_scale(m);
+  if (tid == 0) scale[r] = rs.s;
+  auto put = [&](uint32_t c, const Vec<T>& v) {
+    const uint32_t at = piece<T>(c, cols);
+    int8_t b[Vec<T>::N];
+    quantize_piece(v, rs, b);
+    if (cols - at >= Vec<T>::N) {
+      __builtin_memcpy(out + at, b, sizeof(b));
+    } else {
+      for (uint32_t i = 0; i < Vec<T>::N; i++)
+        if (i < cols - at) out[at + i] = b[i];
+    }
+  };
+#pragma unroll
+  for (int h = 0; h < HELD; h++) {
+    const uint32_t c = tid + h * THREADS;
+    if (c < pieces) put(c, held[h]);
+  }
+  for (uint32_t c = tid + HELD * THREADS; c < pieces; c += THREADS)
+    put(c, row_load(row + piece<T>(c, cols), cols - piece<T>(c, cols)));
 }
 
 static int i8_quantize(zk_context* ctx, const void* x, int type, size_t ld_x, size_t rows, size_t cols, int8_t* q,
                        size_t ld_q, float* scale, hipStream_t st) {
-  if (rows == 0) return ZK_OK;
-  switch (type) {
-    case ZK_F32: return launch_quantize<float>(ctx, x, ld_x, rows, cols, q, ld_q, scale, st);
-    case ZK_F16: return launch_quantize<_Float16>(ctx, x, ld_x, rows, cols, q, ld_q, scale, st);
-    default: return launch_quantize<__bf16>(ctx, x, ld_x, rows, cols, q, ld_q, scale, st);
-  }
+  return by_type(type, [&](auto zero) -> int {
+    typedef decltype(zero) T;
+    const uint32_t pieces = pieces_of<T>((uint32_t)cols);
+    // runs of rows: a launch stays below 2^32 threads
+    for (size_t r = 0; r < rows; r += (size_t)1 << 21) {
+      const uint32_t n = (uint32_t)(rows - r < (size_t)1 << 21 ? rows - r : (size_t)1 << 21);
+      const T* from = (const T*)x + r * ld_x;
+      int8_t* to = q + r * ld_q;
+      // one piece a thread where rows are few (their latency counts), else two
+      // to four of them a thread
+      if (pieces <= 64 || (rows >= 2048 && pieces <= 256))
+        ZK_LAUNCH(ctx, st, "i8_quantize", (k_i8_quantize<T, 64, 4>), dim3(cdiv(n, 4)), dim3(256), 0, from, ld_x, n,
+                  (uint32_t)cols, to, ld_q, scale + r);
+      else if (pieces <= 256 || (rows >= 512 && pieces <= 1024))
+        ZK_LAUNCH(ctx, st, "i8_quantize", (k_i8_quantize<T, 256, 1>), dim3(n), dim3(256), 0, from, ld_x, n,
+                  (uint32_t)cols, to, ld_q, scale + r);
+      else
+        ZK_LAUNCH(ctx, st, "i8_quantize", (k_i8_quantize<T, 1024, 1>), dim3(n), dim3(1024), 0, from, ld_x, n,
+                  (uint32_t)cols, to, ld_q, scale + r);
+    }
+    return ZK_OK;
+  });
 }
 
 // ------------------------------------------------------------ arguments
-static size_t type_bytes(int type) { return type == ZK_F32 || type == ZK_I32 ? 4 : 2; }
-static bool float_type(int type) { return type == ZK_F32 || type == ZK_F16 || type == ZK_BF16; }
-static bool aligned(const void* p, size_t n) { return (uintptr_t)p % n == 0; }
-
 // Checks that the two forms of the product share.
 static int check_product(zk_context* ctx, const I8Args& a, size_t rows, size_t n_out, size_t n_in, int type) {
   if (type != ZK_I32 && !float_type(type)) return ctx->fail(ZK_ERR_INVALID, "i8 product: unknown type of y");
