@@ -97,7 +97,7 @@ __device__ __forceinline__ bool tile_of_block(uint32_t b, uint32_t tiles_t, uint
   constexpr uint32_t G = 8;
   const uint32_t total = tiles_t * tiles_n, per = (total + 7) / 8;
   const uint32_t t = (b & 7) * per + (b >> 3);
-  if (t >= total) return false;
+  if ((b >> 3) >= per || t >= total) return false;
   const uint32_t group = t / (G * tiles_n), at = t % (G * tiles_n);
   const uint32_t size = tiles_t - group * G < G ? tiles_t - group * G : G;
   tt = group * G + at % size;
@@ -105,39 +105,61 @@ __device__ __forceinline__ bool tile_of_block(uint32_t b, uint32_t tiles_t, uint
   return true;
 }
 
-// Rows [r0, r1) and expert of row tile tt of the grouped form: tiles are
-// counted expert by expert, those of the rows without an expert (e = experts)
-// last.  The whole wave takes part; the answer is the same in every lane.
-__device__ __forceinline__ void expert_tile(const I8Args& a, uint32_t tt, uint32_t bt, uint32_t& r0, uint32_t& r1,
-                                            uint32_t& e) {
+// A block's tile: rows [r0, r1) from channel n0 on, and their expert.  Grouped,
+// the row tiles are counted expert by expert, those of the rows without an
+// expert (e = experts) last; the grid is made for the most there can be, and the
+// tiles there are are spread over its first blocks, so that no XCD is left with
+// the empty ones.  The whole wave takes part; the answer is the same in every
+// lane.  False: nothing to do.
+template <bool GROUPED>
+__device__ __forceinline__ bool block_tile(const I8Args& a, uint32_t bt, uint32_t bn, uint32_t tiles_t,
+                                           uint32_t tiles_n, uint32_t& r0, uint32_t& r1, uint32_t& n0, uint32_t& e) {
+  uint32_t tt, tn;
+  if (!GROUPED) {
+    if (!tile_of_block(blockIdx.x, tiles_t, tiles_n, tt, tn)) return false;
+    r0 = tt * bt, r1 = a.rows, n0 = tn * bn, e = 0;
+    return true;
+  }
   const uint32_t lane = threadIdx.x & 63;
-  uint32_t run = 0;
-  for (uint32_t e0 = 0; e0 < a.experts; e0 += 64) {
+  // 64 experts at a time, one a lane: rows [lo, hi), n tiles, s of them up to here
+  uint32_t lo, hi, n, s;
+  auto look = [&](uint32_t e0) {
     const uint32_t me = e0 + lane;
-    uint32_t lo = 0, hi = 0;
+    lo = hi = 0;
     if (me < a.experts) lo = offset_of(a, me), hi = offset_of(a, me + 1);
-    const uint32_t n = hi > lo ? (hi - lo + bt - 1) / bt : 0;
-    uint32_t s = n;
+    n = hi > lo ? (hi - lo + bt - 1) / bt : 0;
+    s = n;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
       const uint32_t o = __shfl_up(s, d);
       if (lane >= (uint32_t)d) s += o;
     }
+  };
+  uint32_t all = 0;
+  for (uint32_t e0 = 64; e0 < a.experts; e0 += 64) look(e0), all += __shfl(s, 63);
+  look(0);
+  all += __shfl(s, 63);
+  const uint32_t end = offset_of(a, a.experts), rest = (a.rows - end + bt - 1) / bt;
+  if (!tile_of_block(blockIdx.x, __builtin_amdgcn_readfirstlane(all + rest), tiles_n, tt, tn)) return false;
+  n0 = tn * bn;
+  uint32_t run = 0;
+  for (uint32_t e0 = 0; e0 < a.experts; e0 += 64) {
+    if (e0) look(e0);
     const uint64_t past = __ballot(run + s > tt);
     if (past) {
       const int l = __ffsll((unsigned long long)past) - 1;
       const uint32_t first = run + __shfl(s, l) - __shfl(n, l);
-      e = e0 + l;
-      r0 = __shfl(lo, l) + (tt - first) * bt;
-      r1 = __shfl(hi, l);
-      return;
+      e = __builtin_amdgcn_readfirstlane(e0 + l);
+      r0 = __builtin_amdgcn_readfirstlane(__shfl(lo, l) + (tt - first) * bt);
+      r1 = __builtin_amdgcn_readfirstlane(__shfl(hi, l));
+      return r0 < r1;
     }
     run += __shfl(s, 63);
   }
   e = a.experts;
-  const uint64_t r = (uint64_t)offset_of(a, a.experts) + (uint64_t)(tt - run) * bt;
+  r0 = __builtin_amdgcn_readfirstlane(end + (tt - run) * bt);
   r1 = a.rows;
-  r0 = r < r1 ? (uint32_t)r : r1;
+  return r0 < r1;
 }
 
 // What rows are padded with: a lane that has no bytes to load takes these.
@@ -265,25 +287,15 @@ __global__ __launch_bounds__(64 * WT * WN) void k_i8_ring(I8Args a, uint32_t til
   __shared__ __align__(16) int8_t lds[5 * SLOT];
   auto swz = [](uint32_t row) { return (row >> 1) & 7u; };
   const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  uint32_t tt, tn;
-  if (!tile_of_block(blockIdx.x, tiles_t, tiles_n, tt, tn)) return;
-  const uint32_t n0 = tn * BN;
-  uint32_t r0 = tt * BT, r1 = a.rows, e = 0;
-  if (GROUPED) expert_tile(a, tt, BT, r0, r1, e);
-  if (r0 >= r1) return;
+  uint32_t r0, r1, n0, e;
+  if (!block_tile<GROUPED>(a, BT, BN, tiles_t, tiles_n, r0, r1, n0, e)) return;
   const bool none = GROUPED && e >= a.experts;
   const int8_t* w = a.w + (none ? 0 : (size_t)e * a.n_out * a.ld_w);
-  Factors<GROUPED, BT, BN, 64 * WAVES> factors;
-  factors.load(a, r0, r1, n0, e);
   const int8_t *xp[PER], *wp[PER];
   auto chunk = [&](uint32_t piece) { return ((lane & 7) ^ swz(piece * 8 + (lane >> 3))) * 16; };
 #pragma unroll
   for (uint32_t i = 0; i < PER; i++) {
     const uint32_t row = (wave * PER + i) * 8 + (lane >> 3);
-    const uint32_t r = r0 + row < r1 ? r0 + row : r1 - 1;
-    int64_t s = GROUPED ? source_row(a, r) : (int64_t)r;
-    if (s < 0) s = 0;
-    xp[i] = a.x + (size_t)s * a.ld_x + chunk(wave * PER + i);
     const uint32_t n = n0 + row < a.n_out ? n0 + row : a.n_out - 1;
     wp[i] = w + (size_t)n * a.ld_w + chunk(wave * PER + i);
   }
@@ -310,18 +322,30 @@ __global__ __launch_bounds__(64 * WT * WN) void k_i8_ring(I8Args a, uint32_t til
     if (r < FN) wf[set][r] = *(const v4i*)(fw + ws * SLOT + r * 32 * BK + ch[s]);
     else xf[set][r - FN] = *(const v4i*)(fx + xs * SLOT + (r - FN) * 32 * BK + ch[s]);
   };
+  // w's first tiles wait for no index of the rows; the factors' chain of loads
+  // runs beside the tiles'
+#pragma unroll
+  for (uint32_t i = 0; i < PER; i++) fill(wp[i], i, 0, 1);
+#pragma unroll
+  for (uint32_t i = 0; i < PER; i++) fill(wp[i], i, 1, 3);
+#pragma unroll
+  for (uint32_t i = 0; i < PER; i++) {
+    const uint32_t row = (wave * PER + i) * 8 + (lane >> 3);
+    const uint32_t r = r0 + row < r1 ? r0 + row : r1 - 1;
+    int64_t s = GROUPED ? source_row(a, r) : (int64_t)r;
+    if (s < 0) s = 0;
+    xp[i] = a.x + (size_t)s * a.ld_x + chunk(wave * PER + i);
+  }
+#pragma unroll
+  for (uint32_t i = 0; i < PER; i++) fill(xp[i], i, 0, 0);
+#pragma unroll
+  for (uint32_t i = 0; i < PER; i++) fill(xp[i], i, 1, 2);
+#pragma unroll
+  for (uint32_t i = 0; i < PER; i++) fill(xp[i], i, 2, 4);
+  Factors<GROUPED, BT, BN, 64 * WAVES> factors;
+  factors.load(a, r0, r1, n0, e);
   if (steps) {
-#pragma unroll
-    for (uint32_t i = 0; i < PER; i++) fill(xp[i], i, 0, 0);
-#pragma unroll
-    for (uint32_t i = 0; i < PER; i++) fill(wp[i], i, 0, 1);
-#pragma unroll
-    for (uint32_t i = 0; i < PER; i++) fill(xp[i], i, 1, 2);
-#pragma unroll
-    for (uint32_t i = 0; i < PER; i++) fill(wp[i], i, 1, 3);
-#pragma unroll
-    for (uint32_t i = 0; i < PER; i++) fill(xp[i], i, 2, 4);
-    if (steps > 2) wait_loads<3 * PER>();
+    if (steps > 2) wait_loads<2 * PER>();
     else wait_loads<0>();
     meet();
     uint32_t xs = 0;  // slot of this step's x
@@ -399,12 +423,8 @@ __global__ __launch_bounds__(64 * WT * WN) void k_i8_odd(I8Args a, uint32_t tile
   __shared__ __align__(16) int8_t lds[2 * STAGE];
   auto swz = [](uint32_t row) { return (row >> 1) & 7u; };
   const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  uint32_t tt, tn;
-  if (!tile_of_block(blockIdx.x, tiles_t, tiles_n, tt, tn)) return;
-  const uint32_t n0 = tn * BN;
-  uint32_t r0 = tt * BT, r1 = a.rows, e = 0;
-  if (GROUPED) expert_tile(a, tt, BT, r0, r1, e);
-  if (r0 >= r1) return;
+  uint32_t r0, r1, n0, e;
+  if (!block_tile<GROUPED>(a, BT, BN, tiles_t, tiles_n, r0, r1, n0, e)) return;
   const bool none = GROUPED && e >= a.experts;
   const int8_t* w = a.w + (none ? 0 : (size_t)e * a.n_out * a.ld_w);
   Factors<GROUPED, BT, BN, 64 * WAVES> factors;
@@ -515,12 +535,8 @@ __global__ __launch_bounds__(64 * KW) void k_i8_direct(I8Args a, uint32_t tiles_
   constexpr int U = FT + FN <= 2 ? 4 : 2;  // steps whose loads are under way together
   __shared__ __align__(16) v4i sums[KW][FN * FT][64];
   const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  uint32_t tt, tn;
-  if (!tile_of_block(blockIdx.x, tiles_t, tiles_n, tt, tn)) return;
-  const uint32_t n0 = tn * BN;
-  uint32_t r0 = tt * BT, r1 = a.rows, e = 0;
-  if (GROUPED) expert_tile(a, tt, BT, r0, r1, e);
-  if (r0 >= r1) return;
+  uint32_t r0, r1, n0, e;
+  if (!block_tile<GROUPED>(a, BT, BN, tiles_t, tiles_n, r0, r1, n0, e)) return;
   const bool none = GROUPED && e >= a.experts;
   const int8_t* w = a.w + (none ? 0 : (size_t)e * a.n_out * a.ld_w);
   const uint32_t fr = lane & 15, c = lane >> 4;
@@ -655,8 +671,9 @@ __global__ __launch_bounds__(256) void k_i8_short(I8Args a) {
 
 // ------------------------------------------------------------ which kernel
 // A tile's time in ns: its own part (first loads, results) and its steps of 128
-// bytes of k, of which a CU has ceil(tiles / 256) tiles to do.  Measured on rows
-// that are multiples of 16 bytes (`odd`: on others).
+// bytes of k, times the tiles that a CU has to do: tiles / 256, rounded up where
+// a tile fills a CU for long (from 64 x 64 on).  Measured on rows that are
+// multiples of 16 bytes (`odd`: on others).
 struct TileCost {
   uint32_t bt, bn, own, step, odd_own, odd_step;
 };
@@ -680,8 +697,9 @@ static int choose_tile(const I8Args& a, bool grouped, bool odd) {
     // an expert's last row tile is half full, or it has only one
     uint64_t tt = cdiv(a.rows, c.bt);
     if (grouped && (tt += groups / 2) < groups) tt = groups;
-    const uint64_t rounds = (tt * cdiv(a.n_out, c.bn) + 255) / 256;
-    const uint64_t t = (odd ? c.odd_own : c.own) + rounds * steps * (odd ? c.odd_step : c.step);
+    uint64_t tiles = tt * cdiv(a.n_out, c.bn);
+    if (tiles < 256 || c.bt >= 64) tiles = (tiles + 255) / 256 * 256;
+    const uint64_t t = (odd ? c.odd_own : c.own) + tiles * steps * (odd ? c.odd_step : c.step) / 256;
     if (t < least) least = t, best = i;
   }
   return best;
@@ -714,7 +732,13 @@ static int launch_product(zk_context* ctx, const I8Args& a, hipStream_t st) {
     case 2: return go(k_i8_direct<T, GROUPED, 1, 2, 8>, 512);
     case 3: return go(k_i8_direct<T, GROUPED, 2, 2, 8>, 512);
     case 4: return odd ? go(k_i8_odd<T, GROUPED, 2, 2, 1, 1>, 256) : go(k_i8_ring<T, GROUPED, 2, 2, 1, 1>, 256);
-    case 5: return odd ? go(k_i8_odd<T, GROUPED, 2, 2, 2, 2>, 256) : go(k_i8_ring<T, GROUPED, 2, 2, 2, 2>, 256);
+    case 5:
+      if (odd) return go(k_i8_odd<T, GROUPED, 2, 2, 2, 2>, 256);
+      // grouped, eight waves share the chain of indexes before the first step
+      // (4096 x 4 rows of 2048, 64 experts: 66 us, 83 with four waves); else four
+      // read LDS less (4096 x 4096 x 4096: 73 us, 77 with eight)
+      if constexpr (GROUPED) return go(k_i8_ring<T, GROUPED, 2, 4, 2, 1>, 512);
+      else return go(k_i8_ring<T, GROUPED, 2, 2, 2, 2>, 256);
     default: return go(k_i8_ring<T, GROUPED, 2, 4, 4, 2>, 512);
   }
 }
