@@ -59,7 +59,7 @@ __global__ __launch_bounds__(SORT_THREADS) void k_sort_place(const int32_t* __re
                                                              int32_t* __restrict__ order,
                                                              int32_t* __restrict__ place) {
   __shared__ uint32_t cnt[SORT_WAVES * ZK_MAX_EXPERTS];
-  __shared__ uint32_t base[ZK_MAX_EXPERTS];
+  __shared__ uint32_t base[ZK_MAX_EXPERTS], sum[ZK_MAX_EXPERTS];
   __shared__ uint32_t scan[SORT_WAVES];
   const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const uint32_t seg0 = blockIdx.x * segment, run = segment / SORT_WAVES;
@@ -69,14 +69,15 @@ __global__ __launch_bounds__(SORT_THREADS) void k_sort_place(const int32_t* __re
   uint32_t* mine = cnt + wave * experts;
   volatile uint32_t* next = mine;  // read and written by different lanes of the wave
   for (uint32_t e = tid; e < SORT_WAVES * experts; e += SORT_THREADS) cnt[e] = 0;
+  if (tid < experts) base[tid] = sum[tid] = 0;
   __syncthreads();
   for (uint32_t i = lo + lane; i < hi; i += 64) {
     const uint32_t e = (uint32_t)expert[i];
     if (e < experts) atomicAdd(&mine[e], 1u);
   }
   __syncthreads();
-  // thread e: the pairs of expert e in the blocks before, in all blocks, and
-  // in each wave of this block before the next
+  // thread e: the pairs of expert e in each wave of this block before the next,
+  // and, over the blocks, in all of them and in those before this one
   uint32_t all = 0, before = 0, here = 0;
   if (tid < experts) {
     for (uint32_t w = 0; w < SORT_WAVES; w++) {
@@ -84,15 +85,20 @@ __global__ __launch_bounds__(SORT_THREADS) void k_sort_place(const int32_t* __re
       cnt[w * experts + tid] = here;
       here += c;
     }
-    if (tot) {
-      for (uint32_t b = 0; b < gridDim.x; b++) {
-        const uint32_t c = tot[(size_t)b * experts + tid];
-        all += c;
-        if (b < blockIdx.x) before += c;
-      }
-    } else {
-      all = here;
+    all = here;
+  }
+  if (tot) {
+    // the blocks' counts are shared out over all threads, so that a thread has
+    // few loads to wait for; the sums are integers, their order does not matter
+    const uint32_t mark = blockIdx.x * experts, last = gridDim.x * experts;
+#pragma unroll 4
+    for (uint32_t i = tid; i < last; i += SORT_THREADS) {
+      const uint32_t c = tot[i], e = i % experts;
+      atomicAdd(&sum[e], c);
+      if (i < mark) atomicAdd(&base[e], c);
     }
+    __syncthreads();
+    if (tid < experts) all = sum[tid], before = base[tid];
   }
   // exclusive scan of `all` over the experts
   uint32_t s = all;
@@ -144,93 +150,144 @@ __global__ __launch_bounds__(SORT_THREADS) void k_sort_place(const int32_t* __re
 }
 
 // ------------------------------------------------------------ rows
-// out[p] = x[order[p] / slots], zeros where order[p] names no token.
-template <class T>
+// out[p] = x[order[p] / slots], zeros where order[p] names no token: 2^log_w
+// threads a row, so that short rows fill a wave.  STREAM: see streams().
+template <class T, bool STREAM>
 __global__ __launch_bounds__(256) void k_gather(const T* __restrict__ x, size_t ld_x,
                                                 const int32_t* __restrict__ order, uint32_t rows, uint32_t tokens,
-                                                uint32_t slots, uint32_t cols, T* __restrict__ out, size_t ld_out) {
-  const uint32_t p = blockIdx.x;
+                                                uint32_t slots, uint32_t cols, uint32_t log_w, T* __restrict__ out,
+                                                size_t ld_out) {
+  const uint32_t p = blockIdx.x * (256u >> log_w) + (threadIdx.x >> log_w);
   if (p >= rows) return;
   const int o = order[p];
   const uint32_t t = o < 0 ? tokens : (uint32_t)o / slots;
   const uint32_t pieces = pieces_of<T>(cols);
-  for (uint32_t c = threadIdx.x; c < pieces; c += 256) {
+  for (uint32_t c = threadIdx.x & ((1u << log_w) - 1); c < pieces; c += 1u << log_w) {
     const uint32_t at = piece<T>(c, cols);
     Vec<T> v = {};
     if (t < tokens) v = row_load(x + (size_t)t * ld_x + at, cols - at);
-    row_store(out + (size_t)p * ld_out + at, cols - at, v);
+    row_store<T, STREAM>(out + (size_t)p * ld_out + at, cols - at, v);
   }
 }
 
-// out[t] = sum_j w[t, j] y[place[t, j]], j ascending, in 32 bits.
-template <class T>
+// out[t] = sum_j w[t, j] y[place[t, j]], j ascending, in 32 bits; 2^log_w threads
+// a token.  Four slots' indexes, then their rows, are loaded together: a token's
+// slots are one chain of two loads per four, not per slot.
+template <class T, bool STREAM>
 __global__ __launch_bounds__(256) void k_combine(const T* __restrict__ y, size_t ld_y,
                                                  const int32_t* __restrict__ place, const float* __restrict__ weight,
-                                                 uint32_t rows, uint32_t slots, uint32_t cols, T* __restrict__ out,
-                                                 size_t ld_out) {
-  const uint32_t t = blockIdx.x;
+                                                 uint32_t rows, uint32_t tokens, uint32_t slots, uint32_t cols,
+                                                 uint32_t log_w, T* __restrict__ out, size_t ld_out) {
+  constexpr int K = 4;
+  const uint32_t t = blockIdx.x * (256u >> log_w) + (threadIdx.x >> log_w);
+  if (t >= tokens) return;
   const uint32_t pieces = pieces_of<T>(cols);
-  for (uint32_t c = threadIdx.x; c < pieces; c += 256) {
-    const uint32_t at = piece<T>(c, cols);
-    float s[Vec<T>::N] = {};
-    for (uint32_t j = 0; j < slots; j++) {
-      const uint32_t p = (uint32_t)place[(size_t)t * slots + j];
-      if (p >= rows) continue;
-      const float w = weight ? weight[(size_t)t * slots + j] : 1.0f;
-      const Vec<T> v = row_load(y + (size_t)p * ld_y + at, cols - at);
-      for (uint32_t i = 0; i < Vec<T>::N; i++) s[i] += w * (float)v.v[i];
+  for (uint32_t c = threadIdx.x & ((1u << log_w) - 1); c < pieces; c += 1u << log_w) {
+  const uint32_t at = piece<T>(c, cols);
+  float s[Vec<T>::N] = {};
+  for (uint32_t j0 = 0; j0 < slots; j0 += K) {
+    uint32_t p[K];
+    float w[K];
+    Vec<T> v[K];
+#pragma unroll
+    for (int k = 0; k < K; k++) {
+      const size_t pair = (size_t)t * slots + j0 + k;
+      const bool on = j0 + k < slots;
+      p[k] = on ? (uint32_t)place[pair] : rows;
+      w[k] = on && weight ? weight[pair] : 1.0f;
     }
-    Vec<T> r;
-    for (uint32_t i = 0; i < Vec<T>::N; i++) r.v[i] = (T)s[i];
-    row_store(out + (size_t)t * ld_out + at, cols - at, r);
+#pragma unroll
+    for (int k = 0; k < K; k++)
+      if (p[k] < rows) v[k] = row_load<T, STREAM>(y + (size_t)p[k] * ld_y + at, cols - at);
+#pragma unroll
+    for (int k = 0; k < K; k++)
+      if (p[k] < rows) {
+#pragma unroll
+        for (uint32_t e = 0; e < Vec<T>::N; e++) s[e] += w[k] * (float)v[k].v[e];
+      }
+  }
+  Vec<T> r;
+#pragma unroll
+  for (uint32_t e = 0; e < Vec<T>::N; e++) r.v[e] = (T)s[e];
+  row_store<T, STREAM>(out + (size_t)t * ld_out + at, cols - at, r);
   }
 }
 
 // dy[place[t, j]] = w[t, j] g[t], dw[t, j] = <g[t], y[place[t, j]]>; rows of dy
-// that hold no pair get zeros.
-template <class T>
+// that hold no pair get zeros.  A block has a token, so that g's row is read
+// once and each dot product ends in one block; four slots go together.
+template <class T, bool STREAM>
 __global__ __launch_bounds__(256) void k_combine_grad(const T* __restrict__ g, size_t ld_g, const T* __restrict__ y,
                                                       size_t ld_y, const int32_t* __restrict__ order,
                                                       const int32_t* __restrict__ place,
                                                       const float* __restrict__ weight, uint32_t rows,
                                                       uint32_t slots, uint32_t cols, T* __restrict__ dy, size_t ld_dy,
                                                       float* __restrict__ dw) {
-  __shared__ float part[4];
+  constexpr int K = 4;
+  __shared__ float part[K][4];
   const uint32_t t = blockIdx.x, tid = threadIdx.x;
   const uint32_t pieces = pieces_of<T>(cols);
-  for (uint32_t j = 0; j < slots; j++) {
-    const size_t i = (size_t)t * slots + j;
-    if (i < rows && order[i] < 0) {
-      for (uint32_t c = tid; c < pieces; c += 256) {
-        const uint32_t at = piece<T>(c, cols);
-        row_store(dy + i * ld_dy + at, cols - at, Vec<T>{});
-      }
+  for (uint32_t j0 = 0; j0 < slots; j0 += K) {
+    const size_t pair = (size_t)t * slots + j0;
+    uint32_t p[K];
+    float w[K], s[K] = {};
+    bool empty[K];  // does position `pair + k` hold no pair?
+#pragma unroll
+    for (int k = 0; k < K; k++) {
+      const bool on = j0 + k < slots;
+      p[k] = on ? (uint32_t)place[pair + k] : rows;
+      w[k] = on && weight ? weight[pair + k] : 1.0f;
+      empty[k] = on && pair + k < rows && order[pair + k] < 0;
     }
-    const uint32_t p = (uint32_t)place[i];
-    float s = 0.0f;
-    if (p < rows) {
-      const float w = weight ? weight[i] : 1.0f;
-      for (uint32_t c = tid; c < pieces; c += 256) {
-        const uint32_t at = piece<T>(c, cols);
-        const uint32_t fresh = c * Vec<T>::N - at;  // elements that the piece before has too
-        const Vec<T> gv = row_load(g + (size_t)t * ld_g + at, cols - at);
-        Vec<T> yv = {};
-        if (dw) yv = row_load(y + (size_t)p * ld_y + at, cols - at);
+    for (uint32_t c = tid; c < pieces; c += 256) {
+      const uint32_t at = piece<T>(c, cols), left = cols - at;
+      const uint32_t fresh = c * Vec<T>::N - at;  // elements that the piece before has too
+      const Vec<T> gv = row_load(g + (size_t)t * ld_g + at, left);
+      Vec<T> yv[K];
+#pragma unroll
+      for (int k = 0; k < K; k++) {
+        yv[k] = Vec<T>{};
+        if (dw && p[k] < rows) yv[k] = row_load<T, STREAM>(y + (size_t)p[k] * ld_y + at, left);
+      }
+#pragma unroll
+      for (int k = 0; k < K; k++) {
+        if (empty[k]) row_store<T, STREAM>(dy + (pair + k) * ld_dy + at, left, Vec<T>{});
+        if (p[k] >= rows) continue;
         Vec<T> r;
+#pragma unroll
         for (uint32_t e = 0; e < Vec<T>::N; e++) {
-          r.v[e] = (T)(w * (float)gv.v[e]);
-          if (e >= fresh) s += (float)gv.v[e] * (float)yv.v[e];
+          r.v[e] = (T)(w[k] * (float)gv.v[e]);
+          if (e >= fresh) s[k] += (float)gv.v[e] * (float)yv[k].v[e];
         }
-        row_store(dy + (size_t)p * ld_dy + at, cols - at, r);
+        row_store<T, STREAM>(dy + (size_t)p[k] * ld_dy + at, left, r);
       }
     }
     if (!dw) continue;
-    for (int d = 32; d; d >>= 1) s += __shfl_xor(s, d);
+#pragma unroll
+    for (int d = 32; d; d >>= 1)
+#pragma unroll
+      for (int k = 0; k < K; k++) s[k] += __shfl_xor(s[k], d);
+    if (j0) __syncthreads();  // the last four's sums are read
+    if ((tid & 63) == 0)
+#pragma unroll
+      for (int k = 0; k < K; k++) part[k][tid >> 6] = s[k];
     __syncthreads();
-    if ((tid & 63) == 0) part[tid >> 6] = s;
-    __syncthreads();
-    if (tid == 0) dw[i] = part[0] + part[1] + part[2] + part[3];
+    if (tid < K && j0 + tid < slots) dw[pair + tid] = part[tid][0] + part[tid][1] + part[tid][2] + part[tid][3];
   }
+}
+
+// Whether a call's rows pass the caches (32 MB of L2): what is read or written
+// once then goes around them and leaves them to the rows that are read again
+// (gather of 65536 rows of 4 KB 69 us, 84 through the caches); smaller rows stay
+// for whoever reads them next.
+static bool streams(size_t rows, size_t cols, size_t size) { return rows * cols * size > (size_t)32 << 20; }
+
+// log2 of the threads that a row gets: its pieces, from 8 to 256.
+template <class T>
+static uint32_t log_threads(size_t cols) {
+  uint32_t l = 3;
+  while (l < 8 && (1u << l) < pieces_of<T>((uint32_t)cols)) l++;
+  return l;
 }
 
 // ------------------------------------------------------------ arguments
@@ -312,9 +369,14 @@ int zk_experts_gather(zk_context* ctx, const void* d_x, int type, size_t ld_x, s
     hipStream_t st = ctx->s(stream);
     return by_type(type, [&](auto zero) -> int {
       typedef decltype(zero) T;
-      ZK_LAUNCH(ctx, st, "experts_gather", k_gather<T>, dim3((uint32_t)rows), dim3(256), 0, (const T*)d_x, ld_x,
-                d_order, (uint32_t)rows, (uint32_t)tokens, (uint32_t)slots, (uint32_t)cols, (T*)d_out, ld_out);
-      return ZK_OK;
+      const uint32_t log_w = log_threads<T>(cols);
+      const dim3 grid(cdiv(rows, 256u >> log_w));
+      auto go = [&](auto kernel) -> int {
+        ZK_LAUNCH(ctx, st, "experts_gather", kernel, grid, dim3(256), 0, (const T*)d_x, ld_x, d_order, (uint32_t)rows,
+                  (uint32_t)tokens, (uint32_t)slots, (uint32_t)cols, log_w, (T*)d_out, ld_out);
+        return ZK_OK;
+      };
+      return streams(rows, cols, sizeof(T)) ? go(k_gather<T, true>) : go(k_gather<T, false>);
     });
   });
 }
@@ -334,9 +396,14 @@ int zk_experts_combine(zk_context* ctx, const void* d_y, int type, size_t ld_y, 
     hipStream_t st = ctx->s(stream);
     return by_type(type, [&](auto zero) -> int {
       typedef decltype(zero) T;
-      ZK_LAUNCH(ctx, st, "experts_combine", k_combine<T>, dim3((uint32_t)tokens), dim3(256), 0, (const T*)d_y, ld_y,
-                d_place, d_weight, (uint32_t)rows, (uint32_t)slots, (uint32_t)cols, (T*)d_out, ld_out);
-      return ZK_OK;
+      const uint32_t log_w = log_threads<T>(cols);
+      const dim3 grid(cdiv(tokens, 256u >> log_w));
+      auto go = [&](auto kernel) -> int {
+        ZK_LAUNCH(ctx, st, "experts_combine", kernel, grid, dim3(256), 0, (const T*)d_y, ld_y, d_place, d_weight,
+                  (uint32_t)rows, (uint32_t)tokens, (uint32_t)slots, (uint32_t)cols, log_w, (T*)d_out, ld_out);
+        return ZK_OK;
+      };
+      return streams(rows, cols, sizeof(T)) ? go(k_combine<T, true>) : go(k_combine<T, false>);
     });
   });
 }
@@ -364,10 +431,13 @@ int zk_experts_combine_grad(zk_context* ctx, const void* d_grad, size_t ld_grad,
     hipStream_t st = ctx->s(stream);
     return by_type(type, [&](auto zero) -> int {
       typedef decltype(zero) T;
-      ZK_LAUNCH(ctx, st, "experts_combine_grad", k_combine_grad<T>, dim3((uint32_t)tokens), dim3(256), 0,
-                (const T*)d_grad, ld_grad, (const T*)d_y, ld_y, d_order, d_place, d_weight, (uint32_t)rows,
-                (uint32_t)slots, (uint32_t)cols, (T*)d_grad_y, ld_grad_y, d_grad_weight);
-      return ZK_OK;
+      auto go = [&](auto kernel) -> int {
+        ZK_LAUNCH(ctx, st, "experts_combine_grad", kernel, dim3((uint32_t)tokens), dim3(256), 0, (const T*)d_grad,
+                  ld_grad, (const T*)d_y, ld_y, d_order, d_place, d_weight, (uint32_t)rows, (uint32_t)slots,
+                  (uint32_t)cols, (T*)d_grad_y, ld_grad_y, d_grad_weight);
+        return ZK_OK;
+      };
+      return streams(rows, cols, sizeof(T)) ? go(k_combine_grad<T, true>) : go(k_combine_grad<T, false>);
     });
   });
 }

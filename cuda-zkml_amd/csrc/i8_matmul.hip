@@ -754,27 +754,33 @@ static int i8_dispatch(zk_context* ctx, const I8Args& a, int type, hipStream_t s
 }
 
 // ------------------------------------------------------------ rows to 8 bits
-// s = max|x| / 127, q = rint(127 x / max|x|).  The quotient is taken by a
-// division, not by a product with the reciprocal, so that it has one rounding
-// and a half-way quotient goes to the even number.  Rows far from 1 are first
-// multiplied by a power of two, so that neither 127 x nor the quotient leaves
-// the type.  A row of zeros gives s = 0 and zeros; a row with an infinity or a
-// NaN gives s = NaN and zeros, so that its products show it.
+// s = a / 127, q = rint(t / a) with t = 127 x and a = max|x|.  The quotient is
+// the correctly rounded one, so that a half-way quotient goes to the even number
+// as in exact arithmetic: t times the rounded reciprocal of a, and one step of
+// Newton's method on the remainder, which two fused operations give exactly
+// (about 10 operations a value; the compiler's division takes 25, and 2048 rows
+// of 4096 then 10.0 us instead of 7.9).  Rows far from 1 are first multiplied by
+// a power of two, so that nothing leaves the normal numbers.  A row of zeros
+// gives s = 0 and zeros; a row with an infinity or a NaN gives s = NaN and zeros,
+// so that its products show it.
 struct RowScale {
-  float s;     // the row's scale
-  float c, a;  // q = rint(127 (x c) / a); a = 0: all zeros
+  float s;      // the row's scale
+  float c, a;   // t = x c, c = 127 times a power of two; a with the same power
+  float inv;    // 1 / a; 0: all zeros
 };
 
 // From the largest magnitude's bits (as integers magnitudes are in the floats'
 // order, NaN above infinity).
 __device__ __forceinline__ RowScale row_scale(uint32_t m) {
   const float a = __uint_as_float(m);
-  RowScale r = {a / 127.0f, 1.0f, 0.0f};
+  RowScale r = {a / 127.0f, 0.0f, 1.0f, 0.0f};
   if (m >= 0x7f800000u) {
     r.s = __uint_as_float(0x7fc00000u);
   } else if (m) {
-    r.c = a >= 0x1p64f ? 0x1p-32f : a < 0x1p-64f ? 0x1p64f : 1.0f;
-    r.a = a * r.c;
+    const float c = a >= 0x1p64f ? 0x1p-32f : a < 0x1p-64f ? 0x1p64f : 1.0f;
+    r.c = 127.0f * c;
+    r.a = a * c;
+    r.inv = 1.0f / r.a;
   }
   return r;
 }
@@ -786,9 +792,25 @@ __device__ __forceinline__ uint32_t magnitude(T x) {
 
 template <class T>
 __device__ __forceinline__ void quantize_piece(const Vec<T>& x, const RowScale& r, int8_t* q) {
+  if (r.inv == 0.0f) {  // where x itself may be an infinity or a NaN
 #pragma unroll
-  for (uint32_t i = 0; i < Vec<T>::N; i++)
-    q[i] = r.a != 0.0f ? (int8_t)rintf((float)x.v[i] * r.c * 127.0f / r.a) : (int8_t)0;
+    for (uint32_t i = 0; i < Vec<T>::N; i++) q[i] = 0;
+    return;
+  }
+#pragma unroll
+  for (uint32_t i = 0; i < Vec<T>::N; i++) {
+    const float t = (float)x.v[i] * r.c, y = t * r.inv;
+    q[i] = (int8_t)rintf(fmaf(fmaf(-y, r.a, t), r.inv, y));
+  }
+}
+
+template <class T>
+__device__ __forceinline__ void look_piece(const Vec<T>& v, uint32_t& m) {
+#pragma unroll
+  for (uint32_t i = 0; i < Vec<T>::N; i++) {
+    const uint32_t u = magnitude(v.v[i]);
+    m = u > m ? u : m;
+  }
 }
 
 // THREADS threads a row, ROWS rows a block.  A thread keeps its first HELD
@@ -808,13 +830,7 @@ __global__ __launch_bounds__(THREADS* ROWS) void k_i8_quantize(const T* __restri
   const uint32_t pieces = pieces_of<T>(cols);
   Vec<T> held[HELD];
   uint32_t m = 0;
-  auto look = [&](const Vec<T>& v) {
-#pragma unroll
-    for (uint32_t i = 0; i < Vec<T>::N; i++) {
-      const uint32_t u = magnitude(v.v[i]);
-      m = u > m ? u : m;
-    }
-  };
+  auto look = [&](const Vec<T>& v) { look_piece(v, m); };
 #pragma unroll
   for (int h = 0; h < HELD; h++) {
     const uint32_t c = tid + h * THREADS;
@@ -885,6 +901,180 @@ static int i8_quantize(zk_context* ctx, const void* x, int type, size_t ld_x, si
                   (uint32_t)cols, to, ld_q, scale + r);
     }
     return ZK_OK;
+  });
+}
+
+// ------------------------------------------------------------ a few rows, quantized on the way
+// The linear layer of at most 16 rows in one launch: each block asks for its
+// first weights, quantizes all of x's rows into LDS while they come (x is small:
+// every block reads it from the L2), and goes on as k_i8_direct with its x
+// fragments from LDS.
+constexpr uint32_t FEW_ROWS = 16, FEW_BYTES = 48 * 1024;
+// A quantized row's stride in LDS: whole steps, and 16 bytes so that the rows of
+// a fragment lie in different banks.
+static __host__ __device__ inline uint32_t few_ld(uint32_t n_in) { return (n_in + 127) / 128 * 128 + 16; }
+
+template <class T, class X, int FN>
+__global__ __launch_bounds__(512) void k_i8_few(I8Args a, const X* __restrict__ x, size_t ld_x) {
+  constexpr uint32_t BN = 16 * FN, BK = 128, KW = 8;
+  constexpr int U = FN == 1 ? 4 : 2, HELD = 4;
+  extern __shared__ __align__(16) int8_t q[];  // rows x few_ld(n_in)
+  __shared__ __align__(16) v4i sums[KW][FN][64];
+  __shared__ uint32_t part[FEW_ROWS][KW];
+  __shared__ float scale[FEW_ROWS];
+  const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t n0 = blockIdx.x * BN, fr = lane & 15, c = lane >> 4, ld = few_ld(a.n_in);
+  const int8_t* wp[FN];
+#pragma unroll
+  for (int i = 0; i < FN; i++) {
+    const uint32_t n = n0 + i * 16 + fr;
+    wp[i] = a.w + (size_t)(n < a.n_out ? n : a.n_out - 1) * a.ld_w;
+  }
+  const uint32_t steps = (a.n_in + BK - 1) / BK, full = a.n_in / BK;
+  v4i wf[U][FN][2];
+  auto load = [&](uint32_t step) {
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      const uint32_t st = step + u * KW, k = st * BK + c * 16;
+      if (st < full) {
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+#pragma unroll
+          for (int i = 0; i < FN; i++) wf[u][i][h] = load16(wp[i] + k + 64 * h);
+      } else if (st < steps) {
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+#pragma unroll
+          for (int i = 0; i < FN; i++) wf[u][i][h] = load16(wp[i] + last_chunk(k + 64 * h, a.n_in).at);
+      }
+    }
+  };
+  load(wave);
+  // ---- x to 8 bits: KW / g rows at a time, g waves a row
+  uint32_t g = KW;
+  while (g > 1 && KW / g < a.rows) g /= 2;
+  const uint32_t at_once = KW / g, first = wave / g, sub = (wave % g) * 64 + lane;
+  const uint32_t pieces = pieces_of<X>(a.n_in);
+  Vec<X> held[HELD];
+  for (uint32_t r = first; r < a.rows; r += at_once) {
+    const X* row = x + (size_t)r * ld_x;
+    uint32_t m = 0;
+#pragma unroll
+    for (int h = 0; h < HELD; h++) {
+      const uint32_t p = sub + h * g * 64;
+      held[h] = Vec<X>{};
+      if (p < pieces) held[h] = row_load(row + piece<X>(p, a.n_in), a.n_in - piece<X>(p, a.n_in));
+    }
+#pragma unroll
+    for (int h = 0; h < HELD; h++) look_piece(held[h], m);
+    for (uint32_t p = sub + HELD * g * 64; p < pieces; p += g * 64)
+      look_piece(row_load(row + piece<X>(p, a.n_in), a.n_in - piece<X>(p, a.n_in)), m);
+#pragma unroll
+    for (int d = 32; d; d >>= 1) {
+      const uint32_t o = (uint32_t)__shfl_xor((int)m, d);
+      m = o > m ? o : m;
+    }
+    if (lane == 0) part[r][wave % g] = m;
+  }
+  wait_lds();
+  meet();
+  for (uint32_t r = first; r < a.rows; r += at_once) {
+    const X* row = x + (size_t)r * ld_x;
+    int8_t* out = q + r * ld;
+    uint32_t m = 0;
+    for (uint32_t i = 0; i < g; i++) m = part[r][i] > m ? part[r][i] : m;
+    const RowScale rs = row_scale(m);
+    if (sub == 0) scale[r] = rs.s;
+    auto put = [&](uint32_t p, const Vec<X>& v) {
+      const uint32_t at = piece<X>(p, a.n_in);
+      int8_t b[Vec<X>::N];
+      quantize_piece(v, rs, b);
+      if (a.n_in - at >= Vec<X>::N) {
+        __builtin_memcpy(out + at, b, sizeof(b));
+      } else {
+        for (uint32_t i = 0; i < a.n_in - at; i++) out[at + i] = b[i];
+      }
+    };
+    const bool again = at_once < a.rows;  // held is the last of several rows
+    if (!again) {
+#pragma unroll
+      for (int h = 0; h < HELD; h++)
+        if (sub + h * g * 64 < pieces) put(sub + h * g * 64, held[h]);
+    }
+    for (uint32_t p = sub + (again ? 0 : HELD * g * 64); p < pieces; p += g * 64)
+      put(p, row_load(row + piece<X>(p, a.n_in), a.n_in - piece<X>(p, a.n_in)));
+  }
+  wait_lds();
+  meet();
+  // ---- the product
+  const uint32_t row = fr < a.rows ? fr : a.rows - 1;
+  const int8_t* xq = q + row * ld;
+  v4i acc[FN] = {};
+  for (uint32_t step = wave; step < steps; step += U * KW) {
+    if (step != wave) load(step);
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      const uint32_t st = step + u * KW;
+      if (st >= steps) break;
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        const uint32_t k = st * BK + c * 16 + 64 * h;
+        v4i xf;
+        if (st < full) {
+          xf = *(const v4i*)(xq + k);
+        } else {
+          const Chunk part = last_chunk(k, a.n_in);
+          xf = load16(xq + part.at) & part.mask;
+        }
+#pragma unroll
+        for (int i = 0; i < FN; i++) acc[i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[u][i][h], xf, acc[i], 0, 0, 0);
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < FN; i++) sums[wave][i][lane] = acc[i];
+  wait_lds();
+  meet();
+  if (wave >= FN) return;
+  v4i sum = sums[0][wave][lane];
+#pragma unroll
+  for (uint32_t k = 1; k < KW; k++) sum += sums[k][wave][lane];
+  const uint32_t n = n0 + wave * 16 + 4 * c;
+  if (fr >= a.rows || n >= a.n_out) return;
+  const float sx = scale[fr];
+  T v[4];
+#pragma unroll
+  for (uint32_t k = 0; k < 4; k++) {
+    const bool in = n + k < a.n_out;
+    v[k] = finish<T>(sum[k], sx * (a.sw && in ? a.sw[n + k] : 1.0f), a.bias && in ? a.bias[n + k] : 0.0f, a.relu);
+  }
+  T* y = (T*)a.y + (size_t)fr * a.ld_y + n;
+  if (n + 4 <= a.n_out) {
+    __builtin_memcpy(y, v, sizeof(v));
+  } else {
+    for (uint32_t k = 0; k < a.n_out - n; k++) y[k] = v[k];
+  }
+}
+
+static bool few_rows(size_t rows, size_t n_in) {
+  return rows <= FEW_ROWS && n_in >= 16 && n_in <= I8_MAX_IN && rows * few_ld((uint32_t)n_in) <= FEW_BYTES;
+}
+
+static int launch_few(zk_context* ctx, const I8Args& a, const void* x, int x_type, size_t ld_x, int y_type,
+                      hipStream_t st) {
+  return by_type(x_type, [&](auto xz) -> int {
+    return by_type(y_type, [&](auto yz) -> int {
+      typedef decltype(xz) X;
+      typedef decltype(yz) T;
+      const uint32_t lds = a.rows * few_ld(a.n_in);
+      // 32 channels a block halve the times that x is quantized; with fewer
+      // than 256 such blocks they would leave CUs without one
+      if (a.n_out >= 8192)
+        ZK_LAUNCH(ctx, st, "i8_linear", (k_i8_few<T, X, 2>), dim3(cdiv(a.n_out, 32)), dim3(512), lds, a, (const X*)x, ld_x);
+      else
+        ZK_LAUNCH(ctx, st, "i8_linear", (k_i8_few<T, X, 1>), dim3(cdiv(a.n_out, 16)), dim3(512), lds, a, (const X*)x, ld_x);
+      return ZK_OK;
+    });
   });
 }
 
@@ -1002,6 +1192,10 @@ int zk_i8_linear(zk_context* ctx, const void* d_x, int x_type, size_t ld_x, cons
     a.x = q, a.w = d_w, a.sx = scale, a.sw = d_w_scale, a.bias = d_bias, a.y = d_y;
     a.ld_x = lw.ld, a.ld_w = ld_w, a.ld_y = ld_y;
     ZK_TRY(check_product(ctx, a, rows, n_out, n_in, y_type));
+    if (few_rows(rows, n_in)) {
+      a.rows = (uint32_t)rows, a.n_out = (uint32_t)n_out, a.n_in = (uint32_t)n_in, a.relu = relu != 0;
+      return launch_few(ctx, a, d_x, x_type, ld_x, y_type, st);
+    }
     ZK_TRY(i8_quantize(ctx, d_x, x_type, ld_x, rows, n_in, q, lw.ld, scale, st));
     return matmul_impl(ctx, q, lw.ld, scale, d_w, ld_w, d_w_scale, d_bias, rows, n_out, n_in, relu, d_y, y_type,
                        ld_y, st);

@@ -16,21 +16,28 @@ struct Vec {
   T v[N];
 };
 
-template <class T>
+typedef int row16 __attribute__((ext_vector_type(4), aligned(1)));
+
+// ONCE: the bytes are used once, so the caches need not keep them.
+template <class T, bool ONCE = false>
 __device__ __forceinline__ Vec<T> row_load(const T* p, uint32_t left) {
   Vec<T> r;
   if (left >= Vec<T>::N) {
-    __builtin_memcpy(&r, p, 16);
+    const row16 v = ONCE ? __builtin_nontemporal_load((const row16*)p) : *(const row16*)p;
+    __builtin_memcpy(&r, &v, 16);
   } else {
     for (uint32_t i = 0; i < Vec<T>::N; i++) r.v[i] = i < left ? p[i] : (T)0.0f;
   }
   return r;
 }
 
-template <class T>
+template <class T, bool ONCE = false>
 __device__ __forceinline__ void row_store(T* p, uint32_t left, const Vec<T>& r) {
   if (left >= Vec<T>::N) {
-    __builtin_memcpy(p, &r, 16);
+    row16 v;
+    __builtin_memcpy(&v, &r, 16);
+    if (ONCE) __builtin_nontemporal_store(v, (row16*)p);
+    else *(row16*)p = v;
   } else {
     for (uint32_t i = 0; i < Vec<T>::N; i++)
       if (i < left) p[i] = r.v[i];
