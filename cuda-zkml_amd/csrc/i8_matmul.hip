@@ -55,13 +55,54 @@ __device__ __forceinline__ Chunk last_chunk(uint32_t k, uint32_t n_in) {
     c.mask[d] = skip <= 4 * d ? -1 : skip >= 4 * d + 4 ? 0 : (int)(~0u << (8 * (skip - 4 * d)));
   return c;
 }
-// 16 bytes from any address: gfx950 loads them whatever its alignment.
-__device__ __forceinline__ v4i load16(const int8_t* p) {
+// 16 bytes from any address: at full rate from whole words, at a third of it
+// from others.
+__device__ __forceinline__ v4i load16_any(const int8_t* p) {
   v4i v;
   __builtin_memcpy(&v, p, 16);
   return v;
 }
-
+// 16 bytes from a multiple of 4 bytes, or, BYTES, from any address as the words
+// that hold them, moved down by the address's part of a word (3 x 5569 x 7061:
+// 11 us, 19 with load16_any).  No word is read that holds none of the bytes.
+typedef int v4i_words __attribute__((ext_vector_type(4), aligned(4)));
+__device__ __forceinline__ v4i move_down(const v4i& v, int next, uint32_t by) {
+  return v4i{(int)__builtin_amdgcn_alignbyte((uint32_t)v[1], (uint32_t)v[0], by),
+             (int)__builtin_amdgcn_alignbyte((uint32_t)v[2], (uint32_t)v[1], by),
+             (int)__builtin_amdgcn_alignbyte((uint32_t)v[3], (uint32_t)v[2], by),
+             (int)__builtin_amdgcn_alignbyte((uint32_t)next, (uint32_t)v[3], by)};
+}
+template <bool BYTES>
+__device__ __forceinline__ v4i load16(const int8_t* p) {
+  if (!BYTES) return *(const v4i_words*)p;
+  const uint32_t by = (uint32_t)(uintptr_t)p & 3u;
+  const int8_t* q = p - by;
+  const v4i v = *(const v4i_words*)q;
+  return move_down(v, *(const int*)(q + (by ? 16 : 12)), by);
+}
+// The last 16 bytes of a row of any length.
+template <bool BYTES>
+__device__ __forceinline__ v4i load16_end(const int8_t* p) {
+  return BYTES ? load16<true>(p) : load16_any(p);
+}
+// Lane c's 32 of a step's 128 bytes, the same ones on both sides of a product:
+// bytes 16 c on of each half, or, BYTES, 32 c on, so that the second 16 bytes'
+// first word is the first ones' next.
+template <bool BYTES>
+__device__ __forceinline__ void load_pair(const int8_t* p, uint32_t c, v4i (&out)[2]) {
+  if (!BYTES) {
+    out[0] = load16<false>(p + c * 16);
+    out[1] = load16<false>(p + c * 16 + 64);
+  } else {
+    const uint32_t by = (uint32_t)(uintptr_t)p & 3u;
+    const int8_t* q = p + c * 32 - by;
+    out[0] = load16<false>(q);
+    out[1] = load16<false>(q + 16);
+    const int next = *(const int*)(q + (by ? 32 : 28));
+    out[0] = move_down(out[0], out[1][0], by);
+    out[1] = move_down(out[1], next, by);
+  }
+}
 template <class T>
 __device__ __forceinline__ T finish(int acc, float s, float b, int relu) {
   float f = (float)acc * s + b;
@@ -282,7 +323,7 @@ __global__ __launch_bounds__(64 * WT * WN) void k_i8_ring(I8Args a, uint32_t til
   constexpr uint32_t WAVES = WT * WN, BT = WT * FT * 32, BN = WN * FN * 32, BK = 128;
   static_assert(BT == BN, "the ring's slots hold either side's tile");
   constexpr uint32_t SLOT = BT * BK, PER = BT / 8 / WAVES;  // 8-row pieces of 1 KB that a wave fills
-  constexpr int HALF = PER / 2;
+  constexpr int FIRST = (PER + 1) / 2;  // of a tile's pieces, those that the first of two quarter steps fills
   constexpr uint32_t OWN = 32 * (FN * 32 * sizeof(T) + 16);  // a wave's part of LDS for its results
   __shared__ __align__(16) int8_t lds[5 * SLOT];
   auto swz = [](uint32_t row) { return (row >> 1) & 7u; };
@@ -383,14 +424,15 @@ __global__ __launch_bounds__(64 * WT * WN) void k_i8_ring(I8Args a, uint32_t til
           }
           acc[m / FT][m % FT] =
               __builtin_amdgcn_mfma_i32_32x32x32_i8(wf[s & 1][m / FT], xf[s & 1][m % FT], acc[m / FT][m % FT], 0, 0, 0);
+          // the tiles of w two steps on and of x three on, as their slots get free
 #pragma unroll
-          for (int d = 0; d < HALF; d++)
-            if (d * M / HALF == m) {
+          for (int d = 0; d < FIRST; d++)
+            if (d * M / FIRST == m) {
               if (s == 3) put(wp[d], d, step + 2, x0);
-              if (LONG || step) {
-                if (s == 0) put(wp[HALF + d], HALF + d, step + 1, w1);
-                if (s == 1) put(xp[d], d, step + 2, x2);
-                if (s == 2) put(xp[HALF + d], HALF + d, step + 2, x2);
+              if (s == 1 && (LONG || step)) put(xp[d], d, step + 2, x2);
+              if (FIRST + d < (int)PER && (LONG || step)) {
+                if (s == 0) put(wp[FIRST + d], FIRST + d, step + 1, w1);
+                if (s == 2) put(xp[FIRST + d], FIRST + d, step + 2, x2);
               }
             }
           __builtin_amdgcn_sched_barrier(0);
@@ -414,6 +456,9 @@ __global__ __launch_bounds__(64 * WT * WN) void k_i8_ring(I8Args a, uint32_t til
 // The same tiles where a row may start at any byte, or end inside a chunk: the
 // steps pass through registers (masked), loaded a step ahead and stored before
 // the stage's turn.
+// (Loads from any address; word loads with the bytes moved down, as the direct
+// kernel has them, hold a register more a piece and made 1194 x 4438 x 5316 98 us
+// instead of 68.)
 template <class T, bool GROUPED, int WT, int WN, int FT, int FN>
 __global__ __launch_bounds__(64 * WT * WN) void k_i8_odd(I8Args a, uint32_t tiles_t, uint32_t tiles_n) {
   constexpr uint32_t WAVES = WT * WN, BT = WT * FT * 32, BN = WN * FN * 32, BK = 128;
@@ -450,18 +495,18 @@ __global__ __launch_bounds__(64 * WT * WN) void k_i8_odd(I8Args a, uint32_t tile
   auto take = [&](uint32_t step) {
     if ((step + 1) * BK <= a.n_in) {
 #pragma unroll
-      for (uint32_t i = 0; i < XR; i++) held[i] = load16(xp[i] + step * BK + chunk(wave * XR + i));
+      for (uint32_t i = 0; i < XR; i++) held[i] = load16_any(xp[i] + step * BK + chunk(wave * XR + i));
 #pragma unroll
-      for (uint32_t i = 0; i < WR; i++) held[XR + i] = load16(wp[i] + step * BK + chunk(wave * WR + i));
+      for (uint32_t i = 0; i < WR; i++) held[XR + i] = load16_any(wp[i] + step * BK + chunk(wave * WR + i));
     } else {
 #pragma unroll
       for (uint32_t i = 0; i < XR; i++) {
         const Chunk c = last_chunk(step * BK + chunk(wave * XR + i), a.n_in);
-        held[i] = load16(xp[i] + c.at) & c.mask;
+        held[i] = load16_any(xp[i] + c.at) & c.mask;
       }
 #pragma unroll
       for (uint32_t i = 0; i < WR; i++)
-        held[XR + i] = load16(wp[i] + last_chunk(step * BK + chunk(wave * WR + i), a.n_in).at);
+        held[XR + i] = load16_any(wp[i] + last_chunk(step * BK + chunk(wave * WR + i), a.n_in).at);
     }
   };
   auto store = [&](uint32_t stage) {
@@ -529,8 +574,8 @@ __global__ __launch_bounds__(64 * WT * WN) void k_i8_odd(I8Args a, uint32_t tile
 // 16 FT tokens x 16 FN channels; its KW waves split k between them in steps of
 // 128 bytes (a cache line of every row) and add up their sums in LDS.  Bound by
 // what the L2 hands over: 16 (FT + FN) rows a block, 9.3 TB/s over the chip.
-template <class T, bool GROUPED, int FT, int FN, int KW>
-__global__ __launch_bounds__(64 * KW) void k_i8_direct(I8Args a, uint32_t tiles_t, uint32_t tiles_n) {
+template <class T, bool GROUPED, bool BYTES, int FT, int FN, int KW>
+__global__ __launch_bounds__(64 * KW, 4) void k_i8_direct(I8Args a, uint32_t tiles_t, uint32_t tiles_n) {
   constexpr uint32_t BT = 16 * FT, BN = 16 * FN, BK = 128;
   constexpr int U = FT + FN <= 2 ? 4 : 2;  // steps whose loads are under way together
   __shared__ __align__(16) v4i sums[KW][FN * FT][64];
@@ -570,14 +615,11 @@ __global__ __launch_bounds__(64 * KW) void k_i8_direct(I8Args a, uint32_t tiles_
   for (; step + (U - 1) * KW < full; step += U * KW) {
 #pragma unroll
     for (int u = 0; u < U; u++) {
-      const uint32_t k = (step + u * KW) * BK + c * 16;
+      const uint32_t k = (step + u * KW) * BK;
 #pragma unroll
-      for (int h = 0; h < 2; h++) {
+      for (int i = 0; i < FN; i++) load_pair<BYTES>(wp[i] + k, c, wf[u][i]);
 #pragma unroll
-        for (int i = 0; i < FN; i++) wf[u][i][h] = load16(wp[i] + k + 64 * h);
-#pragma unroll
-        for (int j = 0; j < FT; j++) xf[u][j][h] = load16(xp[j] + k + 64 * h);
-      }
+      for (int j = 0; j < FT; j++) load_pair<BYTES>(xp[j] + k, c, xf[u][j]);
     }
 #pragma unroll
     for (int u = 0; u < U; u++) multiply(u);
@@ -587,14 +629,14 @@ __global__ __launch_bounds__(64 * KW) void k_i8_direct(I8Args a, uint32_t tiles_
 #pragma unroll
     for (int u = 0; u < U; u++) {
       if (step + u * KW >= steps) break;
-      const uint32_t k = (step + u * KW) * BK + c * 16;
+      const uint32_t k = (step + u * KW) * BK + c * 32;
 #pragma unroll
       for (int h = 0; h < 2; h++) {
-        const Chunk part = last_chunk(k + 64 * h, a.n_in);
+        const Chunk part = last_chunk(k + 16 * h, a.n_in);
 #pragma unroll
-        for (int i = 0; i < FN; i++) wf[u][i][h] = load16(wp[i] + part.at);
+        for (int i = 0; i < FN; i++) wf[u][i][h] = load16_end<BYTES>(wp[i] + part.at);
 #pragma unroll
-        for (int j = 0; j < FT; j++) xf[u][j][h] = load16(xp[j] + part.at) & part.mask;
+        for (int j = 0; j < FT; j++) xf[u][j][h] = load16_end<BYTES>(xp[j] + part.at) & part.mask;
       }
     }
 #pragma unroll
@@ -670,36 +712,40 @@ __global__ __launch_bounds__(256) void k_i8_short(I8Args a) {
 }
 
 // ------------------------------------------------------------ which kernel
-// A tile's time in ns: its own part (first loads, results) and its steps of 128
-// bytes of k, times the tiles that a CU has to do: tiles / 256, rounded up where
-// a tile fills a CU for long (from 64 x 64 on).  Measured on rows that are
-// multiples of 16 bytes (`odd`: on others).
+// A product's time in ns: `base` once, and for each tile that a CU has to do
+// (tiles / 256, rounded up where a tile fills a CU for long) `own` for its first
+// loads and its results and `step` for each 128 bytes of k.  Fitted to products
+// of 1 to 8192 rows, 16 to 8192 long; `odd`: for the tiles that read straight
+// from memory, rows that do not start at whole words, for the others rows that
+// are not multiples of 16 bytes.
 struct TileCost {
-  uint32_t bt, bn, own, step, odd_own, odd_step;
+  uint32_t bt, bn, base, own, step, odd_own, odd_step;
 };
 constexpr TileCost TILE_COST[] = {
-    {16, 16, 600, 114, 600, 170},     {32, 16, 600, 171, 600, 260},     {16, 32, 600, 171, 600, 260},
-    {32, 32, 600, 228, 600, 340},     {64, 64, 1700, 230, 2000, 280},   {128, 128, 4500, 530, 4500, 700},
-    {256, 256, 8500, 1600, 0, 0},
+    {16, 16, 600, 1000, 114, 1000, 150},  {32, 16, 600, 1000, 171, 1000, 220}, {16, 32, 600, 1000, 171, 1000, 200},
+    {32, 32, 600, 1000, 228, 1000, 260},  {64, 64, 1200, 500, 200, 800, 300},  {128, 128, 1000, 2000, 500, 2200, 750},
+    {256, 256, 500, 8000, 1600, 9000, 2500},
 };
 
 // The kernel with the least estimated time: few rows are split over small tiles
 // that read straight from memory, many go through the tiles that read each row
 // fewest times.
-static int choose_tile(const I8Args& a, bool grouped, bool odd) {
+static int choose_tile(const I8Args& a, bool grouped, bool odd_rows, bool bytes) {
   const uint64_t groups = grouped ? (a.experts < a.rows ? a.experts : a.rows) : 0;
   const uint64_t steps = (a.n_in + 127) / 128;
   int best = 0;
   uint64_t least = ~0ull;
   for (int i = 0; i < (int)(sizeof(TILE_COST) / sizeof(TILE_COST[0])); i++) {
     const TileCost& c = TILE_COST[i];
-    if (odd && !c.odd_step) continue;
+    const bool odd = c.bt >= 64 ? odd_rows : bytes;
     // an expert's last row tile is half full, or it has only one
     uint64_t tt = cdiv(a.rows, c.bt);
     if (grouped && (tt += groups / 2) < groups) tt = groups;
     uint64_t tiles = tt * cdiv(a.n_out, c.bn);
     if (tiles < 256 || c.bt >= 64) tiles = (tiles + 255) / 256 * 256;
-    const uint64_t t = (odd ? c.odd_own : c.own) + tiles * steps * (odd ? c.odd_step : c.step) / 256;
+    // grouped, a large tile waits for a chain of indexes first; small ones share a CU
+    const uint64_t own = (odd ? c.odd_own : c.own) + (grouped && c.bt >= 64 ? 2000 : 0);
+    const uint64_t t = c.base + tiles * (own + steps * (odd ? c.odd_step : c.step)) / 256;
     if (t < least) least = t, best = i;
   }
   return best;
@@ -713,8 +759,9 @@ static int launch_product(zk_context* ctx, const I8Args& a, hipStream_t st) {
     ZK_LAUNCH(ctx, st, name, (k_i8_short<T, GROUPED>), dim3(blocks < 65536 ? (uint32_t)blocks : 65536), dim3(256), 0, a);
     return ZK_OK;
   }
-  const bool odd = ((uintptr_t)a.x | (uintptr_t)a.w | a.ld_x | a.ld_w | a.n_in) % 16 != 0;
-  const int c = choose_tile(a, GROUPED, odd);
+  const size_t rows_at = (uintptr_t)a.x | (uintptr_t)a.w | a.ld_x | a.ld_w;
+  const bool odd = (rows_at | a.n_in) % 16 != 0, bytes = rows_at % 4 != 0;
+  const int c = choose_tile(a, GROUPED, odd, bytes);
   auto go = [&](auto kernel, uint32_t threads) -> int {
     // row tiles of the grouped form: whole ones, and a part of one for each
     // expert and for the rows without an expert
@@ -727,19 +774,26 @@ static int launch_product(zk_context* ctx, const I8Args& a, hipStream_t st) {
     return ZK_OK;
   };
   switch (c) {
-    case 0: return go(k_i8_direct<T, GROUPED, 1, 1, 8>, 512);
-    case 1: return go(k_i8_direct<T, GROUPED, 2, 1, 8>, 512);
-    case 2: return go(k_i8_direct<T, GROUPED, 1, 2, 8>, 512);
-    case 3: return go(k_i8_direct<T, GROUPED, 2, 2, 8>, 512);
-    case 4: return odd ? go(k_i8_odd<T, GROUPED, 2, 2, 1, 1>, 256) : go(k_i8_ring<T, GROUPED, 2, 2, 1, 1>, 256);
+    case 0: return bytes ? go(k_i8_direct<T, GROUPED, true, 1, 1, 8>, 512) : go(k_i8_direct<T, GROUPED, false, 1, 1, 8>, 512);
+    case 1: return bytes ? go(k_i8_direct<T, GROUPED, true, 2, 1, 8>, 512) : go(k_i8_direct<T, GROUPED, false, 2, 1, 8>, 512);
+    case 2: return bytes ? go(k_i8_direct<T, GROUPED, true, 1, 2, 8>, 512) : go(k_i8_direct<T, GROUPED, false, 1, 2, 8>, 512);
+    case 3: return bytes ? go(k_i8_direct<T, GROUPED, true, 2, 2, 8>, 512) : go(k_i8_direct<T, GROUPED, false, 2, 2, 8>, 512);
+    case 4:
+      if (odd) return go(k_i8_odd<T, GROUPED, 2, 2, 1, 1>, 256);
+      return go(k_i8_ring<T, GROUPED, 2, 2, 1, 1>, 256);
+    // of short sums a larger part is a tile's own, which more waves do faster
+    // (8192 x 1024 x 8192: 92 us with eight waves of 128 x 128 and 102 with four,
+    // 84 and 88 with sixteen and eight of 256 x 256); fewer waves read LDS less
+    // (8192 x 8192 x 8192: 541 and 513, 441 and 426).  Grouped, all share the chain
+    // of indexes before the first step (66 us and 83, 4096 x 4 rows, 64 experts).
     case 5:
-      if (odd) return go(k_i8_odd<T, GROUPED, 2, 2, 2, 2>, 256);
-      // grouped, eight waves share the chain of indexes before the first step
-      // (4096 x 4 rows of 2048, 64 experts: 66 us, 83 with four waves); else four
-      // read LDS less (4096 x 4096 x 4096: 73 us, 77 with eight)
-      if constexpr (GROUPED) return go(k_i8_ring<T, GROUPED, 2, 4, 2, 1>, 512);
-      else return go(k_i8_ring<T, GROUPED, 2, 2, 2, 2>, 256);
-    default: return go(k_i8_ring<T, GROUPED, 2, 4, 4, 2>, 512);
+      if (odd) return go(k_i8_odd<T, GROUPED, 2, 4, 2, 1>, 512);
+      if (GROUPED || a.n_in <= 2048) return go(k_i8_ring<T, GROUPED, 2, 4, 2, 1>, 512);
+      return go(k_i8_ring<T, false, 2, 2, 2, 2>, 256);
+    default:
+      if (odd) return go(k_i8_odd<T, GROUPED, 2, 4, 4, 2>, 512);
+      if (a.n_in <= 2048) return go(k_i8_ring<T, GROUPED, 4, 4, 2, 2>, 1024);
+      return go(k_i8_ring<T, GROUPED, 2, 4, 4, 2>, 512);
   }
 }
 
@@ -932,22 +986,25 @@ __global__ __launch_bounds__(512) void k_i8_few(I8Args a, const X* __restrict__ 
   }
   const uint32_t steps = (a.n_in + BK - 1) / BK, full = a.n_in / BK;
   v4i wf[U][FN][2];
-  auto load = [&](uint32_t step) {
+  const bool words = (((uint32_t)(uintptr_t)a.w | (uint32_t)a.ld_w) & 3u) == 0;
+  auto load_as = [&](auto bytes, uint32_t step) {
 #pragma unroll
     for (int u = 0; u < U; u++) {
-      const uint32_t st = step + u * KW, k = st * BK + c * 16;
+      const uint32_t st = step + u * KW, k = st * BK + c * 32;
       if (st < full) {
 #pragma unroll
-        for (int h = 0; h < 2; h++)
-#pragma unroll
-          for (int i = 0; i < FN; i++) wf[u][i][h] = load16(wp[i] + k + 64 * h);
+        for (int i = 0; i < FN; i++) load_pair<decltype(bytes)::value>(wp[i] + st * BK, c, wf[u][i]);
       } else if (st < steps) {
 #pragma unroll
         for (int h = 0; h < 2; h++)
 #pragma unroll
-          for (int i = 0; i < FN; i++) wf[u][i][h] = load16(wp[i] + last_chunk(k + 64 * h, a.n_in).at);
+          for (int i = 0; i < FN; i++) wf[u][i][h] = load16_end<decltype(bytes)::value>(wp[i] + last_chunk(k + 16 * h, a.n_in).at);
       }
     }
+  };
+  auto load = [&](uint32_t step) {
+    if (words) load_as(std::false_type(), step);
+    else load_as(std::true_type(), step);
   };
   load(wave);
   // ---- x to 8 bits: KW / g rows at a time, g waves a row
@@ -1018,13 +1075,13 @@ __global__ __launch_bounds__(512) void k_i8_few(I8Args a, const X* __restrict__ 
       if (st >= steps) break;
 #pragma unroll
       for (int h = 0; h < 2; h++) {
-        const uint32_t k = st * BK + c * 16 + 64 * h;
         v4i xf;
         if (st < full) {
-          xf = *(const v4i*)(xq + k);
+          xf = *(const v4i*)(xq + st * BK + (words ? c * 16 + 64 * h : c * 32 + 16 * h));
         } else {
-          const Chunk part = last_chunk(k, a.n_in);
-          xf = load16(xq + part.at) & part.mask;
+          const Chunk part = last_chunk(st * BK + c * 32 + 16 * h, a.n_in);
+          __builtin_memcpy(&xf, xq + part.at, 16);
+          xf &= part.mask;
         }
 #pragma unroll
         for (int i = 0; i < FN; i++) acc[i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[u][i][h], xf, acc[i], 0, 0, 0);
