@@ -683,7 +683,7 @@ __global__ __launch_bounds__(64 * KW, 4) void k_i8_direct(I8Args a, uint32_t til
 }
 
 // ------------------------------------------------------------ rows under 16 bytes
-// A thread takes one result at a time: its sum has 15 terms at the most.
+// A thread takes one result at a time: its sum has 15 terms at the most, or none.
 template <class T, bool GROUPED>
 __global__ __launch_bounds__(256) void k_i8_short(I8Args a) {
   const uint64_t all = (uint64_t)a.rows * a.n_out, stride = (uint64_t)gridDim.x * 256;
@@ -715,15 +715,14 @@ __global__ __launch_bounds__(256) void k_i8_short(I8Args a) {
 // A product's time in ns: `base` once, and for each tile that a CU has to do
 // (tiles / 256, rounded up where a tile fills a CU for long) `own` for its first
 // loads and its results and `step` for each 128 bytes of k.  Fitted to products
-// of 1 to 8192 rows, 16 to 8192 long; `odd`: for the tiles that read straight
-// from memory, rows that do not start at whole words, for the others rows that
-// are not multiples of 16 bytes.
+// of 1 to 8192 rows, 16 to 8192 long; `odd`: for rows that are not multiples of
+// 16 bytes.
 struct TileCost {
   uint32_t bt, bn, base, own, step, odd_own, odd_step;
 };
 constexpr TileCost TILE_COST[] = {
-    {16, 16, 600, 1000, 114, 1000, 150},  {32, 16, 600, 1000, 171, 1000, 220}, {16, 32, 600, 1000, 171, 1000, 200},
-    {32, 32, 600, 1000, 228, 1000, 260},  {64, 64, 1200, 500, 200, 800, 300},  {128, 128, 1000, 2000, 500, 2200, 750},
+    {16, 16, 600, 1000, 0, 1000, 0},     {32, 16, 600, 1000, 0, 1000, 0},     {16, 32, 600, 1000, 0, 1000, 0},
+    {32, 32, 600, 1000, 0, 1000, 0},     {64, 64, 1200, 500, 200, 800, 300},  {128, 128, 1000, 2000, 500, 2200, 750},
     {256, 256, 500, 8000, 1600, 9000, 2500},
 };
 
@@ -737,15 +736,18 @@ static int choose_tile(const I8Args& a, bool grouped, bool odd_rows, bool bytes)
   uint64_t least = ~0ull;
   for (int i = 0; i < (int)(sizeof(TILE_COST) / sizeof(TILE_COST[0])); i++) {
     const TileCost& c = TILE_COST[i];
-    const bool odd = c.bt >= 64 ? odd_rows : bytes;
+    const bool small = c.bt < 64, odd = small ? bytes : odd_rows;
     // an expert's last row tile is half full, or it has only one
     uint64_t tt = cdiv(a.rows, c.bt);
     if (grouped && (tt += groups / 2) < groups) tt = groups;
     uint64_t tiles = tt * cdiv(a.n_out, c.bn);
-    if (tiles < 256 || c.bt >= 64) tiles = (tiles + 255) / 256 * 256;
-    // grouped, a large tile waits for a chain of indexes first; small ones share a CU
-    const uint64_t own = (odd ? c.odd_own : c.own) + (grouped && c.bt >= 64 ? 2000 : 0);
-    const uint64_t t = c.base + tiles * (own + steps * (odd ? c.odd_step : c.step)) / 256;
+    if (tiles < 256 || !small) tiles = (tiles + 255) / 256 * 256;
+    uint64_t own = odd ? c.odd_own : c.own, step = odd ? c.odd_step : c.step;
+    // straight from memory: 128 bytes of each row at 36 bytes/ns a CU, the tile's
+    // missing rows of x being one and the same
+    if (small) step = (c.bn + (a.rows < tt * c.bt ? (a.rows + tt - 1) / tt : c.bt)) * (bytes ? 43 : 36) / 10;
+    if (grouped) own += small ? 1000 : 2000;  // the chain of indexes
+    const uint64_t t = c.base + tiles * (own + steps * step) / 256;
     if (t < least) least = t, best = i;
   }
   return best;
@@ -754,7 +756,7 @@ static int choose_tile(const I8Args& a, bool grouped, bool odd_rows, bool bytes)
 template <class T, bool GROUPED>
 static int launch_product(zk_context* ctx, const I8Args& a, hipStream_t st) {
   const char* name = GROUPED ? "i8_matmul_experts" : "i8_matmul";
-  if (a.n_in < 16) {
+  if (a.n_in < 16 || (GROUPED && !a.tokens)) {  // (without tokens there is no row to read)
     const size_t blocks = ((size_t)a.rows * a.n_out + 255) / 256;
     ZK_LAUNCH(ctx, st, name, (k_i8_short<T, GROUPED>), dim3(blocks < 65536 ? (uint32_t)blocks : 65536), dim3(256), 0, a);
     return ZK_OK;

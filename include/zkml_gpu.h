@@ -262,7 +262,7 @@ int zk_synthetic_r1cs(int num_constraints, int num_public, int num_inputs, uint6
  * them to the real-valued model.
  *
  * zk_i8_matmul: acc[t][n] = sum_k x[t][k] w[n][k] (int8, exact in int32;
- * n_in <= 131071), then
+ * n_in <= 131071, n_out <= 2^26), then
  *   y_type ZK_I32: y = acc (no scales, no bias);
  *   else           y = float(acc) * (x_scale[t] * w_scale[n]) + bias[n],
  * in 32-bit floats, rounded once to y_type; relu != 0 replaces what is below

@@ -106,6 +106,34 @@ def test_strides_and_offsets(ctx, kind, rows, n_out, n_in, lead, pad):
         near(y.read(), want.astype(np.float64), np.abs(want), kind)
 
 
+def wide_sums(x, w):
+    """The exact sums by way of float64, whose 53 bits hold them."""
+    return (x.astype(np.float64) @ w.astype(np.float64).T).astype(np.int64)
+
+
+# sizes whose work fills the chip: the large tiles, whole and ragged, rows that
+# are multiples of 16 bytes, of 4, and of one
+@pytest.mark.parametrize("rows,n_out,n_in", [(1100, 1200, 2080), (1500, 1030, 656), (2050, 2200, 4112),
+                                             (4100, 4090, 1040), (4100, 4200, 2064), (1500, 1030, 660),
+                                             (1100, 1300, 1001), (4000, 4100, 1189), (100, 3000, 1003),
+                                             (9, 7000, 1030), (20, 20, 5569), (3000, 40, 2002)])
+def test_large_tiles(ctx, rows, n_out, n_in):
+    rng = np.random.default_rng([rows, n_out, n_in])
+    x = rng.integers(-128, 128, (rows, n_in), dtype=np.int8)
+    w = rng.integers(-128, 128, (n_out, n_in), dtype=np.int8)
+    say("[i8 large]", rows, n_out, n_in)
+    y = Result(ctx, rows, n_out, "i32", ld=n_out + 3)
+    ctx.i8_matmul(ctx.upload(x), ctx.upload(w), rows, n_out, n_in, y.at, ld_y=n_out + 3)
+    want = wide_sums(x, w)
+    assert np.array_equal(y.read(), want)
+    sx, sw = (np.exp(rng.normal(-6, 0.5, n)).astype(np.float32) for n in (rows, n_out))
+    y = Result(ctx, rows, n_out, "bf16")
+    ctx.i8_matmul(ctx.upload(x), ctx.upload(w), rows, n_out, n_in, y.at, z.BF16, x_scale=ctx.upload(sx),
+                  w_scale=ctx.upload(sw))
+    v = want * (sx.astype(np.float64)[:, None] * sw.astype(np.float64))
+    near(y.read(), v, np.abs(v), "bf16")
+
+
 def test_longest_sum(ctx):
     """The largest sum of the longest row: 2^14 * 131071 < 2^31."""
     n_in = 131071
@@ -242,7 +270,9 @@ def test_quantize_edges(ctx, kind, cols):
 @pytest.mark.parametrize("kind,out", [("f32", "f32"), ("bf16", "bf16"), ("f16", "f16"), ("bf16", "f32")])
 @pytest.mark.parametrize("rows,n_out,n_in,pad", [(1, 100, 4096, 0), (1, 1, 1, 0), (1, 513, 1001, 3), (2, 64, 64, 0),
                                                  (4, 33, 300, 1), (9, 200, 1000, 8), (70, 130, 515, 0),
-                                                 (300, 256, 1024, 0)])
+                                                 (300, 256, 1024, 0), (5, 8200, 9000, 0), (16, 8195, 2900, 1),
+                                                 (3, 70, 15000, 0), (16, 40, 3000, 2), (17, 50, 2000, 0),
+                                                 (2, 30, 16, 0), (2, 30, 15, 0)])
 def test_linear(ctx, kind, out, rows, n_out, n_in, pad):
     """The linear layer is the product over its rows' quantized values: compared
     with the 64-bit product of the library's own q and s, which test_quantize
@@ -328,6 +358,30 @@ def test_experts_product(ctx, kind, tokens, slots, experts, n_out, n_in, dropped
     near(got[:used], v + b[e], np.abs(v) + np.abs(b[e]), kind)
 
 
+@pytest.mark.parametrize("tokens,slots,experts,n_out,n_in,skew", [(2000, 4, 8, 700, 1040, 0.3),
+                                                                  (2000, 4, 8, 700, 1041, 0.3),
+                                                                  (3000, 3, 3, 2100, 1056, 0.5),
+                                                                  (3000, 3, 3, 2100, 1057, 0.5),
+                                                                  (2600, 4, 2, 2100, 2064, 0.2),
+                                                                  (900, 8, 200, 300, 272, 0.02)])
+def test_experts_product_large(ctx, tokens, slots, experts, n_out, n_in, skew):
+    """The large tiles with rows by expert, some of them dropped."""
+    rng = np.random.default_rng([tokens, experts, n_in])
+    offsets, order = routed(rng, tokens, slots, experts, 0.05, skew)
+    x = rng.integers(-127, 128, (tokens, n_in), dtype=np.int8)
+    w = rng.integers(-127, 128, (experts * n_out, n_in), dtype=np.int8)
+    rows = tokens * slots
+    say("[i8 experts large]", tokens, slots, experts, n_out, n_in)
+    y = Result(ctx, rows, n_out, "i32")
+    ctx.i8_matmul_experts(ctx.upload(x), ctx.upload(w), ctx.upload(offsets), rows, experts, n_out, n_in, y.at,
+                          order=ctx.upload(order), slots=slots, tokens=tokens)
+    got = y.read()
+    for e in range(experts):
+        at = slice(offsets[e], offsets[e + 1])
+        assert np.array_equal(got[at], wide_sums(x[order[at] // slots], w[e * n_out:(e + 1) * n_out])), e
+    assert not got[offsets[-1]:].any()
+
+
 def test_experts_product_without_an_order(ctx):
     """Rows that are sorted already: row p of x, its own scale."""
     rng = np.random.default_rng(3)
@@ -355,6 +409,17 @@ def test_experts_product_takes_bad_indexes_as_none(ctx):
     assert (got[0] == 20).all() and not got[1:].any()
 
 
+@pytest.mark.parametrize("n_in", [8, 300])
+def test_experts_product_without_tokens(ctx, n_in):
+    """No token: every row is zero, and nothing of x is read."""
+    order = np.zeros(70, dtype=np.int32)
+    y = Result(ctx, 70, 5, "f32")
+    ctx.i8_matmul_experts(ctx.alloc(1), matrix(ctx, np.ones((2 * 5, n_in), dtype=np.int8)),
+                          ctx.upload(np.array([0, 30, 70], dtype=np.int32)), 70, 2, 5, n_in, y.at, z.F32,
+                          order=ctx.upload(order), slots=1, tokens=0)
+    assert not y.read().any()
+
+
 # ------------------------------------------------------------ refusals, streams
 def test_refusals(ctx):
     d = ctx.alloc(4096)
@@ -371,7 +436,8 @@ def test_refusals(ctx):
                      (dict(x_scale=At(d, 1)), "aligned"), (dict(w_scale=At(d, 2)), "aligned"),
                      (dict(bias=At(d, 3)), "aligned"), (dict(y_type=z.I32, bias=d), "no bias"),
                      (dict(y_type=z.I32, x_scale=d), "no scales"), (dict(n_in=131072, ld_x=131072, ld_w=131072), "131071"),
-                     (dict(rows=1 << 31), "2\\^31"), (dict(n_out=1 << 31, ld_y=1 << 31), "2\\^31")]:
+                     (dict(rows=1 << 31), "2\\^31"), (dict(n_out=1 << 31, ld_y=1 << 31), "2\\^31"),
+                     (dict(n_out=(1 << 26) + 1, ld_y=1 << 27), "2\\^26")]:
         with pytest.raises(z.ZkError, match=why):
             mm(**bad)
     for args, why in [((None, z.F32, 1, 4, d, d), "null"), ((d, z.I32, 1, 4, d, d), "f32, f16 or bf16"),
