@@ -114,6 +114,28 @@ __device__ __forceinline__ int finish<int>(int acc, float, float, int relu) {
   return relu && acc < 0 ? 0 : acc;
 }
 
+// Four neighbouring results, of which the row has `left` from here on.  (Every
+// index is a constant: an array that is indexed by a variable goes to LDS, by way
+// of the launch packet in host memory, and a call of 5 us then took 16.)
+// ONCE: around the caches.
+template <bool ONCE = false, class T>
+__device__ __forceinline__ void store4(T* y, uint32_t left, const T (&v)[4]) {
+  if (left >= 4) {
+    if constexpr (ONCE) {
+      row16 b;
+      static_assert(sizeof(v) == 16, "whole pieces of 16 bytes");
+      __builtin_memcpy(&b, v, 16);
+      __builtin_nontemporal_store(b, (row16*)y);
+    } else {
+      __builtin_memcpy(y, v, sizeof(v));
+    }
+    return;
+  }
+#pragma unroll
+  for (uint32_t k = 0; k < 3; k++)
+    if (k < left) y[k] = v[k];
+}
+
 // Offset of expert e, inside [0, rows] whatever the device array holds.
 __device__ __forceinline__ uint32_t offset_of(const I8Args& a, uint32_t e) {
   const int v = a.offsets[e];
@@ -325,6 +347,7 @@ __global__ __launch_bounds__(64 * WT * WN) void k_i8_ring(I8Args a, uint32_t til
   constexpr uint32_t SLOT = BT * BK, PER = BT / 8 / WAVES;  // 8-row pieces of 1 KB that a wave fills
   constexpr int FIRST = (PER + 1) / 2;  // of a tile's pieces, those that the first of two quarter steps fills
   constexpr uint32_t OWN = 32 * (FN * 32 * sizeof(T) + 16);  // a wave's part of LDS for its results
+  static_assert(WAVES * OWN + 4 * (2 * BT + 2 * BN) <= 5 * SLOT, "the results' LDS is the ring's");
   __shared__ __align__(16) int8_t lds[5 * SLOT];
   auto swz = [](uint32_t row) { return (row >> 1) & 7u; };
   const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -659,12 +682,7 @@ __global__ __launch_bounds__(64 * KW, 4) void k_i8_direct(I8Args a, uint32_t til
       const float sw = a.sw && in ? a.sw[ch + k] : 1.0f, b = a.bias && in ? a.bias[ch + k] : 0.0f;
       v[k] = zero ? (T)0 : finish<T>(sum[k], sx * sw, b, a.relu);
     }
-    T* y = (T*)a.y + (size_t)t * a.ld_y + n;
-    if (n + 4 <= a.n_out) {
-      __builtin_memcpy(y, v, sizeof(v));
-    } else {
-      for (uint32_t k = 0; k < a.n_out - n; k++) y[k] = v[k];
-    }
+    store4((T*)a.y + (size_t)t * a.ld_y + n, a.n_out - n, v);
   };
 #pragma unroll
   for (int i = 0; i < FN; i++)
@@ -679,6 +697,66 @@ __global__ __launch_bounds__(64 * KW, 4) void k_i8_direct(I8Args a, uint32_t til
 #pragma unroll
     for (int k = 1; k < KW; k++) sum += sums[k][sq][lane];
     put(sq / FT, sq % FT, sum);
+  }
+}
+
+// ------------------------------------------------------------ short rows, many of them
+// A small layer over a whole data set: a wave keeps the weights, scales and
+// biases of all 16 FN channels in registers and goes over the tokens, TILES of 16
+// at a time, their rows read once, straight to fragments.  H: halves of 64 bytes
+// that a row has.  Bound by memory, once the launch's own 2 us are past: 100003 x
+// 64 to 32 integers 5.0 us (19 MB), 9.0 through the tiles in LDS, whose blocks
+// have one step each; 500000 x 64 to 32: 16.4.  Results of 4 bytes leave around
+// the caches, which would write them out only at the end (7.6 us); 8-byte pieces
+// do not (4.8 us; 5.2 around the caches, 15 and 35 with 48 channels, 500000 rows).
+template <class T, bool BYTES, int H, int FN>
+__global__ __launch_bounds__(256) void k_i8_thin(I8Args a) {
+  constexpr int TILES = 2;
+  const uint32_t lane = threadIdx.x & 63, fr = lane & 15, c = lane >> 4;
+  Chunk part[H];
+  v4i wf[FN][H];
+  float sw[FN][4], bias[FN][4];
+#pragma unroll
+  for (int h = 0; h < H; h++) part[h] = last_chunk(64 * h + 16 * c, a.n_in);
+#pragma unroll
+  for (int i = 0; i < FN; i++) {
+    const uint32_t row = i * 16 + fr, n = i * 16 + 4 * c;
+    const int8_t* w = a.w + (size_t)(row < a.n_out ? row : a.n_out - 1) * a.ld_w;
+#pragma unroll
+    for (int h = 0; h < H; h++) wf[i][h] = load16_end<BYTES>(w + part[h].at);
+#pragma unroll
+    for (uint32_t k = 0; k < 4; k++) {
+      const bool in = n + k < a.n_out;
+      sw[i][k] = a.sw && in ? a.sw[n + k] : 1.0f, bias[i][k] = a.bias && in ? a.bias[n + k] : 0.0f;
+    }
+  }
+  const uint32_t wave = threadIdx.x >> 6, stride = gridDim.x * 4 * TILES * 16;
+  for (uint32_t t0 = (blockIdx.x * 4 + wave) * TILES * 16; t0 < a.rows; t0 += stride) {
+    v4i xf[TILES][H];
+    float sx[TILES];
+#pragma unroll
+    for (int j = 0; j < TILES; j++) {
+      const uint32_t t = t0 + j * 16 + fr, r = t < a.rows ? t : a.rows - 1;
+#pragma unroll
+      for (int h = 0; h < H; h++) xf[j][h] = load16_end<BYTES>(a.x + (size_t)r * a.ld_x + part[h].at) & part[h].mask;
+      sx[j] = a.sx ? a.sx[r] : 1.0f;
+    }
+#pragma unroll
+    for (int j = 0; j < TILES; j++) {
+      const uint32_t t = t0 + j * 16 + fr;
+#pragma unroll
+      for (int i = 0; i < FN; i++) {
+        v4i acc = {};
+#pragma unroll
+        for (int h = 0; h < H; h++) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[i][h], xf[j][h], acc, 0, 0, 0);
+        const uint32_t n = i * 16 + 4 * c;
+        if (t >= a.rows || n >= a.n_out) continue;
+        T v[4];
+#pragma unroll
+        for (int k = 0; k < 4; k++) v[k] = finish<T>(acc[k], sx[j] * sw[i][k], bias[i][k], a.relu);
+        store4<sizeof(T) == 4>((T*)a.y + (size_t)t * a.ld_y + n, a.n_out - n, v);
+      }
+    }
   }
 }
 
@@ -753,6 +831,12 @@ static int choose_tile(const I8Args& a, bool grouped, bool odd_rows, bool bytes)
   return best;
 }
 
+// Products for k_i8_thin: at 64 channels a token's rows in LDS are worth their
+// steps (100003 x 64 to 64 integers: 9.2 us there, 12.1 here; to 48: 9.2 and 6.8),
+// and under some thousand rows the tiles that split the channels are level with
+// it (4096 x 64 to 32: 3.0 and 3.0; 512: 2.8 and 3.0).
+constexpr uint32_t THIN_ROWS = 4096, THIN_OUT = 48, THIN_IN = 128;
+
 template <class T, bool GROUPED>
 static int launch_product(zk_context* ctx, const I8Args& a, hipStream_t st) {
   const char* name = GROUPED ? "i8_matmul_experts" : "i8_matmul";
@@ -763,6 +847,26 @@ static int launch_product(zk_context* ctx, const I8Args& a, hipStream_t st) {
   }
   const size_t rows_at = (uintptr_t)a.x | (uintptr_t)a.w | a.ld_x | a.ld_w;
   const bool odd = (rows_at | a.n_in) % 16 != 0, bytes = rows_at % 4 != 0;
+  if constexpr (!GROUPED) {
+    if (a.n_in <= THIN_IN && a.rows >= THIN_ROWS && a.n_out <= THIN_OUT) {
+      auto go = [&](auto kernel) -> int {
+        const uint32_t blocks = cdiv(a.rows, 128);
+        ZK_LAUNCH(ctx, st, name, kernel, dim3(blocks < 2048 ? blocks : 2048), dim3(256), 0, a);
+        return ZK_OK;
+      };
+      auto by_out = [&](auto by, auto h) -> int {
+        constexpr bool B = decltype(by)::value;
+        constexpr int H = decltype(h)::value;
+        if (a.n_out <= 16) return go(k_i8_thin<T, B, H, 1>);
+        if (a.n_out <= 32) return go(k_i8_thin<T, B, H, 2>);
+        return go(k_i8_thin<T, B, H, 3>);
+      };
+      auto by_in = [&](auto by) -> int {
+        return a.n_in <= 64 ? by_out(by, std::integral_constant<int, 1>()) : by_out(by, std::integral_constant<int, 2>());
+      };
+      return bytes ? by_in(std::true_type()) : by_in(std::false_type());
+    }
+  }
   const int c = choose_tile(a, GROUPED, odd, bytes);
   auto go = [&](auto kernel, uint32_t threads) -> int {
     // row tiles of the grouped form: whole ones, and a part of one for each
@@ -921,6 +1025,7 @@ __global__ __launch_bounds__(THREADS* ROWS) void k_i8_quantize(const T* __restri
     if (cols - at >= Vec<T>::N) {
       __builtin_memcpy(out + at, b, sizeof(b));
     } else {
+#pragma unroll
       for (uint32_t i = 0; i < Vec<T>::N; i++)
         if (i < cols - at) out[at + i] = b[i];
     }
@@ -1051,7 +1156,9 @@ __global__ __launch_bounds__(512) void k_i8_few(I8Args a, const X* __restrict__ 
       if (a.n_in - at >= Vec<X>::N) {
         __builtin_memcpy(out + at, b, sizeof(b));
       } else {
-        for (uint32_t i = 0; i < a.n_in - at; i++) out[at + i] = b[i];
+#pragma unroll
+        for (uint32_t i = 0; i < Vec<X>::N; i++)
+          if (i < a.n_in - at) out[at + i] = b[i];
       }
     };
     const bool again = at_once < a.rows;  // held is the last of several rows
@@ -1107,12 +1214,7 @@ __global__ __launch_bounds__(512) void k_i8_few(I8Args a, const X* __restrict__ 
     const bool in = n + k < a.n_out;
     v[k] = finish<T>(sum[k], sx * (a.sw && in ? a.sw[n + k] : 1.0f), a.bias && in ? a.bias[n + k] : 0.0f, a.relu);
   }
-  T* y = (T*)a.y + (size_t)fr * a.ld_y + n;
-  if (n + 4 <= a.n_out) {
-    __builtin_memcpy(y, v, sizeof(v));
-  } else {
-    for (uint32_t k = 0; k < a.n_out - n; k++) y[k] = v[k];
-  }
+  store4((T*)a.y + (size_t)fr * a.ld_y + n, a.n_out - n, v);
 }
 
 static bool few_rows(size_t rows, size_t n_in) {

@@ -26,6 +26,7 @@ __device__ __forceinline__ Vec<T> row_load(const T* p, uint32_t left) {
     const row16 v = ONCE ? __builtin_nontemporal_load((const row16*)p) : *(const row16*)p;
     __builtin_memcpy(&r, &v, 16);
   } else {
+#pragma unroll
     for (uint32_t i = 0; i < Vec<T>::N; i++) r.v[i] = i < left ? p[i] : (T)0.0f;
   }
   return r;
@@ -39,6 +40,7 @@ __device__ __forceinline__ void row_store(T* p, uint32_t left, const Vec<T>& r) 
     if (ONCE) __builtin_nontemporal_store(v, (row16*)p);
     else *(row16*)p = v;
   } else {
+#pragma unroll
     for (uint32_t i = 0; i < Vec<T>::N; i++)
       if (i < left) p[i] = r.v[i];
   }

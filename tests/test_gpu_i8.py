@@ -134,6 +134,35 @@ def test_large_tiles(ctx, rows, n_out, n_in):
     near(y.read(), v, np.abs(v), "bf16")
 
 
+# many short rows: one and two halves of 64 bytes, at whole words and not, up to
+# three times 16 channels
+@pytest.mark.parametrize("rows,n_out,n_in,pad,kind", [(4096, 32, 64, 0, "i32"), (5001, 10, 64, 0, "f32"),
+                                                      (5001, 48, 128, 0, "bf16"), (4103, 47, 100, 0, "f32"),
+                                                      (4111, 33, 17, 0, "f16"), (4096, 16, 16, 5, "i32"),
+                                                      (4100, 3, 127, 0, "bf16"), (4099, 31, 65, 2, "i32"),
+                                                      (300001, 1, 33, 0, "i32"), (270000, 21, 63, 1, "f32"),
+                                                      (4095, 48, 128, 0, "i32"), (4096, 49, 64, 0, "i32")])
+def test_many_short_rows(ctx, rows, n_out, n_in, pad, kind):
+    rng = np.random.default_rng([rows, n_out, n_in])
+    x = rng.integers(-128, 128, (rows, n_in), dtype=np.int8)
+    w = rng.integers(-128, 128, (n_out, n_in), dtype=np.int8)
+    say("[i8 short rows]", kind, rows, n_out, n_in, pad)
+    y = Result(ctx, rows, n_out, kind, ld=n_out + pad)
+    padded = lambda a: ctx.upload(np.pad(a, ((0, 0), (0, pad)), constant_values=99))  # noqa: E731
+    want = wide_sums(x, w)
+    if kind == "i32":
+        ctx.i8_matmul(padded(x), padded(w), rows, n_out, n_in, y.at, ld_x=n_in + pad, ld_w=n_in + pad, ld_y=n_out + pad,
+                      relu=True)
+        assert np.array_equal(y.read(), np.maximum(want, 0))
+        return
+    sx, sw = (np.exp(rng.normal(-6, 0.5, n)).astype(np.float32) for n in (rows, n_out))
+    b = rng.normal(0, 1, n_out).astype(np.float32)
+    ctx.i8_matmul(padded(x), padded(w), rows, n_out, n_in, y.at, TYPES[kind], x_scale=ctx.upload(sx), w_scale=ctx.upload(sw),
+                  bias=ctx.upload(b), ld_x=n_in + pad, ld_w=n_in + pad, ld_y=n_out + pad)
+    v = want * (sx.astype(np.float64)[:, None] * sw.astype(np.float64))
+    near(y.read(), v + b, np.abs(v) + np.abs(b), kind)
+
+
 def test_longest_sum(ctx):
     """The largest sum of the longest row: 2^14 * 131071 < 2^31."""
     n_in = 131071
@@ -272,6 +301,7 @@ def test_quantize_edges(ctx, kind, cols):
                                                  (4, 33, 300, 1), (9, 200, 1000, 8), (70, 130, 515, 0),
                                                  (300, 256, 1024, 0), (5, 8200, 9000, 0), (16, 8195, 2900, 1),
                                                  (3, 70, 15000, 0), (16, 40, 3000, 2), (17, 50, 2000, 0),
+                                                 (3, 8200, 16200, 0), (16, 8193, 2900, 0),
                                                  (2, 30, 16, 0), (2, 30, 15, 0)])
 def test_linear(ctx, kind, out, rows, n_out, n_in, pad):
     """The linear layer is the product over its rows' quantized values: compared
