@@ -17,9 +17,15 @@ namespace zk {
 
 // ------------------------------------------------------------ sort
 constexpr int SORT_THREADS = 1024, SORT_WAVES = SORT_THREADS / 64;
-constexpr size_t SORT_ONE = 16384;    // pairs that one block sorts alone
+// Few pairs are sorted by one block, whose time grows with them (128 experts:
+// 66 pairs 3.2 us, 2048 4.6, 8192 11.1, 16384 19.6); more by blocks of 2048 pairs or
+// more, in two launches, the second of which adds up the blocks' counts (16385:
+// 1.6 + 6.2 us, 65536: 2.6 + 7.0, 2^20: 4.8 + 18; a launch costs the host 4 us).
+// Bound by the chain launch, loads, counts, scan, loads; the pairs' own bytes are
+// nothing beside it (65536: 0.8 MB).
+constexpr size_t SORT_ONE = 8192;     // pairs that one block sorts alone
 constexpr size_t SORT_SEGMENT = 2048; // least pairs of a block otherwise
-constexpr size_t SORT_BLOCKS = 128;
+constexpr size_t SORT_BLOCKS = 128;   // (more counts to add up cost more than they save)
 
 struct SortPlan {
   uint32_t blocks, segment;
@@ -152,6 +158,9 @@ __global__ __launch_bounds__(SORT_THREADS) void k_sort_place(const int32_t* __re
 // ------------------------------------------------------------ rows
 // out[p] = x[order[p] / slots], zeros where order[p] names no token: 2^log_w
 // threads a row, so that short rows fill a wave.  STREAM: see streams().
+// Bound by memory: 65536 rows of 4 KB from 16384 in 70 us, 335 MB at 4.8 TB/s
+// (55 us at a copy's 6.05: a token's four rows are wanted far apart in the sorted
+// order, so that some are fetched again).
 template <class T, bool STREAM>
 __global__ __launch_bounds__(256) void k_gather(const T* __restrict__ x, size_t ld_x,
                                                 const int32_t* __restrict__ order, uint32_t rows, uint32_t tokens,
@@ -172,7 +181,8 @@ __global__ __launch_bounds__(256) void k_gather(const T* __restrict__ x, size_t 
 
 // out[t] = sum_j w[t, j] y[place[t, j]], j ascending, in 32 bits; 2^log_w threads
 // a token.  Four slots' indexes, then their rows, are loaded together: a token's
-// slots are one chain of two loads per four, not per slot.
+// slots are one chain of two loads per four, not per slot.  Bound by memory: 16384
+// tokens' four rows of 4 KB in 53 us, 6.3 TB/s.
 template <class T, bool STREAM>
 __global__ __launch_bounds__(256) void k_combine(const T* __restrict__ y, size_t ld_y,
                                                  const int32_t* __restrict__ place, const float* __restrict__ weight,
@@ -183,39 +193,41 @@ __global__ __launch_bounds__(256) void k_combine(const T* __restrict__ y, size_t
   if (t >= tokens) return;
   const uint32_t pieces = pieces_of<T>(cols);
   for (uint32_t c = threadIdx.x & ((1u << log_w) - 1); c < pieces; c += 1u << log_w) {
-  const uint32_t at = piece<T>(c, cols);
-  float s[Vec<T>::N] = {};
-  for (uint32_t j0 = 0; j0 < slots; j0 += K) {
-    uint32_t p[K];
-    float w[K];
-    Vec<T> v[K];
+    const uint32_t at = piece<T>(c, cols);
+    float s[Vec<T>::N] = {};
+    for (uint32_t j0 = 0; j0 < slots; j0 += K) {
+      uint32_t p[K];
+      float w[K];
+      Vec<T> v[K];
 #pragma unroll
-    for (int k = 0; k < K; k++) {
-      const size_t pair = (size_t)t * slots + j0 + k;
-      const bool on = j0 + k < slots;
-      p[k] = on ? (uint32_t)place[pair] : rows;
-      w[k] = on && weight ? weight[pair] : 1.0f;
-    }
-#pragma unroll
-    for (int k = 0; k < K; k++)
-      if (p[k] < rows) v[k] = row_load<T, STREAM>(y + (size_t)p[k] * ld_y + at, cols - at);
-#pragma unroll
-    for (int k = 0; k < K; k++)
-      if (p[k] < rows) {
-#pragma unroll
-        for (uint32_t e = 0; e < Vec<T>::N; e++) s[e] += w[k] * (float)v[k].v[e];
+      for (int k = 0; k < K; k++) {
+        const size_t pair = (size_t)t * slots + j0 + k;
+        const bool on = j0 + k < slots;
+        p[k] = on ? (uint32_t)place[pair] : rows;
+        w[k] = on && weight ? weight[pair] : 1.0f;
       }
-  }
-  Vec<T> r;
 #pragma unroll
-  for (uint32_t e = 0; e < Vec<T>::N; e++) r.v[e] = (T)s[e];
-  row_store<T, STREAM>(out + (size_t)t * ld_out + at, cols - at, r);
+      for (int k = 0; k < K; k++)
+        if (p[k] < rows) v[k] = row_load<T, STREAM>(y + (size_t)p[k] * ld_y + at, cols - at);
+#pragma unroll
+      for (int k = 0; k < K; k++)
+        if (p[k] < rows) {
+#pragma unroll
+          for (uint32_t e = 0; e < Vec<T>::N; e++) s[e] += w[k] * (float)v[k].v[e];
+        }
+    }
+    Vec<T> r;
+#pragma unroll
+    for (uint32_t e = 0; e < Vec<T>::N; e++) r.v[e] = (T)s[e];
+    row_store<T, STREAM>(out + (size_t)t * ld_out + at, cols - at, r);
   }
 }
 
 // dy[place[t, j]] = w[t, j] g[t], dw[t, j] = <g[t], y[place[t, j]]>; rows of dy
 // that hold no pair get zeros.  A block has a token, so that g's row is read
-// once and each dot product ends in one block; four slots go together.
+// once and each dot product ends in one block, whose order is fixed; four slots
+// go together.  Bound by memory: 16384 tokens' four rows of 4 KB in 98 us, 604 MB
+// at 6.2 TB/s.
 template <class T, bool STREAM>
 __global__ __launch_bounds__(256) void k_combine_grad(const T* __restrict__ g, size_t ld_g, const T* __restrict__ y,
                                                       size_t ld_y, const int32_t* __restrict__ order,

@@ -268,7 +268,8 @@ int zk_synthetic_r1cs(int num_constraints, int num_public, int num_inputs, uint6
  * in 32-bit floats, rounded once to y_type; relu != 0 replaces what is below
  * zero by zero (a NaN stays).  d_x_scale (rows), d_w_scale and d_bias (n_out)
  * may be NULL (1, 1 and 0).  ld_* are row strides in elements, at least the
- * row's length; rows of x and w may start at any byte.
+ * row's length; rows of x and w may start at any byte (they may be read in
+ * whole aligned 4-byte words, whose other bytes do not matter).
  * zk_i8_quantize: scale[t] = max_k |x[t][k]| / 127, q[t][k] = the integer
  * nearest to 127 x[t][k] / max_k |x[t][k]| (ties to even).  A row of zeros
  * has scale 0 and zeros; a row that holds an infinity or a NaN has scale NaN
@@ -282,7 +283,8 @@ int zk_synthetic_r1cs(int num_constraints, int num_public, int num_inputs, uint6
  * bias + e * n_out; row p takes row order[p] / slots of x (tokens rows) and
  * its scale, or row p itself when d_order is NULL.  Rows that belong to no
  * expert, or whose order names no token, become zeros.  offsets[0] is 0 and
- * the offsets do not fall.
+ * the offsets do not fall.  At most 2^22 rows; ZK_ERR_SIZE also where rows and
+ * n_out make more than 2^22 tiles.
  * None of these allocates, waits or uses memory of the context, so calls on
  * different streams do not touch each other.  y may not overlap an input.
  * stream may be hipStreamLegacy (the default stream of a program that does

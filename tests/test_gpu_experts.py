@@ -45,7 +45,7 @@ def sort(ctx, e, experts):
     return off.read()[0], order.read()[0], place.read()[0]
 
 
-@pytest.mark.parametrize("pairs", [0, 1, 2, 63, 64, 65, 1000, 1024, 1025, 16384, 16385, 40001, 300000])
+@pytest.mark.parametrize("pairs", [0, 1, 2, 63, 64, 65, 1000, 1024, 1025, 8192, 8193, 16384, 16385, 40001, 300000])
 @pytest.mark.parametrize("experts", [1, 2, 8, 63, 64, 1000, 1024])
 def test_sort(ctx, pairs, experts):
     rng = np.random.default_rng([pairs, experts])
