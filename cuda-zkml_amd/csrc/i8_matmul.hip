@@ -3,7 +3,7 @@
 // matrix cores, with the scales that tie its integers to the real-valued model.
 //
 //   acc[t,n] = sum_k x[t,k] w[n,k]                 int32, exact
-//   y[t,n]   = act(float(acc) (sx[t] sw[n]) + b[n])  or acc itself
+//   y[t,n]   = act((float(acc) sx[t]) sw[n] + b[n])  or acc itself
 //
 // A product of two int8 is at most 2^14, so acc is exact for n_in <= 131071.
 // The grouped form takes its weights by expert: rows offsets[e] to
@@ -103,14 +103,30 @@ __device__ __forceinline__ void load_pair(const int8_t* p, uint32_t c, v4i (&out
     out[1] = move_down(out[1], next, by);
   }
 }
+// A token's scale as the results take it: s * up, where up is a power of two that
+// keeps a sum below 2^31 times s inside the 32-bit floats (row maxima from 10^31 on
+// have such scales, and a channel's scale may bring them back).
+struct TokenScale {
+  float s, up;
+};
+__device__ __forceinline__ TokenScale token_scale(float sx) {
+  const bool big = fabsf(sx) >= 0x1p96f;
+  return TokenScale{big ? sx * 0x1p-32f : sx, big ? 0x1p32f : 1.0f};
+}
+// (float(acc) sx) sw + b, each operation rounded to 32 bits, so that the result is
+// what the elementary operations in this order give bit for bit; times up is exact,
+// and so the fused operation rounds once, as the sum alone does.  (sx sw first could
+// leave the 32-bit floats where the result does not.)
 template <class T>
-__device__ __forceinline__ T finish(int acc, float s, float b, int relu) {
-  float f = (float)acc * s + b;
+__device__ __forceinline__ T finish(int acc, const TokenScale& x, float sw, float b, int relu) {
+  float f = fmaf((float)acc * x.s * sw, x.up, b);
+  // (else the compiler takes an instruction that rounds the f16 from the exact sum)
+  if constexpr (std::is_same<T, _Float16>::value) asm("" : "+v"(f));
   if (relu && f < 0.0f) f = 0.0f;  // a NaN stays
   return (T)f;
 }
 template <>
-__device__ __forceinline__ int finish<int>(int acc, float, float, int relu) {
+__device__ __forceinline__ int finish<int>(int acc, const TokenScale&, float, float, int relu) {
   return relu && acc < 0 ? 0 : acc;
 }
 
@@ -317,7 +333,7 @@ __device__ __forceinline__ void put_results(const I8Args& a, const v16i (&acc)[F
   const float *sw = f + BT + c0, *bias = sw + BN, *has = f + BT + 2 * BN;
 #pragma unroll
   for (int j = 0; j < FT; j++) {
-    const float sx = f[t0 + j * 32 + fr];
+    const TokenScale sx = token_scale(f[t0 + j * 32 + fr]);
     const bool zero = GROUPED && has[t0 + j * 32 + fr] == 0.0f;
 #pragma unroll
     for (int i = 0; i < FN; i++)
@@ -327,7 +343,7 @@ __device__ __forceinline__ void put_results(const I8Args& a, const v16i (&acc)[F
 #pragma unroll
         for (int k = 0; k < 4; k++) {
           const uint32_t c = i * 32 + 8 * q + 4 * hi + k;
-          v[k] = zero ? (T)0 : finish<T>(acc[i][j][4 * q + k], sx * sw[c], bias[c], a.relu);
+          v[k] = zero ? (T)0 : finish<T>(acc[i][j][4 * q + k], sx, sw[c], bias[c], a.relu);
         }
         __builtin_memcpy(own + fr * LD + (i * 32 + 8 * q + 4 * hi) * sizeof(T), v, sizeof(v));
       }
@@ -688,14 +704,14 @@ __global__ __launch_bounds__(64 * KW, 4) void k_i8_direct(I8Args a, uint32_t til
     const uint32_t t = r0 + j * 16 + fr, n = n0 + i * 16 + 4 * c;
     if (t >= r1 || n >= a.n_out) return;
     const bool zero = GROUPED && src[j] < 0;
-    const float sx = a.sx && !zero ? a.sx[src[j]] : 1.0f;
+    const TokenScale sx = token_scale(a.sx && !zero ? a.sx[src[j]] : 1.0f);
     const size_t ch = (none ? 0 : (size_t)e * a.n_out) + n;
     T v[4];
 #pragma unroll
     for (uint32_t k = 0; k < 4; k++) {
       const bool in = n + k < a.n_out;
       const float sw = a.sw && in ? a.sw[ch + k] : 1.0f, b = a.bias && in ? a.bias[ch + k] : 0.0f;
-      v[k] = zero ? (T)0 : finish<T>(sum[k], sx * sw, b, a.relu);
+      v[k] = zero ? (T)0 : finish<T>(sum[k], sx, sw, b, a.relu);
     }
     store4((T*)a.y + (size_t)t * a.ld_y + n, a.n_out - n, v);
   };
@@ -748,13 +764,13 @@ __global__ __launch_bounds__(256) void k_i8_thin(I8Args a) {
   const uint32_t wave = threadIdx.x >> 6, stride = gridDim.x * 4 * TILES * 16;
   for (uint32_t t0 = (blockIdx.x * 4 + wave) * TILES * 16; t0 < a.rows; t0 += stride) {
     v4i xf[TILES][H];
-    float sx[TILES];
+    TokenScale sx[TILES];
 #pragma unroll
     for (int j = 0; j < TILES; j++) {
       const uint32_t t = t0 + j * 16 + fr, r = t < a.rows ? t : a.rows - 1;
 #pragma unroll
       for (int h = 0; h < H; h++) xf[j][h] = load16_end<BYTES>(a.x + (size_t)r * a.ld_x + part[h].at) & part[h].mask;
-      sx[j] = a.sx ? a.sx[r] : 1.0f;
+      sx[j] = token_scale(a.sx ? a.sx[r] : 1.0f);
     }
 #pragma unroll
     for (int j = 0; j < TILES; j++) {
@@ -768,7 +784,7 @@ __global__ __launch_bounds__(256) void k_i8_thin(I8Args a) {
         if (t >= a.rows || n >= a.n_out) continue;
         T v[4];
 #pragma unroll
-        for (int k = 0; k < 4; k++) v[k] = finish<T>(acc[k], sx[j] * sw[i][k], bias[i][k], a.relu);
+        for (int k = 0; k < 4; k++) v[k] = finish<T>(acc[k], sx[j], sw[i][k], bias[i][k], a.relu);
         store4<sizeof(T) == 4>((T*)a.y + (size_t)t * a.ld_y + n, a.n_out - n, v);
       }
     }
@@ -798,7 +814,8 @@ __global__ __launch_bounds__(256) void k_i8_short(I8Args a) {
     if (s >= 0) {
       int acc = 0;
       for (uint32_t k = 0; k < a.n_in; k++) acc += (int)a.x[(size_t)s * a.ld_x + k] * (int)a.w[ch * a.ld_w + k];
-      v = finish<T>(acc, (a.sx ? a.sx[s] : 1.0f) * (a.sw ? a.sw[ch] : 1.0f), a.bias ? a.bias[ch] : 0.0f, a.relu);
+      v = finish<T>(acc, token_scale(a.sx ? a.sx[s] : 1.0f), a.sw ? a.sw[ch] : 1.0f, a.bias ? a.bias[ch] : 0.0f,
+                    a.relu);
     }
     ((T*)a.y)[(size_t)p * a.ld_y + n] = v;
   }
@@ -1227,12 +1244,12 @@ __global__ __launch_bounds__(512) void k_i8_few(I8Args a, const X* __restrict__ 
   for (uint32_t k = 1; k < KW; k++) sum += sums[k][wave][lane];
   const uint32_t n = n0 + wave * 16 + 4 * c;
   if (fr >= a.rows || n >= a.n_out) return;
-  const float sx = scale[fr];
+  const TokenScale sx = token_scale(scale[fr]);
   T v[4];
 #pragma unroll
   for (uint32_t k = 0; k < 4; k++) {
     const bool in = n + k < a.n_out;
-    v[k] = finish<T>(sum[k], sx * (a.sw && in ? a.sw[n + k] : 1.0f), a.bias && in ? a.bias[n + k] : 0.0f, a.relu);
+    v[k] = finish<T>(sum[k], sx, a.sw && in ? a.sw[n + k] : 1.0f, a.bias && in ? a.bias[n + k] : 0.0f, a.relu);
   }
   store4((T*)a.y + (size_t)fr * a.ld_y + n, a.n_out - n, v);
 }

@@ -264,9 +264,10 @@ int zk_synthetic_r1cs(int num_constraints, int num_public, int num_inputs, uint6
  * zk_i8_matmul: acc[t][n] = sum_k x[t][k] w[n][k] (int8, exact in int32;
  * n_in <= 131071, n_out <= 2^26), then
  *   y_type ZK_I32: y = acc (no scales, no bias);
- *   else           y = float(acc) * (x_scale[t] * w_scale[n]) + bias[n],
- * in 32-bit floats, rounded once to y_type; relu != 0 replaces what is below
- * zero by zero (a NaN stays).  d_x_scale (rows), d_w_scale and d_bias (n_out)
+ *   else           y = (float(acc) * x_scale[t]) * w_scale[n] + bias[n],
+ * each operation rounded to 32-bit floats in this order (float(acc) *
+ * x_scale[t] without leaving their range above), then once to y_type; relu !=
+ * 0 replaces what is below zero by zero (a NaN stays).  d_x_scale (rows), d_w_scale and d_bias (n_out)
  * may be NULL (1, 1 and 0).  ld_* are row strides in elements, at least the
  * row's length; rows of x and w may start at any byte (they may be read in
  * whole aligned 4-byte words, whose other bytes do not matter).

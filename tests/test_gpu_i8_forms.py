@@ -1,0 +1,111 @@
+"""GPU tests of what an 8-bit layer makes of its sums (cuda-zkml_amd/csrc/i8_matmul.hip):
+(float(acc) * x_scale) * w_scale + bias with each operation rounded to 32 bits, then
+once to the result's type.  numpy's float32 operations in the same order give the
+same bits, so nothing here has a tolerance.
+"""
+import numpy as np
+import pytest
+
+import zkml_amd as z
+from i8_helpers import TYPES, Result, matrix, words
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def ctx():
+    return z.Context(0)
+
+
+def say(*a):
+    print(*a, flush=True)
+
+
+def elementary(acc, sx, sw, b, relu, kind):
+    """The definition in numpy's float32.  Token scales from 2^96 on: a power of two
+    moved to the channels' scales, which changes no rounding and keeps float(acc) sx
+    inside the 32-bit floats."""
+    up = np.where(np.abs(sx) >= 2.0**96, np.float32(2.0**32), np.float32(1))
+    with np.errstate(over="ignore", under="ignore"):
+        y = (acc.astype(np.float32) * (sx / up)[:, None]) * (sw[None, :] * up[:, None]) + b
+        if relu:
+            y = np.where(y < 0, np.float32(0), y)
+        assert y.dtype == np.float32
+        return words(y, kind)
+
+
+# rows, n_out, n_in: rows under 16 bytes, many short rows, few rows, rows at whole
+# 16 bytes and not
+FORMS = [(5, 7, 8), (5000, 32, 64), (9, 40, 200), (1000, 600, 512), (1000, 600, 513)]
+# the scales' logarithms: ordinary ones; a product below the 32-bit floats, whose
+# results are inside; one above them, where only sums of zero are finite; a token's
+# scale near either end that the channel's brings back
+SCALES = {"ordinary": (-6, -6), "below": (-69, -28), "above": (69, 27), "token high": (80, -70), "token low": (-86, 70)}
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("scales", list(SCALES))
+@pytest.mark.parametrize("rows,n_out,n_in", FORMS)
+def test_results_are_those_of_the_elementary_operations(ctx, kind, scales, rows, n_out, n_in):
+    rng = np.random.default_rng([rows, n_out, n_in, len(scales)])
+    x = rng.integers(-127, 128, (rows, n_in)).astype(np.int8)
+    w = rng.integers(-127, 128, (n_out, n_in)).astype(np.int8)
+    x[1] = 0  # sums of zero are zero whatever the scales are
+    acc = x.astype(np.int64) @ w.astype(np.int64).T
+    lx, lw = SCALES[scales]
+    sx, sw = (np.exp(rng.normal(m, 0.5, n)).astype(np.float32) for m, n in ((lx, rows), (lw, n_out)))
+    b = rng.normal(0, 1, n_out).astype(np.float32) if scales == "ordinary" else np.zeros(n_out, dtype=np.float32)
+    say("[i8 forms]", kind, scales, rows, n_out, n_in)
+    for bias, relu in ((None, False), (b, True)):
+        y = Result(ctx, rows, n_out, kind)
+        ctx.i8_matmul(matrix(ctx, x), matrix(ctx, w), rows, n_out, n_in, y.at, TYPES[kind], x_scale=ctx.upload(sx),
+                      w_scale=ctx.upload(sw), bias=None if bias is None else ctx.upload(bias), relu=relu)
+        want = elementary(acc, sx, sw, np.float32(0) if bias is None else bias, relu, kind)
+        assert np.array_equal(y.read(), want)
+
+
+@pytest.mark.parametrize("rows", [3, 40])
+def test_linear_at_the_ends_of_the_range(ctx, rows):
+    """Rows near the largest 32-bit float and near the smallest, and channels that
+    bring them back: the results are those of the quantized rows."""
+    rng = np.random.default_rng(rows)
+    n_out, n_in = 50, 300
+    for size, back in ((2e38, -76), (1e-34, 66)):
+        x = (rng.uniform(-1, 1, (rows, n_in)) * size).astype(np.float32)
+        w = rng.integers(-127, 128, (n_out, n_in)).astype(np.int8)
+        sw = np.exp(rng.normal(back, 0.5, n_out)).astype(np.float32)
+        xd, q, s = matrix(ctx, x), Result(ctx, rows, n_in, "i8"), Result(ctx, 1, rows, "f32")
+        ctx.i8_quantize(xd, z.F32, rows, n_in, q.at, s.at)
+        y = Result(ctx, rows, n_out, "f32")
+        say("[i8 linear ends]", rows, size)
+        ctx.i8_linear(xd, z.F32, matrix(ctx, w), ctx.upload(sw), rows, n_out, n_in, y.at, z.F32,
+                      ctx.alloc(ctx.i8_linear_work(rows, n_in)))
+        got = y.read()
+        want = elementary(q.read().astype(np.int64) @ w.astype(np.int64).T, s.read()[0], sw, np.float32(0), False, "f32")
+        assert np.array_equal(got, want) and np.isfinite(got).all() and got.any()
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("tokens,slots,experts,n_out,n_in", [(5, 2, 4, 7, 8), (5, 2, 4, 40, 200), (900, 2, 3, 300, 272)])
+def test_experts_results_are_those_of_the_elementary_operations(ctx, kind, tokens, slots, experts, n_out, n_in):
+    rng = np.random.default_rng([tokens, n_out, n_in])
+    rows = tokens * slots
+    e = np.sort(rng.integers(0, experts, rows))
+    offsets = np.searchsorted(e, np.arange(experts + 1)).astype(np.int32)
+    order = rng.permutation(rows).astype(np.int32)
+    x = rng.integers(-127, 128, (tokens, n_in)).astype(np.int8)
+    w = rng.integers(-127, 128, (experts, n_out, n_in)).astype(np.int8)
+    for lx, lw in SCALES.values():
+        sx = np.exp(rng.normal(lx, 0.5, tokens)).astype(np.float32)
+        sw = np.exp(rng.normal(lw, 0.5, (experts, n_out))).astype(np.float32)
+        y = Result(ctx, rows, n_out, kind)
+        say("[i8 experts forms]", kind, tokens, n_out, n_in, lx, lw)
+        ctx.i8_matmul_experts(matrix(ctx, x), matrix(ctx, w.reshape(-1, n_in)), ctx.upload(offsets), rows, experts,
+                              n_out, n_in, y.at, TYPES[kind], x_scale=ctx.upload(sx), w_scale=ctx.upload(sw),
+                              order=ctx.upload(order), slots=slots, tokens=tokens)
+        got = y.read()
+        for i in range(experts):
+            at = slice(offsets[i], offsets[i + 1])
+            t = order[at] // slots
+            acc = x[t].astype(np.int64) @ w[i].astype(np.int64).T
+            assert np.array_equal(got[at], elementary(acc, sx[t], sw[i], np.float32(0), False, kind)), i
