@@ -237,19 +237,19 @@ __global__ __launch_bounds__(256) void k_combine_grad(const T* __restrict__ g, s
                                                       float* __restrict__ dw) {
   constexpr int K = 4;
   __shared__ float part[K][4];
-  const uint32_t t = blockIdx.x, tid = threadIdx.x;
+  const uint32_t t = blockIdx.x, tid = threadIdx.x, pairs = gridDim.x * slots;
   const uint32_t pieces = pieces_of<T>(cols);
   for (uint32_t j0 = 0; j0 < slots; j0 += K) {
     const size_t pair = (size_t)t * slots + j0;
     uint32_t p[K];
     float w[K], s[K] = {};
-    bool empty[K];  // does position `pair + k` hold no pair?
+    bool empty[K];  // does position `pair + k` hold none of the pairs?
 #pragma unroll
     for (int k = 0; k < K; k++) {
       const bool on = j0 + k < slots;
       p[k] = on ? (uint32_t)place[pair + k] : rows;
       w[k] = on && weight ? weight[pair + k] : 1.0f;
-      empty[k] = on && pair + k < rows && order[pair + k] < 0;
+      empty[k] = on && pair + k < rows && (uint32_t)order[pair + k] >= pairs;
     }
     for (uint32_t c = tid; c < pieces; c += 256) {
       const uint32_t at = piece<T>(c, cols), left = cols - at;

@@ -219,6 +219,30 @@ def test_infinite_rows_stay_where_they_are(ctx):
     assert (got[0] == 2).all() and not got[1].any() and (got[2] == 2).all()
 
 
+@pytest.mark.parametrize("cols", [20, 700])
+@pytest.mark.parametrize("slots", [1, 2, 6])
+def test_positions_of_no_pair_get_no_gradient(ctx, cols, slots):
+    """A position whose order is -1, or any other value that names no pair, becomes
+    a row of zeros: as with a position that holds none."""
+    rng = np.random.default_rng([cols, slots])
+    tokens = 6
+    rows = tokens * slots
+    _, order, place = route(rng, tokens, slots, 4, 0.0)
+    dropped = rng.permutation(rows)[:5]
+    place[order[dropped]] = -1
+    order[dropped] = [-1, rows, rows + 1, 1 << 30, -2**31]
+    g, y = rng.normal(0, 1, (tokens, cols)).astype(np.float32), rng.normal(0, 1, (rows, cols)).astype(np.float32)
+    w = rng.random((tokens, slots)).astype(np.float32)
+    gy, gw = Result(ctx, rows, cols, "f32"), Result(ctx, tokens, slots, "f32")
+    ctx.experts_combine_grad(ctx.upload(g), ctx.upload(y), z.F32, cols, ctx.upload(order.astype(np.int32)),
+                             ctx.upload(place.astype(np.int32)), ctx.upload(w), rows, tokens, slots, gy.at, gw.at)
+    at = (order >= 0) & (order < rows)
+    pair = np.where(at, order, 0)
+    want = np.where(at[:, None], w.reshape(-1)[pair][:, None] * g[pair // slots], np.float32(0))
+    assert np.array_equal(gy.read(), want)
+    assert not gw.read()[place.reshape(tokens, slots) < 0].any()
+
+
 @pytest.mark.parametrize("tokens", [0, 3])
 def test_empty(ctx, tokens):
     d = ctx.upload(np.zeros(4096, dtype=np.int32))
