@@ -399,7 +399,13 @@ class Context:
     def i8_matmul_experts(self, x, w, offsets, rows, experts, n_out, n_in, y, y_type=I32, x_scale=None, w_scale=None,
                           bias=None, relu=False, order=None, slots=1, tokens=None, ld_x=None, ld_w=None, ld_y=None,
                           stream=None):
-        """i8_matmul with each expert's weights for its rows (zk_i8_matmul_experts)."""
+        """i8_matmul with each expert's weights for its rows (zk_i8_matmul_experts).
+        tokens: x's rows; with one slot a token it may be left out where they are as
+        many as y's."""
+        if order is not None and slots > 1 and tokens is None:
+            # neither rows nor rows // slots: with a part of the pairs, or more positions
+            # than pairs, it would lose tokens or let a bad order read past x
+            raise ZkError("zk_i8_matmul_experts: an order of several slots needs tokens, the number of x's rows")
         self._check(lib().zk_i8_matmul_experts(
             self.h, _dev(x), n_in if ld_x is None else ld_x, _dev(x_scale), rows if tokens is None else tokens,
             _dev(w), n_in if ld_w is None else ld_w, _dev(w_scale), _dev(bias), _dev(offsets), experts, _dev(order),
