@@ -40,6 +40,14 @@ static SortPlan sort_plan(size_t pairs) {
   return p;
 }
 
+// What a wave's lanes wrote to LDS before it, its other lanes read after it: all
+// lanes meet here, and the compiler moves no access across.  No instruction: one
+// wave's LDS accesses are in order.
+__device__ __forceinline__ void lanes_meet() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
 // Counts of one block's pairs by expert: tot[block][expert].
 __global__ __launch_bounds__(SORT_THREADS) void k_sort_count(const int32_t* __restrict__ expert, uint32_t pairs,
                                                              uint32_t experts, uint32_t segment,
@@ -72,8 +80,7 @@ __global__ __launch_bounds__(SORT_THREADS) void k_sort_place(const int32_t* __re
   const uint32_t lo = seg0 + wave * run;
   uint32_t hi = lo + run;
   if (hi > pairs) hi = pairs;
-  uint32_t* mine = cnt + wave * experts;
-  volatile uint32_t* next = mine;  // read and written by different lanes of the wave
+  uint32_t* mine = cnt + wave * experts;  // read and written by different lanes of the wave
   for (uint32_t e = tid; e < SORT_WAVES * experts; e += SORT_THREADS) cnt[e] = 0;
   if (tid < experts) base[tid] = sum[tid] = 0;
   __syncthreads();
@@ -140,9 +147,11 @@ __global__ __launch_bounds__(SORT_THREADS) void k_sort_place(const int32_t* __re
     }
     const uint32_t rank = (uint32_t)__popcll(same & ((1ull << lane) - 1));
     uint32_t first = 0;
-    // one wave's LDS accesses stay in order: every lane reads before any writes
-    if (e < experts) first = next[e];
-    if (e < experts && rank == 0) next[e] = first + (uint32_t)__popcll(same);
+    // every lane reads before any writes, and the next 64 pairs' lanes after it
+    if (e < experts) first = mine[e];
+    lanes_meet();
+    if (e < experts && rank == 0) mine[e] = first + (uint32_t)__popcll(same);
+    lanes_meet();
     if (i < hi) {
       int32_t p = -1;
       if (e < experts) {
