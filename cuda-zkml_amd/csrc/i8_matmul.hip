@@ -946,12 +946,16 @@ static int i8_dispatch(zk_context* ctx, const I8Args& a, int type, hipStream_t s
 }
 
 // ------------------------------------------------------------ rows to 8 bits
-// s = a / 127, q = rint(t / a) with t = 127 x and a = max|x|.  The quotient is
-// the correctly rounded one, so that a half-way quotient goes to the even number
-// as in exact arithmetic: t times the rounded reciprocal of a, and one step of
-// Newton's method on the remainder, which two fused operations give exactly
-// (about 10 operations a value; the compiler's division takes 25, and 2048 rows
-// of 4096 then 10.0 us instead of 7.9).  Rows far from 1 are first multiplied by
+// s = a / 127, q = rint(t / a) with a = max|x| and t = 127 x, rounded to 32 bits
+// (f16 and bf16: exact).  The quotient is the correctly rounded one: t times the
+// rounded reciprocal of a, and one step of Newton's method on the remainder, which
+// two fused operations give exactly (Markstein's division; about 10 operations a
+// value, where the compiler's takes 25: 2048 rows of 4096 7.9 us instead of 10.0 in
+// turn).  So q is what the elementary operations give, and for 16-bit values, whose
+// quotients beside a half are further from it than the rounding, the integer nearest
+// to the exact quotient.  An f32 quotient within 2^-16 of a half may go to either
+// side: an exact decision would need the remainders of both roundings, and would
+// part from the elementary operations.  Rows far from 1 are first multiplied by
 // a power of two, so that nothing leaves the normal numbers.  A row of zeros
 // gives s = 0 and zeros; a row with an infinity or a NaN gives s = NaN and zeros,
 // so that its products show it.

@@ -272,8 +272,11 @@ int zk_synthetic_r1cs(int num_constraints, int num_public, int num_inputs, uint6
  * row's length; rows of x and w may start at any byte (they may be read in
  * whole aligned 4-byte words, whose other bytes do not matter).
  * zk_i8_quantize: scale[t] = max_k |x[t][k]| / 127, q[t][k] = the integer
- * nearest to 127 x[t][k] / max_k |x[t][k]| (ties to even).  A row of zeros
- * has scale 0 and zeros; a row that holds an infinity or a NaN has scale NaN
+ * nearest to (127 x[t][k]) / max_k |x[t][k]| (ties to even), the product and
+ * the quotient each rounded to 32-bit floats.  For f16 and bf16 rows this is
+ * the integer nearest to the exact quotient; of an f32 row a quotient within
+ * 2^-16 of a half may go to either side.  A row of zeros has scale 0 and
+ * zeros; a row that holds an infinity or a NaN has scale NaN
  * and zeros, so that what is made of it is NaN.
  * zk_i8_linear: zk_i8_quantize of x's rows, then zk_i8_matmul with their
  * scales.  d_work: zk_i8_linear_work(rows, n_in) bytes (0: sizes out of

@@ -85,6 +85,35 @@ def test_linear_at_the_ends_of_the_range(ctx, rows):
         assert np.array_equal(got, want) and np.isfinite(got).all() and got.any()
 
 
+@pytest.mark.parametrize("exponent", [-100, -65, 0, 63, 100])
+def test_f32_quotients_beside_a_half(ctx, exponent):
+    """An f32 row's integers are those of 127 x and its quotient rounded to 32 bits
+    each, also where these roundings end on the other side of a half than the exact
+    quotient (71.49999974 and 60.50000069 in the first two rows)."""
+    rng = np.random.default_rng(exponent + 200)
+    rows, cols = 64, 129
+    x = np.zeros((rows, cols), dtype=np.float32)
+    x[:, 0] = np.concatenate([[11694970, 16616451], rng.integers(1 << 23, 1 << 24, rows - 2)]) * 2.0**-23
+    half = (rng.integers(0, 127, (rows, cols - 1)) + 0.5) * x[:, :1] / 127
+    x[:, 1:] = half.astype(np.float32) + rng.integers(-2, 3, half.shape) * np.spacing(half.astype(np.float32))
+    x[:, 1:] *= rng.choice([-1, 1], half.shape)
+    x[0, 1], x[1, 1] = 6584176 * 2.0**-23, 7915711 * 2.0**-23
+    x = np.clip(x, -x[:, :1], x[:, :1])
+    x = np.ldexp(x, exponent)
+    q, s = Result(ctx, rows, cols, "i8"), Result(ctx, 1, rows, "f32")
+    say("[i8 halves]", exponent)
+    ctx.i8_quantize(matrix(ctx, x), z.F32, rows, cols, q.at, s.at)
+    got, want = q.read(), np.rint((np.float32(127) * x) / x[:, :1])
+    assert want.dtype == np.float32 and np.array_equal(got, want) and got[0, 1] == 72 and got[1, 1] == 60
+    assert np.array_equal(s.read()[0], x[:, 0] / np.float32(127))
+    # and so does the linear layer of few rows, which quantizes on the way
+    w = np.eye(cols, dtype=np.int8)
+    y = Result(ctx, 8, cols, "f32")
+    ctx.i8_linear(matrix(ctx, x[:8]), z.F32, matrix(ctx, w), None, 8, cols, cols, y.at, z.F32,
+                  ctx.alloc(ctx.i8_linear_work(8, cols)))
+    assert np.array_equal(y.read(), want[:8] * s.read()[0][:8, None])
+
+
 @pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("tokens,slots,experts,n_out,n_in", [(5, 2, 4, 7, 8), (5, 2, 4, 40, 200), (900, 2, 3, 300, 272)])
 def test_experts_results_are_those_of_the_elementary_operations(ctx, kind, tokens, slots, experts, n_out, n_in):
