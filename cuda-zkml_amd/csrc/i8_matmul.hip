@@ -836,7 +836,7 @@ constexpr TileCost TILE_COST[] = {
     {256, 256, 500, 8000, 1600, 9000, 2500},
 };
 
-// The kernel with the least estimated time: few rows are split over small tiles
+// The tile with the least estimated time: few rows are split over small tiles
 // that read straight from memory, many go through the tiles that read each row
 // fewest times.
 static int choose_tile(const I8Args& a, bool grouped, bool odd_rows, bool bytes) {
@@ -869,70 +869,101 @@ static int choose_tile(const I8Args& a, bool grouped, bool odd_rows, bool bytes)
 // it (4096 x 64 to 32: 3.0 and 3.0; 512: 2.8 and 3.0).
 constexpr uint32_t THIN_ROWS = 4096, THIN_OUT = 48, THIN_IN = 128;
 
+// A product's kernels; those of tiles in the order of TILE_COST, the tiles in LDS
+// by the waves that share one, or for odd rows.
+enum ProductKernel {
+  K_SHORT, K_THIN, K_DIRECT11, K_DIRECT21, K_DIRECT12, K_DIRECT22, K_RING64, K_ODD64, K_RING128_4, K_RING128_8,
+  K_ODD128, K_RING256_8, K_RING256_16, K_ODD256, K_COUNT
+};
+constexpr const char* KERNEL_NAME[K_COUNT] = {
+    "short", "thin", "direct 16x16", "direct 32x16", "direct 16x32", "direct 32x32", "ring 64x64", "odd 64x64",
+    "ring 128x128, 4 waves", "ring 128x128, 8 waves", "odd 128x128", "ring 256x256, 8 waves",
+    "ring 256x256, 16 waves", "odd 256x256"};
+
+// (Of short sums a larger part is a tile's own, which more waves do faster (8192 x
+// 1024 x 8192: 92 us with eight waves of 128 x 128 and 102 with four, 84 and 88 with
+// sixteen and eight of 256 x 256); fewer waves read LDS less (8192 x 8192 x 8192:
+// 541 and 513, 441 and 426).  Grouped, all share the chain of indexes before the
+// first step (66 us and 83, 4096 x 4 rows, 64 experts).)
+struct ProductChoice {
+  ProductKernel kernel;
+  int tile;    // of TILE_COST
+  bool bytes;  // rows at addresses inside a word
+};
+static ProductChoice choose_kernel(const I8Args& a, bool grouped) {
+  if (a.n_in < 16 || (grouped && !a.tokens)) return {K_SHORT, 0, false};  // (without tokens there is no row to read)
+  const size_t rows_at = (uintptr_t)a.x | (uintptr_t)a.w | a.ld_x | a.ld_w;
+  const bool odd = (rows_at | a.n_in) % 16 != 0, bytes = rows_at % 4 != 0, few_steps = a.n_in <= 2048;
+  if (!grouped && a.n_in <= THIN_IN && a.rows >= THIN_ROWS && a.n_out <= THIN_OUT) return {K_THIN, 0, bytes};
+  const int c = choose_tile(a, grouped, odd, bytes);
+  if (c < 4) return {(ProductKernel)(K_DIRECT11 + c), c, bytes};
+  if (c == 4) return {odd ? K_ODD64 : K_RING64, c, bytes};
+  if (c == 5) return {odd ? K_ODD128 : grouped || few_steps ? K_RING128_8 : K_RING128_4, c, bytes};
+  return {odd ? K_ODD256 : few_steps ? K_RING256_16 : K_RING256_8, c, bytes};
+}
+
 template <class T, bool GROUPED>
 static int launch_product(zk_context* ctx, const I8Args& a, hipStream_t st) {
   const char* name = GROUPED ? "i8_matmul_experts" : "i8_matmul";
-  if (a.n_in < 16 || (GROUPED && !a.tokens)) {  // (without tokens there is no row to read)
-    const size_t blocks = ((size_t)a.rows * a.n_out + 255) / 256;
-    ZK_LAUNCH(ctx, st, name, (k_i8_short<T, GROUPED>), dim3(blocks < 65536 ? (uint32_t)blocks : 65536), dim3(256), 0, a);
+  const ProductChoice c = choose_kernel(a, GROUPED);
+  auto thin = [&](auto kernel) -> int {
+    const uint32_t blocks = cdiv(a.rows, 128);
+    ZK_LAUNCH(ctx, st, name, kernel, dim3(blocks < 2048 ? blocks : 2048), dim3(256), 0, a);
     return ZK_OK;
-  }
-  const size_t rows_at = (uintptr_t)a.x | (uintptr_t)a.w | a.ld_x | a.ld_w;
-  const bool odd = (rows_at | a.n_in) % 16 != 0, bytes = rows_at % 4 != 0;
-  if constexpr (!GROUPED) {
-    if (a.n_in <= THIN_IN && a.rows >= THIN_ROWS && a.n_out <= THIN_OUT) {
-      auto go = [&](auto kernel) -> int {
-        const uint32_t blocks = cdiv(a.rows, 128);
-        ZK_LAUNCH(ctx, st, name, kernel, dim3(blocks < 2048 ? blocks : 2048), dim3(256), 0, a);
-        return ZK_OK;
-      };
-      auto by_out = [&](auto by, auto h) -> int {
-        constexpr bool B = decltype(by)::value;
-        constexpr int H = decltype(h)::value;
-        if (a.n_out <= 16) return go(k_i8_thin<T, B, H, 1>);
-        if (a.n_out <= 32) return go(k_i8_thin<T, B, H, 2>);
-        return go(k_i8_thin<T, B, H, 3>);
-      };
-      auto by_in = [&](auto by) -> int {
-        return a.n_in <= 64 ? by_out(by, std::integral_constant<int, 1>()) : by_out(by, std::integral_constant<int, 2>());
-      };
-      return bytes ? by_in(std::true_type()) : by_in(std::false_type());
-    }
-  }
-  const int c = choose_tile(a, GROUPED, odd, bytes);
+  };
+  auto thin_by = [&](auto by, auto h) -> int {
+    constexpr bool B = decltype(by)::value;
+    constexpr int H = decltype(h)::value;
+    if (a.n_out <= 16) return thin(k_i8_thin<T, B, H, 1>);
+    if (a.n_out <= 32) return thin(k_i8_thin<T, B, H, 2>);
+    return thin(k_i8_thin<T, B, H, 3>);
+  };
   auto go = [&](auto kernel, uint32_t threads) -> int {
     // row tiles of the grouped form: whole ones, and a part of one for each
     // expert and for the rows without an expert
-    const uint32_t bt = TILE_COST[c].bt, groups = a.experts + 1 < a.rows ? a.experts + 1 : a.rows;
+    const uint32_t bt = TILE_COST[c.tile].bt, groups = a.experts + 1 < a.rows ? a.experts + 1 : a.rows;
     const uint32_t tiles_t = GROUPED ? a.rows / bt + groups : cdiv(a.rows, bt);
-    const uint32_t tiles_n = cdiv(a.n_out, TILE_COST[c].bn);
+    const uint32_t tiles_n = cdiv(a.n_out, TILE_COST[c.tile].bn);
     const size_t tiles = (size_t)tiles_t * tiles_n;
     if (tiles > I8_MAX_TILES) return ctx->fail(ZK_ERR_SIZE, "i8 experts: rows and n_out make too many tiles");
     ZK_LAUNCH(ctx, st, name, kernel, dim3(cdiv(tiles, 8) * 8), dim3(threads), 0, a, tiles_t, tiles_n);
     return ZK_OK;
   };
-  switch (c) {
-    case 0: return bytes ? go(k_i8_direct<T, GROUPED, true, 1, 1, 8>, 512) : go(k_i8_direct<T, GROUPED, false, 1, 1, 8>, 512);
-    case 1: return bytes ? go(k_i8_direct<T, GROUPED, true, 2, 1, 8>, 512) : go(k_i8_direct<T, GROUPED, false, 2, 1, 8>, 512);
-    case 2: return bytes ? go(k_i8_direct<T, GROUPED, true, 1, 2, 8>, 512) : go(k_i8_direct<T, GROUPED, false, 1, 2, 8>, 512);
-    case 3: return bytes ? go(k_i8_direct<T, GROUPED, true, 2, 2, 8>, 512) : go(k_i8_direct<T, GROUPED, false, 2, 2, 8>, 512);
-    case 4:
-      if (odd) return go(k_i8_odd<T, GROUPED, 2, 2, 1, 1>, 256);
-      return go(k_i8_ring<T, GROUPED, 2, 2, 1, 1>, 256);
-    // of short sums a larger part is a tile's own, which more waves do faster
-    // (8192 x 1024 x 8192: 92 us with eight waves of 128 x 128 and 102 with four,
-    // 84 and 88 with sixteen and eight of 256 x 256); fewer waves read LDS less
-    // (8192 x 8192 x 8192: 541 and 513, 441 and 426).  Grouped, all share the chain
-    // of indexes before the first step (66 us and 83, 4096 x 4 rows, 64 experts).
-    case 5:
-      if (odd) return go(k_i8_odd<T, GROUPED, 2, 4, 2, 1>, 512);
-      if (GROUPED || a.n_in <= 2048) return go(k_i8_ring<T, GROUPED, 2, 4, 2, 1>, 512);
-      return go(k_i8_ring<T, false, 2, 2, 2, 2>, 256);
-    default:
-      if (odd) return go(k_i8_odd<T, GROUPED, 2, 4, 4, 2>, 512);
-      if (a.n_in <= 2048) return go(k_i8_ring<T, GROUPED, 4, 4, 2, 2>, 1024);
-      return go(k_i8_ring<T, GROUPED, 2, 4, 4, 2>, 512);
+  auto direct = [&](auto ft, auto fn) -> int {
+    constexpr int FT = decltype(ft)::value, FN = decltype(fn)::value;
+    return c.bytes ? go(k_i8_direct<T, GROUPED, true, FT, FN, 8>, 512) : go(k_i8_direct<T, GROUPED, false, FT, FN, 8>, 512);
+  };
+  const std::integral_constant<int, 1> one;
+  const std::integral_constant<int, 2> two;
+  switch (c.kernel) {
+    case K_SHORT: {
+      const size_t blocks = ((size_t)a.rows * a.n_out + 255) / 256;
+      ZK_LAUNCH(ctx, st, name, (k_i8_short<T, GROUPED>), dim3(blocks < 65536 ? (uint32_t)blocks : 65536), dim3(256), 0, a);
+      return ZK_OK;
+    }
+    case K_THIN:
+      if constexpr (!GROUPED) {
+        if (c.bytes) return a.n_in <= 64 ? thin_by(std::true_type(), one) : thin_by(std::true_type(), two);
+        return a.n_in <= 64 ? thin_by(std::false_type(), one) : thin_by(std::false_type(), two);
+      }
+      break;
+    case K_DIRECT11: return direct(one, one);
+    case K_DIRECT21: return direct(two, one);
+    case K_DIRECT12: return direct(one, two);
+    case K_DIRECT22: return direct(two, two);
+    case K_RING64: return go(k_i8_ring<T, GROUPED, 2, 2, 1, 1>, 256);
+    case K_ODD64: return go(k_i8_odd<T, GROUPED, 2, 2, 1, 1>, 256);
+    case K_RING128_4:
+      if constexpr (!GROUPED) return go(k_i8_ring<T, false, 2, 2, 2, 2>, 256);
+      break;
+    case K_RING128_8: return go(k_i8_ring<T, GROUPED, 2, 4, 2, 1>, 512);
+    case K_ODD128: return go(k_i8_odd<T, GROUPED, 2, 4, 2, 1>, 512);
+    case K_RING256_8: return go(k_i8_ring<T, GROUPED, 2, 4, 4, 2>, 512);
+    case K_RING256_16: return go(k_i8_ring<T, GROUPED, 4, 4, 2, 2>, 1024);
+    case K_ODD256: return go(k_i8_odd<T, GROUPED, 2, 4, 4, 2>, 512);
+    default: break;
   }
+  return ctx->fail(ZK_ERR_INVALID, "i8 product: no kernel");
 }
 
 template <bool GROUPED>
@@ -1367,6 +1398,17 @@ int zk_i8_matmul(zk_context* ctx, const int8_t* d_x, size_t ld_x, const float* d
     return matmul_impl(ctx, d_x, ld_x, d_x_scale, d_w, ld_w, d_w_scale, d_bias, rows, n_out, n_in, relu, d_y, y_type,
                        ld_y, ctx->s(stream));
   });
+}
+
+const char* zk_debug_i8_kernel(size_t rows, size_t n_out, size_t n_in, size_t ld_x, size_t ld_w, size_t address,
+                               int experts) {
+  using namespace zk;
+  if (rows > 0x7fffffffu || n_out > 0x7fffffffu || n_in > I8_MAX_IN || experts < 0) return nullptr;
+  I8Args a = {};
+  a.x = (const int8_t*)address, a.ld_x = ld_x, a.ld_w = ld_w;
+  a.rows = (uint32_t)rows, a.n_out = (uint32_t)n_out, a.n_in = (uint32_t)n_in;
+  a.experts = (uint32_t)experts, a.tokens = a.rows;
+  return KERNEL_NAME[choose_kernel(a, experts > 0).kernel];
 }
 
 size_t zk_i8_linear_work(size_t rows, size_t n_in) {

@@ -112,6 +112,8 @@ def lib():
         sz, ci = ctypes.c_size_t, ctypes.c_int
         L.zk_i8_matmul.argtypes = [vp, vp, sz, vp, vp, sz, vp, vp, sz, sz, sz, ci, vp, ci, sz, vp]
         L.zk_i8_quantize.argtypes = [vp, vp, ci, sz, sz, sz, vp, sz, vp, vp]
+        L.zk_debug_i8_kernel.argtypes = [sz] * 6 + [ci]
+        L.zk_debug_i8_kernel.restype = ctypes.c_char_p
         L.zk_i8_linear_work.argtypes = [sz, sz]
         L.zk_i8_linear_work.restype = sz
         L.zk_i8_linear.argtypes = [vp, vp, ci, sz, vp, sz, vp, vp, sz, sz, sz, ci, vp, ci, sz, vp, sz, vp]

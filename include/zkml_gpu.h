@@ -310,6 +310,12 @@ int zk_i8_matmul_experts(zk_context* ctx, const int8_t* d_x, size_t ld_x, const 
                          const int32_t* d_offsets, int experts, const int32_t* d_order, int slots, size_t rows,
                          size_t n_out, size_t n_in, int relu, void* d_y, int y_type, size_t ld_y, void* stream);
 
+/* Test hook: the name of the kernel that zk_i8_matmul takes for these sizes and
+ * strides, x and w at addresses with the low bits of `address`; with experts > 0
+ * that of zk_i8_matmul_experts.  NULL: sizes out of range.  Host only. */
+const char* zk_debug_i8_kernel(size_t rows, size_t n_out, size_t n_in, size_t ld_x, size_t ld_w, size_t address,
+                               int experts);
+
 /* ---- routed experts ---------------------------------------------------------
  * No counterpart in the reference, whose routing ends with each sample's class
  * and flag (src/prover/statement_v2.cuh:243-266).  Samples ("tokens") sorted by

@@ -7,7 +7,8 @@ import numpy as np
 import pytest
 
 import zkml_amd as z
-from i8_helpers import TYPES, Result, matrix, words
+from i8_helpers import TYPES, At, Result, matrix, values, words
+from i8_sizes import GROUPED, PLAIN, listed
 
 pytestmark = pytest.mark.gpu
 
@@ -138,3 +139,125 @@ def test_experts_results_are_those_of_the_elementary_operations(ctx, kind, token
             t = order[at] // slots
             acc = x[t].astype(np.int64) @ w[i].astype(np.int64).T
             assert np.array_equal(got[at], elementary(acc, sx[t], sw[i], np.float32(0), False, kind)), i
+
+
+# ------------------------------------------------------------ every kernel, every type
+def sums(x, w):
+    """The exact sums by way of float64, whose 53 bits hold them."""
+    return (x.astype(np.float64) @ w.astype(np.float64).T).astype(np.int64)
+
+
+# by type: bias, ReLU
+EPILOGUES = {"i32": (False, True), "f32": (True, True), "f16": (True, False), "bf16": (False, True)}
+
+
+@pytest.mark.parametrize("kernel,rows,n_out,n_in", listed(PLAIN))
+def test_every_kernel_in_every_type(ctx, kernel, rows, n_out, n_in):
+    rng = np.random.default_rng([rows, n_out, n_in])
+    x = rng.integers(-128, 128, (rows, n_in), dtype=np.int8)
+    w = rng.integers(-128, 128, (n_out, n_in), dtype=np.int8)
+    sx, sw = (np.exp(rng.normal(-6, 0.5, n)).astype(np.float32) for n in (rows, n_out))
+    b = rng.normal(0, 1, n_out).astype(np.float32)
+    xd, wd, sxd, swd, bd = (ctx.upload(a) for a in (x, w, sx, sw, b))
+    acc = sums(x, w)
+    for kind, (bias, relu) in EPILOGUES.items():
+        say("[i8 kernels]", kernel, kind, rows, n_out, n_in)
+        y = Result(ctx, rows, n_out, kind, ld=n_out + 3)
+        scaled = {} if kind == "i32" else dict(x_scale=sxd, w_scale=swd, bias=bd if bias else None)
+        ctx.i8_matmul(xd, wd, rows, n_out, n_in, y.at, TYPES[kind], relu=relu, ld_y=n_out + 3, **scaled)
+        if kind == "i32":
+            want = np.maximum(acc, 0) if relu else acc
+        else:
+            want = elementary(acc, sx, sw, b if bias else np.float32(0), relu, kind)
+        assert np.array_equal(y.read(), want), kind
+
+
+@pytest.mark.parametrize("kernel,rows,n_out,n_in,experts", listed(GROUPED))
+def test_every_kernel_by_expert_in_every_type(ctx, kernel, rows, n_out, n_in, experts):
+    """Unevenly filled experts, one of them empty where there are several, and rows
+    of none behind them."""
+    rng = np.random.default_rng([rows, n_out, n_in, experts])
+    slots = 2 if rows % 2 == 0 else 1
+    tokens = rows // slots
+    e = rng.choice(experts, size=rows, p=(p := np.exp(-0.3 * np.arange(experts))) / p.sum())
+    if experts > 2:
+        e[e == 1] = 0
+    e[rng.random(rows) < 0.05] = experts
+    order = np.argsort(e, kind="stable").astype(np.int32)
+    offsets = np.searchsorted(e[order], np.arange(experts + 1)).astype(np.int32)
+    used = offsets[-1]
+    order[used:] = -1
+    x = rng.integers(-127, 128, (tokens, n_in), dtype=np.int8)
+    w = rng.integers(-127, 128, (experts, n_out, n_in), dtype=np.int8)
+    sx = np.exp(rng.normal(-6, 0.5, tokens)).astype(np.float32)
+    sw = np.exp(rng.normal(-6, 0.5, (experts, n_out))).astype(np.float32)
+    b = rng.normal(0, 1, (experts, n_out)).astype(np.float32)
+    xd, wd, sxd, swd, bd, fd, od = (ctx.upload(a) for a in (x, w, sx, sw, b, offsets, order))
+    at = [slice(offsets[i], offsets[i + 1]) for i in range(experts)]
+    acc = [sums(x[order[a] // slots], w[i]) for i, a in enumerate(at)]
+    for kind, (bias, relu) in EPILOGUES.items():
+        say("[i8 kernels by expert]", kernel, kind, rows, n_out, n_in, experts)
+        y = Result(ctx, rows, n_out, kind, ld=n_out + 3)
+        scaled = {} if kind == "i32" else dict(x_scale=sxd, w_scale=swd, bias=bd if bias else None)
+        ctx.i8_matmul_experts(xd, wd, fd, rows, experts, n_out, n_in, y.at, TYPES[kind], relu=relu, order=od,
+                              slots=slots, tokens=tokens, ld_y=n_out + 3, **scaled)
+        got = y.read()
+        assert not got[used:].any(), kind
+        for i, a in enumerate(at):
+            if kind == "i32":
+                want = np.maximum(acc[i], 0) if relu else acc[i]
+            else:
+                want = elementary(acc[i], sx[order[a] // slots], sw[i], b[i] if bias else np.float32(0), relu, kind)
+            assert np.array_equal(got[a], want), (kind, i)
+
+
+def test_rows_in_two_launches(ctx):
+    """More than 2^22 tiles of 16 x 16: the rows from the 256th on are a launch of
+    their own, with their own part of x, of the scales and of y."""
+    rows, n_out, n_in, at = 259, 1 << 22, 16, 253
+    rng = np.random.default_rng(2)
+    x = rng.integers(-128, 128, (rows, n_in), dtype=np.int8)
+    w = rng.integers(-128, 128, (n_out, n_in), dtype=np.int8)
+    sx, sw = (np.exp(rng.normal(-6, 0.5, n)).astype(np.float32) for n in (rows, n_out))
+    y = ctx.alloc(rows * n_out * 2)
+    say("[i8 two launches]")
+    ctx.i8_matmul(ctx.upload(x), ctx.upload(w), rows, n_out, n_in, y, z.BF16, x_scale=ctx.upload(sx),
+                  w_scale=ctx.upload(sw))
+    got = ctx.d2h(At(y, at * n_out * 2), (rows - at, n_out), np.uint16)
+    # (sums below 2^24 are exact in 32-bit floats)
+    acc = x[at:].astype(np.float32) @ w.astype(np.float32).T
+    assert np.array_equal(got, elementary(acc, sx[at:], sw, np.float32(0), False, "bf16"))
+
+
+# ------------------------------------------------------------ many rows to 8 bits
+# pieces of 16 bytes a row: up to 64, to 256 and to 1024 at 2048 rows, at 512 and at
+# fewer, and more
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("rows,cols", [(2100, 201), (2100, 1001), (600, 1001), (600, 4001), (600, 9001), (2100, 2501)])
+def test_quantize_many_rows(ctx, kind, rows, cols):
+    rng = np.random.default_rng([rows, cols])
+    x = words(rng.normal(0, 1, (rows, cols)) * np.exp(rng.normal(0, 2, (rows, 1))), kind)
+    q, s = Result(ctx, rows, cols, "i8", ld=cols + 1), Result(ctx, 1, rows, "f32")
+    say("[i8 quantize]", kind, rows, cols)
+    ctx.i8_quantize(ctx.upload(x), TYPES[kind], rows, cols, q.at, s.at, ld_q=cols + 1)
+    v = values(x, kind).astype(np.float32)
+    a = np.abs(v).max(axis=1)
+    assert np.array_equal(q.read(), np.rint(np.float32(127) * v / a[:, None]))
+    assert np.array_equal(s.read()[0], a / np.float32(127))
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("rows,n_out,n_in", [(700, 130, 4001), (2100, 300, 1008)])
+def test_linear_of_many_rows(ctx, kind, rows, n_out, n_in):
+    rng = np.random.default_rng([rows, n_in])
+    x = words(rng.normal(0, 1, (rows, n_in)), kind)
+    w = rng.integers(-127, 128, (n_out, n_in), dtype=np.int8)
+    sw, b = np.exp(rng.normal(-5, 0.5, n_out)).astype(np.float32), rng.normal(0, 1, n_out).astype(np.float32)
+    y = Result(ctx, rows, n_out, kind)
+    say("[i8 linear]", kind, rows, n_out, n_in)
+    ctx.i8_linear(ctx.upload(x), TYPES[kind], ctx.upload(w), ctx.upload(sw), rows, n_out, n_in, y.at, TYPES[kind],
+                  ctx.alloc(ctx.i8_linear_work(rows, n_in)), bias=ctx.upload(b))
+    v = values(x, kind).astype(np.float32)
+    a = np.abs(v).max(axis=1)
+    q = np.rint(np.float32(127) * v / a[:, None]).astype(np.int8)
+    assert np.array_equal(y.read(), elementary(sums(q, w), a / np.float32(127), sw, b, False, kind))
