@@ -1312,8 +1312,9 @@ static int launch_few(zk_context* ctx, const I8Args& a, const void* x, int x_typ
 }
 
 // ------------------------------------------------------------ arguments
-// Checks that the two forms of the product share.
-static int check_product(zk_context* ctx, const I8Args& a, size_t rows, size_t n_out, size_t n_in, int type) {
+// Checks that the two forms of the product share.  reads_x: x has rows at all.
+static int check_product(zk_context* ctx, const I8Args& a, size_t rows, size_t n_out, size_t n_in, int type,
+                         bool reads_x = true) {
   if (type != ZK_I32 && !float_type(type)) return ctx->fail(ZK_ERR_INVALID, "i8 product: unknown type of y");
   if (type == ZK_I32 && (a.sx || a.sw || a.bias))
     return ctx->fail(ZK_ERR_INVALID, "i8 product: integer sums take no scales and no bias");
@@ -1322,7 +1323,7 @@ static int check_product(zk_context* ctx, const I8Args& a, size_t rows, size_t n
   if (n_out > 16 * I8_MAX_TILES) return ctx->fail(ZK_ERR_SIZE, "i8 product: n_out above 2^26");
   if (a.ld_x < n_in || a.ld_w < n_in || a.ld_y < n_out)
     return ctx->fail(ZK_ERR_INVALID, "i8 product: a row stride below the row's length");
-  if (rows && n_out && (!a.y || (n_in && (!a.x || !a.w))))
+  if (rows && n_out && (!a.y || (n_in && ((!a.x && reads_x) || !a.w))))
     return ctx->fail(ZK_ERR_INVALID, "i8 product: null pointer");
   if (!aligned(a.y, type_bytes(type)) || !aligned(a.sx, 4) || !aligned(a.sw, 4) || !aligned(a.bias, 4))
     return ctx->fail(ZK_ERR_INVALID, "i8 product: a pointer is not aligned to its type");
@@ -1459,7 +1460,7 @@ int zk_i8_matmul_experts(zk_context* ctx, const int8_t* d_x, size_t ld_x, const 
     if (experts < 1 || experts > ZK_MAX_EXPERTS)
       return ctx->fail(ZK_ERR_SIZE, "i8 experts: between 1 and 1024 experts");
     if (slots < 1) return ctx->fail(ZK_ERR_INVALID, "i8 experts: slots is at least 1");
-    ZK_TRY(check_product(ctx, a, rows, n_out, n_in, y_type));
+    ZK_TRY(check_product(ctx, a, rows, n_out, n_in, y_type, tokens > 0));
     if (rows > ZK_MAX_EXPERT_ROWS || tokens > 0x7fffffffu)
       return ctx->fail(ZK_ERR_SIZE, "i8 experts: too many rows");
     if (!rows || !n_out) return ZK_OK;

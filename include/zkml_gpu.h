@@ -286,8 +286,8 @@ int zk_synthetic_r1cs(int num_constraints, int num_public, int num_inputs, uint6
  * zk_experts_sort) use expert e's weights, d_w + e * n_out * ld_w, w_scale and
  * bias + e * n_out; row p takes row order[p] / slots of x (tokens rows) and
  * its scale, or row p itself when d_order is NULL.  Rows that belong to no
- * expert, or whose order names no token, become zeros.  offsets[0] is 0 and
- * the offsets do not fall.  At most 2^22 rows; ZK_ERR_SIZE also where rows and
+ * expert, or whose order names no token, become zeros (no tokens: d_x may be
+ * NULL).  offsets[0] is 0 and the offsets do not fall.  At most 2^22 rows; ZK_ERR_SIZE also where rows and
  * n_out make more than 2^22 tiles.
  * None of these allocates, waits or uses memory of the context, so calls on
  * different streams do not touch each other.  y may not overlap an input.

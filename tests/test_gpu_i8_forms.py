@@ -211,6 +211,18 @@ def test_every_kernel_by_expert_in_every_type(ctx, kernel, rows, n_out, n_in, ex
             assert np.array_equal(got[a], want), (kind, i)
 
 
+@pytest.mark.parametrize("n_in", [8, 300])
+def test_no_tokens_need_no_x(ctx, n_in):
+    """An empty x has no address (a torch tensor's is 0): every row is zero."""
+    y = Result(ctx, 70, 5, "f32")
+    w = ctx.upload(np.ones((2 * 5, n_in), dtype=np.int8))
+    offsets, order = ctx.upload(np.array([0, 30, 70], dtype=np.int32)), ctx.upload(np.zeros(70, dtype=np.int32))
+    ctx.i8_matmul_experts(None, w, offsets, 70, 2, 5, n_in, y.at, z.F32, order=order, slots=1, tokens=0)
+    assert not y.read().any()
+    with pytest.raises(z.ZkError, match="null"):
+        ctx.i8_matmul_experts(None, w, offsets, 70, 2, 5, n_in, y.at, z.F32, order=order, slots=1, tokens=1)
+
+
 def test_rows_in_two_launches(ctx):
     """More than 2^22 tiles of 16 x 16: the rows from the 256th on are a launch of
     their own, with their own part of x, of the scales and of y."""
