@@ -1139,10 +1139,14 @@ static int i8_quantize(zk_context* ctx, const void* x, int type, size_t ld_x, si
 // first weights, quantizes all of x's rows into LDS while they come (x is small:
 // every block reads it from the L2), and goes on as k_i8_direct with its x
 // fragments from LDS.  Bound by the chain of x's maximum, its bytes and the
-// product: 1 x 8192 x 1024 in 9.2 us, 4.0 + 7.3 in two launches.  x's quantization
-// is repeated in every block, which costs more than a launch once x is large: 8 x
-// 4062 x 1024 9.2 us, 3.2 + 6.7 in two; 16 x 4062 x 1024 (64 KB) 14.0, 3.3 + 7.4.
-constexpr uint32_t FEW_ROWS = 16, FEW_BYTES = 48 * 1024;
+// product: 1 x 8192 x 1024 f16 in 9.7 us, 3.9 + 7.2 in two launches.  x's
+// quantization is repeated in every block, which costs more than the host's second
+// launch once x is large.  A call, this way and in two launches (medians, us): 1 x
+// 4096 x 4096 bf16 13.4 and 16.0, 8 x 4062 x 1024 (32 KB) 13.6 and 15.7, in f32 14.9
+// and 15.7; 3 x 15000 x 1000 (44 KB) 20.2 and 15.6, 16 x 2900 x 8195 (46 KB) 19.5 and
+// 15.4.  On the GPU alone, where nothing waits for the host, two launches are level
+// from about 16 KB on (4 x 4096 x 4096 9.3 and 3.4 + 5.8; 8 rows 12.5 and 3.6 + 6.2).
+constexpr uint32_t FEW_ROWS = 16, FEW_BYTES = 36 * 1024;
 // A quantized row's stride in LDS: whole steps, and 16 bytes so that the rows of
 // a fragment lie in different banks.
 static __host__ __device__ inline uint32_t few_ld(uint32_t n_in) { return (n_in + 127) / 128 * 128 + 16; }

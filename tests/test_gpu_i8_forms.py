@@ -258,6 +258,16 @@ def test_quantize_many_rows(ctx, kind, rows, cols):
     assert np.array_equal(s.read()[0], a / np.float32(127))
 
 
+# at most 16 rows of at most 36 KB in 8 bits are quantized on the way, 16 channels a
+# block or 32 (from 8192 on); more go through the quantizer
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("rows,n_out,n_in", [(1, 33, 17), (16, 70, 2047), (8, 100, 4062), (2, 100, 18000),
+                                             (16, 8195, 2001), (8, 8200, 4062), (1, 8193, 36000), (3, 8193, 129),
+                                             (9, 100, 4095), (1, 50, 37000), (17, 50, 300)])
+def test_linear_of_few_rows(ctx, kind, rows, n_out, n_in):
+    test_linear_of_many_rows(ctx, kind, rows, n_out, n_in)
+
+
 @pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("rows,n_out,n_in", [(700, 130, 4001), (2100, 300, 1008)])
 def test_linear_of_many_rows(ctx, kind, rows, n_out, n_in):
