@@ -18,9 +18,10 @@ namespace zk {
 // ------------------------------------------------------------ sort
 constexpr int SORT_THREADS = 1024, SORT_WAVES = SORT_THREADS / 64;
 // Few pairs are sorted by one block, whose time grows with them (128 experts:
-// 66 pairs 3.2 us, 2048 4.6, 8192 11.1, 16384 19.6); more by blocks of 2048 pairs or
-// more, in two launches, the second of which adds up the blocks' counts (16385:
-// 1.6 + 6.2 us, 65536: 2.6 + 7.0, 2^20: 4.8 + 18; a launch costs the host 4 us).
+// 2048 pairs 4.9 us, 8192 10.9, 16384 would be 19.6; 66 pairs to 8 experts 3.3); more
+// by blocks of 2048 pairs or more, in two launches, the second of which adds up the
+// blocks' counts (16384: 2.4 + 5.9 us, 65536: 2.4 + 6.8, 2^20: 4.1 + 17.5, to 1024
+// experts 4.9 + 53; a launch costs the host 4 us).
 // Bound by the chain launch, loads, counts, scan, loads; the pairs' own bytes are
 // nothing beside it (65536: 0.8 MB).
 constexpr size_t SORT_ONE = 8192;     // pairs that one block sorts alone
@@ -167,7 +168,7 @@ __global__ __launch_bounds__(SORT_THREADS) void k_sort_place(const int32_t* __re
 // ------------------------------------------------------------ rows
 // out[p] = x[order[p] / slots], zeros where order[p] names no token: 2^log_w
 // threads a row, so that short rows fill a wave.  STREAM: see streams().
-// Bound by memory: 65536 rows of 4 KB from 16384 in 70 us, 335 MB at 4.8 TB/s
+// Bound by memory: 65536 rows of 4 KB from 16384 in 73 us, 335 MB at 4.6 TB/s
 // (55 us at a copy's 6.05: a token's four rows are wanted far apart in the sorted
 // order, so that some are fetched again).
 template <class T, bool STREAM>
@@ -235,8 +236,8 @@ __global__ __launch_bounds__(256) void k_combine(const T* __restrict__ y, size_t
 // dy[place[t, j]] = w[t, j] g[t], dw[t, j] = <g[t], y[place[t, j]]>; rows of dy
 // that hold no pair get zeros.  A block has a token, so that g's row is read
 // once and each dot product ends in one block, whose order is fixed; four slots
-// go together.  Bound by memory: 16384 tokens' four rows of 4 KB in 98 us, 604 MB
-// at 6.2 TB/s.
+// go together.  Bound by memory: 16384 tokens' four rows of 4 KB in 102 us, 604 MB
+// at 5.9 TB/s.
 template <class T, bool STREAM>
 __global__ __launch_bounds__(256) void k_combine_grad(const T* __restrict__ g, size_t ld_g, const T* __restrict__ y,
                                                       size_t ld_y, const int32_t* __restrict__ order,
@@ -299,7 +300,7 @@ __global__ __launch_bounds__(256) void k_combine_grad(const T* __restrict__ g, s
 
 // Whether a call's rows pass the caches (32 MB of L2): what is read or written
 // once then goes around them and leaves them to the rows that are read again
-// (gather of 65536 rows of 4 KB 69 us, 84 through the caches); smaller rows stay
+// (in turn, gather of 65536 rows of 4 KB 69 us, 84 through the caches); smaller rows stay
 // for whoever reads them next.
 static bool streams(size_t rows, size_t cols, size_t size) { return rows * cols * size > (size_t)32 << 20; }
 

@@ -63,8 +63,8 @@ __device__ __forceinline__ v4i load16_any(const int8_t* p) {
   return v;
 }
 // 16 bytes from a multiple of 4 bytes, or, BYTES, from any address as the words
-// that hold them, moved down by the address's part of a word (3 x 5569 x 7061:
-// 11 us, 19 with load16_any).  No word is read that holds none of the bytes.
+// that hold them, moved down by the address's part of a word (3 rows, 5569 to
+// 7061, in turn: 11 us, 19 with load16_any).  No word is read that holds none of the bytes.
 typedef int v4i_words __attribute__((ext_vector_type(4), aligned(4)));
 __device__ __forceinline__ v4i move_down(const v4i& v, int next, uint32_t by) {
   return v4i{(int)__builtin_amdgcn_alignbyte((uint32_t)v[1], (uint32_t)v[0], by),
@@ -250,16 +250,20 @@ __device__ const v4i zeros16 = {0, 0, 0, 0};
 // four neighbouring channels of one token).  Steps of 128 bytes of k, a whole
 // cache line of each row, pass through LDS: byte chunk c of row r lies at chunk
 // c ^ (r / 2 % 8), so that the 32 rows of a fragment meet no bank twice (the
-// conflict counter stays at zero).
+// conflict counter does not grow with n_in: what it counts are the results).
 //
 // Rows of whole 16-byte chunks go straight from memory to LDS, with no register
 // and no instruction between, into a ring of five slots of one side's tile each:
 // this step's two tiles, the next step's two, and x's of the one after, each slot
 // asked for again half a step after everybody has read it.  Loads and LDS reads
 // are placed between the matrix instructions, which then have no pause longer
-// than a barrier.  Bound by the matrix cores at the clock that the card's power
-// leaves them: 8192 x 8192 x 8192 in 445 us, 2.47 POPS (355 us with zeros for data),
-// 2048 x 4096 x 4096 in 39.6 us, 1.74 POPS (512 tiles, two for each CU).
+// than a barrier.  8192 x 8192 x 8192: 457 us a call, 2.40 POPS (traced, median of
+// sixty in a row 479, 457 to 591); 309 with zeros for data.  The matrix cores are
+// busy in 0.67 to 0.73 of the cycles with either data (a tile's first loads and
+// results take 0.07 by the fit below, waits within the steps the rest); the clock
+// makes the difference, 2.1 to 2.2 GHz on zeros and 1.3 to 1.7 with random data,
+// where the card's power limits it.  2048 rows, 4096 to 4096: 40.4 us, 1.70 POPS
+// (512 tiles, two for each CU).
 
 // 16 bytes a lane from `p` to LDS at `at` + 16 * lane (`at` the same in the
 // whole wave).  Only wait_loads() waits for it: to the compiler's own counting
@@ -506,10 +510,11 @@ __global__ __launch_bounds__(64 * WT * WN) void k_i8_ring(I8Args a, uint32_t til
 // The same tiles where a row may start at any byte, or end inside a chunk: the
 // steps pass through registers (masked), loaded a step ahead and stored before
 // the stage's turn.  Bound by those loads, which take three times as long from
-// addresses inside a word: 777 x 1001 x 1234 in 10.3 us.
+// addresses inside a word: 777 rows, 1001 to 1234, in 10.6 us, 1194 rows, 4438 to
+// 5316 f32, in 65.
 // (Loads from any address; word loads with the bytes moved down, as the direct
-// kernel has them, hold a register more a piece and made 1194 x 4438 x 5316 98 us
-// instead of 68.)
+// kernel has them, hold a register more a piece and made the latter 98 us instead
+// of 68, in turn.)
 template <class T, bool GROUPED, int WT, int WN, int FT, int FN>
 __global__ __launch_bounds__(64 * WT * WN) void k_i8_odd(I8Args a, uint32_t tiles_t, uint32_t tiles_n) {
   constexpr uint32_t WAVES = WT * WN, BT = WT * FT * 32, BN = WN * FN * 32, BK = 128;
@@ -626,8 +631,8 @@ __global__ __launch_bounds__(64 * WT * WN) void k_i8_odd(I8Args a, uint32_t tile
 // 128 bytes (a cache line of every row) and add up their sums in LDS.  Bound by
 // what the L2 hands over: 16 (FT + FN) rows a block, 9.3 TB/s over the chip; one
 // row by the chain of the launch, a block's loads (all under way together) and
-// its sums: 1 x 4096 x 4096 in 5.7 us (17 MB; an empty launch takes 2.4), 5 tokens
-// at two of 16 experts each, 4096 x 2048, in 12.5.
+// its sums: one row, 4096 to 4096, in 5.8 us (17 MB; an empty launch takes 2.4), 5
+// tokens at two of 16 experts each, 4096 to 2048, in 13.8 (12.6 to 18.3; 64 MB).
 template <class T, bool GROUPED, bool BYTES, int FT, int FN, int KW>
 __global__ __launch_bounds__(64 * KW, 4) void k_i8_direct(I8Args a, uint32_t tiles_t, uint32_t tiles_n) {
   constexpr uint32_t BT = 16 * FT, BN = 16 * FN, BK = 128;
@@ -735,11 +740,12 @@ __global__ __launch_bounds__(64 * KW, 4) void k_i8_direct(I8Args a, uint32_t til
 // A small layer over a whole data set: a wave keeps the weights, scales and
 // biases of all 16 FN channels in registers and goes over the tokens, TILES of 16
 // at a time, their rows read once, straight to fragments.  H: halves of 64 bytes
-// that a row has.  Bound by memory, once the launch's own 2 us are past: 100003 x
-// 64 to 32 integers 5.0 us (19 MB), 9.0 through the tiles in LDS, whose blocks
-// have one step each; 500000 x 64 to 32: 16.4.  Results of 4 bytes leave around
-// the caches, which would write them out only at the end (7.6 us); 8-byte pieces
-// do not (4.8 us; 5.2 around the caches, 15 and 35 with 48 channels, 500000 rows).
+// that a row has.  Bound by memory, once the launch's own 2 us are past: 100003 rows,
+// 64 to 32 integers, 5.6 us (19 MB); 500000: 20.3 (96 MB).  Measured in turn at
+// 100003: 5.0 here and 9.0 through the tiles in LDS, whose blocks have one step
+// each.  Results of 4 bytes leave around the caches, which would write them out only
+// at the end (5.0 and 7.6 us); 8-byte pieces do not (4.8 us; 5.2 around the caches,
+// 15 and 35 with 48 channels, 500000 rows).
 template <class T, bool BYTES, int H, int FN>
 __global__ __launch_bounds__(256) void k_i8_thin(I8Args a) {
   constexpr int TILES = 2;
@@ -864,9 +870,9 @@ static int choose_tile(const I8Args& a, bool grouped, bool odd_rows, bool bytes)
 }
 
 // Products for k_i8_thin: at 64 channels a token's rows in LDS are worth their
-// steps (100003 x 64 to 64 integers: 9.2 us there, 12.1 here; to 48: 9.2 and 6.8),
-// and under some thousand rows the tiles that split the channels are level with
-// it (4096 x 64 to 32: 3.0 and 3.0; 512: 2.8 and 3.0).
+// steps (in turn, 100003 rows, 64 to 64 integers: 9.2 us there, 12.1 here; to 48: 9.2
+// and 6.8), and under some thousand rows the tiles that split the channels are level
+// with it (4096 rows, 64 to 32: 3.0 and 3.0; 512: 2.8 and 3.0).
 constexpr uint32_t THIN_ROWS = 4096, THIN_OUT = 48, THIN_IN = 128;
 
 // A product's kernels; those of tiles in the order of TILE_COST, the tiles in LDS
@@ -880,11 +886,11 @@ constexpr const char* KERNEL_NAME[K_COUNT] = {
     "ring 128x128, 4 waves", "ring 128x128, 8 waves", "odd 128x128", "ring 256x256, 8 waves",
     "ring 256x256, 16 waves", "odd 256x256"};
 
-// (Of short sums a larger part is a tile's own, which more waves do faster (8192 x
-// 1024 x 8192: 92 us with eight waves of 128 x 128 and 102 with four, 84 and 88 with
-// sixteen and eight of 256 x 256); fewer waves read LDS less (8192 x 8192 x 8192:
-// 541 and 513, 441 and 426).  Grouped, all share the chain of indexes before the
-// first step (66 us and 83, 4096 x 4 rows, 64 experts).)
+// (Of short sums a larger part is a tile's own, which more waves do faster (in turn,
+// 8192 rows, 1024 to 8192: 92 us with eight waves of 128 x 128 and 102 with four, 84
+// and 88 with sixteen and eight of 256 x 256); fewer waves read LDS less (8192 to
+// 8192: 541 and 513, 441 and 426).  Grouped, all share the chain of indexes before
+// the first step (66 us and 83, 4096 x 4 rows, 64 experts).)
 struct ProductChoice {
   ProductKernel kernel;
   int tile;    // of TILE_COST
@@ -1043,7 +1049,8 @@ __device__ __forceinline__ void look_piece(const Vec<T>& v, uint32_t& m) {
 // THREADS threads a row, ROWS rows a block.  A thread keeps its first HELD
 // pieces of 16 bytes from the pass for the maximum to the pass that divides, so
 // that rows of up to 64 KB are read once.  Bound by its own chain (load, maximum
-// over the block, divide, store): 2048 rows of 4096 bf16 in 8.5 us, 25 MB at 3 TB/s.
+// over the block, divide, store): 2048 rows of 4096 bf16 in 9.9 us (8.2 to 10.2), 25 MB
+// at 2.5 TB/s.
 template <class T, int THREADS, int ROWS>
 __global__ __launch_bounds__(THREADS* ROWS) void k_i8_quantize(const T* __restrict__ x, size_t ld_x, uint32_t rows,
                                                                uint32_t cols, int8_t* __restrict__ q, size_t ld_q,
@@ -1139,13 +1146,14 @@ static int i8_quantize(zk_context* ctx, const void* x, int type, size_t ld_x, si
 // first weights, quantizes all of x's rows into LDS while they come (x is small:
 // every block reads it from the L2), and goes on as k_i8_direct with its x
 // fragments from LDS.  Bound by the chain of x's maximum, its bytes and the
-// product: 1 x 8192 x 1024 f16 in 9.7 us, 3.9 + 7.2 in two launches.  x's
+// product: one row, 8192 to 1024 f16, in 9.9 us, 3.9 + 7.2 in two launches.  x's
 // quantization is repeated in every block, which costs more than the host's second
-// launch once x is large.  A call, this way and in two launches (medians, us): 1 x
-// 4096 x 4096 bf16 13.4 and 16.0, 8 x 4062 x 1024 (32 KB) 13.6 and 15.7, in f32 14.9
-// and 15.7; 3 x 15000 x 1000 (44 KB) 20.2 and 15.6, 16 x 2900 x 8195 (46 KB) 19.5 and
-// 15.4.  On the GPU alone, where nothing waits for the host, two launches are level
-// from about 16 KB on (4 x 4096 x 4096 9.3 and 3.4 + 5.8; 8 rows 12.5 and 3.6 + 6.2).
+// launch once x is large.  A call, this way and in two launches (medians, us): one
+// row, 4096 to 4096 bf16, 13.4 and 16.0; 8 rows, 4062 to 1024 (32 KB), 13.6 and 15.7,
+// in f32 14.9 and 15.7; 3 rows, 15000 to 1000 (44 KB), 20.2 and 15.6; 16 rows, 2900 to
+// 8195 (46 KB), 19.5 and 15.4.  On the GPU alone, where nothing waits for the host,
+// two launches are level from about 16 KB on (4096 to 4096: 4 rows 9.3 and 3.4 + 5.8,
+// 8 rows 12.5 and 3.6 + 6.2).
 constexpr uint32_t FEW_ROWS = 16, FEW_BYTES = 36 * 1024;
 // A quantized row's stride in LDS: whole steps, and 16 bytes so that the rows of
 // a fragment lie in different banks.
