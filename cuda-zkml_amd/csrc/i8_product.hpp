@@ -1,0 +1,178 @@
+// What the products of 8-bit rows share: their arguments, the tile of a block
+// (dense, and grouped by expert), copies from memory straight to LDS, and the
+// stores of neighbouring results.
+#pragma once
+#include "rows.hpp"
+#include "zk_internal.hpp"
+
+namespace zk {
+
+typedef int v4i __attribute__((ext_vector_type(4)));
+typedef int v16i __attribute__((ext_vector_type(16)));
+
+constexpr size_t I8_MAX_TILES = (size_t)1 << 22;  // blocks of one launch (its threads stay below 2^32)
+
+// What a product's kernel is given.
+struct I8Args {
+  const int8_t* x;
+  const int8_t* w;
+  const float* sx;  // per token, or null: 1
+  const float* sw;  // per channel, or null: 1
+  const float* bias;
+  void* y;
+  size_t ld_x, ld_w, ld_y;
+  uint32_t rows, n_out, n_in;
+  int relu;
+  // grouped form
+  const int32_t* offsets;
+  const int32_t* order;
+  uint32_t experts, slots, tokens;
+};
+
+// Four neighbouring results, of which the row has `left` from here on.  (Every
+// index is a constant: an array that is indexed by a variable goes to LDS, by way
+// of the launch packet in host memory, and a call of 5 us then took 16.)
+// ONCE: around the caches.
+template <bool ONCE = false, class T>
+__device__ __forceinline__ void store4(T* y, uint32_t left, const T (&v)[4]) {
+  if (left >= 4) {
+    if constexpr (ONCE) {
+      row16 b;
+      static_assert(sizeof(v) == 16, "whole pieces of 16 bytes");
+      __builtin_memcpy(&b, v, 16);
+      __builtin_nontemporal_store(b, (row16*)y);
+    } else {
+      __builtin_memcpy(y, v, sizeof(v));
+    }
+    return;
+  }
+#pragma unroll
+  for (uint32_t k = 0; k < 3; k++)
+    if (k < left) y[k] = v[k];
+}
+
+// Offset of expert e, inside [0, rows] whatever the device array holds.
+__device__ __forceinline__ uint32_t offset_of(const I8Args& a, uint32_t e) {
+  const int v = a.offsets[e];
+  return v < 0 ? 0u : (uint32_t)v > a.rows ? a.rows : (uint32_t)v;
+}
+
+// Row of x behind position p (grouped form), or -1: the position holds none.
+__device__ __forceinline__ int64_t source_row(const I8Args& a, uint32_t p) {
+  if (!a.order) return p < a.tokens ? (int64_t)p : -1;
+  const int o = a.order[p];
+  if (o < 0) return -1;
+  const uint32_t t = (uint32_t)o / a.slots;
+  return t < a.tokens ? (int64_t)t : -1;
+}
+
+// Tile (tt, tn) of block b.  Blocks b, b + 8, b + 16, ... share an XCD and its
+// L2: each XCD gets one run of the tiles, and a run goes over 8 token tiles
+// before it takes the next channel tile, so that the 32 blocks an XCD holds at
+// a time read about 8 + 4 tiles of rows between them.
+__device__ __forceinline__ bool tile_of_block(uint32_t b, uint32_t tiles_t, uint32_t tiles_n, uint32_t& tt,
+                                              uint32_t& tn) {
+  constexpr uint32_t G = 8;
+  const uint32_t total = tiles_t * tiles_n, per = (total + 7) / 8;
+  const uint32_t t = (b & 7) * per + (b >> 3);
+  if ((b >> 3) >= per || t >= total) return false;
+  const uint32_t group = t / (G * tiles_n), at = t % (G * tiles_n);
+  const uint32_t size = tiles_t - group * G < G ? tiles_t - group * G : G;
+  tt = group * G + at % size;
+  tn = at / size;
+  return true;
+}
+
+// A block's tile: rows [r0, r1) from channel n0 on, and their expert.  Grouped,
+// the row tiles are counted expert by expert, those of the rows without an
+// expert (e = experts) last; the grid is made for the most there can be, and the
+// tiles there are are spread over its first blocks, so that no XCD is left with
+// the empty ones.  The whole wave takes part; the answer is the same in every
+// lane.  False: nothing to do.
+template <bool GROUPED>
+__device__ __forceinline__ bool block_tile(const I8Args& a, uint32_t bt, uint32_t bn, uint32_t tiles_t,
+                                           uint32_t tiles_n, uint32_t& r0, uint32_t& r1, uint32_t& n0, uint32_t& e) {
+  uint32_t tt, tn;
+  if (!GROUPED) {
+    if (!tile_of_block(blockIdx.x, tiles_t, tiles_n, tt, tn)) return false;
+    r0 = tt * bt, r1 = a.rows, n0 = tn * bn, e = 0;
+    return true;
+  }
+  const uint32_t lane = threadIdx.x & 63;
+  // 64 experts at a time, one a lane: rows [lo, hi), n tiles, s of them up to here
+  uint32_t lo, hi, n, s;
+  auto look = [&](uint32_t e0) {
+    const uint32_t me = e0 + lane;
+    lo = hi = 0;
+    if (me < a.experts) lo = offset_of(a, me), hi = offset_of(a, me + 1);
+    n = hi > lo ? (hi - lo + bt - 1) / bt : 0;
+    s = n;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const uint32_t o = __shfl_up(s, d);
+      if (lane >= (uint32_t)d) s += o;
+    }
+  };
+  uint32_t all = 0;
+  for (uint32_t e0 = 64; e0 < a.experts; e0 += 64) look(e0), all += __shfl(s, 63);
+  look(0);
+  all += __shfl(s, 63);
+  const uint32_t end = offset_of(a, a.experts), rest = (a.rows - end + bt - 1) / bt;
+  if (!tile_of_block(blockIdx.x, __builtin_amdgcn_readfirstlane(all + rest), tiles_n, tt, tn)) return false;
+  n0 = tn * bn;
+  uint32_t run = 0;
+  for (uint32_t e0 = 0; e0 < a.experts; e0 += 64) {
+    if (e0) look(e0);
+    const uint64_t past = __ballot(run + s > tt);
+    if (past) {
+      const int l = __ffsll((unsigned long long)past) - 1;
+      const uint32_t first = run + __shfl(s, l) - __shfl(n, l);
+      e = __builtin_amdgcn_readfirstlane(e0 + l);
+      r0 = __builtin_amdgcn_readfirstlane(__shfl(lo, l) + (tt - first) * bt);
+      r1 = __builtin_amdgcn_readfirstlane(__shfl(hi, l));
+      return r0 < r1;
+    }
+    run += __shfl(s, 63);
+  }
+  e = a.experts;
+  r0 = __builtin_amdgcn_readfirstlane(end + (tt - run) * bt);
+  r1 = a.rows;
+  return r0 < r1;
+}
+
+// What rows are padded with: a lane that has no bytes to load takes these.
+__device__ const v4i zeros16 = {0, 0, 0, 0};
+
+// ------------------------------------------------------------ memory to LDS
+// 16 bytes a lane from `p` to LDS at `at` + 16 * lane (`at` the same in the
+// whole wave).  Only wait_loads() waits for it: to the compiler's own counting
+// it is unknown, which makes the compiler's waits longer, never shorter.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"  // m0 is named so that nothing of the compiler's is kept in it
+__device__ __forceinline__ void load_to_lds(const int8_t* p, uint32_t at) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(at), "v"(p) : "m0");
+}
+#pragma clang diagnostic pop
+// Until at most N of the wave's loads are under way.
+template <int N>
+__device__ __forceinline__ void wait_loads() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+__device__ __forceinline__ void meet() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+// ---- rows to 8 bits (i8_matmul.hip)
+int i8_quantize(zk_context* ctx, const void* x, int type, size_t ld_x, size_t rows, size_t cols, int8_t* q,
+                size_t ld_q, float* scale, hipStream_t st);
+int check_quantize(zk_context* ctx, const void* x, int type, size_t ld_x, size_t rows, size_t cols);
+// Layout of a quantizing layer's workspace: the rows' scales, then the rows' bytes.
+struct LinearWork {
+  size_t ld, q, bytes;
+};
+LinearWork linear_work(size_t rows, size_t n_in);
+
+}  // namespace zk

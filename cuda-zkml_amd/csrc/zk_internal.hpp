@@ -150,6 +150,21 @@ int guard(zk_context* ctx, Fn&& fn) noexcept {
   return code;
 }
 
+// The context's device as the current one for as long as this lives: a caller's
+// thread may have another one current.
+struct OnDevice {
+  int before = -1;
+  explicit OnDevice(const zk_context* ctx) {
+    int now = -1;
+    if (hipGetDevice(&now) == hipSuccess && now != ctx->device && hipSetDevice(ctx->device) == hipSuccess) before = now;
+  }
+  ~OnDevice() {
+    if (before >= 0) (void)hipSetDevice(before);
+  }
+  OnDevice(const OnDevice&) = delete;
+  OnDevice& operator=(const OnDevice&) = delete;
+};
+
 // Issue priority of the quotient's kernels (sparse products, NTTs, pointwise
 // step).  In a proof they run beside the G2 MSM's accumulation and the H MSM
 // waits for them: their waves outrank the MSM waves sharing a SIMD.

@@ -125,6 +125,21 @@ def lib():
         L.zk_experts_gather.argtypes = [vp, vp, ci, sz, sz, vp, sz, sz, ci, vp, sz, vp]
         L.zk_experts_combine.argtypes = [vp, vp, ci, sz, sz, vp, vp, sz, sz, ci, vp, sz, vp]
         L.zk_experts_combine_grad.argtypes = [vp, vp, sz, vp, sz, ci, sz, vp, vp, vp, sz, sz, ci, vp, sz, vp, vp]
+        L.zk_i4_row_bytes.argtypes = [sz]
+        L.zk_i4_row_bytes.restype = sz
+        L.zk_i4_quantize.argtypes = [vp, vp, ci, sz, sz, sz, ci, vp, sz, vp, ci, vp]
+        L.zk_i4_matmul.argtypes = [vp, vp, sz, vp, vp, sz, vp, ci, ci, vp, sz, sz, sz, ci, vp, ci, sz, vp]
+        L.zk_i4_linear_work.argtypes = [sz, sz]
+        L.zk_i4_linear_work.restype = sz
+        L.zk_i4_linear.argtypes = [vp, vp, ci, sz, vp, sz, vp, ci, ci, vp, sz, sz, sz, ci, vp, ci, sz, vp, sz, vp]
+        L.zk_i4_matmul_experts.argtypes = [vp, vp, sz, vp, sz, vp, sz, vp, ci, ci, vp, vp, ci, vp, ci, sz, sz, sz, ci,
+                                           vp, ci, sz, vp]
+        fl = ctypes.c_float
+        L.zk_experts_route_work.argtypes = [sz, ci]
+        L.zk_experts_route_work.restype = sz
+        L.zk_experts_route.argtypes = [vp, vp, ci, sz, sz, ci, ci, fl, ci, vp, vp, vp, vp, vp, vp, sz, vp]
+        L.zk_experts_balance.argtypes = [vp, vp, ci, sz, sz, ci, ci, fl, vp, vp, vp, vp, vp, sz, vp]
+        L.zk_experts_route_grad.argtypes = [vp, vp, ci, sz, sz, ci, ci, fl, ci, vp, vp, vp, vp, vp, sz, vp]
         L.zk_poseidon_permute.argtypes = [vp]
         L.zk_poseidon_hash2.argtypes = [vp, vp, vp]
         L.zk_poseidon_commit.argtypes = [vp, ctypes.c_size_t, ctypes.c_uint64, vp]
@@ -444,6 +459,85 @@ class Context:
             self.h, _dev(grad), cols if ld_grad is None else ld_grad, _dev(y), cols if ld_y is None else ld_y,
             rows_type, cols, _dev(order), _dev(place), _dev(weight), rows, tokens, slots, _dev(grad_y),
             cols if ld_grad_y is None else ld_grad_y, _dev(grad_weight), stream), "zk_experts_combine_grad")
+
+    # ---- layers with 4-bit weights
+    @staticmethod
+    def i4_row_bytes(n_in):
+        """Bytes of a channel's 4-bit weights (zk_i4_row_bytes)."""
+        return lib().zk_i4_row_bytes(n_in)
+
+    def i4_quantize(self, w, w_type, rows, cols, group, q, scale, scale_type=F32, ld_w=None, ld_q=None, stream=None):
+        """Weights to 4 bits with a scale per group (zk_i4_quantize); q: rows *
+        i4_row_bytes(cols) bytes, scale: (groups, rows)."""
+        self._check(lib().zk_i4_quantize(self.h, _dev(w), w_type, cols if ld_w is None else ld_w, rows, cols, group,
+                                         _dev(q), (cols + 127) // 128 * 64 if ld_q is None else ld_q, _dev(scale),
+                                         scale_type, stream), "zk_i4_quantize")
+
+    def i4_matmul(self, x, w, w_scale, rows, n_out, n_in, group, y, y_type=F32, scale_type=F32, x_scale=None,
+                  bias=None, relu=False, ld_x=None, ld_w=None, ld_y=None, stream=None):
+        """y = x w^T, x int8 and w in 4 bits with a scale per group (zk_i4_matmul)."""
+        self._check(lib().zk_i4_matmul(self.h, _dev(x), n_in if ld_x is None else ld_x, _dev(x_scale), _dev(w),
+                                       (n_in + 127) // 128 * 64 if ld_w is None else ld_w, _dev(w_scale), scale_type,
+                                       group, _dev(bias), rows, n_out, n_in, relu, _dev(y), y_type,
+                                       n_out if ld_y is None else ld_y, stream), "zk_i4_matmul")
+
+    @staticmethod
+    def i4_linear_work(rows, n_in):
+        return lib().zk_i4_linear_work(rows, n_in)
+
+    def i4_linear(self, x, x_type, w, w_scale, rows, n_out, n_in, group, y, y_type, work, scale_type=F32, bias=None,
+                  relu=False, ld_x=None, ld_w=None, ld_y=None, stream=None):
+        """Quantizes x's rows to 8 bits and multiplies (zk_i4_linear); work:
+        i4_linear_work(rows, n_in) bytes."""
+        self._check(lib().zk_i4_linear(self.h, _dev(x), x_type, n_in if ld_x is None else ld_x, _dev(w),
+                                       (n_in + 127) // 128 * 64 if ld_w is None else ld_w, _dev(w_scale), scale_type,
+                                       group, _dev(bias), rows, n_out, n_in, relu, _dev(y), y_type,
+                                       n_out if ld_y is None else ld_y, _dev(work), _nbytes(work), stream),
+                    "zk_i4_linear")
+
+    def i4_matmul_experts(self, x, w, w_scale, offsets, rows, experts, n_out, n_in, group, y, y_type=F32,
+                          scale_type=F32, x_scale=None, bias=None, relu=False, order=None, slots=1, tokens=None,
+                          ld_x=None, ld_w=None, ld_y=None, stream=None):
+        """i4_matmul with each expert's weights for its rows (zk_i4_matmul_experts).
+        tokens: x's rows, as in i8_matmul_experts."""
+        if order is not None and slots > 1 and tokens is None:
+            raise ZkError("zk_i4_matmul_experts: an order of several slots needs tokens, the number of x's rows")
+        self._check(lib().zk_i4_matmul_experts(
+            self.h, _dev(x), n_in if ld_x is None else ld_x, _dev(x_scale), rows if tokens is None else tokens,
+            _dev(w), (n_in + 127) // 128 * 64 if ld_w is None else ld_w, _dev(w_scale), scale_type, group, _dev(bias),
+            _dev(offsets), experts, _dev(order), slots, rows, n_out, n_in, relu, _dev(y), y_type,
+            n_out if ld_y is None else ld_y, stream), "zk_i4_matmul_experts")
+
+    # ---- the experts' router
+    @staticmethod
+    def experts_route_work(tokens, experts):
+        return lib().zk_experts_route_work(tokens, experts)
+
+    def experts_route(self, scores, scores_type, tokens, experts, slots, expert, weight, scale=1.0, renormalize=True,
+                      count=None, prob=None, loss=None, work=None, ld=None, stream=None):
+        """Each token's experts and weights, and with count (experts + 1 words), prob
+        and loss their balance (zk_experts_route); work: experts_route_work bytes."""
+        self._check(lib().zk_experts_route(self.h, _dev(scores), scores_type, experts if ld is None else ld, tokens,
+                                           experts, slots, scale, renormalize, _dev(expert), _dev(weight),
+                                           _dev(count), _dev(prob), _dev(loss), _dev(work), _nbytes(work), stream),
+                    "zk_experts_route")
+
+    def experts_balance(self, scores, scores_type, tokens, experts, slots, expert, count, prob, loss, work=None,
+                        scale=1.0, ld=None, stream=None):
+        """Counts, mean probabilities and balance loss of given routes (zk_experts_balance)."""
+        self._check(lib().zk_experts_balance(self.h, _dev(scores), scores_type, experts if ld is None else ld, tokens,
+                                             experts, slots, scale, _dev(expert), _dev(count), _dev(prob), _dev(loss),
+                                             _dev(work), _nbytes(work), stream), "zk_experts_balance")
+
+    def experts_route_grad(self, scores, scores_type, tokens, experts, slots, expert, grad_scores, scale=1.0,
+                           renormalize=True, grad_weight=None, count=None, grad_loss=None, ld=None, ld_grad=None,
+                           stream=None):
+        """Gradient of the scores from the weights' and the loss's (zk_experts_route_grad)."""
+        self._check(lib().zk_experts_route_grad(self.h, _dev(scores), scores_type, experts if ld is None else ld,
+                                                tokens, experts, slots, scale, renormalize, _dev(expert),
+                                                _dev(grad_weight), _dev(count), _dev(grad_loss), _dev(grad_scores),
+                                                experts if ld_grad is None else ld_grad, stream),
+                    "zk_experts_route_grad")
 
     # ---- Groth16
     def r1cs(self, num_constraints, num_variables, num_public, A, B, C):

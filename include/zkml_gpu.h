@@ -316,6 +316,56 @@ int zk_i8_matmul_experts(zk_context* ctx, const int8_t* d_x, size_t ld_x, const 
 const char* zk_debug_i8_kernel(size_t rows, size_t n_out, size_t n_in, size_t ld_x, size_t ld_w, size_t address,
                                int experts);
 
+/* ---- layers with 4-bit weights ----------------------------------------------
+ * No counterpart in the reference.  The 8-bit rows above (int8 with a scale
+ * each) times weights of 4 bits, -8 to 7, with a scale for each group of `group`
+ * (32, 64 or a multiple of 128) neighbouring weights of a channel, the last of
+ * which may be shorter.
+ * Layout: a channel's weights are zk_i4_row_bytes(n_in) = 64 ceil(n_in / 128)
+ * bytes (0: n_in above 2^24); in each 64 of them, which are 128 weights, byte b
+ * holds weight b in its low and weight 64 + b in its high four bits, two's
+ * complement.  What lies behind a row's last weight does not matter.  Rows start
+ * at multiples of 16 bytes (d_w and ld_w, in bytes).  The scale of group g of
+ * channel n is d_w_scale[g * n_out + n], of type scale_type (ZK_F32, ZK_F16 or
+ * ZK_BF16).
+ *
+ * zk_i4_quantize: a matrix of rows x cols to this layout.  scale = max |w| of the
+ * group / 7, rounded to scale_type; q = the integer nearest to w / scale (ties to
+ * even), between -8 and 7.  A group of zeros, or whose scale rounds to zero, has
+ * scale 0 and zeros, one that holds an infinity or a NaN scale NaN and zeros.
+ * Padding becomes zero.
+ * zk_i4_matmul: y[t][n] = x_scale[t] * sum_g w_scale[g][n] acc[t][n][g] + bias[n]
+ * with acc[t][n][g] = sum_k x[t][k] q[n][k] over group g.  Sums within 128
+ * weights are exact; the groups' terms are added in 32-bit floats, in an order that
+ * depends on the sizes alone; the token's scale and the bias follow in one fused
+ * operation, then one rounding to y_type (ZK_F32, ZK_F16, ZK_BF16).  relu,
+ * strides, NULL scales and biases and rows of x at any byte as in zk_i8_matmul
+ * (d_w_scale may not be NULL); at most 2^26 channels.
+ * zk_i4_linear: zk_i8_quantize of x's rows, then zk_i4_matmul.  d_work:
+ * zk_i4_linear_work(rows, n_in) bytes (0: sizes out of range), 16-byte aligned,
+ * free again when the call's work on the stream is done.
+ * zk_i4_matmul_experts: as zk_i8_matmul_experts; expert e's weights begin at
+ * d_w + e * n_out * ld_w bytes, its scales at d_w_scale[e * groups * n_out], its
+ * biases at d_bias[e * n_out].
+ * None of these allocates, waits or uses memory of the context.  Outputs may not
+ * overlap an input. */
+size_t zk_i4_row_bytes(size_t n_in);
+int zk_i4_quantize(zk_context* ctx, const void* d_w, int w_type, size_t ld_w, size_t rows, size_t cols, int group,
+                   void* d_q, size_t ld_q, void* d_scale, int scale_type, void* stream);
+int zk_i4_matmul(zk_context* ctx, const int8_t* d_x, size_t ld_x, const float* d_x_scale, const void* d_w, size_t ld_w,
+                 const void* d_w_scale, int scale_type, int group, const float* d_bias, size_t rows, size_t n_out,
+                 size_t n_in, int relu, void* d_y, int y_type, size_t ld_y, void* stream);
+size_t zk_i4_linear_work(size_t rows, size_t n_in);
+int zk_i4_linear(zk_context* ctx, const void* d_x, int x_type, size_t ld_x, const void* d_w, size_t ld_w,
+                 const void* d_w_scale, int scale_type, int group, const float* d_bias, size_t rows, size_t n_out,
+                 size_t n_in, int relu, void* d_y, int y_type, size_t ld_y, void* d_work, size_t work_bytes,
+                 void* stream);
+int zk_i4_matmul_experts(zk_context* ctx, const int8_t* d_x, size_t ld_x, const float* d_x_scale, size_t tokens,
+                         const void* d_w, size_t ld_w, const void* d_w_scale, int scale_type, int group,
+                         const float* d_bias, const int32_t* d_offsets, int experts, const int32_t* d_order, int slots,
+                         size_t rows, size_t n_out, size_t n_in, int relu, void* d_y, int y_type, size_t ld_y,
+                         void* stream);
+
 /* ---- routed experts ---------------------------------------------------------
  * No counterpart in the reference, whose routing ends with each sample's class
  * and flag (src/prover/statement_v2.cuh:243-266).  Samples ("tokens") sorted by
@@ -353,6 +403,52 @@ int zk_experts_combine_grad(zk_context* ctx, const void* d_grad, size_t ld_grad,
                             int type, size_t cols, const int32_t* d_order, const int32_t* d_place,
                             const float* d_weight, size_t rows, size_t tokens, int slots, void* d_grad_y,
                             size_t ld_grad_y, float* d_grad_weight, void* stream);
+
+/* ---- the experts' router ------------------------------------------------------
+ * No counterpart in the reference.  Which experts a token's gate scores name, with
+ * which weights, how evenly, and the gradients.  scores: tokens x experts, ZK_F32,
+ * ZK_F16, ZK_BF16, or ZK_I32 (a gate's exact sums from zk_i8_matmul), rows at
+ * stride ld.  p[t] = softmax over the experts of scale * scores[t] (scale positive
+ * and finite), in 32-bit floats.  A score of minus infinity (ZK_I32: INT32_MIN) is
+ * a masked expert: never chosen, probability 0.
+ *
+ * zk_experts_route: a token's `slots` experts (1 to 32) by falling score, of equal
+ * scores the lower expert first, as zk_experts_sort takes them, and their weights:
+ * p of the chosen, or with renormalize != 0 these divided by their sum.  A token
+ * with fewer unmasked experts has expert -1 and weight 0 in the slots that are
+ * left (all of them in a masked row: padding); one with a NaN or an infinity above
+ * has experts -1 and weights NaN.
+ * With d_count, d_prob and d_loss (all or none) also, over the n tokens that have
+ * a score other than masked,
+ *   count[e] = routes that name e (experts + 1 words; count[experts] = n),
+ *   prob[e] = sum_t p[t][e] / n,
+ *   loss = experts * sum_e count[e] / (n * slots) * prob[e]       (1 if all are even),
+ * prob and loss 0 without such a token, NaN with a NaN or an infinity above.
+ * d_work: zk_experts_route_work(tokens, experts) bytes (0: sizes out of range),
+ * 4-byte aligned, used only with these outputs.
+ * zk_experts_balance: the same three for given routes (tokens x slots); a route
+ * outside [0, experts) names none.
+ * zk_experts_route_grad: the gradient with regard to the scores of what depends
+ * on the weights by grad_weight (tokens x slots; NULL: nothing does) and on the
+ * loss by grad_loss[0] (d_count NULL: nothing does; else the counts of
+ * zk_experts_route or zk_experts_balance, constants to the gradient).  expert,
+ * scale and renormalize as in the forward call; the same expert twice counts
+ * twice.  Masked scores get 0, a row with a NaN or an infinity above NaN.
+ * At most 1024 experts and 2^22 pairs.  No result depends on the order of
+ * execution.  None of these allocates, waits or uses memory of the context; calls
+ * that overlap need a workspace each. */
+enum { ZK_MAX_SLOTS = 32 };
+size_t zk_experts_route_work(size_t tokens, int experts);
+int zk_experts_route(zk_context* ctx, const void* d_scores, int type, size_t ld, size_t tokens, int experts, int slots,
+                     float scale, int renormalize, int32_t* d_expert, float* d_weight, int32_t* d_count,
+                     float* d_prob, float* d_loss, void* d_work, size_t work_bytes, void* stream);
+int zk_experts_balance(zk_context* ctx, const void* d_scores, int type, size_t ld, size_t tokens, int experts,
+                       int slots, float scale, const int32_t* d_expert, int32_t* d_count, float* d_prob,
+                       float* d_loss, void* d_work, size_t work_bytes, void* stream);
+int zk_experts_route_grad(zk_context* ctx, const void* d_scores, int type, size_t ld, size_t tokens, int experts,
+                          int slots, float scale, int renormalize, const int32_t* d_expert,
+                          const float* d_grad_weight, const int32_t* d_count, const float* d_grad_loss,
+                          void* d_grad_scores, size_t ld_grad, void* stream);
 
 /* ---- pairing and verification (host code, no device needed) -------------
  * zk_pairing replaces bn254::pairing (src/curve/pairing.cuh:198-282): the
