@@ -22,15 +22,10 @@ constexpr size_t I4_MAX_IN = (size_t)1 << 24;  // (indexes inside a row stay far
 struct I4Args : I8Args {
   const void* scale;  // groups x n_out, for each expert
   uint32_t group, groups;
+  int y_type;
 };
 
 static __host__ __device__ inline size_t i4_row_bytes(size_t n_in) { return (n_in + 127) / 128 * 64; }
-
-// Weight k of a packed row.
-__device__ __forceinline__ int weight_at(const int8_t* row, uint32_t k) {
-  const int b = row[(k >> 7) * 64 + (k & 63)];
-  return k & 64 ? b >> 4 : (int)((uint32_t)b << 28) >> 28;
-}
 
 // sx sum + b in one rounding; what is below zero becomes zero, a NaN stays.
 __device__ __forceinline__ float i4_finish(float sum, float sx, float b, int relu) {
@@ -38,55 +33,194 @@ __device__ __forceinline__ float i4_finish(float sum, float sx, float b, int rel
   return relu && f < 0.0f ? 0.0f : f;
 }
 
-// A thread takes one result at a time.
-template <class T, class S, bool GROUPED>
-__global__ __launch_bounds__(256) void k_i4_plain(I4Args a) {
-  const uint64_t all = (uint64_t)a.rows * a.n_out, stride = (uint64_t)gridDim.x * 256;
-  for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += stride) {
-    const uint32_t p = (uint32_t)(i / a.n_out), n = (uint32_t)(i % a.n_out);
-    int64_t s = p;
-    uint32_t e = 0;
-    if (GROUPED) {
-      uint32_t hi = a.experts;  // the last expert whose rows begin at p or before, with p among them
-      while (e < hi) {
-        const uint32_t mid = (e + hi) / 2;
-        if (offset_of(a, mid + 1) <= p) e = mid + 1;
-        else hi = mid;
-      }
-      s = e < a.experts ? source_row(a, p) : -1;
+// Zeros for rows that have no token to read.
+template <class T>
+__global__ __launch_bounds__(256) void k_i4_zeros(T* __restrict__ y, size_t ld_y, uint32_t rows, uint32_t n_out) {
+  const uint64_t all = (uint64_t)rows * n_out, stride = (uint64_t)gridDim.x * 256;
+  for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += stride)
+    y[(size_t)(i / n_out) * ld_y + i % n_out] = (T)0.0f;
+}
+
+// ------------------------------------------------------------ few rows
+typedef float v4f __attribute__((ext_vector_type(4)));
+
+// 16 bytes of a row of x from byte k on, zeros from its end on; nothing outside the
+// row is read.
+__device__ __forceinline__ v4i x_piece(const int8_t* row, uint32_t k, uint32_t n_in) {
+  v4i v = {0, 0, 0, 0};
+  if (k + 16 <= n_in) {
+    __builtin_memcpy(&v, row + k, 16);
+  } else if (k < n_in) {
+    if (n_in >= 16) {
+      unsigned __int128 w;
+      __builtin_memcpy(&w, row + n_in - 16, 16);
+      w >>= 8 * (16 - (n_in - k));
+      __builtin_memcpy(&v, &w, 16);
+    } else {
+      for (uint32_t j = 0; j < n_in - k; j++) v[j >> 2] |= (int)((uint32_t)(uint8_t)row[k + j] << (8 * (j & 3)));
     }
-    float v = 0.0f;
-    if (s >= 0) {
-      const size_t ch = (size_t)e * a.n_out + n;
-      const S* scale = (const S*)a.scale + (size_t)e * a.groups * a.n_out + n;
-      float sum = 0.0f;
-      for (uint32_t g = 0; g < a.groups; g++) {
-        const uint32_t end = (g + 1) * a.group < a.n_in ? (g + 1) * a.group : a.n_in;
-        // (in parts whose sums are exact as floats)
-        for (uint32_t k0 = g * a.group; k0 < end; k0 += 8192) {
-          int acc = 0;
-          for (uint32_t k = k0; k < end && k < k0 + 8192; k++)
-            acc += (int)a.x[(size_t)s * a.ld_x + k] * weight_at(a.w + ch * a.ld_w, k);
-          sum = fmaf((float)acc, (float)scale[(size_t)g * a.n_out], sum);
+  }
+  return v;
+}
+
+// Result of row t's channel n.
+__device__ __forceinline__ void i4_put(const I4Args& a, uint32_t t, uint32_t n, float v) {
+  const size_t at = (size_t)t * a.ld_y + n;
+  if (a.y_type == ZK_F32) ((float*)a.y)[at] = v;
+  else if (a.y_type == ZK_F16) ((_Float16*)a.y)[at] = (_Float16)v;
+  else ((__bf16*)a.y)[at] = (__bf16)v;
+}
+
+// A block has 16 FT tokens x 16 FN channels, its KW waves a part of k each, in
+// steps of 128; their sums meet in LDS.  The matrix instruction takes 16 tokens (D's
+// rows) and 16 channels (its columns): a lane holds four tokens of one channel, and
+// needs one scale.  16 packed bytes of a lane are its operands of two instructions, 16
+// times the weights, which the results take back.  G: 128 for groups of whole steps,
+// 64, or 32, where an instruction's two groups are told apart by x: the lanes of the
+// other group hold zeros.  D's row 4 c + i is token 4 i + c of the 16, so that up to
+// four tokens (NI = 1) are one register of each lane.
+template <class S, int G, bool GROUPED, int FT, int FN, int NI, int KW, int U>
+__global__ __launch_bounds__(64 * KW) void k_i4_direct(I4Args a, uint32_t tiles_t, uint32_t tiles_n) {
+  constexpr uint32_t BT = NI < 4 ? 4 * NI : 16 * FT, BN = 16 * FN;
+  __shared__ __align__(16) float sums[KW][FN * FT][NI][64];
+  const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  uint32_t r0, r1, n0, e;
+  if (!block_tile<GROUPED>(a, BT, BN, tiles_t, tiles_n, r0, r1, n0, e)) return;
+  const bool none = GROUPED && e >= a.experts;
+  const uint32_t fr = lane & 15, c = lane >> 4;
+  const size_t ch = none ? 0 : (size_t)e * a.n_out;
+  const int8_t *xp[FT], *wp[FN];
+  const S* sp[FN];
+#pragma unroll
+  for (int i = 0; i < FN; i++) {
+    const uint32_t n = n0 + i * 16 + fr, m = n < a.n_out ? n : a.n_out - 1;
+    wp[i] = a.w + (ch + m) * a.ld_w + 16 * c;
+    sp[i] = (const S*)a.scale + ch * a.groups + m;
+  }
+#pragma unroll
+  for (int j = 0; j < FT; j++) {
+    const uint32_t t = r0 + j * 16 + (NI > 1 ? (fr & 3) * 4 : 0) + (fr >> 2), r = t < r1 ? t : r1 - 1;
+    const int64_t s = GROUPED ? source_row(a, r) : (int64_t)r;
+    xp[j] = a.x + (size_t)(s < 0 ? 0 : s) * a.ld_x;
+  }
+  float acc[FN][FT][NI] = {};
+  const uint32_t steps = none ? 0 : (a.n_in + 127) / 128, full = a.n_in / 128;
+  const uint32_t per = (steps + KW - 1) / KW;
+  const uint32_t first = wave * per, last = first + per < steps ? first + per : steps;
+  constexpr int NS = G >= 128 ? 1 : 128 / G;  // scales of a step
+  // G = 128: the step's group and how many of its steps are past
+  const uint32_t whole = a.group / 128;
+  uint32_t group = 0, past = 0;
+  if (G >= 128) group = first / whole, past = first % whole;
+  for (uint32_t s0 = first; s0 < last; s0 += U) {
+    v4i wf[U][FN], xf[U][FT][2];
+    S sc[U][FN][NS];
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      const uint32_t step = s0 + u < last ? s0 + u : last - 1;  // (again the last one, not used)
+#pragma unroll
+      for (int i = 0; i < FN; i++) wf[u][i] = *(const v4i*)(wp[i] + (size_t)step * 64);
+#pragma unroll
+      for (int k = 0; k < NS; k++) {
+        uint32_t g = G >= 128 ? group : step * NS + k;
+        if (G < 128 && g >= a.groups) g = a.groups - 1;  // (behind the row's end: x is zero)
+#pragma unroll
+        for (int i = 0; i < FN; i++) sc[u][i][k] = sp[i][(size_t)g * a.n_out];
+      }
+      if (G >= 128 && s0 + u + 1 < last && ++past == whole) past = 0, group++;
+      if (step < full) {
+#pragma unroll
+        for (int j = 0; j < FT; j++)
+#pragma unroll
+          for (int h = 0; h < 2; h++) __builtin_memcpy(&xf[u][j][h], xp[j] + step * 128 + 64 * h + 16 * c, 16);
+      } else {
+#pragma unroll
+        for (int j = 0; j < FT; j++)
+#pragma unroll
+          for (int h = 0; h < 2; h++) xf[u][j][h] = x_piece(xp[j], step * 128 + 64 * h + 16 * c, a.n_in);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      if (s0 + u >= last) break;
+#pragma unroll
+      for (int i = 0; i < FN; i++) {
+        const v4i high = wf[u][i] & (int)0xf0f0f0f0, low = (wf[u][i] << 4) & (int)0xf0f0f0f0;
+#pragma unroll
+        for (int j = 0; j < FT; j++) {
+          const v4i zero = {0, 0, 0, 0};
+          v4i part[NS];
+          if (G >= 128) {
+            part[0] = __builtin_amdgcn_mfma_i32_16x16x64_i8(xf[u][j][0], low, zero, 0, 0, 0);
+            part[0] = __builtin_amdgcn_mfma_i32_16x16x64_i8(xf[u][j][1], high, part[0], 0, 0, 0);
+          } else if (G == 64) {
+            part[0] = __builtin_amdgcn_mfma_i32_16x16x64_i8(xf[u][j][0], low, zero, 0, 0, 0);
+            part[NS - 1] = __builtin_amdgcn_mfma_i32_16x16x64_i8(xf[u][j][1], high, zero, 0, 0, 0);
+          } else {
+#pragma unroll
+            for (int k = 0; k < NS; k++) {
+              const v4i x = (int)c / 2 == k % 2 ? xf[u][j][k / 2] : zero;
+              part[k] = __builtin_amdgcn_mfma_i32_16x16x64_i8(x, k < 2 ? low : high, zero, 0, 0, 0);
+            }
+          }
+#pragma unroll
+          for (int k = 0; k < NS; k++)
+#pragma unroll
+            for (int q = 0; q < NI; q++) acc[i][j][q] = fmaf((float)part[k][q], (float)sc[u][i][k], acc[i][j][q]);
         }
       }
-      v = i4_finish(sum, a.sx ? a.sx[s] : 1.0f, a.bias ? a.bias[ch] : 0.0f, a.relu);
     }
-    ((T*)a.y)[(size_t)p * a.ld_y + n] = (T)v;
+  }
+#pragma unroll
+  for (int i = 0; i < FN; i++)
+#pragma unroll
+    for (int j = 0; j < FT; j++)
+#pragma unroll
+      for (int q = 0; q < NI; q++) sums[wave][i * FT + j][q][lane] = acc[i][j][q];
+  __syncthreads();
+  // a wave adds up every KW-th register of the squares
+#pragma unroll
+  for (int r = 0; r < FN * FT * NI; r++) {
+    if ((uint32_t)r % KW != wave) continue;
+    const int sq = r / NI, q = r % NI;
+    const uint32_t t = r0 + (sq % FT) * 16 + 4 * q + c, n = n0 + (sq / FT) * 16 + fr;
+    if (t >= r1 || t >= r0 + BT || n >= a.n_out) continue;
+    float sum = sums[0][sq][q][lane];
+#pragma unroll
+    for (int k = 1; k < KW; k++) sum += sums[k][sq][q][lane];
+    const int64_t s = none ? -1 : GROUPED ? source_row(a, t) : (int64_t)t;
+    float v = 0.0f;
+    if (s >= 0) v = i4_finish(sum * 0.0625f, a.sx ? a.sx[s] : 1.0f, a.bias ? a.bias[ch + n] : 0.0f, a.relu);
+    i4_put(a, t, n, v);
   }
 }
 
-template <bool GROUPED>
-static int i4_dispatch(zk_context* ctx, const I4Args& a, int scale_type, int type, hipStream_t st) {
+template <class S, int G, bool GROUPED>
+static int i4_launch(zk_context* ctx, const I4Args& a, hipStream_t st) {
   const char* name = GROUPED ? "i4_matmul_experts" : "i4_matmul";
-  return by_type(type, [&](auto yz) -> int {
-    return by_type(scale_type, [&](auto sz) -> int {
-      typedef decltype(yz) T;
-      typedef decltype(sz) S;
-      const size_t blocks = ((size_t)a.rows * a.n_out + 255) / 256;
-      ZK_LAUNCH(ctx, st, name, (k_i4_plain<T, S, GROUPED>), dim3(blocks < 65536 ? (uint32_t)blocks : 65536), dim3(256), 0, a);
-      return ZK_OK;
-    });
+  auto go = [&](auto kernel, uint32_t threads, uint32_t bt, uint32_t bn) -> int {
+    const uint32_t groups = a.experts + 1 < a.rows ? a.experts + 1 : a.rows;
+    const uint32_t tiles_t = GROUPED ? a.rows / bt + groups : cdiv(a.rows, bt), tiles_n = cdiv(a.n_out, bn);
+    const size_t tiles = (size_t)tiles_t * tiles_n;
+    if (tiles > I8_MAX_TILES) return ctx->fail(ZK_ERR_SIZE, "i4 product: rows and n_out make too many tiles");
+    ZK_LAUNCH(ctx, st, name, kernel, dim3(cdiv(tiles, 8) * 8), dim3(threads), 0, a, tiles_t, tiles_n);
+    return ZK_OK;
+  };
+  // rows of one expert, about
+  const uint32_t rows = GROUPED ? cdiv(a.rows, a.experts < a.rows ? a.experts : a.rows) : a.rows;
+  if (rows <= 4) return go(k_i4_direct<S, G, GROUPED, 1, 1, 1, 8, 4>, 512, 4, 16);
+  if (rows <= 16) return go(k_i4_direct<S, G, GROUPED, 1, 1, 4, 8, 4>, 512, 16, 16);
+  if (rows <= 32) return go(k_i4_direct<S, G, GROUPED, 2, 2, 4, 8, 2>, 512, 32, 32);
+  return go(k_i4_direct<S, G, GROUPED, 4, 2, 4, 8, 2>, 512, 64, 32);
+}
+
+template <bool GROUPED>
+static int i4_dispatch(zk_context* ctx, const I4Args& a, int scale_type, hipStream_t st) {
+  return by_type(scale_type, [&](auto sz) -> int {
+    typedef decltype(sz) S;
+    if (a.group == 32) return i4_launch<S, 32, GROUPED>(ctx, a, st);
+    if (a.group == 64) return i4_launch<S, 64, GROUPED>(ctx, a, st);
+    return i4_launch<S, 128, GROUPED>(ctx, a, st);
   });
 }
 
@@ -171,7 +305,8 @@ static int check_i4(zk_context* ctx, const I4Args& a, size_t rows, size_t n_out,
   return ZK_OK;
 }
 
-static void set_sizes(I4Args& a, size_t rows, size_t n_out, size_t n_in, int group, int relu) {
+static void set_sizes(I4Args& a, size_t rows, size_t n_out, size_t n_in, int group, int relu, int type) {
+  a.y_type = type;
   a.rows = (uint32_t)rows, a.n_out = (uint32_t)n_out, a.n_in = (uint32_t)n_in, a.relu = relu != 0;
   a.group = (uint32_t)group, a.groups = cdiv(n_in, group);
 }
@@ -185,7 +320,7 @@ static int i4_matmul(zk_context* ctx, const I4Args& a, int scale_type, int type,
     b.x = a.x ? a.x + r * a.ld_x : a.x;
     b.sx = a.sx ? a.sx + r : a.sx;
     b.y = (uint8_t*)a.y + r * a.ld_y * type_bytes(type);
-    ZK_TRY(i4_dispatch<false>(ctx, b, scale_type, type, st));
+    ZK_TRY(i4_dispatch<false>(ctx, b, scale_type, st));
   }
   return ZK_OK;
 }
@@ -241,7 +376,7 @@ int zk_i4_matmul(zk_context* ctx, const int8_t* d_x, size_t ld_x, const float* d
     a.ld_x = ld_x, a.ld_w = ld_w, a.ld_y = ld_y;
     ZK_TRY(check_i4(ctx, a, rows, n_out, n_in, group, scale_type, y_type));
     if (!rows || !n_out) return ZK_OK;
-    set_sizes(a, rows, n_out, n_in, group, relu);
+    set_sizes(a, rows, n_out, n_in, group, relu, y_type);
     OnDevice on(ctx);
     return i4_matmul(ctx, a, scale_type, y_type, ctx->s(stream));
   });
@@ -270,7 +405,7 @@ int zk_i4_linear(zk_context* ctx, const void* d_x, int x_type, size_t ld_x, cons
     if (!rows || !n_out) return ZK_OK;
     if (!d_work || !aligned(d_work, 16) || work_bytes < lw.bytes)
       return ctx->fail(ZK_ERR_INVALID, "i4 linear: workspace missing, too small or not aligned to 16 bytes");
-    set_sizes(a, rows, n_out, n_in, group, relu);
+    set_sizes(a, rows, n_out, n_in, group, relu, y_type);
     OnDevice on(ctx);
     hipStream_t st = ctx->s(stream);
     ZK_TRY(i8_quantize(ctx, d_x, x_type, ld_x, rows, n_in, (int8_t*)d_work + lw.q, lw.ld, (float*)d_work, st));
@@ -299,11 +434,20 @@ int zk_i4_matmul_experts(zk_context* ctx, const int8_t* d_x, size_t ld_x, const 
     if (!d_offsets) return ctx->fail(ZK_ERR_INVALID, "i4 experts: null pointer");
     if (!aligned(d_offsets, 4) || !aligned(d_order, 4))
       return ctx->fail(ZK_ERR_INVALID, "i4 experts: a pointer is not aligned to its type");
-    set_sizes(a, rows, n_out, n_in, group, relu);
+    set_sizes(a, rows, n_out, n_in, group, relu, y_type);
     a.offsets = d_offsets, a.order = d_order, a.experts = (uint32_t)experts, a.slots = (uint32_t)slots;
     a.tokens = (uint32_t)tokens;
     OnDevice on(ctx);
-    return i4_dispatch<true>(ctx, a, scale_type, y_type, ctx->s(stream));
+    if (!tokens) {
+      const size_t blocks = (rows * n_out + 255) / 256;
+      return by_type(y_type, [&](auto zero) -> int {
+        ZK_LAUNCH(ctx, ctx->s(stream), "i4_matmul_experts", k_i4_zeros<decltype(zero)>,
+                  dim3(blocks < 65536 ? (uint32_t)blocks : 65536), dim3(256), 0, (decltype(zero)*)d_y, ld_y, a.rows,
+                  a.n_out);
+        return ZK_OK;
+      });
+    }
+    return i4_dispatch<true>(ctx, a, scale_type, ctx->s(stream));
   });
 }
 
