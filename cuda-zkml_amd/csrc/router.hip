@@ -27,6 +27,9 @@
 namespace zk {
 
 constexpr int ROUTE_THREADS = 256;
+// Threads of a block that also makes counts and sums: many waves, so that few
+// blocks' sums are left to be added up.
+constexpr int balance_threads(int lanes) { return lanes == 16 ? 1024 : 512; }
 
 struct RouteArgs {
   const void* scores;
@@ -36,37 +39,79 @@ struct RouteArgs {
   int renormalize;
   int32_t* expert;   // tokens x slots; given where the routes are
   float* weight;     // tokens x slots
-  float* part_prob;  // of each block: sums of p by expert
-  uint32_t* part_count;  // of each block: counts by expert, and tokens with a score
 };
 
+// exp(a) for a <= 0 (or NaN): the hardware's 2^x of a's product with log2(e), whose
+// rounding error and whose factor's are made good by one step; below 2^-126 zero.
+__device__ __forceinline__ float exp_down(float a) {
+  constexpr float L = 1.44269504f, REST = 1.925963033e-8f, LN2 = 0.693147181f;  // log2(e) = L + REST
+  a = fmaxf(a, -200.0f);
+  const float t = a * L, lost = fmaf(a, REST, fmaf(a, L, -t)), p = __builtin_amdgcn_exp2f(t);
+  return fmaf(p, lost * LN2, p);
+}
+
 // What scores are compared as: floats, or integers; NONE is a masked expert's.
+// 16-bit scores have a key each, which orders them and names their expert: no
+// two keys of a row are equal, and one maximum finds the next expert.
 template <class T>
 struct Score {
   typedef float W;
+  static constexpr bool KEYED = sizeof(T) == 2;
   static __device__ __forceinline__ float none() { return -INFINITY; }
   static __device__ __forceinline__ float read(T s) { return (float)s + 0.0f; }  // (-0 and 0 are equal)
   // NaN and infinity leave a row without a softmax
   static __device__ __forceinline__ bool bad(float v) { return !(v < INFINITY); }
   // exp(scale (v - m)); v <= m, m a score
-  static __device__ __forceinline__ float ex(float v, float m, float scale) { return expf((v - m) * scale); }
+  static __device__ __forceinline__ float ex(float v, float m, float scale) { return exp_down((v - m) * scale); }
+  // 0: masked, else the score's rank among all of the type above, the expert below
+  static __device__ __forceinline__ uint32_t key(float v, uint32_t e) {
+    uint16_t b;
+    const T s = (T)v;
+    __builtin_memcpy(&b, &s, 2);
+    const uint32_t rank = b & 0x8000u ? (uint16_t)~b : b | 0x8000u;
+    return v == none() ? 0u : rank << 16 | (0xffffu - e);
+  }
+  static __device__ __forceinline__ float of_key(uint32_t key) {
+    const uint32_t rank = key >> 16;
+    const uint16_t b = (uint16_t)(rank & 0x8000u ? rank & 0x7fffu : ~rank);
+    T s;
+    __builtin_memcpy(&s, &b, 2);
+    return (float)s;
+  }
 };
 template <>
 struct Score<int> {
   typedef int W;
+  static constexpr bool KEYED = false;
   static __device__ __forceinline__ int none() { return INT32_MIN; }
   static __device__ __forceinline__ int read(int s) { return s; }
   static __device__ __forceinline__ bool bad(int) { return false; }
   static __device__ __forceinline__ float ex(int v, int m, float scale) {
-    return v == none() ? 0.0f : expf(-(float)((uint32_t)m - (uint32_t)v) * scale);
+    return v == none() ? 0.0f : exp_down(-(float)((uint32_t)m - (uint32_t)v) * scale);
   }
 };
 
-template <int L, class X, class F>
-__device__ __forceinline__ X over_lanes(X v, F&& f) {
-#pragma unroll
-  for (int d = L / 2; d; d >>= 1) v = f(v, __shfl_xor(v, d));
+// What a lane's partner holds: the lanes of a row of 16 by data-parallel moves, which
+// take no trip through LDS; after the steps before, all lanes of the partner's half
+// hold the same.
+template <int D, class X>
+__device__ __forceinline__ X partner(X v) {
+  static_assert(sizeof(X) == 4, "one register");
+  int b;
+  __builtin_memcpy(&b, &v, 4);
+  if constexpr (D == 1) b = __builtin_amdgcn_update_dpp(b, b, 0xb1, 0xf, 0xf, false);         // quad: 1 0 3 2
+  else if constexpr (D == 2) b = __builtin_amdgcn_update_dpp(b, b, 0x4e, 0xf, 0xf, false);    // quad: 2 3 0 1
+  else if constexpr (D == 4) b = __builtin_amdgcn_update_dpp(b, b, 0x141, 0xf, 0xf, false);   // half row, mirrored
+  else if constexpr (D == 8) b = __builtin_amdgcn_update_dpp(b, b, 0x140, 0xf, 0xf, false);   // row, mirrored
+  else b = __shfl_xor(b, D);
+  __builtin_memcpy(&v, &b, 4);
   return v;
+}
+// f over a token's L lanes; every lane has the result, and the same one.
+template <int L, int D = 1, class X, class F>
+__device__ __forceinline__ X over_lanes(X v, F&& f) {
+  if constexpr (D < L) return over_lanes<L, 2 * D>(f(v, partner<D>(v)), f);
+  else return v;
 }
 template <int L, class X>
 __device__ __forceinline__ X max_over(X v) {
@@ -96,19 +141,57 @@ __device__ __forceinline__ void load_scores(const T* row, uint32_t first, uint32
   }
 }
 
+// Counts and sums of p of all tokens to count, prob and loss, by a block's threads;
+// expert e's from get(e) (its count, and its sum of p), loss's part of these experts
+// from the first thread.  Counts below 2^24, sums in 64 bits.
+template <int THREADS, class Get>
+__device__ __forceinline__ double balance_of(uint32_t lo, uint32_t hi, uint32_t n, uint32_t experts, uint32_t slots,
+                                             int32_t* count, float* prob, Get&& get) {
+  __shared__ double part[THREADS / 64];
+  double x = 0.0;
+  for (uint32_t e = lo + threadIdx.x; e < hi; e += THREADS) {
+    uint32_t c;
+    double s;
+    get(e, c, s);
+    const double mean = n ? s / n : 0.0;
+    count[e] = (int32_t)c;
+    prob[e] = (float)mean;
+    if (n) x += mean * c / ((double)n * slots);
+  }
+#pragma unroll
+  for (int d = 32; d; d >>= 1) x += __shfl_xor(x, d);
+  if (threadIdx.x % 64 == 0) part[threadIdx.x / 64] = x;
+  __syncthreads();
+  if (threadIdx.x == 0)
+    for (int w = 1; w < THREADS / 64; w++) x += part[w];
+  return x * experts;
+}
+
+// Where a call's sums go: of each block, then by expert to the caller's arrays.
+struct BalanceOut {
+  int32_t* count;
+  float* prob;
+  float* loss;
+  double* loss_part;  // of each block of the last step
+  uint32_t* ticket;   // blocks of the last step that are done
+  float* part_prob;      // of each block: sums of p by expert
+  uint32_t* part_count;  // of each block: counts by expert, and tokens with a score
+};
+
 // CHOOSE: a token's experts and weights are found; else given.  BALANCE: counts
-// and sums of p are made.
+// and sums of p are made; one block alone makes the caller's results of them.
 template <class T, int L, int V, bool CHOOSE, bool BALANCE>
-__global__ __launch_bounds__(ROUTE_THREADS) void k_route(RouteArgs a) {
+__global__ __launch_bounds__(BALANCE ? balance_threads(L) : ROUTE_THREADS) void k_route(RouteArgs a, BalanceOut out) {
   typedef Score<T> S;
   typedef typename S::W W;
-  constexpr uint32_t GROUPS = ROUTE_THREADS / L, WAVES = ROUTE_THREADS / 64;
+  constexpr uint32_t THREADS = BALANCE ? balance_threads(L) : ROUTE_THREADS, GROUPS = THREADS / L, WAVES = THREADS / 64;
   constexpr int KEPT = (ZK_MAX_SLOTS + L - 1) / L;
   __shared__ uint32_t count[BALANCE ? L * V + 1 : 1];
   __shared__ float sums[BALANCE ? WAVES * L * V : 1];
   const uint32_t tid = threadIdx.x, l = tid % L, first = l * V;
   if (BALANCE) {
-    for (uint32_t e = tid; e <= a.experts; e += ROUTE_THREADS) count[e] = 0;
+    for (uint32_t e = tid; e <= a.experts; e += THREADS) count[e] = 0;
+    if (blockIdx.x == 0 && tid == 0 && gridDim.x > 1) *out.ticket = 0;
     __syncthreads();
   }
   float psum[V] = {};
@@ -116,6 +199,11 @@ __global__ __launch_bounds__(ROUTE_THREADS) void k_route(RouteArgs a) {
   for (uint32_t t0 = blockIdx.x * GROUPS; t0 < a.tokens; t0 += gridDim.x * GROUPS) {
     const uint32_t t = t0 + tid / L;
     if (t >= a.tokens) continue;  // (all of the token's lanes)
+    int given[KEPT];
+    if (!CHOOSE) {
+#pragma unroll
+      for (int k = 0; k < KEPT; k++) given[k] = l + k * L < a.slots ? a.expert[(size_t)t * a.slots + l + k * L] : -1;
+    }
     W v[V];
     load_scores<T, V>((const T*)a.scores + (size_t)t * a.ld, first, a.experts, v);
     W top = S::none();
@@ -147,10 +235,9 @@ __global__ __launch_bounds__(ROUTE_THREADS) void k_route(RouteArgs a) {
       if (l == 0 && !empty) atomicAdd(&count[a.experts], 1u);
     }
     if (!CHOOSE) {
-      for (uint32_t j = l; j < a.slots; j += L) {
-        const uint32_t e = (uint32_t)a.expert[(size_t)t * a.slots + j];
-        if (e < a.experts) atomicAdd(&count[e], 1u);
-      }
+#pragma unroll
+      for (int k = 0; k < KEPT; k++)
+        if ((uint32_t)given[k] < a.experts) atomicAdd(&count[given[k]], 1u);
       continue;
     }
     int kept_e[KEPT];
@@ -158,25 +245,42 @@ __global__ __launch_bounds__(ROUTE_THREADS) void k_route(RouteArgs a) {
 #pragma unroll
     for (int k = 0; k < KEPT; k++) kept_e[k] = -1, kept_w[k] = bad ? NAN : 0.0f;
     float total = 0.0f;
+    uint32_t key[S::KEYED ? V : 1];
+    if constexpr (S::KEYED) {
+#pragma unroll
+      for (int i = 0; i < V; i++) key[i] = S::key(v[i], first + i);
+    }
     for (uint32_t j = 0; j < a.slots && !bad; j++) {
-      // a lane's first largest score, then the lowest expert that has the largest of all
-      W b = S::none();
+      W best = S::none();
       uint32_t e = a.experts;
+      if constexpr (S::KEYED) {
+        uint32_t b = 0;
 #pragma unroll
-      for (int i = 0; i < V; i++)
-        if (v[i] > b) b = v[i], e = first + i;
-      const W best = max_over<L>(b);
-      if (best == S::none()) break;
-      e = min_over<L>(b == best ? e : a.experts);
+        for (int i = 0; i < V; i++) b = key[i] > b ? key[i] : b;
+        b = max_over<L>(b);
+        if (!b) break;
 #pragma unroll
-      for (int i = 0; i < V; i++)
-        if (first + i == e) v[i] = S::none();
+        for (int i = 0; i < V; i++) key[i] = key[i] == b ? 0u : key[i];
+        e = 0xffffu - (b & 0xffffu);
+        best = S::of_key(b);
+      } else {
+        // a lane's first largest score, then the lowest expert that has the largest of all
+        W b = S::none();
+#pragma unroll
+        for (int i = 0; i < V; i++)
+          if (v[i] > b) b = v[i], e = first + i;
+        best = max_over<L>(b);
+        if (best == S::none()) break;
+        e = min_over<L>(b == best ? e : a.experts);
+#pragma unroll
+        for (int i = 0; i < V; i++)
+          if (first + i == e) v[i] = S::none();
+      }
       const float w = S::ex(best, m, a.scale);
       total += w;
 #pragma unroll
       for (int k = 0; k < KEPT; k++)
         if (j == l + k * L) kept_e[k] = (int)e, kept_w[k] = w;
-      if (BALANCE && l == 0) atomicAdd(&count[e], 1u);
     }
     const float by = a.renormalize ? (total > 0.0f ? 1.0f / total : 0.0f) : inv;
 #pragma unroll
@@ -185,66 +289,82 @@ __global__ __launch_bounds__(ROUTE_THREADS) void k_route(RouteArgs a) {
         const size_t at = (size_t)t * a.slots + l + k * L;
         a.expert[at] = kept_e[k];
         a.weight[at] = bad ? kept_w[k] : kept_w[k] * by;
+        if (BALANCE && kept_e[k] >= 0) atomicAdd(&count[kept_e[k]], 1u);
       }
   }
-  if (!BALANCE) return;
-  // the wave's tokens, then the waves, in a fixed order
+  if constexpr (BALANCE) {
+    // the wave's tokens, then the waves, in a fixed order
 #pragma unroll
-  for (int i = 0; i < V; i++) {
+    for (int i = 0; i < V; i++) {
 #pragma unroll
-    for (int d = L; d < 64; d <<= 1) psum[i] += __shfl_xor(psum[i], d);
-    if (tid % 64 < L) sums[(tid / 64) * L * V + first + i] = psum[i];
-  }
-  __syncthreads();
-  for (uint32_t e = tid; e <= a.experts; e += ROUTE_THREADS) {
-    a.part_count[(size_t)blockIdx.x * (a.experts + 1) + e] = count[e];
-    if (e == a.experts) break;
-    float s = sums[e];
+      for (int d = L; d < 64; d <<= 1) psum[i] += __shfl_xor(psum[i], d);
+      if (tid % 64 < L) sums[(tid / 64) * L * V + first + i] = psum[i];
+    }
+    __syncthreads();
+    auto sum = [&](uint32_t e) {
+      float s = sums[e];
 #pragma unroll
-    for (uint32_t w = 1; w < WAVES; w++) s += sums[w * L * V + e];
-    a.part_prob[(size_t)blockIdx.x * a.experts + e] = s;
+      for (uint32_t w = 1; w < WAVES; w++) s += sums[w * L * V + e];
+      return s;
+    };
+    if (gridDim.x == 1) {
+      const uint32_t n = count[a.experts];
+      const double loss = balance_of<THREADS>(0, a.experts, n, a.experts, a.slots, out.count, out.prob,
+                                              [&](uint32_t e, uint32_t& c, double& s) { c = count[e], s = sum(e); });
+      if (tid == 0) *out.loss = (float)loss, out.count[a.experts] = (int32_t)n;
+      return;
+    }
+    for (uint32_t e = tid; e <= a.experts; e += THREADS) {
+      out.part_count[(size_t)blockIdx.x * (a.experts + 1) + e] = count[e];
+      if (e < a.experts) out.part_prob[(size_t)blockIdx.x * a.experts + e] = sum(e);
+    }
   }
 }
 
-// The blocks' counts and sums to count, prob and loss; sums in 64 bits, in the
-// order of the blocks.
-__global__ __launch_bounds__(1024) void k_balance_finish(const float* __restrict__ part_prob,
-                                                         const uint32_t* __restrict__ part_count, uint32_t blocks,
-                                                         uint32_t experts, uint32_t slots,
-                                                         int32_t* __restrict__ count, float* __restrict__ prob,
-                                                         float* __restrict__ loss) {
-  __shared__ uint32_t tokens;
-  __shared__ double part[16];
-  const uint32_t e = threadIdx.x;
-  uint32_t c = 0;
+// The blocks' counts and sums to the caller's: a block has 32 experts and shares the
+// blocks' rows among eight threads each, in a fixed order; the loss is put together by
+// the block that is done last, from all blocks' parts in their order.
+constexpr uint32_t FINISH_EXPERTS = 32;
+__global__ __launch_bounds__(256) void k_balance_finish(BalanceOut out, uint32_t blocks, uint32_t experts,
+                                                        uint32_t slots) {
+  constexpr uint32_t E = FINISH_EXPERTS, PARTS = 256 / E;
+  __shared__ uint32_t c_part[PARTS][E], n_part[4];
+  __shared__ double s_part[PARTS][E];
+  const uint32_t tid = threadIdx.x, x = tid % E, y = tid / E, e = blockIdx.x * E + x;
+  uint32_t c = 0, n = 0;
   double s = 0.0;
-  if (e < experts)
-    for (uint32_t b = 0; b < blocks; b++) {
-      c += part_count[(size_t)b * (experts + 1) + e];
-      s += part_prob[(size_t)b * experts + e];
-    }
-  if (e == 0) {
-    uint32_t n = 0;
-    for (uint32_t b = 0; b < blocks; b++) n += part_count[(size_t)b * (experts + 1) + experts];
-    tokens = n;
-    count[experts] = (int32_t)n;
-  }
-  __syncthreads();
-  const uint32_t n = tokens;
-  const double mean = n ? s / n : 0.0;
   if (e < experts) {
-    count[e] = (int32_t)c;
-    prob[e] = (float)mean;
+#pragma unroll 8
+    for (uint32_t b = y; b < blocks; b += PARTS) {
+      c += out.part_count[(size_t)b * (experts + 1) + e];
+      s += out.part_prob[(size_t)b * experts + e];
+    }
   }
-  double x = n && e < experts ? mean * c / ((double)n * slots) : 0.0;
+  for (uint32_t b = tid; b < blocks; b += 256) n += out.part_count[(size_t)b * (experts + 1) + experts];
 #pragma unroll
-  for (int d = 32; d; d >>= 1) x += __shfl_xor(x, d);
-  if (e % 64 == 0) part[e / 64] = x;
+  for (int d = 32; d; d >>= 1) n += __shfl_xor(n, d);
+  if (tid % 64 == 0) n_part[tid / 64] = n;
+  c_part[y][x] = c, s_part[y][x] = s;
   __syncthreads();
-  if (e == 0) {
-    for (int w = 1; w < 16; w++) x += part[w];
-    *loss = (float)(x * experts);
+  n = n_part[0] + n_part[1] + n_part[2] + n_part[3];
+  const uint32_t lo = blockIdx.x * E, hi = lo + E < experts ? lo + E : experts;
+  double loss = balance_of<256>(lo, hi, n, experts, slots, out.count, out.prob,
+                                [&](uint32_t f, uint32_t& fc, double& fs) {
+                                  fc = 0, fs = 0.0;
+#pragma unroll
+                                  for (uint32_t p = 0; p < PARTS; p++) fc += c_part[p][f - lo], fs += s_part[p][f - lo];
+                                });
+  if (tid) return;
+  if (blockIdx.x == 0) out.count[experts] = (int32_t)n;
+  if (gridDim.x > 1) {
+    __hip_atomic_store(&out.loss_part[blockIdx.x], loss, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    const uint32_t done = __hip_atomic_fetch_add(out.ticket, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
+    if (done + 1 < gridDim.x) return;
+    loss = 0.0;
+    for (uint32_t b = 0; b < gridDim.x; b++)
+      loss += __hip_atomic_load(&out.loss_part[b], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   }
+  *out.loss = (float)loss;
 }
 
 // ------------------------------------------------------------ gradient
@@ -253,7 +373,6 @@ struct RouteGradArgs {
   size_t ld, ld_grad;
   uint32_t tokens, experts, slots;
   float scale;
-  int renormalize;
   const int32_t* expert;
   const float* grad_weight;  // or null
   const int32_t* count;      // or null
@@ -261,10 +380,11 @@ struct RouteGradArgs {
   void* grad;
 };
 
-template <class T, int L, int V>
+template <class T, int L, int V, bool NORMAL>
 __global__ __launch_bounds__(ROUTE_THREADS) void k_route_grad(RouteGradArgs a) {
   typedef Score<T> S;
   constexpr uint32_t GROUPS = ROUTE_THREADS / L;
+  constexpr int KEPT = (ZK_MAX_SLOTS + L - 1) / L;
   const uint32_t tid = threadIdx.x, l = tid % L, first = l * V;
   // the loss's factors of this lane's experts: g experts / n, and f
   float f[V] = {}, c = 0.0f;
@@ -282,6 +402,16 @@ __global__ __launch_bounds__(ROUTE_THREADS) void k_route_grad(RouteGradArgs a) {
     const uint32_t t = t0 + tid / L;
     if (t >= a.tokens) continue;  // (all of the token's lanes)
     float v[V], p[V], d[V];
+    // the token's routes, a lane each (two where there are more than lanes)
+    int named[KEPT];
+    float gw[KEPT];
+#pragma unroll
+    for (int k = 0; k < KEPT; k++) {
+      const bool on = a.grad_weight && l + k * L < a.slots;
+      const size_t at = (size_t)t * a.slots + l + k * L;
+      named[k] = on ? a.expert[at] : -1;
+      gw[k] = on ? a.grad_weight[at] : 0.0f;
+    }
     load_scores<T, V>((const T*)a.scores + (size_t)t * a.ld, first, a.experts, v);
     float top = S::none();
     bool bad = false;
@@ -311,13 +441,20 @@ __global__ __launch_bounds__(ROUTE_THREADS) void k_route_grad(RouteGradArgs a) {
       if (a.grad_weight) {
         float g[V] = {}, times[V] = {};
         for (uint32_t j = 0; j < a.slots; j++) {
-          const uint32_t e = (uint32_t)a.expert[(size_t)t * a.slots + j];
-          const float gj = a.grad_weight[(size_t)t * a.slots + j];
+          int e = __shfl(named[0], j, L);
+          float gj = __shfl(gw[0], j, L);
+          if constexpr (KEPT > 1) {
+            if (j >= L) e = __shfl(named[1], j - L, L), gj = __shfl(gw[1], j - L, L);
+          }
+          if ((uint32_t)e >= a.experts) continue;
 #pragma unroll
           for (int i = 0; i < V; i++)
-            if (first + i < a.experts && first + i == e) g[i] += gj, times[i] += 1.0f;
+            if (first + i == (uint32_t)e) {
+              g[i] += gj;
+              if (NORMAL) times[i] += 1.0f;
+            }
         }
-        if (a.renormalize) {
+        if constexpr (NORMAL) {
           // softmax over the chosen alone: their own maximum, sum and mean
           float mc = S::none(), zc = 0.0f, gc = 0.0f;
 #pragma unroll
@@ -360,30 +497,40 @@ __global__ __launch_bounds__(ROUTE_THREADS) void k_route_grad(RouteGradArgs a) {
 }
 
 // ------------------------------------------------------------ which lanes
-// Calls fn with the lanes a token gets and the scores of a lane.
+// Calls fn with the lanes a token gets and the scores of a lane: 16 lanes, whose
+// reductions need no LDS, as long as their scores fit the registers.
 template <class Fn>
 static int by_experts(uint32_t experts, Fn&& fn) {
   using std::integral_constant;
-  const integral_constant<int, 16> quarter;
-  const integral_constant<int, 64> whole;
-  if (experts <= 16) return fn(quarter, integral_constant<int, 1>());
-  if (experts <= 32) return fn(quarter, integral_constant<int, 2>());
-  if (experts <= 64) return fn(quarter, integral_constant<int, 4>());
-  if (experts <= 128) return fn(quarter, integral_constant<int, 8>());
-  if (experts <= 256) return fn(whole, integral_constant<int, 4>());
-  if (experts <= 512) return fn(whole, integral_constant<int, 8>());
-  return fn(whole, integral_constant<int, 16>());
+  const integral_constant<int, 16> row;
+  if (experts <= 16) return fn(row, integral_constant<int, 1>());
+  if (experts <= 32) return fn(row, integral_constant<int, 2>());
+  if (experts <= 64) return fn(row, integral_constant<int, 4>());
+  if (experts <= 128) return fn(row, integral_constant<int, 8>());
+  if (experts <= 256) return fn(row, integral_constant<int, 16>());
+  if (experts <= 512) return fn(integral_constant<int, 32>(), integral_constant<int, 16>());
+  return fn(integral_constant<int, 64>(), integral_constant<int, 16>());
 }
+static int lanes_of(int experts) { return experts <= 256 ? 16 : experts <= 512 ? 32 : 64; }
 
-constexpr uint32_t ROUTE_BLOCKS = 1024;    // of a launch at the most (then a block has several tokens a group)
-constexpr uint32_t BALANCE_BLOCKS = 128;   // whose sums one block adds up
+constexpr uint32_t ROUTE_BLOCKS = 2048;   // of a launch at the most (then a block has several tokens a group)
+constexpr uint32_t BALANCE_BLOCKS = 256;  // one a CU
+constexpr size_t BALANCE_ONE = 256;       // tokens that one block takes alone, in one launch
 
-static uint32_t route_blocks(size_t tokens, int lanes, uint32_t most) {
-  const uint32_t b = cdiv(tokens, ROUTE_THREADS / lanes);
+static uint32_t route_blocks(size_t tokens, uint32_t a_block, uint32_t most) {
+  const uint32_t b = cdiv(tokens, a_block);
   return b < most ? b : most;
 }
 static uint32_t balance_blocks(size_t tokens, int experts) {
-  return route_blocks(tokens, experts <= 128 ? 16 : 64, BALANCE_BLOCKS);
+  if (tokens <= BALANCE_ONE) return 1;
+  const int lanes = lanes_of(experts);
+  return route_blocks(tokens, balance_threads(lanes) / lanes, BALANCE_BLOCKS);
+}
+// A workspace: the last step's parts of the loss and ticket, then the blocks' sums and
+// counts; none for one block.
+static size_t balance_work(size_t tokens, int experts) {
+  const uint32_t blocks = balance_blocks(tokens, experts);
+  return blocks > 1 ? 8 * (ZK_MAX_EXPERTS / FINISH_EXPERTS + 1) + (size_t)blocks * (2 * experts + 1) * 4 : 0;
 }
 
 // ------------------------------------------------------------ arguments
@@ -419,35 +566,39 @@ static int by_score_type(int type, Fn&& fn) {
 }
 
 template <bool CHOOSE>
-static int route(zk_context* ctx, RouteArgs a, int type, int32_t* count, float* prob, float* loss, void* work,
-                 size_t work_bytes, hipStream_t st) {
-  const bool balance = count != nullptr;
+static int route(zk_context* ctx, const RouteArgs& a, int type, BalanceOut out, void* work, size_t work_bytes,
+                 hipStream_t st) {
+  const bool balance = out.count != nullptr;
   const uint32_t blocks = balance_blocks(a.tokens, (int)a.experts);
   if (balance) {
-    const size_t need = zk_experts_route_work(a.tokens, (int)a.experts);
-    if (need && (!work || !aligned(work, 4) || work_bytes < need))
-      return ctx->fail(ZK_ERR_INVALID, "experts' route: workspace missing, too small or not aligned to 4 bytes");
-    a.part_prob = (float*)work;
-    a.part_count = (uint32_t*)work + (size_t)blocks * a.experts;
+    const size_t need = balance_work(a.tokens, (int)a.experts);
+    if (need && (!work || !aligned(work, 8) || work_bytes < need))
+      return ctx->fail(ZK_ERR_INVALID, "experts' route: workspace missing, too small or not aligned to 8 bytes");
+    constexpr size_t PARTS = ZK_MAX_EXPERTS / FINISH_EXPERTS;
+    out.loss_part = (double*)work;
+    out.ticket = (uint32_t*)(out.loss_part + PARTS);
+    out.part_prob = (float*)(out.loss_part + PARTS + 1);
+    out.part_count = (uint32_t*)(out.part_prob + (size_t)blocks * a.experts);
+  } else if (!a.tokens) {
+    return ZK_OK;
   }
   const char* name = CHOOSE ? "experts_route" : "experts_balance";
-  if (a.tokens)
-    ZK_TRY(by_score_type(type, [&](auto zero) -> int {
-      typedef decltype(zero) T;
-      return by_experts(a.experts, [&](auto lanes, auto per) -> int {
-        constexpr int L = decltype(lanes)::value, V = decltype(per)::value;
-        if (balance) {
-          ZK_LAUNCH(ctx, st, name, (k_route<T, L, V, CHOOSE, true>), dim3(blocks), dim3(ROUTE_THREADS), 0, a);
-        } else if constexpr (CHOOSE) {
-          ZK_LAUNCH(ctx, st, name, (k_route<T, L, V, true, false>), dim3(route_blocks(a.tokens, L, ROUTE_BLOCKS)),
-                    dim3(ROUTE_THREADS), 0, a);
-        }
-        return ZK_OK;
-      });
-    }));
-  if (balance)
-    ZK_LAUNCH(ctx, st, name, k_balance_finish, dim3(1), dim3(1024), 0, a.part_prob, a.part_count,
-              a.tokens ? blocks : 0, a.experts, a.slots, count, prob, loss);
+  ZK_TRY(by_score_type(type, [&](auto zero) -> int {
+    typedef decltype(zero) T;
+    return by_experts(a.experts, [&](auto lanes, auto per) -> int {
+      constexpr int L = decltype(lanes)::value, V = decltype(per)::value;
+      if (balance) {
+        ZK_LAUNCH(ctx, st, name, (k_route<T, L, V, CHOOSE, true>), dim3(blocks), dim3(balance_threads(L)), 0, a, out);
+      } else if constexpr (CHOOSE) {
+        ZK_LAUNCH(ctx, st, name, (k_route<T, L, V, true, false>),
+                  dim3(route_blocks(a.tokens, ROUTE_THREADS / L, ROUTE_BLOCKS)), dim3(ROUTE_THREADS), 0, a, out);
+      }
+      return ZK_OK;
+    });
+  }));
+  if (balance && blocks > 1)
+    ZK_LAUNCH(ctx, st, name, k_balance_finish, dim3(cdiv(a.experts, FINISH_EXPERTS)), dim3(256), 0, out, blocks,
+              a.experts, a.slots);
   return ZK_OK;
 }
 
@@ -458,7 +609,7 @@ extern "C" {
 size_t zk_experts_route_work(size_t tokens, int experts) {
   using namespace zk;
   if (experts < 1 || experts > ZK_MAX_EXPERTS || tokens > ZK_MAX_EXPERT_ROWS) return 0;
-  return (size_t)balance_blocks(tokens, experts) * (2 * experts + 1) * 4;
+  return balance_work(tokens, experts);
 }
 
 int zk_experts_route(zk_context* ctx, const void* d_scores, int type, size_t ld, size_t tokens, int experts, int slots,
@@ -472,8 +623,9 @@ int zk_experts_route(zk_context* ctx, const void* d_scores, int type, size_t ld,
     if (d_count || d_prob || d_loss) ZK_TRY(check_route_words(ctx, d_count, d_prob, d_loss));
     OnDevice on(ctx);
     const RouteArgs a = {d_scores, ld, (uint32_t)tokens, (uint32_t)experts, (uint32_t)slots, scale, renormalize != 0,
-                         d_expert, d_weight, nullptr, nullptr};
-    return route<true>(ctx, a, type, d_count, d_prob, d_loss, d_work, work_bytes, ctx->s(stream));
+                         d_expert, d_weight};
+    const BalanceOut out = {d_count, d_prob, d_loss, nullptr, nullptr, nullptr, nullptr};
+    return route<true>(ctx, a, type, out, d_work, work_bytes, ctx->s(stream));
   });
 }
 
@@ -488,8 +640,9 @@ int zk_experts_balance(zk_context* ctx, const void* d_scores, int type, size_t l
     ZK_TRY(check_route_words(ctx, d_count, d_prob, d_loss));
     OnDevice on(ctx);
     const RouteArgs a = {d_scores, ld, (uint32_t)tokens, (uint32_t)experts, (uint32_t)slots, scale, 0,
-                         (int32_t*)d_expert, nullptr, nullptr, nullptr};
-    return route<false>(ctx, a, type, d_count, d_prob, d_loss, d_work, work_bytes, ctx->s(stream));
+                         (int32_t*)d_expert, nullptr};
+    const BalanceOut out = {d_count, d_prob, d_loss, nullptr, nullptr, nullptr, nullptr};
+    return route<false>(ctx, a, type, out, d_work, work_bytes, ctx->s(stream));
   });
 }
 
@@ -514,14 +667,17 @@ int zk_experts_route_grad(zk_context* ctx, const void* d_scores, int type, size_
       return ctx->fail(ZK_ERR_INVALID, "experts' route: a pointer is not aligned to its type");
     OnDevice on(ctx);
     const RouteGradArgs a = {d_scores, ld, ld_grad, (uint32_t)tokens, (uint32_t)experts, (uint32_t)slots, scale,
-                             renormalize != 0, d_expert, d_grad_weight, d_count, d_grad_loss, d_grad_scores};
+                             d_expert, d_grad_weight, d_count, d_grad_loss, d_grad_scores};
     hipStream_t st = ctx->s(stream);
     return by_type(type, [&](auto zero) -> int {
       typedef decltype(zero) T;
       return by_experts(a.experts, [&](auto lanes, auto per) -> int {
         constexpr int L = decltype(lanes)::value, V = decltype(per)::value;
-        ZK_LAUNCH(ctx, st, "experts_route_grad", (k_route_grad<T, L, V>), dim3(route_blocks(tokens, L, ROUTE_BLOCKS)),
-                  dim3(ROUTE_THREADS), 0, a);
+        const dim3 grid(route_blocks(tokens, ROUTE_THREADS / L, ROUTE_BLOCKS));
+        if (renormalize && d_grad_weight)
+          ZK_LAUNCH(ctx, st, "experts_route_grad", (k_route_grad<T, L, V, true>), grid, dim3(ROUTE_THREADS), 0, a);
+        else
+          ZK_LAUNCH(ctx, st, "experts_route_grad", (k_route_grad<T, L, V, false>), grid, dim3(ROUTE_THREADS), 0, a);
         return ZK_OK;
       });
     });

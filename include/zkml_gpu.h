@@ -424,8 +424,8 @@ int zk_experts_combine_grad(zk_context* ctx, const void* d_grad, size_t ld_grad,
  *   prob[e] = sum_t p[t][e] / n,
  *   loss = experts * sum_e count[e] / (n * slots) * prob[e]       (1 if all are even),
  * prob and loss 0 without such a token, NaN with a NaN or an infinity above.
- * d_work: zk_experts_route_work(tokens, experts) bytes (0: sizes out of range),
- * 4-byte aligned, used only with these outputs.
+ * d_work: zk_experts_route_work(tokens, experts) bytes (0: none needed, may be
+ * NULL), 8-byte aligned, used only with these outputs.
  * zk_experts_balance: the same three for given routes (tokens x slots); a route
  * outside [0, experts) names none.
  * zk_experts_route_grad: the gradient with regard to the scores of what depends

@@ -55,7 +55,7 @@ def work_of(ctx, tokens, experts):
 
 
 # tokens, experts, slots
-SIZES = [(1, 1, 1), (1, 8, 2), (3, 2, 2), (5, 3, 8), (33, 8, 2), (17, 16, 4), (64, 17, 3), (100, 32, 6), (70, 60, 4),
+SIZES = [(1, 1, 1), (1, 8, 2), (3, 2, 2), (5, 3, 8), (33, 8, 2), (17, 16, 4), (64, 17, 3), (100, 32, 6), (70, 60, 4), (257, 60, 2), (300, 1024, 3), (700, 400, 2),
          (65, 64, 8), (129, 65, 5), (300, 128, 8), (40, 129, 4), (31, 256, 32), (50, 300, 17), (9, 512, 8),
          (20, 1000, 10), (7, 1024, 32), (3000, 24, 2)]
 
@@ -270,12 +270,12 @@ def test_no_tokens(ctx):
 
 def test_refusals(ctx):
     d = ctx.upload(np.zeros(1 << 14, dtype=np.int32))
-    work = ctx.alloc(ctx.experts_route_work(4, 8))
-    short = ctx.alloc(ctx.experts_route_work(4, 8) - 4)
-    route = dict(scores=d, scores_type=z.F32, tokens=4, experts=8, slots=2, expert=ctx.alloc(64), weight=ctx.alloc(64),
-                 count=ctx.alloc(64), prob=ctx.alloc(64), loss=ctx.alloc(64), work=work)
+    work = ctx.alloc(ctx.experts_route_work(400, 8))
+    short = ctx.alloc(ctx.experts_route_work(400, 8) - 4)
+    route = dict(scores=d, scores_type=z.F32, tokens=400, experts=8, slots=2, expert=ctx.alloc(3200),
+                 weight=ctx.alloc(3200), count=ctx.alloc(64), prob=ctx.alloc(64), loss=ctx.alloc(64), work=work)
     balance = {k: x for k, x in route.items() if k != "weight"}
-    grad = dict(scores=d, scores_type=z.F32, tokens=4, experts=8, slots=2, expert=d, grad_scores=ctx.alloc(256),
+    grad = dict(scores=d, scores_type=z.F32, tokens=400, experts=8, slots=2, expert=d, grad_scores=ctx.alloc(12800),
                 grad_weight=d, count=d, grad_loss=d)
     shared = [(dict(experts=0), "1024"), (dict(experts=1025), "1024"), (dict(slots=0), "32 slots"),
               (dict(slots=33), "32 slots"), (dict(tokens=1 << 22), "2\\^22"), (dict(tokens=(1 << 22) + 1), "2\\^22"),
@@ -285,7 +285,7 @@ def test_refusals(ctx):
               (dict(scores_type=9), "type")]
     both = [(dict(count=None), "null"), (dict(prob=None), "null"), (dict(loss=None), "null"),
             (dict(loss=At(d, 2)), "aligned"), (dict(work=None), "workspace"), (dict(work=short), "workspace"),
-            (dict(work=At(d, 2)), "workspace")]
+            (dict(work=At(d, 4)), "workspace")]
     for f, a, more in [(ctx.experts_route, route, both + [(dict(weight=None), "null")]),
                        (ctx.experts_balance, balance, both),
                        (ctx.experts_route_grad, grad, [
