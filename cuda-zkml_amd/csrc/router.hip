@@ -31,6 +31,10 @@ constexpr int ROUTE_THREADS = 256;
 // blocks' sums are left to be added up.
 constexpr int balance_threads(int lanes) { return lanes == 16 ? 1024 : 512; }
 
+constexpr uint32_t ROUTE_BLOCKS = 2048;   // of a launch at the most (then a block has several tokens a group)
+constexpr uint32_t BALANCE_BLOCKS = 256;  // one a CU
+constexpr size_t BALANCE_ONE = 256;       // tokens that one block takes alone, in one launch
+
 struct RouteArgs {
   const void* scores;
   size_t ld;
@@ -41,12 +45,16 @@ struct RouteArgs {
   float* weight;     // tokens x slots
 };
 
-// exp(a) for a <= 0 (or NaN): the hardware's 2^x of a's product with log2(e), whose
-// rounding error and whose factor's are made good by one step; below 2^-126 zero.
-__device__ __forceinline__ float exp_down(float a) {
-  constexpr float L = 1.44269504f, REST = 1.925963033e-8f, LN2 = 0.693147181f;  // log2(e) = L + REST
-  a = fmaxf(a, -200.0f);
-  const float t = a * L, lost = fmaf(a, REST, fmaf(a, L, -t)), p = __builtin_amdgcn_exp2f(t);
+// exp(scale x) for x <= 0: the hardware's 2^y of y = x scale log2(e).  EXACT: y's own
+// rounding is made good, so that what is left of an error is that of the hardware
+// (1 ulp), of the factor (2^-26 |y|) and of x scale; else y is off by two roundings,
+// which 16-bit results do not show.  Below 2^-126 it gives zero.
+template <bool EXACT>
+__device__ __forceinline__ float exp_down(float x, float scale) {
+  constexpr float LOG2E = 1.44269504f, LN2 = 0.693147181f;
+  if constexpr (!EXACT) return __builtin_amdgcn_exp2f(x * (scale * LOG2E));
+  const float a = fmaxf(x * scale, -200.0f);
+  const float y = a * LOG2E, lost = fmaf(a, LOG2E, -y), p = __builtin_amdgcn_exp2f(y);
   return fmaf(p, lost * LN2, p);
 }
 
@@ -58,11 +66,13 @@ struct Score {
   typedef float W;
   static constexpr bool KEYED = sizeof(T) == 2;
   static __device__ __forceinline__ float none() { return -INFINITY; }
+  static __device__ __forceinline__ float larger(float a, float b) { return __builtin_elementwise_maximum(a, b); }
   static __device__ __forceinline__ float read(T s) { return (float)s + 0.0f; }  // (-0 and 0 are equal)
-  // NaN and infinity leave a row without a softmax
-  static __device__ __forceinline__ bool bad(float v) { return !(v < INFINITY); }
+  // A row whose largest score this is has no softmax: it holds a NaN or an infinity.
+  static __device__ __forceinline__ bool bad(float m) { return !(m < INFINITY); }
   // exp(scale (v - m)); v <= m, m a score
-  static __device__ __forceinline__ float ex(float v, float m, float scale) { return exp_down((v - m) * scale); }
+  template <bool EXACT>
+  static __device__ __forceinline__ float ex(float v, float m, float scale) { return exp_down<EXACT>(v - m, scale); }
   // 0: masked, else the score's rank among all of the type above, the expert below
   static __device__ __forceinline__ uint32_t key(float v, uint32_t e) {
     uint16_t b;
@@ -84,10 +94,12 @@ struct Score<int> {
   typedef int W;
   static constexpr bool KEYED = false;
   static __device__ __forceinline__ int none() { return INT32_MIN; }
+  static __device__ __forceinline__ int larger(int a, int b) { return a > b ? a : b; }
   static __device__ __forceinline__ int read(int s) { return s; }
   static __device__ __forceinline__ bool bad(int) { return false; }
+  template <bool EXACT>
   static __device__ __forceinline__ float ex(int v, int m, float scale) {
-    return v == none() ? 0.0f : exp_down(-(float)((uint32_t)m - (uint32_t)v) * scale);
+    return v == none() ? 0.0f : exp_down<EXACT>(-(float)((uint32_t)m - (uint32_t)v), scale);
   }
 };
 
@@ -126,19 +138,45 @@ __device__ __forceinline__ float sum_over(float v) {
   return over_lanes<L>(v, [](float a, float b) { return a + b; });
 }
 
+// N bytes at an address that is a multiple of an element's, in one piece.
+template <int N, class P>
+__device__ __forceinline__ void copy_piece(const P* from, P* to) {  // (one of them in registers)
+  typedef int word __attribute__((aligned(2)));
+  typedef int words2 __attribute__((ext_vector_type(2), aligned(2)));
+  typedef int words4 __attribute__((ext_vector_type(4), aligned(2)));
+  if constexpr (N == 2) *to = *from;
+  else if constexpr (N == 4) *(word*)to = *(const word*)from;
+  else if constexpr (N == 8) *(words2*)to = *(const words2*)from;
+  else *(words4*)to = *(const words4*)from;
+}
+
+// Which of a token's experts a lane has: pieces of up to 16 bytes, so that a
+// token's lanes take neighbouring ones.  Their numbers grow with i.
+template <class T, int L, int V>
+struct Part {
+  static constexpr int C = V * sizeof(T) < 16 ? V : 16 / sizeof(T);
+  static __device__ __forceinline__ uint32_t expert(uint32_t l, int i) { return (i / C) * (L * C) + l * C + i % C; }
+};
+
 // A lane's V scores of a row; those beyond its end are masked.
-template <class T, int V>
-__device__ __forceinline__ void load_scores(const T* row, uint32_t first, uint32_t experts,
+template <class T, int L, int V>
+__device__ __forceinline__ void load_scores(const T* row, uint32_t l, uint32_t experts,
                                             typename Score<T>::W (&v)[V]) {
+  typedef Part<T, L, V> P;
   T raw[V];
-  if (first + V <= experts) {
-    __builtin_memcpy(raw, row + first, sizeof(raw));
 #pragma unroll
-    for (int i = 0; i < V; i++) v[i] = Score<T>::read(raw[i]);
-  } else {
+  for (int c = 0; c < V; c += P::C) {
+    const uint32_t e = P::expert(l, c);
+    if (e + P::C <= experts) {
+      copy_piece<P::C * sizeof(T)>(row + e, raw + c);
+    } else {
+      // (read again the row's last score, so that no load waits for another)
 #pragma unroll
-    for (int i = 0; i < V; i++) v[i] = first + i < experts ? Score<T>::read(row[first + i]) : Score<T>::none();
+      for (int i = 0; i < P::C; i++) raw[c + i] = row[e + i < experts ? e + i : experts - 1];
+    }
   }
+#pragma unroll
+  for (int i = 0; i < V; i++) v[i] = P::expert(l, i) < experts ? Score<T>::read(raw[i]) : Score<T>::none();
 }
 
 // Counts and sums of p of all tokens to count, prob and loss, by a block's threads;
@@ -183,12 +221,13 @@ struct BalanceOut {
 template <class T, int L, int V, bool CHOOSE, bool BALANCE>
 __global__ __launch_bounds__(BALANCE ? balance_threads(L) : ROUTE_THREADS) void k_route(RouteArgs a, BalanceOut out) {
   typedef Score<T> S;
+  typedef Part<T, L, V> P;
   typedef typename S::W W;
   constexpr uint32_t THREADS = BALANCE ? balance_threads(L) : ROUTE_THREADS, GROUPS = THREADS / L, WAVES = THREADS / 64;
   constexpr int KEPT = (ZK_MAX_SLOTS + L - 1) / L;
   __shared__ uint32_t count[BALANCE ? L * V + 1 : 1];
   __shared__ float sums[BALANCE ? WAVES * L * V : 1];
-  const uint32_t tid = threadIdx.x, l = tid % L, first = l * V;
+  const uint32_t tid = threadIdx.x, l = tid % L;
   if (BALANCE) {
     for (uint32_t e = tid; e <= a.experts; e += THREADS) count[e] = 0;
     if (blockIdx.x == 0 && tid == 0 && gridDim.x > 1) *out.ticket = 0;
@@ -205,22 +244,17 @@ __global__ __launch_bounds__(BALANCE ? balance_threads(L) : ROUTE_THREADS) void 
       for (int k = 0; k < KEPT; k++) given[k] = l + k * L < a.slots ? a.expert[(size_t)t * a.slots + l + k * L] : -1;
     }
     W v[V];
-    load_scores<T, V>((const T*)a.scores + (size_t)t * a.ld, first, a.experts, v);
+    load_scores<T, L, V>((const T*)a.scores + (size_t)t * a.ld, l, a.experts, v);
     W top = S::none();
-    bool bad = false;
 #pragma unroll
-    for (int i = 0; i < V; i++) {
-      top = v[i] > top ? v[i] : top;
-      bad |= S::bad(v[i]);
-    }
-    const W m = max_over<L>(top);
-    bad = max_over<L>((int)bad) != 0;
-    const bool empty = !bad && m == S::none();
+    for (int i = 0; i < V; i++) top = S::larger(top, v[i]);
+    const W m = over_lanes<L>(top, S::larger);
+    const bool bad = S::bad(m), empty = m == S::none();
     float inv = 0.0f;
     if (all && !bad && !empty) {
       float p[V], z = 0.0f;
 #pragma unroll
-      for (int i = 0; i < V; i++) z += p[i] = S::ex(v[i], m, a.scale);
+      for (int i = 0; i < V; i++) z += p[i] = S::template ex<true>(v[i], m, a.scale);
       inv = 1.0f / sum_over<L>(z);
       if (BALANCE) {
 #pragma unroll
@@ -241,14 +275,13 @@ __global__ __launch_bounds__(BALANCE ? balance_threads(L) : ROUTE_THREADS) void 
       continue;
     }
     int kept_e[KEPT];
-    float kept_w[KEPT];
+    W kept[KEPT];
 #pragma unroll
-    for (int k = 0; k < KEPT; k++) kept_e[k] = -1, kept_w[k] = bad ? NAN : 0.0f;
-    float total = 0.0f;
+    for (int k = 0; k < KEPT; k++) kept_e[k] = -1, kept[k] = S::none();
     uint32_t key[S::KEYED ? V : 1];
     if constexpr (S::KEYED) {
 #pragma unroll
-      for (int i = 0; i < V; i++) key[i] = S::key(v[i], first + i);
+      for (int i = 0; i < V; i++) key[i] = S::key(v[i], P::expert(l, i));
     }
     for (uint32_t j = 0; j < a.slots && !bad; j++) {
       W best = S::none();
@@ -268,27 +301,34 @@ __global__ __launch_bounds__(BALANCE ? balance_threads(L) : ROUTE_THREADS) void 
         W b = S::none();
 #pragma unroll
         for (int i = 0; i < V; i++)
-          if (v[i] > b) b = v[i], e = first + i;
-        best = max_over<L>(b);
+          if (v[i] > b) b = v[i], e = P::expert(l, i);
+        best = over_lanes<L>(b, S::larger);
         if (best == S::none()) break;
         e = min_over<L>(b == best ? e : a.experts);
 #pragma unroll
         for (int i = 0; i < V; i++)
-          if (first + i == e) v[i] = S::none();
+          if (P::expert(l, i) == e) v[i] = S::none();
       }
-      const float w = S::ex(best, m, a.scale);
-      total += w;
 #pragma unroll
       for (int k = 0; k < KEPT; k++)
-        if (j == l + k * L) kept_e[k] = (int)e, kept_w[k] = w;
+        if (j == l + k * L) kept_e[k] = (int)e, kept[k] = best;
     }
-    const float by = a.renormalize ? (total > 0.0f ? 1.0f / total : 0.0f) : inv;
+    // the weights, each by the lane that keeps it
+    float w[KEPT], total = 0.0f;
+#pragma unroll
+    for (int k = 0; k < KEPT; k++) total += w[k] = kept_e[k] < 0 ? 0.0f : S::template ex<true>(kept[k], m, a.scale);
+    float by = inv;
+    if (a.renormalize) {
+      total = sum_over<L>(total);
+      by = total > 0.0f ? 1.0f / total : 0.0f;
+    }
+    if (bad) by = NAN;
 #pragma unroll
     for (int k = 0; k < KEPT; k++)
       if (l + k * L < a.slots) {
         const size_t at = (size_t)t * a.slots + l + k * L;
         a.expert[at] = kept_e[k];
-        a.weight[at] = bad ? kept_w[k] : kept_w[k] * by;
+        a.weight[at] = w[k] * by;
         if (BALANCE && kept_e[k] >= 0) atomicAdd(&count[kept_e[k]], 1u);
       }
   }
@@ -298,7 +338,7 @@ __global__ __launch_bounds__(BALANCE ? balance_threads(L) : ROUTE_THREADS) void 
     for (int i = 0; i < V; i++) {
 #pragma unroll
       for (int d = L; d < 64; d <<= 1) psum[i] += __shfl_xor(psum[i], d);
-      if (tid % 64 < L) sums[(tid / 64) * L * V + first + i] = psum[i];
+      if (tid % 64 < L) sums[(tid / 64) * L * V + P::expert(l, i)] = psum[i];
     }
     __syncthreads();
     auto sum = [&](uint32_t e) {
@@ -333,14 +373,24 @@ __global__ __launch_bounds__(256) void k_balance_finish(BalanceOut out, uint32_t
   const uint32_t tid = threadIdx.x, x = tid % E, y = tid / E, e = blockIdx.x * E + x;
   uint32_t c = 0, n = 0;
   double s = 0.0;
-  if (e < experts) {
-#pragma unroll 8
-    for (uint32_t b = y; b < blocks; b += PARTS) {
-      c += out.part_count[(size_t)b * (experts + 1) + e];
-      s += out.part_prob[(size_t)b * experts + e];
+  static_assert(BALANCE_BLOCKS <= 256, "a thread a block");
+  if (tid < blocks) n = out.part_count[(size_t)tid * (experts + 1) + experts];
+  // (loads of rows and experts that are not there are of others, so that 16 rows' are
+  // under way together)
+  const uint32_t col = e < experts ? e : experts - 1;
+  for (uint32_t b0 = y; b0 < blocks; b0 += 16 * PARTS) {
+    uint32_t ci[16];
+    float si[16];
+#pragma unroll
+    for (uint32_t i = 0; i < 16; i++) {
+      const uint32_t b = b0 + i * PARTS < blocks ? b0 + i * PARTS : b0;
+      ci[i] = out.part_count[(size_t)b * (experts + 1) + col];
+      si[i] = out.part_prob[(size_t)b * experts + col];
     }
+#pragma unroll
+    for (uint32_t i = 0; i < 16; i++)
+      if (b0 + i * PARTS < blocks) c += ci[i], s += si[i];
   }
-  for (uint32_t b = tid; b < blocks; b += 256) n += out.part_count[(size_t)b * (experts + 1) + experts];
 #pragma unroll
   for (int d = 32; d; d >>= 1) n += __shfl_xor(n, d);
   if (tid % 64 == 0) n_part[tid / 64] = n;
@@ -383,25 +433,28 @@ struct RouteGradArgs {
 template <class T, int L, int V, bool NORMAL>
 __global__ __launch_bounds__(ROUTE_THREADS) void k_route_grad(RouteGradArgs a) {
   typedef Score<T> S;
+  typedef Part<T, L, V> P;
   constexpr uint32_t GROUPS = ROUTE_THREADS / L;
   constexpr int KEPT = (ZK_MAX_SLOTS + L - 1) / L;
-  const uint32_t tid = threadIdx.x, l = tid % L, first = l * V;
-  // the loss's factors of this lane's experts: g experts / n, and f
-  float f[V] = {}, c = 0.0f;
+  constexpr bool EXACT = sizeof(T) == 4;
+  const uint32_t tid = threadIdx.x, l = tid % L;
+  // the loss's gradients of the mean probabilities, g experts / n f, by way of LDS: a
+  // few lines of counts that every lane of the chip asks the L2 for cost 11 us of 20
+  // (32768 tokens, 256 experts)
+  float f[V] = {};
   if (a.count) {
-    const int n = a.count[a.experts];
-    if (n > 0) {
-      c = *a.grad_loss * ((float)a.experts / (float)n);
-      const float per = 1.0f / ((float)n * (float)a.slots);
+    __shared__ float shared[L * V];
+    const float n = (float)a.count[a.experts], g = *a.grad_loss;
+    const float per = n > 0.0f ? g * ((float)a.experts / (n * n * (float)a.slots)) : 0.0f;
+    for (uint32_t e = tid; e < L * V; e += ROUTE_THREADS) shared[e] = e < a.experts ? (float)a.count[e] * per : 0.0f;
+    __syncthreads();
 #pragma unroll
-      for (int i = 0; i < V; i++)
-        if (first + i < a.experts) f[i] = (float)a.count[first + i] * per;
-    }
+    for (int i = 0; i < V; i++) f[i] = shared[P::expert(l, i)];
   }
   for (uint32_t t0 = blockIdx.x * GROUPS; t0 < a.tokens; t0 += gridDim.x * GROUPS) {
     const uint32_t t = t0 + tid / L;
     if (t >= a.tokens) continue;  // (all of the token's lanes)
-    float v[V], p[V], d[V];
+    float v[V], d[V];
     // the token's routes, a lane each (two where there are more than lanes)
     int named[KEPT];
     float gw[KEPT];
@@ -412,86 +465,75 @@ __global__ __launch_bounds__(ROUTE_THREADS) void k_route_grad(RouteGradArgs a) {
       named[k] = on ? a.expert[at] : -1;
       gw[k] = on ? a.grad_weight[at] : 0.0f;
     }
-    load_scores<T, V>((const T*)a.scores + (size_t)t * a.ld, first, a.experts, v);
+    load_scores<T, L, V>((const T*)a.scores + (size_t)t * a.ld, l, a.experts, v);
     float top = S::none();
-    bool bad = false;
+#pragma unroll
+    for (int i = 0; i < V; i++) top = S::larger(top, v[i]);
+    const float m = over_lanes<L>(top, S::larger);
+    const bool bad = S::bad(m), empty = m == S::none();
+    // g: gradients of the experts' weights; times: routes that name them
+    float g[V] = {}, times[V] = {};
+    if (a.grad_weight)
+      for (uint32_t j = 0; j < a.slots; j++) {
+        int e = __shfl(named[0], j, L);
+        float gj = __shfl(gw[0], j, L);
+        if constexpr (KEPT > 1) {
+          if (j >= L) e = __shfl(named[1], j - L, L), gj = __shfl(gw[1], j - L, L);
+        }
+        if ((uint32_t)e >= a.experts) continue;
+#pragma unroll
+        for (int i = 0; i < V; i++)
+          if (P::expert(l, i) == (uint32_t)e) {
+            g[i] += gj;
+            if (NORMAL) times[i] += 1.0f;
+          }
+      }
+    // with p = e / z: all that depends on p has the gradient p (G - sum p G)
+    float z = 0.0f, dot = 0.0f, ez[V];
 #pragma unroll
     for (int i = 0; i < V; i++) {
-      top = v[i] > top ? v[i] : top;
-      bad |= S::bad(v[i]);
+      const float G = NORMAL ? f[i] : f[i] + g[i];
+      z += ez[i] = S::template ex<EXACT>(v[i], m, a.scale);
+      dot = fmaf(ez[i], G, dot);
     }
-    const float m = max_over<L>(top);
-    bad = max_over<L>((int)bad) != 0;
-    const bool empty = !bad && m == S::none();
+    const float inv = 1.0f / sum_over<L>(z);
+    dot = sum_over<L>(dot) * inv;
+    const float by = inv * a.scale;
 #pragma unroll
-    for (int i = 0; i < V; i++) d[i] = bad ? NAN : 0.0f;
-    if (!bad && !empty) {
-      float z = 0.0f, dot = 0.0f;
+    for (int i = 0; i < V; i++) d[i] = ez[i] * by * ((NORMAL ? f[i] : f[i] + g[i]) - dot);
+    if constexpr (NORMAL) {
+      // softmax over the chosen alone: their own maximum, sum and mean
+      float mc = S::none(), zc = 0.0f, gc = 0.0f;
 #pragma unroll
-      for (int i = 0; i < V; i++) z += p[i] = S::ex(v[i], m, a.scale);
-      const float inv = 1.0f / sum_over<L>(z);
+      for (int i = 0; i < V; i++) mc = times[i] > 0.0f ? S::larger(mc, v[i]) : mc;
+      mc = over_lanes<L>(mc, S::larger);
 #pragma unroll
       for (int i = 0; i < V; i++) {
-        p[i] *= inv;
-        dot += p[i] * f[i];
+        ez[i] = times[i] > 0.0f && v[i] > S::none() ? S::template ex<EXACT>(v[i], mc, a.scale) : 0.0f;
+        zc = fmaf(times[i], ez[i], zc);
+        gc = fmaf(g[i], ez[i], gc);
       }
-      if (a.count) dot = sum_over<L>(dot);
+      zc = sum_over<L>(zc), gc = sum_over<L>(gc);
+      const float ic = zc > 0.0f ? 1.0f / zc : 0.0f, byc = ic * a.scale;
+      gc *= ic;
 #pragma unroll
-      for (int i = 0; i < V; i++) d[i] = c * p[i] * (f[i] - dot);
-      if (a.grad_weight) {
-        float g[V] = {}, times[V] = {};
-        for (uint32_t j = 0; j < a.slots; j++) {
-          int e = __shfl(named[0], j, L);
-          float gj = __shfl(gw[0], j, L);
-          if constexpr (KEPT > 1) {
-            if (j >= L) e = __shfl(named[1], j - L, L), gj = __shfl(gw[1], j - L, L);
-          }
-          if ((uint32_t)e >= a.experts) continue;
-#pragma unroll
-          for (int i = 0; i < V; i++)
-            if (first + i == (uint32_t)e) {
-              g[i] += gj;
-              if (NORMAL) times[i] += 1.0f;
-            }
-        }
-        if constexpr (NORMAL) {
-          // softmax over the chosen alone: their own maximum, sum and mean
-          float mc = S::none(), zc = 0.0f, gc = 0.0f;
-#pragma unroll
-          for (int i = 0; i < V; i++)
-            if (times[i] > 0.0f && v[i] > mc) mc = v[i];
-          mc = max_over<L>(mc);
-#pragma unroll
-          for (int i = 0; i < V; i++) {
-            p[i] = times[i] > 0.0f && v[i] > S::none() ? S::ex(v[i], mc, a.scale) : 0.0f;
-            zc += times[i] * p[i];
-            gc += g[i] * p[i];
-          }
-          zc = sum_over<L>(zc), gc = sum_over<L>(gc);
-          const float ic = zc > 0.0f ? 1.0f / zc : 0.0f;
-          gc *= ic;
-#pragma unroll
-          for (int i = 0; i < V; i++) d[i] += p[i] * ic * (g[i] - times[i] * gc);
-        } else {
-          float gp = 0.0f;
-#pragma unroll
-          for (int i = 0; i < V; i++) gp += g[i] * p[i];
-          gp = sum_over<L>(gp);
-#pragma unroll
-          for (int i = 0; i < V; i++) d[i] += p[i] * (g[i] - gp);
-        }
-      }
+      for (int i = 0; i < V; i++) d[i] = fmaf(ez[i] * byc, fmaf(-times[i], gc, g[i]), d[i]);
     }
     T out[V];
+    // a masked row's sums are of nothing, an impossible one's are NaN
 #pragma unroll
-    for (int i = 0; i < V; i++) out[i] = (T)(d[i] * a.scale);
-    T* row = (T*)a.grad + (size_t)t * a.ld_grad + first;
-    if (first + V <= a.experts) {
-      __builtin_memcpy(row, out, sizeof(out));
-    } else {
+    for (int i = 0; i < V; i++) out[i] = (T)(empty ? 0.0f : bad ? NAN : d[i]);
+    T* row = (T*)a.grad + (size_t)t * a.ld_grad;
 #pragma unroll
-      for (int i = 0; i < V; i++)
-        if (first + i < a.experts) row[i] = out[i];
+    for (int k = 0; k < V; k += P::C) {
+      const uint32_t e = P::expert(l, k);
+      if (e + P::C <= a.experts) {
+        copy_piece<P::C * sizeof(T)>(out + k, row + e);
+      } else {
+#pragma unroll
+        for (int i = 0; i < P::C; i++)
+          if (e + i < a.experts) row[e + i] = out[k + i];
+      }
     }
   }
 }
@@ -512,10 +554,6 @@ static int by_experts(uint32_t experts, Fn&& fn) {
   return fn(integral_constant<int, 64>(), integral_constant<int, 16>());
 }
 static int lanes_of(int experts) { return experts <= 256 ? 16 : experts <= 512 ? 32 : 64; }
-
-constexpr uint32_t ROUTE_BLOCKS = 2048;   // of a launch at the most (then a block has several tokens a group)
-constexpr uint32_t BALANCE_BLOCKS = 256;  // one a CU
-constexpr size_t BALANCE_ONE = 256;       // tokens that one block takes alone, in one launch
 
 static uint32_t route_blocks(size_t tokens, uint32_t a_block, uint32_t most) {
   const uint32_t b = cdiv(tokens, a_block);
