@@ -22,7 +22,7 @@ constexpr size_t I4_MAX_IN = (size_t)1 << 24;  // (indexes inside a row stay far
 struct I4Args : I8Args {
   const void* scale;  // groups x n_out, for each expert
   uint32_t group, groups;
-  int y_type;
+  int scale_type, y_type;
 };
 
 static __host__ __device__ inline size_t i4_row_bytes(size_t n_in) { return (n_in + 127) / 128 * 64; }
@@ -195,15 +195,283 @@ __global__ __launch_bounds__(64 * KW) void k_i4_direct(I4Args a, uint32_t tiles_
   }
 }
 
+// ------------------------------------------------------------ many rows
+// Eight neighbouring results of a row, of which it has `left` from here on.
+template <class T>
+__device__ __forceinline__ void put8(T* y, uint32_t left, const float (&v)[8]) {
+  T r[8];
+#pragma unroll
+  for (int k = 0; k < 8; k++) r[k] = (T)v[k];
+  if (left >= 8) {
+#pragma unroll
+    for (int k = 0; k < (int)sizeof(r) / 16; k++) ((row16*)y)[k] = ((const row16*)r)[k];
+  } else {
+#pragma unroll
+    for (uint32_t k = 0; k < 7; k++)
+      if (k < left) y[k] = r[k];
+  }
+}
+
+__device__ __forceinline__ float i4_scale(const I4Args& a, size_t at) {
+  if (a.scale_type == ZK_F32) return ((const float*)a.scale)[at];
+  if (a.scale_type == ZK_F16) return (float)((const _Float16*)a.scale)[at];
+  return (float)((const __bf16*)a.scale)[at];
+}
+
+// A block computes BT tokens x BN channels, its WT x WN waves a grid of FT x FN
+// squares of 32 x 32 each (D's rows are tokens, its columns channels, so that a lane
+// holds one channel's results and needs one scale).  Steps of 128 of k, a cache line of
+// x's rows and half a one of w's, go straight from memory to LDS, into three stages: while one is
+// multiplied the next is there and the one after under way.  Chunk c (16 bytes) of x's
+// row r lies at c ^ (r / 2 % 8), of w's at c ^ (r / 4 % 4): the rows that a fragment
+// reads together meet no bank twice.  w is unpacked in registers, once for the wave's FT
+// squares; a group's integer sums become floats and go to the results with its scale,
+// which is what bounds this kernel beside the matrix cores: 32 operations a square and
+// group for four matrix instructions of a step.  Scales come through registers to LDS, four
+// groups' at a time.  ODD: x's rows start at any byte or end inside a chunk; they come
+// through registers, masked.
+template <int G, bool GROUPED, bool ODD, int WT, int WN, int FT, int FN>
+__global__ __launch_bounds__(64 * WT * WN) void k_i4_ring(I4Args a, uint32_t tiles_t, uint32_t tiles_n) {
+  constexpr uint32_t WAVES = WT * WN, THREADS = 64 * WAVES, BT = WT * FT * 32, BN = WN * FN * 32;
+  constexpr uint32_t XB = BT * 128, WB = BN * 64, STAGE = XB + WB, STAGES = 3;
+  constexpr uint32_t XR = BT / 8 / WAVES, WR = BN / 16 / WAVES;  // 1 KB pieces of a stage that a wave fills
+  constexpr int NS = G >= 128 ? 1 : 128 / G;                     // scales of a step
+  constexpr uint32_t ROWS = 4, W = ROWS / NS;                    // rows of scales, and steps, of a window
+  constexpr uint32_t SR = ROWS * BN / THREADS;                   // scales of a window that a thread loads
+  constexpr uint32_t LD = FN * 32 + 4, OWN = 32 * LD * 4;        // a wave's results of 32 tokens
+  static_assert(WAVES * OWN + 4 * (2 * BT + BN) <= STAGES * STAGE, "the results' LDS is the stages'");
+  static_assert(XR * 8 * WAVES == BT && WR * 16 * WAVES == BN && SR * THREADS == ROWS * BN, "whole pieces");
+  __shared__ __align__(16) int8_t lds[STAGES * STAGE];
+  __shared__ float scales[2][ROWS][BN];
+  const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  uint32_t r0, r1, n0, e;
+  if (!block_tile<GROUPED>(a, BT, BN, tiles_t, tiles_n, r0, r1, n0, e)) return;
+  const bool none = GROUPED && e >= a.experts;
+  const size_t ch = none ? 0 : (size_t)e * a.n_out;
+  const uint32_t steps = none ? 0 : (a.n_in + 127) / 128, full = a.n_in / 128;
+  const uint32_t base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) int8_t*)lds;
+  // ---- what a lane fetches: chunk xc of x's row, chunk wc of w's
+  const int8_t *xp[XR], *wp[WR];
+  uint32_t xc[XR];
+#pragma unroll
+  for (uint32_t i = 0; i < WR; i++) {
+    const uint32_t row = (wave * WR + i) * 16 + (lane >> 2), n = n0 + row < a.n_out ? n0 + row : a.n_out - 1;
+    wp[i] = a.w + (ch + n) * a.ld_w + ((lane & 3) ^ (row >> 2 & 3)) * 16;
+  }
+#pragma unroll
+  for (uint32_t i = 0; i < XR; i++) {
+    const uint32_t row = (wave * XR + i) * 8 + (lane >> 3), r = r0 + row < r1 ? r0 + row : r1 - 1;
+    int64_t s = GROUPED ? source_row(a, r) : (int64_t)r;
+    if (s < 0) s = 0;
+    xc[i] = ((lane & 7) ^ (row >> 1 & 7)) * 16;
+    xp[i] = a.x + (size_t)s * a.ld_x + (ODD ? 0 : xc[i]);
+  }
+  v4i held[ODD ? XR : 1];
+  auto fetch = [&](uint32_t step, uint32_t stage) {
+    const uint32_t at = base + stage * STAGE;
+    if constexpr (ODD) {
+#pragma unroll
+      for (uint32_t i = 0; i < XR; i++) {
+        if (step < full) __builtin_memcpy(&held[i], xp[i] + step * 128 + xc[i], 16);
+        else held[i] = x_piece(xp[i], step * 128 + xc[i], a.n_in);
+      }
+    } else {
+#pragma unroll
+      for (uint32_t i = 0; i < XR; i++)
+        load_to_lds(step < full || step * 128 + xc[i] < a.n_in ? xp[i] + (size_t)step * 128 : (const int8_t*)&zeros16,
+                    at + (wave * XR + i) * 1024);
+    }
+#pragma unroll
+    for (uint32_t i = 0; i < WR; i++) load_to_lds(wp[i] + (size_t)step * 64, at + XB + (wave * WR + i) * 1024);
+  };
+  auto put_held = [&](uint32_t stage) {
+    if constexpr (ODD) {
+#pragma unroll
+      for (uint32_t i = 0; i < XR; i++) *(v4i*)(lds + stage * STAGE + (wave * XR + i) * 1024 + lane * 16) = held[i];
+    }
+  };
+  float sc[SR];
+  const uint32_t whole = G >= 128 ? a.group / 128 : 1;  // steps of a group
+  auto fetch_scales = [&](uint32_t window) {
+#pragma unroll
+    for (uint32_t i = 0; i < SR; i++) {
+      const uint32_t k = tid + i * THREADS, n = n0 + k % BN < a.n_out ? n0 + k % BN : a.n_out - 1;
+      uint32_t g = window * ROWS + k / BN;
+      if (G >= 128) g /= whole;
+      if (g >= a.groups) g = a.groups - 1;  // (behind the row's end: x is zero)
+      sc[i] = i4_scale(a, ch * a.groups + (size_t)g * a.n_out + n);
+    }
+  };
+  auto put_scales = [&](uint32_t window) {
+#pragma unroll
+    for (uint32_t i = 0; i < SR; i++) {
+      const uint32_t k = tid + i * THREADS;
+      scales[window & 1][k / BN][k % BN] = sc[i];
+    }
+  };
+  // the results' factors, a few for each thread, there when they are needed
+  constexpr uint32_t FACTORS = (2 * BT + BN + THREADS - 1) / THREADS;
+  float factor[FACTORS];
+#pragma unroll
+  for (uint32_t i = 0; i < FACTORS; i++) {
+    const uint32_t k = tid + i * THREADS;
+    factor[i] = 0.0f;
+    if (k < 2 * BT) {  // tokens' scales, and whether they are there
+      const uint32_t t = r0 + k % BT;
+      int64_t s = -1;
+      if (t < r1 && !none) s = GROUPED ? source_row(a, t) : (int64_t)t;
+      factor[i] = s < 0 ? 0.0f : k < BT && a.sx ? a.sx[s] : 1.0f;
+    } else if (k < 2 * BT + BN) {
+      const uint32_t n = n0 + k - 2 * BT;
+      factor[i] = a.bias && n < a.n_out ? a.bias[ch + n] : 0.0f;
+    }
+  }
+  // ---- where a lane reads its fragments
+  const uint32_t wave_t = wave % WT, wave_n = wave / WT, fr = lane & 31, hi = lane >> 5;
+  const int8_t* fx = lds + (wave_t * FT * 32 + fr) * 128;
+  const int8_t* fw = lds + XB + (wave_n * FN * 32 + fr) * 64;
+  uint32_t cx[4], cw[2];
+#pragma unroll
+  for (uint32_t s = 0; s < 4; s++) cx[s] = ((2 * s + hi) ^ (fr >> 1 & 7)) * 16;
+#pragma unroll
+  for (uint32_t s = 0; s < 2; s++) cw[s] = ((2 * s + hi) ^ (fr >> 2 & 3)) * 16;
+  float acc[FN][FT][16] = {};
+  if (steps) {
+    fetch_scales(0);
+    fetch(0, 0);
+    put_held(0);
+    if (steps > 1) fetch(1, 1);
+    uint32_t stage = 0;
+    for (uint32_t step = 0; step < steps; step++) {
+      const uint32_t next = stage + 1 < STAGES ? stage + 1 : 0, after = next + 1 < STAGES ? next + 1 : 0;
+      if (step + 1 < steps) put_held(next);
+      if (step % W == 0) put_scales(step / W);
+      // this step's pieces are in, also those of the other waves; all have read the last one's
+      if (step + 1 < steps) wait_loads<(ODD ? 0 : XR) + WR>();
+      else wait_loads<0>();
+      wait_lds();
+      meet();
+      if (step % W == 0 && step + W < steps) fetch_scales(step / W + 1);
+      if (step + 2 < steps) fetch(step + 2, after);
+      const int8_t *sx = fx + stage * STAGE, *sw = fw + stage * STAGE;
+      v4i wf[FN][4];
+      float ws[FN][NS];
+#pragma unroll
+      for (int i = 0; i < FN; i++) {
+#pragma unroll
+        for (int q = 0; q < 2; q++) {
+          const v4i p = *(const v4i*)(sw + i * 32 * 64 + cw[q]);
+          wf[i][q] = (p << 4) & (int)0xf0f0f0f0;
+          wf[i][q + 2] = p & (int)0xf0f0f0f0;
+        }
+#pragma unroll
+        for (int k = 0; k < NS; k++)
+          ws[i][k] = scales[step / W & 1][step % W * NS + k][wave_n * FN * 32 + i * 32 + fr];
+      }
+#pragma unroll
+      for (int j = 0; j < FT; j++) {
+        v4i xf[4];
+#pragma unroll
+        for (int s = 0; s < 4; s++) xf[s] = *(const v4i*)(sx + j * 32 * 128 + cx[s]);
+#pragma unroll
+        for (int i = 0; i < FN; i++) {
+          v16i part = {};
+#pragma unroll
+          for (int s = 0; s < 4; s++) {
+            part = __builtin_amdgcn_mfma_i32_32x32x32_i8(xf[s], wf[i][s], part, 0, 0, 0);
+            if ((s + 1) % (4 / NS) == 0) {
+#pragma unroll
+              for (int r = 0; r < 16; r++) acc[i][j][r] = fmaf((float)part[r], ws[i][s * NS / 4], acc[i][j][r]);
+              part = v16i{};
+            }
+          }
+        }
+      }
+      stage = next;
+    }
+  }
+  // ---- results: a wave's 32 tokens at a time, by way of its own LDS
+  wait_lds();
+  meet();
+  float* f = (float*)(lds + WAVES * OWN);
+#pragma unroll
+  for (uint32_t i = 0; i < FACTORS; i++)
+    if (tid + i * THREADS < 2 * BT + BN) f[tid + i * THREADS] = factor[i];
+  wait_lds();
+  meet();
+  float* own = (float*)(lds + wave * OWN);
+  constexpr uint32_t PIECES = FN * 4, PER = 64 / PIECES;  // of eight channels in a row; rows of one store
+  const uint32_t c = lane % PIECES * 8, n = n0 + wave_n * FN * 32 + c;
+  float bias[8];
+#pragma unroll
+  for (int k = 0; k < 8; k++) bias[k] = f[2 * BT + wave_n * FN * 32 + c + k];
+#pragma unroll
+  for (int j = 0; j < FT; j++) {
+#pragma unroll
+    for (int i = 0; i < FN; i++)
+#pragma unroll
+      for (int r = 0; r < 16; r++) own[(8 * (r / 4) + 4 * hi + r % 4) * LD + i * 32 + fr] = acc[i][j][r];
+    wait_lds();  // one wave's LDS accesses are in order; this keeps the compiler to it
+#pragma unroll
+    for (uint32_t s = 0; s < 32; s += PER) {
+      const uint32_t row = s + lane / PIECES, tt = wave_t * FT * 32 + j * 32 + row, t = r0 + tt;
+      if (t < r1 && n < a.n_out) {
+        float v[8];
+        const float sx = f[tt], has = f[BT + tt];
+#pragma unroll
+        for (int k = 0; k < 8; k++)
+          v[k] = has != 0.0f ? i4_finish(own[row * LD + c + k] * 0.0625f, sx, bias[k], a.relu) : 0.0f;
+        const size_t at = (size_t)t * a.ld_y + n;
+        if (a.y_type == ZK_F32) put8((float*)a.y + at, a.n_out - n, v);
+        else if (a.y_type == ZK_F16) put8((_Float16*)a.y + at, a.n_out - n, v);
+        else put8((__bf16*)a.y + at, a.n_out - n, v);
+      }
+    }
+    wait_lds();
+  }
+}
+
+template <bool GROUPED>
+static int i4_tiles(zk_context* ctx, const I4Args& a, uint32_t bt, uint32_t bn, uint32_t& tiles_t, uint32_t& tiles_n,
+                    uint32_t& blocks) {
+  // row tiles of the grouped form: whole ones, and a part of one for each expert and
+  // for the rows without an expert
+  const uint32_t groups = a.experts + 1 < a.rows ? a.experts + 1 : a.rows;
+  tiles_t = GROUPED ? a.rows / bt + groups : cdiv(a.rows, bt);
+  tiles_n = cdiv(a.n_out, bn);
+  const size_t tiles = (size_t)tiles_t * tiles_n;
+  if (tiles > I8_MAX_TILES) return ctx->fail(ZK_ERR_SIZE, "i4 product: rows and n_out make too many tiles");
+  blocks = cdiv(tiles, 8) * 8;
+  return ZK_OK;
+}
+
+template <int G, bool GROUPED>
+static int i4_launch_ring(zk_context* ctx, const I4Args& a, hipStream_t st) {
+  const char* name = GROUPED ? "i4_matmul_experts" : "i4_matmul";
+  const bool odd = (((uintptr_t)a.x | a.ld_x | a.n_in) & 15) != 0;
+  auto go = [&](auto kernel, uint32_t threads, uint32_t bt, uint32_t bn) -> int {
+    uint32_t tiles_t, tiles_n, blocks;
+    ZK_TRY(i4_tiles<GROUPED>(ctx, a, bt, bn, tiles_t, tiles_n, blocks));
+    ZK_LAUNCH(ctx, st, name, kernel, dim3(blocks), dim3(threads), 0, a, tiles_t, tiles_n);
+    return ZK_OK;
+  };
+  auto by_tile = [&](auto is_odd) -> int {
+    constexpr bool ODD = decltype(is_odd)::value;
+    const size_t t256 = (size_t)cdiv(a.rows, 256) * cdiv(a.n_out, 256), t128 = (size_t)cdiv(a.rows, 128) * cdiv(a.n_out, 128);
+    if (t256 >= 256 && !GROUPED) return go(k_i4_ring<G, GROUPED, ODD, 2, 4, 4, 2>, 512, 256, 256);
+    if (t128 >= 128) return go(k_i4_ring<G, GROUPED, ODD, 2, 2, 2, 2>, 256, 128, 128);
+    return go(k_i4_ring<G, GROUPED, ODD, 2, 2, 1, 1>, 256, 64, 64);
+  };
+  return odd ? by_tile(std::true_type()) : by_tile(std::false_type());
+}
+
 template <class S, int G, bool GROUPED>
 static int i4_launch(zk_context* ctx, const I4Args& a, hipStream_t st) {
   const char* name = GROUPED ? "i4_matmul_experts" : "i4_matmul";
   auto go = [&](auto kernel, uint32_t threads, uint32_t bt, uint32_t bn) -> int {
-    const uint32_t groups = a.experts + 1 < a.rows ? a.experts + 1 : a.rows;
-    const uint32_t tiles_t = GROUPED ? a.rows / bt + groups : cdiv(a.rows, bt), tiles_n = cdiv(a.n_out, bn);
-    const size_t tiles = (size_t)tiles_t * tiles_n;
-    if (tiles > I8_MAX_TILES) return ctx->fail(ZK_ERR_SIZE, "i4 product: rows and n_out make too many tiles");
-    ZK_LAUNCH(ctx, st, name, kernel, dim3(cdiv(tiles, 8) * 8), dim3(threads), 0, a, tiles_t, tiles_n);
+    uint32_t tiles_t, tiles_n, blocks;
+    ZK_TRY(i4_tiles<GROUPED>(ctx, a, bt, bn, tiles_t, tiles_n, blocks));
+    ZK_LAUNCH(ctx, st, name, kernel, dim3(blocks), dim3(threads), 0, a, tiles_t, tiles_n);
     return ZK_OK;
   };
   // rows of one expert, about
@@ -211,7 +479,8 @@ static int i4_launch(zk_context* ctx, const I4Args& a, hipStream_t st) {
   if (rows <= 4) return go(k_i4_direct<S, G, GROUPED, 1, 1, 1, 8, 4>, 512, 4, 16);
   if (rows <= 16) return go(k_i4_direct<S, G, GROUPED, 1, 1, 4, 8, 4>, 512, 16, 16);
   if (rows <= 32) return go(k_i4_direct<S, G, GROUPED, 2, 2, 4, 8, 2>, 512, 32, 32);
-  return go(k_i4_direct<S, G, GROUPED, 4, 2, 4, 8, 2>, 512, 64, 32);
+  if (rows <= 48) return go(k_i4_direct<S, G, GROUPED, 4, 2, 4, 8, 2>, 512, 64, 32);
+  return i4_launch_ring<G, GROUPED>(ctx, a, st);
 }
 
 template <bool GROUPED>
@@ -305,8 +574,9 @@ static int check_i4(zk_context* ctx, const I4Args& a, size_t rows, size_t n_out,
   return ZK_OK;
 }
 
-static void set_sizes(I4Args& a, size_t rows, size_t n_out, size_t n_in, int group, int relu, int type) {
-  a.y_type = type;
+static void set_sizes(I4Args& a, size_t rows, size_t n_out, size_t n_in, int group, int relu, int scale_type,
+                      int type) {
+  a.scale_type = scale_type, a.y_type = type;
   a.rows = (uint32_t)rows, a.n_out = (uint32_t)n_out, a.n_in = (uint32_t)n_in, a.relu = relu != 0;
   a.group = (uint32_t)group, a.groups = cdiv(n_in, group);
 }
@@ -376,7 +646,7 @@ int zk_i4_matmul(zk_context* ctx, const int8_t* d_x, size_t ld_x, const float* d
     a.ld_x = ld_x, a.ld_w = ld_w, a.ld_y = ld_y;
     ZK_TRY(check_i4(ctx, a, rows, n_out, n_in, group, scale_type, y_type));
     if (!rows || !n_out) return ZK_OK;
-    set_sizes(a, rows, n_out, n_in, group, relu, y_type);
+    set_sizes(a, rows, n_out, n_in, group, relu, scale_type, y_type);
     OnDevice on(ctx);
     return i4_matmul(ctx, a, scale_type, y_type, ctx->s(stream));
   });
@@ -405,7 +675,7 @@ int zk_i4_linear(zk_context* ctx, const void* d_x, int x_type, size_t ld_x, cons
     if (!rows || !n_out) return ZK_OK;
     if (!d_work || !aligned(d_work, 16) || work_bytes < lw.bytes)
       return ctx->fail(ZK_ERR_INVALID, "i4 linear: workspace missing, too small or not aligned to 16 bytes");
-    set_sizes(a, rows, n_out, n_in, group, relu, y_type);
+    set_sizes(a, rows, n_out, n_in, group, relu, scale_type, y_type);
     OnDevice on(ctx);
     hipStream_t st = ctx->s(stream);
     ZK_TRY(i8_quantize(ctx, d_x, x_type, ld_x, rows, n_in, (int8_t*)d_work + lw.q, lw.ld, (float*)d_work, st));
@@ -434,7 +704,7 @@ int zk_i4_matmul_experts(zk_context* ctx, const int8_t* d_x, size_t ld_x, const 
     if (!d_offsets) return ctx->fail(ZK_ERR_INVALID, "i4 experts: null pointer");
     if (!aligned(d_offsets, 4) || !aligned(d_order, 4))
       return ctx->fail(ZK_ERR_INVALID, "i4 experts: a pointer is not aligned to its type");
-    set_sizes(a, rows, n_out, n_in, group, relu, y_type);
+    set_sizes(a, rows, n_out, n_in, group, relu, scale_type, y_type);
     a.offsets = d_offsets, a.order = d_order, a.experts = (uint32_t)experts, a.slots = (uint32_t)slots;
     a.tokens = (uint32_t)tokens;
     OnDevice on(ctx);

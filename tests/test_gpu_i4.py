@@ -81,7 +81,8 @@ def test_strides_and_offsets(ctx, kind, rows, n_out, n_in, group, lead, pad):
 # many rows: whole and ragged tiles, rows of whole 16-byte pieces and not
 @pytest.mark.parametrize("group", [32, 64, 128, 256])
 @pytest.mark.parametrize("rows,n_out,n_in", [(700, 1200, 2048), (1500, 1030, 656), (2050, 2200, 1040),
-                                             (1100, 1300, 1001), (129, 4100, 3001)])
+                                             (1100, 1300, 1001), (129, 4100, 3001), (4100, 4200, 272),
+                                             (4099, 4100, 157)])
 def test_many_rows(ctx, rows, n_out, n_in, group):
     rng = np.random.default_rng([rows, n_out, n_in, group])
     x, sx, q, s, sv = inputs(rng, rows, n_out, n_in, group, "f16")
