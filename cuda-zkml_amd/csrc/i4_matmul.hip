@@ -212,10 +212,17 @@ __device__ __forceinline__ void put8(T* y, uint32_t left, const float (&v)[8]) {
   }
 }
 
-__device__ __forceinline__ float i4_scale(const I4Args& a, size_t at) {
-  if (a.scale_type == ZK_F32) return ((const float*)a.scale)[at];
-  if (a.scale_type == ZK_F16) return (float)((const _Float16*)a.scale)[at];
-  return (float)((const __bf16*)a.scale)[at];
+// A scale's bits, and what they are worth (apart, so that a load waits for nothing).
+__device__ __forceinline__ uint32_t scale_bits(const I4Args& a, size_t at) {
+  return a.scale_type == ZK_F32 ? ((const uint32_t*)a.scale)[at] : ((const uint16_t*)a.scale)[at];
+}
+__device__ __forceinline__ float scale_of(const I4Args& a, uint32_t bits) {
+  if (a.scale_type == ZK_F32) return __uint_as_float(bits);
+  if (a.scale_type == ZK_BF16) return __uint_as_float(bits << 16);
+  const uint16_t b = (uint16_t)bits;
+  _Float16 h;
+  __builtin_memcpy(&h, &b, 2);
+  return (float)h;
 }
 
 // A block computes BT tokens x BN channels, its WT x WN waves a grid of FT x FN
@@ -231,7 +238,7 @@ __device__ __forceinline__ float i4_scale(const I4Args& a, size_t at) {
 // groups' at a time.  ODD: x's rows start at any byte or end inside a chunk; they come
 // through registers, masked.
 template <int G, bool GROUPED, bool ODD, int WT, int WN, int FT, int FN>
-__global__ __launch_bounds__(64 * WT * WN) void k_i4_ring(I4Args a, uint32_t tiles_t, uint32_t tiles_n) {
+__global__ __launch_bounds__(64 * WT * WN, 2) void k_i4_ring(I4Args a, uint32_t tiles_t, uint32_t tiles_n) {
   constexpr uint32_t WAVES = WT * WN, THREADS = 64 * WAVES, BT = WT * FT * 32, BN = WN * FN * 32;
   constexpr uint32_t XB = BT * 128, WB = BN * 64, STAGE = XB + WB, STAGES = 3;
   constexpr uint32_t XR = BT / 8 / WAVES, WR = BN / 16 / WAVES;  // 1 KB pieces of a stage that a wave fills
@@ -250,21 +257,28 @@ __global__ __launch_bounds__(64 * WT * WN) void k_i4_ring(I4Args a, uint32_t til
   const size_t ch = none ? 0 : (size_t)e * a.n_out;
   const uint32_t steps = none ? 0 : (a.n_in + 127) / 128, full = a.n_in / 128;
   const uint32_t base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) int8_t*)lds;
-  // ---- what a lane fetches: chunk xc of x's row, chunk wc of w's
-  const int8_t *xp[XR], *wp[WR];
-  uint32_t xc[XR];
+  // ---- what a lane fetches: a chunk of x's rows and one of w's.  NEAR: 32 bits from a
+  // base that the block has in common.
+  const int8_t* wbase = a.w + (ch + n0) * a.ld_w;
+  const int8_t* xbase = GROUPED ? a.x : a.x + (size_t)r0 * a.ld_x;
+  typedef std::conditional_t<ODD, const int8_t*, uint32_t> Place;
+  Place xp[XR], wp[WR];
+  auto x_chunk = [&](uint32_t i) { return ((lane & 7) ^ (((wave * XR + i) * 8 + (lane >> 3)) >> 1 & 7)) * 16; };
 #pragma unroll
   for (uint32_t i = 0; i < WR; i++) {
-    const uint32_t row = (wave * WR + i) * 16 + (lane >> 2), n = n0 + row < a.n_out ? n0 + row : a.n_out - 1;
-    wp[i] = a.w + (ch + n) * a.ld_w + ((lane & 3) ^ (row >> 2 & 3)) * 16;
+    const uint32_t row = (wave * WR + i) * 16 + (lane >> 2), n = n0 + row < a.n_out ? row : a.n_out - 1 - n0;
+    const size_t off = (size_t)n * a.ld_w + ((lane & 3) ^ (row >> 2 & 3)) * 16;
+    if constexpr (ODD) wp[i] = wbase + off;
+    else wp[i] = (uint32_t)off;
   }
 #pragma unroll
   for (uint32_t i = 0; i < XR; i++) {
     const uint32_t row = (wave * XR + i) * 8 + (lane >> 3), r = r0 + row < r1 ? r0 + row : r1 - 1;
-    int64_t s = GROUPED ? source_row(a, r) : (int64_t)r;
+    int64_t s = GROUPED ? source_row(a, r) : (int64_t)(r - r0);
     if (s < 0) s = 0;
-    xc[i] = ((lane & 7) ^ (row >> 1 & 7)) * 16;
-    xp[i] = a.x + (size_t)s * a.ld_x + (ODD ? 0 : xc[i]);
+    const size_t off = (size_t)s * a.ld_x;
+    if constexpr (ODD) xp[i] = xbase + off;
+    else xp[i] = (uint32_t)off + x_chunk(i);
   }
   v4i held[ODD ? XR : 1];
   auto fetch = [&](uint32_t step, uint32_t stage) {
@@ -272,17 +286,35 @@ __global__ __launch_bounds__(64 * WT * WN) void k_i4_ring(I4Args a, uint32_t til
     if constexpr (ODD) {
 #pragma unroll
       for (uint32_t i = 0; i < XR; i++) {
-        if (step < full) __builtin_memcpy(&held[i], xp[i] + step * 128 + xc[i], 16);
-        else held[i] = x_piece(xp[i], step * 128 + xc[i], a.n_in);
+        if (step < full) __builtin_memcpy(&held[i], xp[i] + step * 128 + x_chunk(i), 16);
+        else held[i] = x_piece(xp[i], step * 128 + x_chunk(i), a.n_in);
       }
+#pragma unroll
+      for (uint32_t i = 0; i < WR; i++) load_to_lds(wp[i] + (size_t)step * 64, at + XB + (wave * WR + i) * 1024);
     } else {
+      if (step < full) {
+#pragma unroll
+        for (uint32_t i = 0; i < XR; i++) load_to_lds(xbase + (size_t)step * 128, xp[i], at + (wave * XR + i) * 1024);
+      } else {
+        // chunks behind the row's end: its first one, to be cleared
+#pragma unroll
+        for (uint32_t i = 0; i < XR; i++) {
+          const uint32_t c = x_chunk(i);
+          load_to_lds(xbase, step * 128 + c < a.n_in ? xp[i] + step * 128 : xp[i] - c, at + (wave * XR + i) * 1024);
+        }
+      }
+#pragma unroll
+      for (uint32_t i = 0; i < WR; i++) load_to_lds(wbase + (size_t)step * 64, wp[i], at + XB + (wave * WR + i) * 1024);
+    }
+  };
+  // (once the wave's own pieces of the last step, which is not a whole one, are there)
+  auto clear_end = [&](uint32_t step, uint32_t stage) {
+    if constexpr (!ODD) {
 #pragma unroll
       for (uint32_t i = 0; i < XR; i++)
-        load_to_lds(step < full || step * 128 + xc[i] < a.n_in ? xp[i] + (size_t)step * 128 : (const int8_t*)&zeros16,
-                    at + (wave * XR + i) * 1024);
+        if (step * 128 + x_chunk(i) >= a.n_in)
+          *(v4i*)(lds + stage * STAGE + (wave * XR + i) * 1024 + lane * 16) = v4i{0, 0, 0, 0};
     }
-#pragma unroll
-    for (uint32_t i = 0; i < WR; i++) load_to_lds(wp[i] + (size_t)step * 64, at + XB + (wave * WR + i) * 1024);
   };
   auto put_held = [&](uint32_t stage) {
     if constexpr (ODD) {
@@ -290,7 +322,7 @@ __global__ __launch_bounds__(64 * WT * WN) void k_i4_ring(I4Args a, uint32_t til
       for (uint32_t i = 0; i < XR; i++) *(v4i*)(lds + stage * STAGE + (wave * XR + i) * 1024 + lane * 16) = held[i];
     }
   };
-  float sc[SR];
+  uint32_t sc[SR];
   const uint32_t whole = G >= 128 ? a.group / 128 : 1;  // steps of a group
   auto fetch_scales = [&](uint32_t window) {
 #pragma unroll
@@ -299,14 +331,14 @@ __global__ __launch_bounds__(64 * WT * WN) void k_i4_ring(I4Args a, uint32_t til
       uint32_t g = window * ROWS + k / BN;
       if (G >= 128) g /= whole;
       if (g >= a.groups) g = a.groups - 1;  // (behind the row's end: x is zero)
-      sc[i] = i4_scale(a, ch * a.groups + (size_t)g * a.n_out + n);
+      sc[i] = scale_bits(a, ch * a.groups + (size_t)g * a.n_out + n);
     }
   };
   auto put_scales = [&](uint32_t window) {
 #pragma unroll
     for (uint32_t i = 0; i < SR; i++) {
       const uint32_t k = tid + i * THREADS;
-      scales[window & 1][k / BN][k % BN] = sc[i];
+      scales[window & 1][k / BN][k % BN] = scale_of(a, sc[i]);
     }
   };
   // the results' factors, a few for each thread, there when they are needed
@@ -335,7 +367,17 @@ __global__ __launch_bounds__(64 * WT * WN) void k_i4_ring(I4Args a, uint32_t til
   for (uint32_t s = 0; s < 4; s++) cx[s] = ((2 * s + hi) ^ (fr >> 1 & 7)) * 16;
 #pragma unroll
   for (uint32_t s = 0; s < 2; s++) cw[s] = ((2 * s + hi) ^ (fr >> 2 & 3)) * 16;
-  float acc[FN][FT][16] = {};
+  // A step's units, their matrix instructions, and whether a step's last unit is left
+  // to the next step.
+  constexpr int UNITS = FN * FT * NS, M = 4 / NS;
+  constexpr bool DEFER = UNITS % 2 == 0;
+  float acc[FN][FT][16] = {}, last = 0.0f;
+  v16i part[2] = {};
+  auto add_last = [&] {
+#pragma unroll
+    for (int r = 0; r < 16; r++)
+      acc[FN - 1][FT - 1][r] = fmaf((float)part[(UNITS - 1) & 1][r], last, acc[FN - 1][FT - 1][r]);
+  };
   if (steps) {
     fetch_scales(0);
     fetch(0, 0);
@@ -349,13 +391,16 @@ __global__ __launch_bounds__(64 * WT * WN) void k_i4_ring(I4Args a, uint32_t til
       // this step's pieces are in, also those of the other waves; all have read the last one's
       if (step + 1 < steps) wait_loads<(ODD ? 0 : XR) + WR>();
       else wait_loads<0>();
+      if (step >= full) clear_end(step, stage);
       wait_lds();
       meet();
       if (step % W == 0 && step + W < steps) fetch_scales(step / W + 1);
       if (step + 2 < steps) fetch(step + 2, after);
       const int8_t *sx = fx + stage * STAGE, *sw = fw + stage * STAGE;
-      v4i wf[FN][4];
+      v4i wf[FN][4], xf[4];
       float ws[FN][NS];
+#pragma unroll
+      for (int s = 0; s < 4; s++) xf[s] = *(const v4i*)(sx + cx[s]);
 #pragma unroll
       for (int i = 0; i < FN; i++) {
 #pragma unroll
@@ -368,27 +413,35 @@ __global__ __launch_bounds__(64 * WT * WN) void k_i4_ring(I4Args a, uint32_t til
         for (int k = 0; k < NS; k++)
           ws[i][k] = scales[step / W & 1][step % W * NS + k][wave_n * FN * 32 + i * 32 + fr];
       }
+      // unit u: square u / NS, its group u % NS; the sums of the unit before go to the
+      // results between this one's matrix instructions
 #pragma unroll
-      for (int j = 0; j < FT; j++) {
-        v4i xf[4];
+      for (int u = 0; u < UNITS; u++) {
+        const int j = u / NS / FN, i = u / NS % FN, k = u % NS;
 #pragma unroll
-        for (int s = 0; s < 4; s++) xf[s] = *(const v4i*)(sx + j * 32 * 128 + cx[s]);
+        for (int m = 0; m < M; m++) {
+          const int s = k * M + m;
+          const v16i zero = {};
+          part[u & 1] = __builtin_amdgcn_mfma_i32_32x32x32_i8(xf[s], wf[i][s], m ? part[u & 1] : zero, 0, 0, 0);
+          // (the fragment's last use: the next tokens' takes its place)
+          if (i == FN - 1 && j + 1 < FT) xf[s] = *(const v4i*)(sx + (j + 1) * 32 * 128 + cx[s]);
+          __builtin_amdgcn_sched_barrier(0);
+          if (u || DEFER) {
+            const int v = u ? u - 1 : UNITS - 1;
+            const float w = u ? ws[v / NS % FN][v % NS] : last;
+            // (not after the first, whose turn the sums before are not there yet)
 #pragma unroll
-        for (int i = 0; i < FN; i++) {
-          v16i part = {};
-#pragma unroll
-          for (int s = 0; s < 4; s++) {
-            part = __builtin_amdgcn_mfma_i32_32x32x32_i8(xf[s], wf[i][s], part, 0, 0, 0);
-            if ((s + 1) % (4 / NS) == 0) {
-#pragma unroll
-              for (int r = 0; r < 16; r++) acc[i][j][r] = fmaf((float)part[r], ws[i][s * NS / 4], acc[i][j][r]);
-              part = v16i{};
-            }
+            for (int r = M > 1 ? (m ? (m - 1) * 16 / (M - 1) : 0) : 0; r < (M > 1 ? m * 16 / (M - 1) : 16); r++)
+              acc[v / NS % FN][v / NS / FN][r] = fmaf((float)part[v & 1][r], w, acc[v / NS % FN][v / NS / FN][r]);
           }
+          __builtin_amdgcn_sched_barrier(0);
         }
       }
+      last = ws[FN - 1][NS - 1];
+      if (!DEFER) add_last();
       stage = next;
     }
+    if (DEFER) add_last();
   }
   // ---- results: a wave's 32 tokens at a time, by way of its own LDS
   wait_lds();
@@ -412,7 +465,7 @@ __global__ __launch_bounds__(64 * WT * WN) void k_i4_ring(I4Args a, uint32_t til
 #pragma unroll
       for (int r = 0; r < 16; r++) own[(8 * (r / 4) + 4 * hi + r % 4) * LD + i * 32 + fr] = acc[i][j][r];
     wait_lds();  // one wave's LDS accesses are in order; this keeps the compiler to it
-#pragma unroll
+#pragma unroll 1
     for (uint32_t s = 0; s < 32; s += PER) {
       const uint32_t row = s + lane / PIECES, tt = wave_t * FT * 32 + j * 32 + row, t = r0 + tt;
       if (t < r1 && n < a.n_out) {
@@ -448,7 +501,9 @@ static int i4_tiles(zk_context* ctx, const I4Args& a, uint32_t bt, uint32_t bn, 
 template <int G, bool GROUPED>
 static int i4_launch_ring(zk_context* ctx, const I4Args& a, hipStream_t st) {
   const char* name = GROUPED ? "i4_matmul_experts" : "i4_matmul";
-  const bool odd = (((uintptr_t)a.x | a.ld_x | a.n_in) & 15) != 0;
+  // rows of whole chunks whose places in a block's reach 32 bits hold
+  const bool odd = (((uintptr_t)a.x | a.ld_x | a.n_in) & 15) != 0 || a.ld_w >> 23 || a.ld_x >> 23 ||
+                   (GROUPED && (uint64_t)a.tokens * a.ld_x >> 32);
   auto go = [&](auto kernel, uint32_t threads, uint32_t bt, uint32_t bn) -> int {
     uint32_t tiles_t, tiles_n, blocks;
     ZK_TRY(i4_tiles<GROUPED>(ctx, a, bt, bn, tiles_t, tiles_n, blocks));
@@ -458,7 +513,8 @@ static int i4_launch_ring(zk_context* ctx, const I4Args& a, hipStream_t st) {
   auto by_tile = [&](auto is_odd) -> int {
     constexpr bool ODD = decltype(is_odd)::value;
     const size_t t256 = (size_t)cdiv(a.rows, 256) * cdiv(a.n_out, 256), t128 = (size_t)cdiv(a.rows, 128) * cdiv(a.n_out, 128);
-    if (t256 >= 256 && !GROUPED) return go(k_i4_ring<G, GROUPED, ODD, 2, 4, 4, 2>, 512, 256, 256);
+    if constexpr (!ODD && !GROUPED)
+      if (t256 >= 256) return go(k_i4_ring<G, GROUPED, ODD, 2, 4, 4, 2>, 512, 256, 256);
     if (t128 >= 128) return go(k_i4_ring<G, GROUPED, ODD, 2, 2, 2, 2>, 256, 128, 128);
     return go(k_i4_ring<G, GROUPED, ODD, 2, 2, 1, 1>, 256, 64, 64);
   };

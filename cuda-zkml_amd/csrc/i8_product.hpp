@@ -152,6 +152,10 @@ __device__ const v4i zeros16 = {0, 0, 0, 0};
 __device__ __forceinline__ void load_to_lds(const int8_t* p, uint32_t at) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(at), "v"(p) : "m0");
 }
+// The same from `p` + off, p the same in the whole wave: one register for an address.
+__device__ __forceinline__ void load_to_lds(const int8_t* p, uint32_t off, uint32_t at) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(at), "v"(off), "s"(p) : "m0");
+}
 #pragma clang diagnostic pop
 // Until at most N of the wave's loads are under way.
 template <int N>
