@@ -242,6 +242,7 @@ __global__ __launch_bounds__(64 * WT * WN, 2) void k_i4_ring(I4Args a, uint32_t 
   constexpr uint32_t WAVES = WT * WN, THREADS = 64 * WAVES, BT = WT * FT * 32, BN = WN * FN * 32;
   constexpr uint32_t XB = BT * 128, WB = BN * 64, STAGE = XB + WB, STAGES = 3;
   constexpr uint32_t XR = BT / 8 / WAVES, WR = BN / 16 / WAVES;  // 1 KB pieces of a stage that a wave fills
+  constexpr int LOADS = (ODD ? 0 : XR) + WR;                     // of them straight to LDS
   constexpr int NS = G >= 128 ? 1 : 128 / G;                     // scales of a step
   constexpr uint32_t ROWS = 4, W = ROWS / NS;                    // rows of scales, and steps, of a window
   constexpr uint32_t SR = ROWS * BN / THREADS;                   // scales of a window that a thread loads
@@ -281,18 +282,20 @@ __global__ __launch_bounds__(64 * WT * WN, 2) void k_i4_ring(I4Args a, uint32_t 
     else xp[i] = (uint32_t)off + x_chunk(i);
   }
   v4i held[ODD ? XR : 1];
-  auto fetch = [&](uint32_t step, uint32_t stage) {
+  // LONG: a whole step.
+  auto fetch = [&](auto is_long, uint32_t step, uint32_t stage) {
+    constexpr bool LONG = decltype(is_long)::value;
     const uint32_t at = base + stage * STAGE;
     if constexpr (ODD) {
 #pragma unroll
       for (uint32_t i = 0; i < XR; i++) {
-        if (step < full) __builtin_memcpy(&held[i], xp[i] + step * 128 + x_chunk(i), 16);
+        if (LONG || step < full) __builtin_memcpy(&held[i], xp[i] + step * 128 + x_chunk(i), 16);
         else held[i] = x_piece(xp[i], step * 128 + x_chunk(i), a.n_in);
       }
 #pragma unroll
       for (uint32_t i = 0; i < WR; i++) load_to_lds(wp[i] + (size_t)step * 64, at + XB + (wave * WR + i) * 1024);
     } else {
-      if (step < full) {
+      if (LONG || step < full) {
 #pragma unroll
         for (uint32_t i = 0; i < XR; i++) load_to_lds(xbase + (size_t)step * 128, xp[i], at + (wave * XR + i) * 1024);
       } else {
@@ -378,29 +381,35 @@ __global__ __launch_bounds__(64 * WT * WN, 2) void k_i4_ring(I4Args a, uint32_t 
     for (int r = 0; r < 16; r++)
       acc[FN - 1][FT - 1][r] = fmaf((float)part[(UNITS - 1) & 1][r], last, acc[FN - 1][FT - 1][r]);
   };
+  // Stage of step s, in its slot, becomes every wave's to read: its pieces are in, those
+  // of the other waves too, and all have read the stage before the last; the one after the
+  // next is asked for in that one's place.
+  auto up = [](uint32_t slot) { return slot + 1 < STAGES ? slot + 1 : 0; };
+  auto turn = [&](auto is_long, uint32_t s, uint32_t slot) {
+    constexpr bool LONG = decltype(is_long)::value;
+    if (LONG || s + 1 < steps) put_held(up(slot));
+    if (s % W == 0) put_scales(s / W);
+    if (LONG || s + 1 < steps) wait_loads<LOADS>();
+    else wait_loads<0>();
+    if (!LONG && s >= full) clear_end(s, slot);
+    wait_lds();
+    meet();
+    if (s % W == 0 && s + W < steps) fetch_scales(s / W + 1);
+    if (LONG || s + 2 < steps) fetch(is_long, s + 2, up(up(slot)));
+  };
   if (steps) {
     fetch_scales(0);
-    fetch(0, 0);
+    fetch(std::false_type(), 0, 0);
     put_held(0);
-    if (steps > 1) fetch(1, 1);
-    uint32_t stage = 0;
-    for (uint32_t step = 0; step < steps; step++) {
-      const uint32_t next = stage + 1 < STAGES ? stage + 1 : 0, after = next + 1 < STAGES ? next + 1 : 0;
-      if (step + 1 < steps) put_held(next);
-      if (step % W == 0) put_scales(step / W);
-      // this step's pieces are in, also those of the other waves; all have read the last one's
-      if (step + 1 < steps) wait_loads<(ODD ? 0 : XR) + WR>();
-      else wait_loads<0>();
-      if (step >= full) clear_end(step, stage);
-      wait_lds();
-      meet();
-      if (step % W == 0 && step + W < steps) fetch_scales(step / W + 1);
-      if (step + 2 < steps) fetch(step + 2, after);
-      const int8_t *sx = fx + stage * STAGE, *sw = fw + stage * STAGE;
+    if (steps > 1) fetch(std::false_type(), 1, 1);
+    uint32_t slot = 0;
+    auto run = [&](auto is_long, uint32_t step) {
+      turn(is_long, step, slot);
+      const int8_t *sx = fx + slot * STAGE, *sw = fw + slot * STAGE;
       v4i wf[FN][4], xf[4];
       float ws[FN][NS];
 #pragma unroll
-      for (int s = 0; s < 4; s++) xf[s] = *(const v4i*)(sx + cx[s]);
+      for (int q = 0; q < 4; q++) xf[q] = *(const v4i*)(sx + cx[q]);
 #pragma unroll
       for (int i = 0; i < FN; i++) {
 #pragma unroll
@@ -420,27 +429,34 @@ __global__ __launch_bounds__(64 * WT * WN, 2) void k_i4_ring(I4Args a, uint32_t 
         const int j = u / NS / FN, i = u / NS % FN, k = u % NS;
 #pragma unroll
         for (int m = 0; m < M; m++) {
-          const int s = k * M + m;
+          const int q = k * M + m;
           const v16i zero = {};
-          part[u & 1] = __builtin_amdgcn_mfma_i32_32x32x32_i8(xf[s], wf[i][s], m ? part[u & 1] : zero, 0, 0, 0);
+          part[u & 1] = __builtin_amdgcn_mfma_i32_32x32x32_i8(xf[q], wf[i][q], m ? part[u & 1] : zero, 0, 0, 0);
           // (the fragment's last use: the next tokens' takes its place)
-          if (i == FN - 1 && j + 1 < FT) xf[s] = *(const v4i*)(sx + (j + 1) * 32 * 128 + cx[s]);
+          if (i == FN - 1 && j + 1 < FT) xf[q] = *(const v4i*)(sx + (j + 1) * 32 * 128 + cx[q]);
           __builtin_amdgcn_sched_barrier(0);
           if (u || DEFER) {
             const int v = u ? u - 1 : UNITS - 1;
             const float w = u ? ws[v / NS % FN][v % NS] : last;
             // (not after the first, whose turn the sums before are not there yet)
+            constexpr int SHARE = M > 1 ? M - 1 : 1;
+            const int lo = M == 1 || m == 0 ? 0 : (m - 1) * 16 / SHARE, to = M == 1 ? 16 : m * 16 / SHARE;
 #pragma unroll
-            for (int r = M > 1 ? (m ? (m - 1) * 16 / (M - 1) : 0) : 0; r < (M > 1 ? m * 16 / (M - 1) : 16); r++)
-              acc[v / NS % FN][v / NS / FN][r] = fmaf((float)part[v & 1][r], w, acc[v / NS % FN][v / NS / FN][r]);
+            for (int r = 0; r < 16; r++)
+              if (r >= lo && r < to)
+                acc[v / NS % FN][v / NS / FN][r] = fmaf((float)part[v & 1][r], w, acc[v / NS % FN][v / NS / FN][r]);
           }
           __builtin_amdgcn_sched_barrier(0);
         }
       }
       last = ws[FN - 1][NS - 1];
       if (!DEFER) add_last();
-      stage = next;
-    }
+      slot = up(slot);
+    };
+    uint32_t step = 0;
+    if constexpr (FT * FN < 8)  // (the largest squares' registers do not suffice for two loops)
+      for (; step + 2 < full; step++) run(std::true_type(), step);
+    for (; step < steps; step++) run(std::false_type(), step);
     if (DEFER) add_last();
   }
   // ---- results: a wave's 32 tokens at a time, by way of its own LDS
@@ -515,8 +531,8 @@ static int i4_launch_ring(zk_context* ctx, const I4Args& a, hipStream_t st) {
     const size_t t256 = (size_t)cdiv(a.rows, 256) * cdiv(a.n_out, 256), t128 = (size_t)cdiv(a.rows, 128) * cdiv(a.n_out, 128);
     if constexpr (!ODD && !GROUPED)
       if (t256 >= 256) return go(k_i4_ring<G, GROUPED, ODD, 2, 4, 4, 2>, 512, 256, 256);
-    if (t128 >= 128) return go(k_i4_ring<G, GROUPED, ODD, 2, 2, 2, 2>, 256, 128, 128);
-    return go(k_i4_ring<G, GROUPED, ODD, 2, 2, 1, 1>, 256, 64, 64);
+    if (t128 >= 512 && !GROUPED) return go(k_i4_ring<G, GROUPED, ODD, 2, 2, 2, 2>, 256, 128, 128);
+    return go(k_i4_ring<G, GROUPED, ODD, 1, 4, 2, 1>, 256, 64, 128);
   };
   return odd ? by_tile(std::true_type()) : by_tile(std::false_type());
 }
