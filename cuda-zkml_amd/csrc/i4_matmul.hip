@@ -71,127 +71,197 @@ __device__ __forceinline__ void i4_put(const I4Args& a, uint32_t t, uint32_t n, 
   else ((__bf16*)a.y)[at] = (__bf16)v;
 }
 
-// A block has 16 FT tokens x 16 FN channels, its KW waves a part of k each, in
-// steps of 128; their sums meet in LDS.  The matrix instruction takes 16 tokens (D's
-// rows) and 16 channels (its columns): a lane holds four tokens of one channel, and
-// needs one scale.  16 packed bytes of a lane are its operands of two instructions, 16
-// times the weights, which the results take back.  G: 128 for groups of whole steps,
-// 64, or 32, where an instruction's two groups are told apart by x: the lanes of the
-// other group hold zeros.  D's row 4 c + i is token 4 i + c of the 16, so that up to
-// four tokens (NI = 1) are one register of each lane.
-template <class S, int G, bool GROUPED, int FT, int FN, int NI, int KW, int U>
-__global__ __launch_bounds__(64 * KW) void k_i4_direct(I4Args a, uint32_t tiles_t, uint32_t tiles_n) {
+// A scale's bits, and what they are worth (apart, so that a load waits for nothing).
+__device__ __forceinline__ uint32_t scale_bits(const I4Args& a, size_t at) {
+  return a.scale_type == ZK_F32 ? ((const uint32_t*)a.scale)[at] : ((const uint16_t*)a.scale)[at];
+}
+__device__ __forceinline__ float scale_of(const I4Args& a, uint32_t bits) {
+  if (a.scale_type == ZK_F32) return __uint_as_float(bits);
+  if (a.scale_type == ZK_BF16) return __uint_as_float(bits << 16);
+  const uint16_t b = (uint16_t)bits;
+  _Float16 h;
+  __builtin_memcpy(&h, &b, 2);
+  return (float)h;
+}
+
+// Few tokens (decoding), or a small layer: w is read once.  A block has 16 FT tokens x
+// 16 FN channels, its KW waves a part of k each, in steps of 128; their sums meet in LDS.
+// A wave's rows come by lanes that lie side by side in them, straight from memory into
+// LDS of its own, U steps ahead (a fragment's 64 lanes, sixteen rows apart, are sixty-four
+// accesses of 16 bytes to the vector cache, which does one a cycle: 48 tokens, 8192 to
+// 8192, took 20 us that way), so that waves wait for nobody until the end.
+// The matrix instruction takes 16 tokens (D's rows) and 16 channels (its columns): a lane
+// holds four tokens of one channel, and needs one scale.  16 packed bytes of a lane are its
+// operands of two instructions, 16 times the weights, which the results take back.  G: 128
+// for groups of whole steps, 64, or 32, where an instruction's two groups are told apart by
+// x: the lanes of the other group hold zeros.  D's row 4 c + i is token 4 i + c of the 16, so
+// that up to four tokens (NI = 1) are one register of each lane.  ODD: x's rows start at
+// any byte or end inside a chunk of 16; they come through registers, masked.
+template <int G, bool GROUPED, bool ODD, int FT, int FN, int NI, int KW, int U>
+__global__ __launch_bounds__(64 * KW) void k_i4_wave(I4Args a, uint32_t tiles_t, uint32_t tiles_n) {
   constexpr uint32_t BT = NI < 4 ? 4 * NI : 16 * FT, BN = 16 * FN;
-  __shared__ __align__(16) float sums[KW][FN * FT][NI][64];
+  constexpr uint32_t XROWS = NI < 4 ? 4 : 16 * FT;               // of x in LDS
+  constexpr uint32_t XB = XROWS * 128, WB = BN * 64, STEP = XB + WB, OWN = 2 * U * STEP;
+  constexpr int XP = U * (int)XB / 1024;                         // 1 KB pieces of x in U steps
+  constexpr int LOADS = (ODD ? 0 : XP) + U * FN;
+  constexpr int NS = G >= 128 ? 1 : 128 / G;                     // scales of a step
+  constexpr uint32_t ROWS = 16, W = ROWS / NS;                   // rows of scales, and steps, of a window
+  constexpr uint32_t SUMS = FN * FT * NI * 64 * 4;
+  static_assert(XP * 1024 == U * (int)XB && KW * OWN >= KW * SUMS, "whole pieces; the sums' LDS is the rows'");
+  __shared__ __align__(16) int8_t lds[KW * OWN];
+  __shared__ float scales[KW][ROWS][BN];
   const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   uint32_t r0, r1, n0, e;
   if (!block_tile<GROUPED>(a, BT, BN, tiles_t, tiles_n, r0, r1, n0, e)) return;
   const bool none = GROUPED && e >= a.experts;
   const uint32_t fr = lane & 15, c = lane >> 4;
   const size_t ch = none ? 0 : (size_t)e * a.n_out;
-  const int8_t *xp[FT], *wp[FN];
-  const S* sp[FN];
+  const uint32_t steps = none ? 0 : (a.n_in + 127) / 128;
+  const uint32_t per = (steps + KW - 1) / KW, first = wave * per, last = first + per < steps ? first + per : steps;
+  // ---- what a lane fetches: x's piece p is its rows 8 p to 8 p + 7 of the U steps' one after
+  // the other; chunk s of a row r lies at s ^ (r / 2 % 8), w's at s ^ (r / 4 % 4)
+  const int8_t *xp[XP], *wp[FN];
+  auto x_step = [&](int p) { return (p * 8 + (lane >> 3)) / XROWS; };
+  auto x_chunk = [&](int p) { return ((lane & 7) ^ (((p * 8 + (lane >> 3)) % XROWS) >> 1 & 7)) * 16; };
 #pragma unroll
   for (int i = 0; i < FN; i++) {
-    const uint32_t n = n0 + i * 16 + fr, m = n < a.n_out ? n : a.n_out - 1;
-    wp[i] = a.w + (ch + m) * a.ld_w + 16 * c;
-    sp[i] = (const S*)a.scale + ch * a.groups + m;
+    const uint32_t row = i * 16 + (lane >> 2), n = n0 + row < a.n_out ? n0 + row : a.n_out - 1;
+    wp[i] = a.w + (ch + n) * a.ld_w + ((lane & 3) ^ (row >> 2 & 3)) * 16;
   }
 #pragma unroll
-  for (int j = 0; j < FT; j++) {
-    const uint32_t t = r0 + j * 16 + (NI > 1 ? (fr & 3) * 4 : 0) + (fr >> 2), r = t < r1 ? t : r1 - 1;
+  for (int p = 0; p < XP; p++) {
+    const uint32_t row = (p * 8 + (lane >> 3)) % XROWS;
+    const uint32_t t = r0 + (NI < 4 ? row : row / 16 * 16 + (row & 3) * 4 + (row % 16 >> 2)), r = t < r1 ? t : r1 - 1;
     const int64_t s = GROUPED ? source_row(a, r) : (int64_t)r;
-    xp[j] = a.x + (size_t)(s < 0 ? 0 : s) * a.ld_x;
+    xp[p] = a.x + (size_t)(s < 0 ? 0 : s) * a.ld_x;
   }
-  float acc[FN][FT][NI] = {};
-  const uint32_t steps = none ? 0 : (a.n_in + 127) / 128, full = a.n_in / 128;
-  const uint32_t per = (steps + KW - 1) / KW;
-  const uint32_t first = wave * per, last = first + per < steps ? first + per : steps;
-  constexpr int NS = G >= 128 ? 1 : 128 / G;  // scales of a step
-  // G = 128: the step's group and how many of its steps are past
-  const uint32_t whole = a.group / 128;
-  uint32_t group = 0, past = 0;
-  if (G >= 128) group = first / whole, past = first % whole;
-  for (uint32_t s0 = first; s0 < last; s0 += U) {
-    v4i wf[U][FN], xf[U][FT][2];
-    S sc[U][FN][NS];
+  // the results that the thread will finish: their factors
+  constexpr int DONE = (FN * FT * NI + KW - 1) / KW;
+  float fx[DONE], fb[DONE];
+  bool has[DONE];
 #pragma unroll
-    for (int u = 0; u < U; u++) {
-      const uint32_t step = s0 + u < last ? s0 + u : last - 1;  // (again the last one, not used)
+  for (int d = 0; d < DONE; d++) {
+    const uint32_t r = wave + d * KW, sq = r / NI, t = r0 + sq % FT * 16 + 4 * (r % NI) + c, n = n0 + sq / FT * 16 + fr;
+    const bool in = r < FN * FT * NI && t < r1 && t < r0 + BT && n < a.n_out;
+    int64_t s = -1;
+    if (in && !none) s = GROUPED ? source_row(a, t) : (int64_t)t;
+    has[d] = s >= 0;
+    fx[d] = has[d] && a.sx ? a.sx[s] : 1.0f;
+    fb[d] = has[d] && a.bias ? a.bias[ch + n] : 0.0f;
+  }
+  int8_t* own = lds + wave * OWN;
+  const uint32_t base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) int8_t*)lds + wave * OWN;
+  // U steps from s on into one half of the wave's LDS: x's rows of each, then w's
+  auto fetch = [&](uint32_t s, uint32_t half) {
+    const uint32_t at = base + half * U * STEP;
+    if constexpr (ODD) {
+      v4i held[XP];
 #pragma unroll
-      for (int i = 0; i < FN; i++) wf[u][i] = *(const v4i*)(wp[i] + (size_t)step * 64);
+      for (int p = 0; p < XP; p++) held[p] = x_piece(xp[p], (s + x_step(p)) * 128 + x_chunk(p), a.n_in);
 #pragma unroll
-      for (int k = 0; k < NS; k++) {
-        uint32_t g = G >= 128 ? group : step * NS + k;
-        if (G < 128 && g >= a.groups) g = a.groups - 1;  // (behind the row's end: x is zero)
+      for (int p = 0; p < XP; p++) *(v4i*)(own + half * U * STEP + p * 1024 + lane * 16) = held[p];
+    } else {
 #pragma unroll
-        for (int i = 0; i < FN; i++) sc[u][i][k] = sp[i][(size_t)g * a.n_out];
-      }
-      if (G >= 128 && s0 + u + 1 < last && ++past == whole) past = 0, group++;
-      if (step < full) {
-#pragma unroll
-        for (int j = 0; j < FT; j++)
-#pragma unroll
-          for (int h = 0; h < 2; h++) __builtin_memcpy(&xf[u][j][h], xp[j] + step * 128 + 64 * h + 16 * c, 16);
-      } else {
-#pragma unroll
-        for (int j = 0; j < FT; j++)
-#pragma unroll
-          for (int h = 0; h < 2; h++) xf[u][j][h] = x_piece(xp[j], step * 128 + 64 * h + 16 * c, a.n_in);
+      for (int p = 0; p < XP; p++) {
+        const uint32_t k = (s + x_step(p)) * 128 + x_chunk(p);
+        load_to_lds(k < a.n_in ? xp[p] + k : (const int8_t*)&zeros16, at + p * 1024);
       }
     }
 #pragma unroll
     for (int u = 0; u < U; u++) {
-      if (s0 + u >= last) break;
+      const uint32_t step = s + u < last ? s + u : last - 1;  // (again the last one, not used)
 #pragma unroll
-      for (int i = 0; i < FN; i++) {
-        const v4i high = wf[u][i] & (int)0xf0f0f0f0, low = (wf[u][i] << 4) & (int)0xf0f0f0f0;
+      for (int i = 0; i < FN; i++) load_to_lds(wp[i] + (size_t)step * 64, at + U * XB + u * WB + i * 1024);
+    }
+  };
+  float acc[FN][FT][NI] = {};
+  const uint32_t whole = G >= 128 ? a.group / 128 : 1;  // steps of a group
+  for (uint32_t w0 = first; w0 < last; w0 += W) {
+    const uint32_t end = w0 + W < last ? w0 + W : last;
+    uint32_t sc[4 * FN];
+#pragma unroll
+    for (int i = 0; i < 4 * FN; i++) {
+      const uint32_t k = lane + i * 64, n = n0 + k % BN < a.n_out ? n0 + k % BN : a.n_out - 1;
+      uint32_t g = w0 * NS + k / BN;
+      if (G >= 128) g /= whole;
+      if (g >= a.groups) g = a.groups - 1;  // (behind the row's end: x is zero)
+      sc[i] = scale_bits(a, ch * a.groups + (size_t)g * a.n_out + n);
+    }
+    fetch(w0, 0);
+    if (w0 + U < end) fetch(w0 + U, 1);
+#pragma unroll
+    for (int i = 0; i < 4 * FN; i++) scales[wave][(lane + i * 64) / BN][(lane + i * 64) % BN] = scale_of(a, sc[i]);
+    uint32_t half = 0;
+    for (uint32_t s0 = w0; s0 < end; s0 += U) {
+      if (s0 + U < end) wait_loads<LOADS>();
+      else wait_loads<0>();
+      wait_lds();
+      const int8_t *sx = own + half * U * STEP, *sw = sx + U * XB;
+#pragma unroll
+      for (int u = 0; u < U; u++) {
+        if (s0 + u >= end) break;
+        v4i xf[FT][2];
 #pragma unroll
         for (int j = 0; j < FT; j++) {
-          const v4i zero = {0, 0, 0, 0};
-          v4i part[NS];
-          if (G >= 128) {
-            part[0] = __builtin_amdgcn_mfma_i32_16x16x64_i8(xf[u][j][0], low, zero, 0, 0, 0);
-            part[0] = __builtin_amdgcn_mfma_i32_16x16x64_i8(xf[u][j][1], high, part[0], 0, 0, 0);
-          } else if (G == 64) {
-            part[0] = __builtin_amdgcn_mfma_i32_16x16x64_i8(xf[u][j][0], low, zero, 0, 0, 0);
-            part[NS - 1] = __builtin_amdgcn_mfma_i32_16x16x64_i8(xf[u][j][1], high, zero, 0, 0, 0);
-          } else {
+          const uint32_t row = NI < 4 ? fr >> 2 : j * 16 + fr;
 #pragma unroll
-            for (int k = 0; k < NS; k++) {
-              const v4i x = (int)c / 2 == k % 2 ? xf[u][j][k / 2] : zero;
-              part[k] = __builtin_amdgcn_mfma_i32_16x16x64_i8(x, k < 2 ? low : high, zero, 0, 0, 0);
+          for (int h = 0; h < 2; h++)
+            xf[j][h] = *(const v4i*)(sx + u * XB + row * 128 + ((4 * h + c) ^ (row >> 1 & 7)) * 16);
+        }
+#pragma unroll
+        for (int i = 0; i < FN; i++) {
+          const v4i p = *(const v4i*)(sw + u * WB + (i * 16 + fr) * 64 + (c ^ (fr >> 2)) * 16);
+          const v4i high = p & (int)0xf0f0f0f0, low = (p << 4) & (int)0xf0f0f0f0, zero = {0, 0, 0, 0};
+          float ws[NS];
+#pragma unroll
+          for (int k = 0; k < NS; k++) ws[k] = scales[wave][(s0 - w0 + u) * NS + k][i * 16 + fr];
+#pragma unroll
+          for (int j = 0; j < FT; j++) {
+            v4i part[NS];
+            if (G >= 128) {
+              part[0] = __builtin_amdgcn_mfma_i32_16x16x64_i8(xf[j][0], low, zero, 0, 0, 0);
+              part[0] = __builtin_amdgcn_mfma_i32_16x16x64_i8(xf[j][1], high, part[0], 0, 0, 0);
+            } else if (G == 64) {
+              part[0] = __builtin_amdgcn_mfma_i32_16x16x64_i8(xf[j][0], low, zero, 0, 0, 0);
+              part[NS - 1] = __builtin_amdgcn_mfma_i32_16x16x64_i8(xf[j][1], high, zero, 0, 0, 0);
+            } else {
+#pragma unroll
+              for (int k = 0; k < NS; k++) {
+                const v4i x = (int)c / 2 == k % 2 ? xf[j][k / 2] : zero;
+                part[k] = __builtin_amdgcn_mfma_i32_16x16x64_i8(x, k < 2 ? low : high, zero, 0, 0, 0);
+              }
             }
+#pragma unroll
+            for (int k = 0; k < NS; k++)
+#pragma unroll
+              for (int q = 0; q < NI; q++) acc[i][j][q] = fmaf((float)part[k][q], ws[k], acc[i][j][q]);
           }
-#pragma unroll
-          for (int k = 0; k < NS; k++)
-#pragma unroll
-            for (int q = 0; q < NI; q++) acc[i][j][q] = fmaf((float)part[k][q], (float)sc[u][i][k], acc[i][j][q]);
         }
       }
+      wait_lds();  // this half is read
+      if (s0 + 2 * U < end) fetch(s0 + 2 * U, half);
+      half ^= 1;
     }
   }
+  meet();  // (every wave's loads are done and read)
+  float(*sums)[FN * FT * NI][64] = (float(*)[FN * FT * NI][64])lds;
 #pragma unroll
   for (int i = 0; i < FN; i++)
 #pragma unroll
     for (int j = 0; j < FT; j++)
 #pragma unroll
-      for (int q = 0; q < NI; q++) sums[wave][i * FT + j][q][lane] = acc[i][j][q];
-  __syncthreads();
+      for (int q = 0; q < NI; q++) sums[wave][(i * FT + j) * NI + q][lane] = acc[i][j][q];
+  wait_lds();
+  meet();
   // a wave adds up every KW-th register of the squares
 #pragma unroll
-  for (int r = 0; r < FN * FT * NI; r++) {
-    if ((uint32_t)r % KW != wave) continue;
-    const int sq = r / NI, q = r % NI;
-    const uint32_t t = r0 + (sq % FT) * 16 + 4 * q + c, n = n0 + (sq / FT) * 16 + fr;
-    if (t >= r1 || t >= r0 + BT || n >= a.n_out) continue;
-    float sum = sums[0][sq][q][lane];
+  for (int d = 0; d < DONE; d++) {
+    const uint32_t r = wave + d * KW, sq = r / NI, t = r0 + sq % FT * 16 + 4 * (r % NI) + c, n = n0 + sq / FT * 16 + fr;
+    if (r >= FN * FT * NI || t >= r1 || t >= r0 + BT || n >= a.n_out) continue;
+    float sum = sums[0][r][lane];
 #pragma unroll
-    for (int k = 1; k < KW; k++) sum += sums[k][sq][q][lane];
-    const int64_t s = none ? -1 : GROUPED ? source_row(a, t) : (int64_t)t;
-    float v = 0.0f;
-    if (s >= 0) v = i4_finish(sum * 0.0625f, a.sx ? a.sx[s] : 1.0f, a.bias ? a.bias[ch + n] : 0.0f, a.relu);
-    i4_put(a, t, n, v);
+    for (int k = 1; k < KW; k++) sum += sums[k][r][lane];
+    i4_put(a, t, n, has[d] ? i4_finish(sum * 0.0625f, fx[d], fb[d], a.relu) : 0.0f);
   }
 }
 
@@ -210,19 +280,6 @@ __device__ __forceinline__ void put8(T* y, uint32_t left, const float (&v)[8]) {
     for (uint32_t k = 0; k < 7; k++)
       if (k < left) y[k] = r[k];
   }
-}
-
-// A scale's bits, and what they are worth (apart, so that a load waits for nothing).
-__device__ __forceinline__ uint32_t scale_bits(const I4Args& a, size_t at) {
-  return a.scale_type == ZK_F32 ? ((const uint32_t*)a.scale)[at] : ((const uint16_t*)a.scale)[at];
-}
-__device__ __forceinline__ float scale_of(const I4Args& a, uint32_t bits) {
-  if (a.scale_type == ZK_F32) return __uint_as_float(bits);
-  if (a.scale_type == ZK_BF16) return __uint_as_float(bits << 16);
-  const uint16_t b = (uint16_t)bits;
-  _Float16 h;
-  __builtin_memcpy(&h, &b, 2);
-  return (float)h;
 }
 
 // A block computes BT tokens x BN channels, its WT x WN waves a grid of FT x FN
@@ -537,32 +594,40 @@ static int i4_launch_ring(zk_context* ctx, const I4Args& a, hipStream_t st) {
   return odd ? by_tile(std::true_type()) : by_tile(std::false_type());
 }
 
-template <class S, int G, bool GROUPED>
-static int i4_launch(zk_context* ctx, const I4Args& a, hipStream_t st) {
+template <int G, bool GROUPED>
+static int i4_launch_wave(zk_context* ctx, const I4Args& a, uint32_t rows, hipStream_t st) {
   const char* name = GROUPED ? "i4_matmul_experts" : "i4_matmul";
+  const bool odd = (((uintptr_t)a.x | a.ld_x | a.n_in) & 15) != 0;
   auto go = [&](auto kernel, uint32_t threads, uint32_t bt, uint32_t bn) -> int {
     uint32_t tiles_t, tiles_n, blocks;
     ZK_TRY(i4_tiles<GROUPED>(ctx, a, bt, bn, tiles_t, tiles_n, blocks));
     ZK_LAUNCH(ctx, st, name, kernel, dim3(blocks), dim3(threads), 0, a, tiles_t, tiles_n);
     return ZK_OK;
   };
+  auto by_rows = [&](auto is_odd) -> int {
+    constexpr bool ODD = decltype(is_odd)::value;
+    if (rows <= 4) return go(k_i4_wave<G, GROUPED, ODD, 1, 1, 1, 8, 2>, 512, 4, 16);
+    if (rows <= 16) return go(k_i4_wave<G, GROUPED, ODD, 1, 1, 4, 8, 2>, 512, 16, 16);
+    if (rows <= 32) return go(k_i4_wave<G, GROUPED, ODD, 2, 2, 4, 8, 1>, 512, 32, 32);
+    if (rows <= 48) return go(k_i4_wave<G, GROUPED, ODD, 3, 2, 4, 8, 1>, 512, 48, 32);
+    return go(k_i4_wave<G, GROUPED, ODD, 4, 2, 4, 4, 1>, 256, 64, 32);
+  };
+  return odd ? by_rows(std::true_type()) : by_rows(std::false_type());
+}
+
+template <int G, bool GROUPED>
+static int i4_launch(zk_context* ctx, const I4Args& a, hipStream_t st) {
   // rows of one expert, about
   const uint32_t rows = GROUPED ? cdiv(a.rows, a.experts < a.rows ? a.experts : a.rows) : a.rows;
-  if (rows <= 4) return go(k_i4_direct<S, G, GROUPED, 1, 1, 1, 8, 4>, 512, 4, 16);
-  if (rows <= 16) return go(k_i4_direct<S, G, GROUPED, 1, 1, 4, 8, 4>, 512, 16, 16);
-  if (rows <= 32) return go(k_i4_direct<S, G, GROUPED, 2, 2, 4, 8, 2>, 512, 32, 32);
-  if (rows <= 48) return go(k_i4_direct<S, G, GROUPED, 4, 2, 4, 8, 2>, 512, 64, 32);
+  if (rows <= (GROUPED ? 32 : 64)) return i4_launch_wave<G, GROUPED>(ctx, a, rows, st);
   return i4_launch_ring<G, GROUPED>(ctx, a, st);
 }
 
 template <bool GROUPED>
-static int i4_dispatch(zk_context* ctx, const I4Args& a, int scale_type, hipStream_t st) {
-  return by_type(scale_type, [&](auto sz) -> int {
-    typedef decltype(sz) S;
-    if (a.group == 32) return i4_launch<S, 32, GROUPED>(ctx, a, st);
-    if (a.group == 64) return i4_launch<S, 64, GROUPED>(ctx, a, st);
-    return i4_launch<S, 128, GROUPED>(ctx, a, st);
-  });
+static int i4_dispatch(zk_context* ctx, const I4Args& a, hipStream_t st) {
+  if (a.group == 32) return i4_launch<32, GROUPED>(ctx, a, st);
+  if (a.group == 64) return i4_launch<64, GROUPED>(ctx, a, st);
+  return i4_launch<128, GROUPED>(ctx, a, st);
 }
 
 // ------------------------------------------------------------ weights to 4 bits
@@ -653,7 +718,7 @@ static void set_sizes(I4Args& a, size_t rows, size_t n_out, size_t n_in, int gro
   a.group = (uint32_t)group, a.groups = cdiv(n_in, group);
 }
 
-static int i4_matmul(zk_context* ctx, const I4Args& a, int scale_type, int type, hipStream_t st) {
+static int i4_matmul(zk_context* ctx, const I4Args& a, hipStream_t st) {
   // rows in runs of at most I8_MAX_TILES tiles of 16 x 16
   const size_t most = I8_MAX_TILES / cdiv(a.n_out, 16) * 16;
   for (size_t r = 0; r < a.rows; r += most) {
@@ -661,8 +726,8 @@ static int i4_matmul(zk_context* ctx, const I4Args& a, int scale_type, int type,
     b.rows = (uint32_t)(a.rows - r < most ? a.rows - r : most);
     b.x = a.x ? a.x + r * a.ld_x : a.x;
     b.sx = a.sx ? a.sx + r : a.sx;
-    b.y = (uint8_t*)a.y + r * a.ld_y * type_bytes(type);
-    ZK_TRY(i4_dispatch<false>(ctx, b, scale_type, st));
+    b.y = (uint8_t*)a.y + r * a.ld_y * type_bytes(a.y_type);
+    ZK_TRY(i4_dispatch<false>(ctx, b, st));
   }
   return ZK_OK;
 }
@@ -720,7 +785,7 @@ int zk_i4_matmul(zk_context* ctx, const int8_t* d_x, size_t ld_x, const float* d
     if (!rows || !n_out) return ZK_OK;
     set_sizes(a, rows, n_out, n_in, group, relu, scale_type, y_type);
     OnDevice on(ctx);
-    return i4_matmul(ctx, a, scale_type, y_type, ctx->s(stream));
+    return i4_matmul(ctx, a, ctx->s(stream));
   });
 }
 
@@ -751,7 +816,7 @@ int zk_i4_linear(zk_context* ctx, const void* d_x, int x_type, size_t ld_x, cons
     OnDevice on(ctx);
     hipStream_t st = ctx->s(stream);
     ZK_TRY(i8_quantize(ctx, d_x, x_type, ld_x, rows, n_in, (int8_t*)d_work + lw.q, lw.ld, (float*)d_work, st));
-    return i4_matmul(ctx, a, scale_type, y_type, st);
+    return i4_matmul(ctx, a, st);
   });
 }
 
@@ -789,7 +854,7 @@ int zk_i4_matmul_experts(zk_context* ctx, const int8_t* d_x, size_t ld_x, const 
         return ZK_OK;
       });
     }
-    return i4_dispatch<true>(ctx, a, scale_type, ctx->s(stream));
+    return i4_dispatch<true>(ctx, a, ctx->s(stream));
   });
 }
 
