@@ -557,77 +557,102 @@ __global__ __launch_bounds__(64 * WT * WN, 2) void k_i4_ring(I4Args a, uint32_t 
   }
 }
 
-template <bool GROUPED>
-static int i4_tiles(zk_context* ctx, const I4Args& a, uint32_t bt, uint32_t bn, uint32_t& tiles_t, uint32_t& tiles_n,
-                    uint32_t& blocks) {
-  // row tiles of the grouped form: whole ones, and a part of one for each expert and
-  // for the rows without an expert
-  const uint32_t groups = a.experts + 1 < a.rows ? a.experts + 1 : a.rows;
-  tiles_t = GROUPED ? a.rows / bt + groups : cdiv(a.rows, bt);
-  tiles_n = cdiv(a.n_out, bn);
-  const size_t tiles = (size_t)tiles_t * tiles_n;
-  if (tiles > I8_MAX_TILES) return ctx->fail(ZK_ERR_SIZE, "i4 product: rows and n_out make too many tiles");
-  blocks = cdiv(tiles, 8) * 8;
-  return ZK_OK;
+// ------------------------------------------------------------ which kernel
+// A product's time in ns: that of its first tile on a CU, and of each more, both with a
+// part for every step of 128 of k (fitted to products of 1 to 4096 rows, 128 to 8192 long,
+// and to 2 to 6400 rows of 8 to 64 experts; the rule's choices took 2, 2.5 and 3% longer
+// than the best of all on the average, 27% at the most).  Rows of x of whole chunks, at any
+// byte, and grouped by expert; 0: not a choice.  Smaller groups lengthen a step.
+struct I4Cost {
+  uint32_t first, step, more, more_step;
+};
+struct I4Tile {
+  const char* name;
+  uint32_t bt, bn;
+  I4Cost whole, odd, grouped;
+  uint32_t step64, step32;  // percent of a step with groups of 64 and 32
+};
+enum I4Kernel { I4_4x16, I4_4x32, I4_16x16, I4_16x32, I4_32x32, I4_48x32, I4_32x128, I4_64x128, I4_256, I4_COUNT };
+constexpr I4Tile I4_TILES[I4_COUNT] = {
+    {"wave 4x16", 4, 16, {3866, 18, 846, 21}, {3681, 34, 810, 26}, {4541, 5, 1260, 23}, 100, 110},
+    {"wave 4x32", 4, 32, {}, {}, {4680, 44, 800, 40}, 100, 110},
+    {"wave 16x16", 16, 16, {4164, 30, 1896, 41}, {4215, 66, 2237, 67}, {}, 105, 130},
+    {"wave 16x32", 16, 32, {4468, 88, 491, 44}, {4404, 129, 393, 64}, {5568, 44, 552, 57}, 105, 130},
+    {"wave 32x32", 32, 32, {4757, 79, 3039, 76}, {5149, 125, 3493, 122}, {}, 105, 130},
+    {"wave 48x32", 48, 32, {5101, 98, 3758, 96}, {5731, 167, 4720, 156}, {}, 105, 130},
+    {"stages 32x128", 32, 128, {4453, 451, 756, 145}, {4514, 505, 1157, 154}, {4874, 457, 993, 186}, 155, 200},
+    {"stages 64x128", 64, 128, {5150, 537, 2169, 282}, {5432, 617, 2748, 336}, {5764, 542, 74, 378}, 135, 175},
+    {"stages 256x256", 256, 256, {12066, 1852, 21966, 2325}, {}, {}, 160, 290},
+};
+
+// Whether x's rows are in whole chunks of 16 bytes, and, for the stages, a block's rows
+// within 32 bits of one another.
+static bool whole_rows(const I4Args& a) { return (((uintptr_t)a.x | a.ld_x | a.n_in) & 15) == 0; }
+static bool near_rows(const I4Args& a, bool grouped) {
+  return !(a.ld_w >> 23) && !(a.ld_x >> 23) && (!grouped || !((uint64_t)a.tokens * a.ld_x >> 32));
 }
 
-template <int G, bool GROUPED>
-static int i4_launch_ring(zk_context* ctx, const I4Args& a, hipStream_t st) {
-  const char* name = GROUPED ? "i4_matmul_experts" : "i4_matmul";
-  // rows of whole chunks whose places in a block's reach 32 bits hold
-  const bool odd = (((uintptr_t)a.x | a.ld_x | a.n_in) & 15) != 0 || a.ld_w >> 23 || a.ld_x >> 23 ||
-                   (GROUPED && (uint64_t)a.tokens * a.ld_x >> 32);
-  auto go = [&](auto kernel, uint32_t threads, uint32_t bt, uint32_t bn) -> int {
-    uint32_t tiles_t, tiles_n, blocks;
-    ZK_TRY(i4_tiles<GROUPED>(ctx, a, bt, bn, tiles_t, tiles_n, blocks));
-    ZK_LAUNCH(ctx, st, name, kernel, dim3(blocks), dim3(threads), 0, a, tiles_t, tiles_n);
+static I4Kernel choose_i4(const I4Args& a, bool grouped) {
+  const bool whole = whole_rows(a), near = near_rows(a, grouped);
+  const uint64_t steps = (a.n_in + 127) / 128, groups = grouped ? (a.experts < a.rows ? a.experts : a.rows) : 0;
+  I4Kernel best = I4_4x16;
+  uint64_t least = ~0ull;
+  for (int i = 0; i < I4_COUNT; i++) {
+    const I4Tile& t = I4_TILES[i];
+    const I4Cost& c = grouped ? t.grouped : whole && (near || i < I4_32x128) ? t.whole : t.odd;
+    if (!c.first) continue;
+    // an expert's last row tile is half full, or it has only one
+    uint64_t tt = cdiv(a.rows, t.bt);
+    if (grouped && (tt += groups / 2) < groups) tt = groups;
+    const uint64_t tiles = tt * cdiv(a.n_out, t.bn), more = tiles > 256 ? tiles - 256 : 0;
+    const uint64_t k = steps * (a.group == 32 ? t.step32 : a.group == 64 ? t.step64 : 100);
+    const uint64_t time = c.first + c.step * k / 100 + (c.more * more + c.more_step * k / 100 * more) / 256;
+    if (time < least) least = time, best = (I4Kernel)i;
+  }
+  return best;
+}
+
+template <int G, bool GROUPED, bool ODD>
+static int launch_i4_as(zk_context* ctx, const I4Args& a, I4Kernel k, hipStream_t st) {
+  auto go = [&](auto kernel, uint32_t threads) -> int {
+    // row tiles of the grouped form: whole ones, and a part of one for each expert and
+    // for the rows without an expert
+    const uint32_t bt = I4_TILES[k].bt, groups = a.experts + 1 < a.rows ? a.experts + 1 : a.rows;
+    const uint32_t tiles_t = GROUPED ? a.rows / bt + groups : cdiv(a.rows, bt);
+    const uint32_t tiles_n = cdiv(a.n_out, I4_TILES[k].bn);
+    const size_t tiles = (size_t)tiles_t * tiles_n;
+    if (tiles > I8_MAX_TILES) return ctx->fail(ZK_ERR_SIZE, "i4 product: rows and n_out make too many tiles");
+    ZK_LAUNCH(ctx, st, GROUPED ? "i4_matmul_experts" : "i4_matmul", kernel, dim3(cdiv(tiles, 8) * 8), dim3(threads), 0,
+              a, tiles_t, tiles_n);
     return ZK_OK;
   };
-  auto by_tile = [&](auto is_odd) -> int {
-    constexpr bool ODD = decltype(is_odd)::value;
-    const size_t t256 = (size_t)cdiv(a.rows, 256) * cdiv(a.n_out, 256), t128 = (size_t)cdiv(a.rows, 128) * cdiv(a.n_out, 128);
-    if constexpr (!ODD && !GROUPED)
-      if (t256 >= 256) return go(k_i4_ring<G, GROUPED, ODD, 2, 4, 4, 2>, 512, 256, 256);
-    if (t128 >= 512 && !GROUPED) return go(k_i4_ring<G, GROUPED, ODD, 2, 2, 2, 2>, 256, 128, 128);
-    return go(k_i4_ring<G, GROUPED, ODD, 1, 4, 2, 1>, 256, 64, 128);
-  };
-  return odd ? by_tile(std::true_type()) : by_tile(std::false_type());
-}
-
-template <int G, bool GROUPED>
-static int i4_launch_wave(zk_context* ctx, const I4Args& a, uint32_t rows, hipStream_t st) {
-  const char* name = GROUPED ? "i4_matmul_experts" : "i4_matmul";
-  const bool odd = (((uintptr_t)a.x | a.ld_x | a.n_in) & 15) != 0;
-  auto go = [&](auto kernel, uint32_t threads, uint32_t bt, uint32_t bn) -> int {
-    uint32_t tiles_t, tiles_n, blocks;
-    ZK_TRY(i4_tiles<GROUPED>(ctx, a, bt, bn, tiles_t, tiles_n, blocks));
-    ZK_LAUNCH(ctx, st, name, kernel, dim3(blocks), dim3(threads), 0, a, tiles_t, tiles_n);
-    return ZK_OK;
-  };
-  auto by_rows = [&](auto is_odd) -> int {
-    constexpr bool ODD = decltype(is_odd)::value;
-    if (rows <= 4) return go(k_i4_wave<G, GROUPED, ODD, 1, 1, 1, 8, 2>, 512, 4, 16);
-    if (rows <= 16) return go(k_i4_wave<G, GROUPED, ODD, 1, 1, 4, 8, 2>, 512, 16, 16);
-    if (rows <= 32) return go(k_i4_wave<G, GROUPED, ODD, 2, 2, 4, 8, 1>, 512, 32, 32);
-    if (rows <= 48) return go(k_i4_wave<G, GROUPED, ODD, 3, 2, 4, 8, 1>, 512, 48, 32);
-    return go(k_i4_wave<G, GROUPED, ODD, 4, 2, 4, 4, 1>, 256, 64, 32);
-  };
-  return odd ? by_rows(std::true_type()) : by_rows(std::false_type());
-}
-
-template <int G, bool GROUPED>
-static int i4_launch(zk_context* ctx, const I4Args& a, hipStream_t st) {
-  // rows of one expert, about
-  const uint32_t rows = GROUPED ? cdiv(a.rows, a.experts < a.rows ? a.experts : a.rows) : a.rows;
-  if (rows <= (GROUPED ? 32 : 64)) return i4_launch_wave<G, GROUPED>(ctx, a, rows, st);
-  return i4_launch_ring<G, GROUPED>(ctx, a, st);
+  if (k == I4_4x16) return go(k_i4_wave<G, GROUPED, ODD, 1, 1, 1, 8, 2>, 512);
+  if (k == I4_16x32) return go(k_i4_wave<G, GROUPED, ODD, 1, 2, 4, 4, 1>, 256);
+  if (k == I4_32x128) return go(k_i4_ring<G, GROUPED, ODD, 1, 4, 1, 1>, 256);
+  if (k == I4_64x128) return go(k_i4_ring<G, GROUPED, ODD, 1, 4, 2, 1>, 256);
+  if constexpr (GROUPED) {
+    if (k == I4_4x32) return go(k_i4_wave<G, true, ODD, 1, 2, 1, 4, 2>, 256);
+  } else {
+    if (k == I4_16x16) return go(k_i4_wave<G, false, ODD, 1, 1, 4, 8, 2>, 512);
+    if (k == I4_32x32) return go(k_i4_wave<G, false, ODD, 2, 2, 4, 8, 1>, 512);
+    if (k == I4_48x32) return go(k_i4_wave<G, false, ODD, 3, 2, 4, 8, 1>, 512);
+    if constexpr (!ODD)
+      if (k == I4_256) return go(k_i4_ring<G, false, false, 2, 4, 4, 2>, 512);
+  }
+  return ctx->fail(ZK_ERR_INVALID, "i4 product: no kernel");
 }
 
 template <bool GROUPED>
 static int i4_dispatch(zk_context* ctx, const I4Args& a, hipStream_t st) {
-  if (a.group == 32) return i4_launch<32, GROUPED>(ctx, a, st);
-  if (a.group == 64) return i4_launch<64, GROUPED>(ctx, a, st);
-  return i4_launch<128, GROUPED>(ctx, a, st);
+  const I4Kernel k = choose_i4(a, GROUPED);
+  const bool odd = !whole_rows(a) || (k >= I4_32x128 && !near_rows(a, GROUPED));
+  auto by_odd = [&](auto g) -> int {
+    constexpr int G = decltype(g)::value;
+    return odd ? launch_i4_as<G, GROUPED, true>(ctx, a, k, st) : launch_i4_as<G, GROUPED, false>(ctx, a, k, st);
+  };
+  if (a.group == 32) return by_odd(std::integral_constant<int, 32>());
+  if (a.group == 64) return by_odd(std::integral_constant<int, 64>());
+  return by_odd(std::integral_constant<int, 128>());
 }
 
 // ------------------------------------------------------------ weights to 4 bits
@@ -787,6 +812,17 @@ int zk_i4_matmul(zk_context* ctx, const int8_t* d_x, size_t ld_x, const float* d
     OnDevice on(ctx);
     return i4_matmul(ctx, a, ctx->s(stream));
   });
+}
+
+const char* zk_debug_i4_kernel(size_t rows, size_t n_out, size_t n_in, size_t ld_x, size_t address, int group,
+                               int experts) {
+  using namespace zk;
+  if (!rows || !n_out || rows > 0x7fffffffu || n_out > 16 * I8_MAX_TILES || n_in > I4_MAX_IN || experts < 0) return nullptr;
+  I4Args a = {};
+  a.x = (const int8_t*)address, a.ld_x = ld_x, a.ld_w = i4_row_bytes(n_in);
+  set_sizes(a, rows, n_out, n_in, group, 0, ZK_F32, ZK_F32);
+  a.experts = (uint32_t)experts, a.tokens = a.rows;
+  return I4_TILES[choose_i4(a, experts > 0)].name;
 }
 
 size_t zk_i4_linear_work(size_t rows, size_t n_in) {

@@ -129,6 +129,8 @@ def lib():
         L.zk_i4_row_bytes.restype = sz
         L.zk_i4_quantize.argtypes = [vp, vp, ci, sz, sz, sz, ci, vp, sz, vp, ci, vp]
         L.zk_i4_matmul.argtypes = [vp, vp, sz, vp, vp, sz, vp, ci, ci, vp, sz, sz, sz, ci, vp, ci, sz, vp]
+        L.zk_debug_i4_kernel.argtypes = [sz] * 5 + [ci, ci]
+        L.zk_debug_i4_kernel.restype = ctypes.c_char_p
         L.zk_i4_linear_work.argtypes = [sz, sz]
         L.zk_i4_linear_work.restype = sz
         L.zk_i4_linear.argtypes = [vp, vp, ci, sz, vp, sz, vp, ci, ci, vp, sz, sz, sz, ci, vp, ci, sz, vp, sz, vp]

@@ -42,6 +42,24 @@ def product(x, q, scale, group, sx, bias, relu):
     return (np.maximum(y, 0) if relu else y), size
 
 
+def wide_product(x, q, scale, group, sx, bias, relu):
+    """product() for many results: a group of up to 128 at a time, whose sums are exact
+    in 32-bit floats (below 128 * 128 * 8), a term's size from the magnitudes' sum."""
+    n_in, run = x.shape[1], min(group, 128)
+    y = np.zeros((x.shape[0], q.shape[0]))
+    size = np.zeros_like(y)
+    xf, qf = x.astype(np.float32), q.astype(np.float32)
+    for k in range(0, n_in, run):
+        s = scale[k // group]
+        y += (xf[:, k:k + run] @ qf[:, k:k + run].T) * s
+        size += (np.abs(xf[:, k:k + run]) @ np.abs(qf[:, k:k + run]).T) * np.abs(s)
+    s = 1.0 if sx is None else sx.astype(np.float64)[:, None]
+    y, size = y * s, size * np.abs(s)
+    if bias is not None:
+        y, size = y + bias, size + np.abs(bias)
+    return (np.maximum(y, 0) if relu else y), size
+
+
 def near(got, want, size, n_in, kind):
     """Within a rounding of 2^-24 of the terms' size for each 32 weights and three
     more (a term itself, the token's scale, the bias), and one of the result's type."""
@@ -61,4 +79,5 @@ def inputs(rng, rows, n_out, n_in, group, scale_kind="f32", experts=1):
     return x, sx, q, s, values(s, scale_kind)
 
 
-__all__ = ["packed", "unpacked", "product", "near", "inputs", "Result", "matrix", "TYPES", "values", "words", "z"]
+__all__ = ["packed", "unpacked", "product", "wide_product", "near", "inputs", "Result", "matrix", "TYPES", "values", "words",
+           "z"]

@@ -56,7 +56,8 @@ def balance(s, scale, expert):
     # a lane adds its tokens one after the other
     lim = (p * R).sum(axis=0) / max(n, 1) + (n + FEW) * 2.0**-24 * prob + 2.0**-126
     f = count[:-1] / max(1, n * slots)
-    return count, prob, experts * (f * prob).sum(), lim, experts * (f * lim).sum() + 2.0**-22 * experts * (f * prob).sum()
+    loss = experts * (f * prob).sum()
+    return count, prob, loss, lim, experts * (f * lim).sum() + 2.0**-22 * loss
 
 
 def gradient(s, scale, expert, renormalize, gw=None, count=None, gl=None):

@@ -55,7 +55,8 @@ def work_of(ctx, tokens, experts):
 
 
 # tokens, experts, slots
-SIZES = [(1, 1, 1), (1, 8, 2), (3, 2, 2), (5, 3, 8), (33, 8, 2), (17, 16, 4), (64, 17, 3), (100, 32, 6), (70, 60, 4), (257, 60, 2), (300, 1024, 3), (700, 400, 2),
+SIZES = [(1, 1, 1), (1, 8, 2), (3, 2, 2), (5, 3, 8), (33, 8, 2), (17, 16, 4), (64, 17, 3), (100, 32, 6), (70, 60, 4), (257, 60, 2),
+         (300, 1024, 3), (700, 400, 2),
          (65, 64, 8), (129, 65, 5), (300, 128, 8), (40, 129, 4), (31, 256, 32), (50, 300, 17), (9, 512, 8),
          (20, 1000, 10), (7, 1024, 32), (3000, 24, 2)]
 
@@ -76,8 +77,8 @@ def test_route(ctx, kind, renormalize, masked, ties, pad, tokens, experts, slots
     for balance in (False, True):
         o = outputs(ctx, tokens, experts, slots, balance)
         more = dict({k: r.at for k, r in o.items()}, work=work_of(ctx, tokens, experts) if balance else None)
-        ctx.experts_route(d, TYPES[kind], tokens, experts, slots, scale=scale, renormalize=renormalize, ld=experts + pad,
-                          **more)
+        ctx.experts_route(d, TYPES[kind], tokens, experts, slots, scale=scale, renormalize=renormalize,
+                          ld=experts + pad, **more)
         assert np.array_equal(o["expert"].read(), want)
         within(o["weight"].read(), w, lim)
         if balance:
@@ -290,7 +291,8 @@ def test_refusals(ctx):
                        (ctx.experts_balance, balance, both),
                        (ctx.experts_route_grad, grad, [
                            (dict(grad_scores=None), "null"), (dict(grad_scores=At(d, 2)), "aligned"),
-                           (dict(grad_loss=None), "null"), (dict(ld_grad=7), "stride"), (dict(scores_type=z.I32), "gradient"),
+                           (dict(grad_loss=None), "null"), (dict(ld_grad=7), "stride"),
+                           (dict(scores_type=z.I32), "gradient"),
                            (dict(grad_weight=None, count=None), "neither")])]:
         f(**a)
         for bad, why in shared + more:
