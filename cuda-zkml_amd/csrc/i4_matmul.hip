@@ -84,6 +84,25 @@ __device__ __forceinline__ float scale_of(const I4Args& a, uint32_t bits) {
   return (float)h;
 }
 
+// A step's products of 16 tokens and 16 channels, a sum for each of its groups, 16 times
+// too large: p a lane's packed weights, x its two fragments.  Groups of 32: an instruction's
+// two are told apart by x, the lanes of the other one hold zeros.
+template <int G, int NS>
+__device__ __forceinline__ void i4_multiply(const v4i (&x)[2], const v4i& p, uint32_t c, v4i (&sums)[NS]) {
+  const v4i high = p & (int)0xf0f0f0f0, low = (p << 4) & (int)0xf0f0f0f0, zero = {0, 0, 0, 0};
+  if constexpr (G >= 128) {
+    sums[0] = __builtin_amdgcn_mfma_i32_16x16x64_i8(x[0], low, zero, 0, 0, 0);
+    sums[0] = __builtin_amdgcn_mfma_i32_16x16x64_i8(x[1], high, sums[0], 0, 0, 0);
+  } else if constexpr (G == 64) {
+    sums[0] = __builtin_amdgcn_mfma_i32_16x16x64_i8(x[0], low, zero, 0, 0, 0);
+    sums[1] = __builtin_amdgcn_mfma_i32_16x16x64_i8(x[1], high, zero, 0, 0, 0);
+  } else {
+#pragma unroll
+    for (int k = 0; k < NS; k++)
+      sums[k] = __builtin_amdgcn_mfma_i32_16x16x64_i8((int)c / 2 == k % 2 ? x[k / 2] : zero, k < 2 ? low : high, zero, 0, 0, 0);
+  }
+}
+
 // Few tokens (decoding), or a small layer: w is read once.  A block has 16 FT tokens x
 // 16 FN channels, its KW waves a part of k each, in steps of 128; their sums meet in LDS.
 // A wave's rows come by lanes that lie side by side in them, straight from memory into
@@ -93,8 +112,7 @@ __device__ __forceinline__ float scale_of(const I4Args& a, uint32_t bits) {
 // The matrix instruction takes 16 tokens (D's rows) and 16 channels (its columns): a lane
 // holds four tokens of one channel, and needs one scale.  16 packed bytes of a lane are its
 // operands of two instructions, 16 times the weights, which the results take back.  G: 128
-// for groups of whole steps, 64, or 32, where an instruction's two groups are told apart by
-// x: the lanes of the other group hold zeros.  D's row 4 c + i is token 4 i + c of the 16, so
+// for groups of whole steps, 64 or 32.  D's row 4 c + i is token 4 i + c of the 16, so
 // that up to four tokens (NI = 1) are one register of each lane.  ODD: x's rows start at
 // any byte or end inside a chunk of 16; they come through registers, masked.
 template <int G, bool GROUPED, bool ODD, int FT, int FN, int NI, int KW, int U>
@@ -211,26 +229,13 @@ __global__ __launch_bounds__(64 * KW) void k_i4_wave(I4Args a, uint32_t tiles_t,
 #pragma unroll
         for (int i = 0; i < FN; i++) {
           const v4i p = *(const v4i*)(sw + u * WB + (i * 16 + fr) * 64 + (c ^ (fr >> 2)) * 16);
-          const v4i high = p & (int)0xf0f0f0f0, low = (p << 4) & (int)0xf0f0f0f0, zero = {0, 0, 0, 0};
           float ws[NS];
 #pragma unroll
           for (int k = 0; k < NS; k++) ws[k] = scales[wave][(s0 - w0 + u) * NS + k][i * 16 + fr];
 #pragma unroll
           for (int j = 0; j < FT; j++) {
             v4i part[NS];
-            if (G >= 128) {
-              part[0] = __builtin_amdgcn_mfma_i32_16x16x64_i8(xf[j][0], low, zero, 0, 0, 0);
-              part[0] = __builtin_amdgcn_mfma_i32_16x16x64_i8(xf[j][1], high, part[0], 0, 0, 0);
-            } else if (G == 64) {
-              part[0] = __builtin_amdgcn_mfma_i32_16x16x64_i8(xf[j][0], low, zero, 0, 0, 0);
-              part[NS - 1] = __builtin_amdgcn_mfma_i32_16x16x64_i8(xf[j][1], high, zero, 0, 0, 0);
-            } else {
-#pragma unroll
-              for (int k = 0; k < NS; k++) {
-                const v4i x = (int)c / 2 == k % 2 ? xf[j][k / 2] : zero;
-                part[k] = __builtin_amdgcn_mfma_i32_16x16x64_i8(x, k < 2 ? low : high, zero, 0, 0, 0);
-              }
-            }
+            i4_multiply<G>(xf[j], p, c, part);
 #pragma unroll
             for (int k = 0; k < NS; k++)
 #pragma unroll
@@ -263,6 +268,125 @@ __global__ __launch_bounds__(64 * KW) void k_i4_wave(I4Args a, uint32_t tiles_t,
     for (int k = 1; k < KW; k++) sum += sums[k][r][lane];
     i4_put(a, t, n, has[d] ? i4_finish(sum * 0.0625f, fx[d], fb[d], a.relu) : 0.0f);
   }
+}
+
+// ------------------------------------------------------------ a few rows, quantized on the way
+// The linear layer of at most 16 rows in one launch: each block asks for its first weights,
+// quantizes all of x's rows into LDS while they come, and goes on as k_i4_wave with its x
+// fragments from there.  Bound by the chain of x's maximum, its bytes and the product.
+// That every block quantizes x again pays as long as all blocks run at once (two a CU) and
+// x is small; in turn, a call this way and in two launches: one row, 8192 to 1024 f16,
+// 8.9 and 12.4 us.
+constexpr uint32_t I4_FEW_OUT = 2 * 256 * 16;
+
+template <class X, int G, int NI>
+__global__ __launch_bounds__(512) void k_i4_few(I4Args a, const X* __restrict__ x, size_t ld_x) {
+  constexpr uint32_t KW = 8, U = 2, BN = 16, WB = BN * 64, OWN = 2 * U * WB;
+  constexpr int NS = G >= 128 ? 1 : 128 / G;
+  constexpr uint32_t ROWS = 16, W = ROWS / NS;
+  extern __shared__ __align__(16) int8_t q[];  // rows x few_ld(n_in)
+  __shared__ __align__(16) int8_t lds[KW * OWN];
+  __shared__ float scales[KW][ROWS][BN];
+  __shared__ uint32_t part[FEW_ROWS][KW];
+  __shared__ float sx[FEW_ROWS];
+  const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t n0 = blockIdx.x * BN, fr = lane & 15, c = lane >> 4, ld = few_ld(a.n_in);
+  const uint32_t steps = (a.n_in + 127) / 128, per = (steps + KW - 1) / KW;
+  const uint32_t first = wave * per, last = first + per < steps ? first + per : steps;
+  const uint32_t wrow = n0 + (lane >> 2) < a.n_out ? n0 + (lane >> 2) : a.n_out - 1;
+  const int8_t* wp = a.w + (size_t)wrow * a.ld_w + ((lane & 3) ^ (lane >> 4)) * 16;
+  const int8_t* own = lds + wave * OWN;
+  const uint32_t base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) int8_t*)lds + wave * OWN;
+  auto fetch = [&](uint32_t s, uint32_t half) {
+#pragma unroll
+    for (uint32_t u = 0; u < U; u++) {
+      const uint32_t step = s + u < last ? s + u : last - 1;  // (again the last one, not used)
+      load_to_lds(wp + (size_t)step * 64, base + (half * U + u) * WB);
+    }
+  };
+  const uint32_t whole = G >= 128 ? a.group / 128 : 1;  // steps of a group
+  uint32_t sc[4], end = 0;
+  auto begin = [&](uint32_t w0) {
+    end = w0 + W < last ? w0 + W : last;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const uint32_t k = lane + i * 64, n = n0 + k % BN < a.n_out ? n0 + k % BN : a.n_out - 1;
+      uint32_t g = w0 * NS + k / BN;
+      if (G >= 128) g /= whole;
+      if (g >= a.groups) g = a.groups - 1;  // (behind the row's end: x is zero)
+      sc[i] = scale_bits(a, (size_t)g * a.n_out + n);
+    }
+    fetch(w0, 0);
+    if (w0 + U < end) fetch(w0 + U, 1);
+  };
+  if (first < last) begin(first);
+  for (uint32_t i = threadIdx.x; i < a.rows * 128; i += 512) {  // behind the rows' ends
+    const uint32_t k = a.n_in / 128 * 128 + i % 128;
+    if (k >= a.n_in) q[i / 128 * ld + k] = 0;
+  }
+  quantize_rows<X, KW>(x, ld_x, a.rows, a.n_in, q, ld, part, sx);
+  // ---- the product
+  const uint32_t token = NI < 4 ? fr >> 2 : (fr & 3) * 4 + (fr >> 2);
+  const int8_t* xq = q + (token < a.rows ? token : a.rows - 1) * ld + 16 * c;
+  float acc[NI] = {};
+  for (uint32_t w0 = first; w0 < last; w0 += W) {
+    if (w0 != first) begin(w0);
+#pragma unroll
+    for (int i = 0; i < 4; i++) scales[wave][(lane + i * 64) / BN][(lane + i * 64) % BN] = scale_of(a, sc[i]);
+    uint32_t half = 0;
+    for (uint32_t s0 = w0; s0 < end; s0 += U) {
+      if (s0 + U < end) wait_loads<U>();
+      else wait_loads<0>();
+      wait_lds();
+#pragma unroll
+      for (uint32_t u = 0; u < U; u++) {
+        if (s0 + u >= end) break;
+        v4i xf[2];
+#pragma unroll
+        for (int h = 0; h < 2; h++) xf[h] = *(const v4i*)(xq + (s0 + u) * 128 + 64 * h);
+        const v4i p = *(const v4i*)(own + (half * U + u) * WB + fr * 64 + (c ^ (fr >> 2)) * 16);
+        v4i sums[NS];
+        i4_multiply<G>(xf, p, c, sums);
+#pragma unroll
+        for (int k = 0; k < NS; k++) {
+          const float w = scales[wave][(s0 - w0 + u) * NS + k][fr];
+#pragma unroll
+          for (int i = 0; i < NI; i++) acc[i] = fmaf((float)sums[k][i], w, acc[i]);
+        }
+      }
+      wait_lds();  // this half is read
+      if (s0 + 2 * U < end) fetch(s0 + 2 * U, half);
+      half ^= 1;
+    }
+  }
+  meet();  // (every wave's loads are done and read)
+  float(*sums)[NI][64] = (float(*)[NI][64])lds;
+#pragma unroll
+  for (int i = 0; i < NI; i++) sums[wave][i][lane] = acc[i];
+  wait_lds();
+  meet();
+  const uint32_t t = 4 * wave + c, n = n0 + fr;
+  if (wave >= NI || t >= a.rows || n >= a.n_out) return;
+  float sum = sums[0][wave][lane];
+#pragma unroll
+  for (uint32_t k = 1; k < KW; k++) sum += sums[k][wave][lane];
+  i4_put(a, t, n, i4_finish(sum * 0.0625f, sx[t], a.bias ? a.bias[n] : 0.0f, a.relu));
+}
+
+static bool i4_few(size_t rows, size_t n_out, size_t n_in) {
+  return rows <= FEW_ROWS && n_in >= 16 && n_out <= I4_FEW_OUT && rows * few_ld((uint32_t)n_in) <= FEW_BYTES;
+}
+
+template <int G>
+static int i4_launch_few(zk_context* ctx, const I4Args& a, const void* x, int x_type, size_t ld_x, hipStream_t st) {
+  return by_type(x_type, [&](auto xz) -> int {
+    typedef decltype(xz) X;
+    const dim3 grid(cdiv(a.n_out, 16));
+    const uint32_t lds = a.rows * few_ld(a.n_in);
+    if (a.rows <= 4) ZK_LAUNCH(ctx, st, "i4_linear", (k_i4_few<X, G, 1>), grid, dim3(512), lds, a, (const X*)x, ld_x);
+    else ZK_LAUNCH(ctx, st, "i4_linear", (k_i4_few<X, G, 4>), grid, dim3(512), lds, a, (const X*)x, ld_x);
+    return ZK_OK;
+  });
 }
 
 // ------------------------------------------------------------ many rows
@@ -851,6 +975,11 @@ int zk_i4_linear(zk_context* ctx, const void* d_x, int x_type, size_t ld_x, cons
     set_sizes(a, rows, n_out, n_in, group, relu, scale_type, y_type);
     OnDevice on(ctx);
     hipStream_t st = ctx->s(stream);
+    if (i4_few(rows, n_out, n_in)) {
+      if (group == 32) return i4_launch_few<32>(ctx, a, d_x, x_type, ld_x, st);
+      if (group == 64) return i4_launch_few<64>(ctx, a, d_x, x_type, ld_x, st);
+      return i4_launch_few<128>(ctx, a, d_x, x_type, ld_x, st);
+    }
     ZK_TRY(i8_quantize(ctx, d_x, x_type, ld_x, rows, n_in, (int8_t*)d_work + lw.q, lw.ld, (float*)d_work, st));
     return i4_matmul(ctx, a, st);
   });

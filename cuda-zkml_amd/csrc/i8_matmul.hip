@@ -826,69 +826,6 @@ static int i8_dispatch(zk_context* ctx, const I8Args& a, int type, hipStream_t s
 }
 
 // ------------------------------------------------------------ rows to 8 bits
-// s = a / 127, q = rint(t / a) with a = max|x| and t = 127 x, rounded to 32 bits
-// (f16 and bf16: exact).  The quotient is the correctly rounded one: t times the
-// rounded reciprocal of a, and one step of Newton's method on the remainder, which
-// two fused operations give exactly (Markstein's division; about 10 operations a
-// value, where the compiler's takes 25: 2048 rows of 4096 7.9 us instead of 10.0 in
-// turn).  So q is what the elementary operations give, and for 16-bit values, whose
-// quotients beside a half are further from it than the rounding, the integer nearest
-// to the exact quotient.  An f32 quotient within 2^-16 of a half may go to either
-// side: an exact decision would need the remainders of both roundings, and would
-// part from the elementary operations.  Rows far from 1 are first multiplied by
-// a power of two, so that nothing leaves the normal numbers.  A row of zeros
-// gives s = 0 and zeros; a row with an infinity or a NaN gives s = NaN and zeros,
-// so that its products show it.
-struct RowScale {
-  float s;      // the row's scale
-  float c, a;   // t = x c, c = 127 times a power of two; a with the same power
-  float inv;    // 1 / a; 0: all zeros
-};
-
-// From the largest magnitude's bits (as integers magnitudes are in the floats'
-// order, NaN above infinity).
-__device__ __forceinline__ RowScale row_scale(uint32_t m) {
-  const float a = __uint_as_float(m);
-  RowScale r = {a / 127.0f, 0.0f, 1.0f, 0.0f};
-  if (m >= 0x7f800000u) {
-    r.s = __uint_as_float(0x7fc00000u);
-  } else if (m) {
-    const float c = a >= 0x1p64f ? 0x1p-32f : a < 0x1p-64f ? 0x1p64f : 1.0f;
-    r.c = 127.0f * c;
-    r.a = a * c;
-    r.inv = 1.0f / r.a;
-  }
-  return r;
-}
-
-template <class T>
-__device__ __forceinline__ uint32_t magnitude(T x) {
-  return __float_as_uint((float)x) & 0x7fffffffu;
-}
-
-template <class T>
-__device__ __forceinline__ void quantize_piece(const Vec<T>& x, const RowScale& r, int8_t* q) {
-  if (r.inv == 0.0f) {  // where x itself may be an infinity or a NaN
-#pragma unroll
-    for (uint32_t i = 0; i < Vec<T>::N; i++) q[i] = 0;
-    return;
-  }
-#pragma unroll
-  for (uint32_t i = 0; i < Vec<T>::N; i++) {
-    const float t = (float)x.v[i] * r.c, y = t * r.inv;
-    q[i] = (int8_t)rintf(fmaf(fmaf(-y, r.a, t), r.inv, y));
-  }
-}
-
-template <class T>
-__device__ __forceinline__ void look_piece(const Vec<T>& v, uint32_t& m) {
-#pragma unroll
-  for (uint32_t i = 0; i < Vec<T>::N; i++) {
-    const uint32_t u = magnitude(v.v[i]);
-    m = u > m ? u : m;
-  }
-}
-
 // THREADS threads a row, ROWS rows a block.  A thread keeps its first HELD
 // pieces of 16 bytes from the pass for the maximum to the pass that divides, so
 // that rows of up to 64 KB are read once.  Bound by its own chain (load, maximum
@@ -997,15 +934,10 @@ int i8_quantize(zk_context* ctx, const void* x, int type, size_t ld_x, size_t ro
 // 8195 (46 KB), 19.5 and 15.4.  On the GPU alone, where nothing waits for the host,
 // two launches are level from about 16 KB on (4096 to 4096: 4 rows 9.3 and 3.4 + 5.8,
 // 8 rows 12.5 and 3.6 + 6.2).
-constexpr uint32_t FEW_ROWS = 16, FEW_BYTES = 36 * 1024;
-// A quantized row's stride in LDS: whole steps, and 16 bytes so that the rows of
-// a fragment lie in different banks.
-static __host__ __device__ inline uint32_t few_ld(uint32_t n_in) { return (n_in + 127) / 128 * 128 + 16; }
-
 template <class T, class X, int FN>
 __global__ __launch_bounds__(512) void k_i8_few(I8Args a, const X* __restrict__ x, size_t ld_x) {
   constexpr uint32_t BN = 16 * FN, BK = 128, KW = 8;
-  constexpr int U = FN == 1 ? 4 : 2, HELD = 4;
+  constexpr int U = FN == 1 ? 4 : 2;
   extern __shared__ __align__(16) int8_t q[];  // rows x few_ld(n_in)
   __shared__ __align__(16) v4i sums[KW][FN][64];
   __shared__ uint32_t part[FEW_ROWS][KW];
@@ -1041,64 +973,7 @@ __global__ __launch_bounds__(512) void k_i8_few(I8Args a, const X* __restrict__ 
     else load_as(std::true_type(), step);
   };
   load(wave);
-  // ---- x to 8 bits: KW / g rows at a time, g waves a row
-  uint32_t g = KW;
-  while (g > 1 && KW / g < a.rows) g /= 2;
-  const uint32_t at_once = KW / g, first = wave / g, sub = (wave % g) * 64 + lane;
-  const uint32_t pieces = pieces_of<X>(a.n_in);
-  Vec<X> held[HELD];
-  for (uint32_t r = first; r < a.rows; r += at_once) {
-    const X* row = x + (size_t)r * ld_x;
-    uint32_t m = 0;
-#pragma unroll
-    for (int h = 0; h < HELD; h++) {
-      const uint32_t p = sub + h * g * 64;
-      held[h] = Vec<X>{};
-      if (p < pieces) held[h] = row_load(row + piece<X>(p, a.n_in), a.n_in - piece<X>(p, a.n_in));
-    }
-#pragma unroll
-    for (int h = 0; h < HELD; h++) look_piece(held[h], m);
-    for (uint32_t p = sub + HELD * g * 64; p < pieces; p += g * 64)
-      look_piece(row_load(row + piece<X>(p, a.n_in), a.n_in - piece<X>(p, a.n_in)), m);
-#pragma unroll
-    for (int d = 32; d; d >>= 1) {
-      const uint32_t o = (uint32_t)__shfl_xor((int)m, d);
-      m = o > m ? o : m;
-    }
-    if (lane == 0) part[r][wave % g] = m;
-  }
-  wait_lds();
-  meet();
-  for (uint32_t r = first; r < a.rows; r += at_once) {
-    const X* row = x + (size_t)r * ld_x;
-    int8_t* out = q + r * ld;
-    uint32_t m = 0;
-    for (uint32_t i = 0; i < g; i++) m = part[r][i] > m ? part[r][i] : m;
-    const RowScale rs = row_scale(m);
-    if (sub == 0) scale[r] = rs.s;
-    auto put = [&](uint32_t p, const Vec<X>& v) {
-      const uint32_t at = piece<X>(p, a.n_in);
-      int8_t b[Vec<X>::N];
-      quantize_piece(v, rs, b);
-      if (a.n_in - at >= Vec<X>::N) {
-        __builtin_memcpy(out + at, b, sizeof(b));
-      } else {
-#pragma unroll
-        for (uint32_t i = 0; i < Vec<X>::N; i++)
-          if (i < a.n_in - at) out[at + i] = b[i];
-      }
-    };
-    const bool again = at_once < a.rows;  // held is the last of several rows
-    if (!again) {
-#pragma unroll
-      for (int h = 0; h < HELD; h++)
-        if (sub + h * g * 64 < pieces) put(sub + h * g * 64, held[h]);
-    }
-    for (uint32_t p = sub + (again ? 0 : HELD * g * 64); p < pieces; p += g * 64)
-      put(p, row_load(row + piece<X>(p, a.n_in), a.n_in - piece<X>(p, a.n_in)));
-  }
-  wait_lds();
-  meet();
+  quantize_rows<X, KW>(x, ld_x, a.rows, a.n_in, q, ld, part, scale);
   // ---- the product
   const uint32_t row = fr < a.rows ? fr : a.rows - 1;
   const int8_t* xq = q + row * ld;

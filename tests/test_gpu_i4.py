@@ -206,7 +206,8 @@ def test_quantize_of_what_has_no_scale(ctx):
 
 
 LINEAR = [(1, 100, 64, 32), (1, 1024, 8192, 128), (3, 70, 1001, 64), (16, 33, 500, 128), (17, 200, 1024, 128),
-          (40, 129, 2100, 64), (300, 257, 640, 128), (8, 100, 20000, 128)]
+          (40, 129, 2100, 64), (300, 257, 640, 128), (8, 100, 20000, 128), (2, 20, 7, 32), (5, 40, 16, 64), (4, 50, 33, 128),
+          (16, 300, 2200, 256), (1, 8200, 256, 128), (2, 8192, 130, 32), (13, 31, 1500, 64), (1, 70, 36000, 128)]
 
 
 @pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
