@@ -33,7 +33,11 @@ constexpr int balance_threads(int lanes) { return lanes == 16 ? 1024 : 512; }
 
 constexpr uint32_t ROUTE_BLOCKS = 2048;   // of a launch at the most (then a block has several tokens a group)
 constexpr uint32_t BALANCE_BLOCKS = 256;  // one a CU
-constexpr size_t BALANCE_ONE = 256;       // tokens that one block takes alone, in one launch
+// Tokens times (experts + 64) that one block takes alone: a second launch costs the host
+// 3.7 us and the GPU 2.5 to 4, by which time it has done 256 tokens' choice of 60 experts
+// (14.3 us with the gradient on the GPU, 12.0 in two launches; a call 14.2 and 17.9), or
+// counted 500 tokens' (12.6 and 10.2; 13.8 and 17.8).
+constexpr size_t BALANCE_ONE_CHOICE = (size_t)1 << 15, BALANCE_ONE = (size_t)1 << 16;
 
 struct RouteArgs {
   const void* scores;
@@ -559,15 +563,15 @@ static uint32_t route_blocks(size_t tokens, uint32_t a_block, uint32_t most) {
   const uint32_t b = cdiv(tokens, a_block);
   return b < most ? b : most;
 }
-static uint32_t balance_blocks(size_t tokens, int experts) {
-  if (tokens <= BALANCE_ONE) return 1;
+static uint32_t balance_blocks(size_t tokens, int experts, bool choose) {
+  if (tokens * (experts + 64) <= (choose ? BALANCE_ONE_CHOICE : BALANCE_ONE)) return 1;
   const int lanes = lanes_of(experts);
   return route_blocks(tokens, balance_threads(lanes) / lanes, BALANCE_BLOCKS);
 }
 // A workspace: the last step's parts of the loss and ticket, then the blocks' sums and
 // counts; none for one block.
-static size_t balance_work(size_t tokens, int experts) {
-  const uint32_t blocks = balance_blocks(tokens, experts);
+static size_t balance_work(size_t tokens, int experts, bool choose) {
+  const uint32_t blocks = balance_blocks(tokens, experts, choose);
   return blocks > 1 ? 8 * (ZK_MAX_EXPERTS / FINISH_EXPERTS + 1) + (size_t)blocks * (2 * experts + 1) * 4 : 0;
 }
 
@@ -607,9 +611,9 @@ template <bool CHOOSE>
 static int route(zk_context* ctx, const RouteArgs& a, int type, BalanceOut out, void* work, size_t work_bytes,
                  hipStream_t st) {
   const bool balance = out.count != nullptr;
-  const uint32_t blocks = balance_blocks(a.tokens, (int)a.experts);
+  const uint32_t blocks = balance_blocks(a.tokens, (int)a.experts, CHOOSE);
   if (balance) {
-    const size_t need = balance_work(a.tokens, (int)a.experts);
+    const size_t need = balance_work(a.tokens, (int)a.experts, CHOOSE);
     if (need && (!work || !aligned(work, 8) || work_bytes < need))
       return ctx->fail(ZK_ERR_INVALID, "experts' route: workspace missing, too small or not aligned to 8 bytes");
     constexpr size_t PARTS = ZK_MAX_EXPERTS / FINISH_EXPERTS;
@@ -647,7 +651,7 @@ extern "C" {
 size_t zk_experts_route_work(size_t tokens, int experts) {
   using namespace zk;
   if (experts < 1 || experts > ZK_MAX_EXPERTS || tokens > ZK_MAX_EXPERT_ROWS) return 0;
-  return balance_work(tokens, experts);
+  return balance_work(tokens, experts, true);  // (the more of the two)
 }
 
 int zk_experts_route(zk_context* ctx, const void* d_scores, int type, size_t ld, size_t tokens, int experts, int slots,

@@ -271,12 +271,12 @@ def test_no_tokens(ctx):
 
 def test_refusals(ctx):
     d = ctx.upload(np.zeros(1 << 14, dtype=np.int32))
-    work = ctx.alloc(ctx.experts_route_work(400, 8))
-    short = ctx.alloc(ctx.experts_route_work(400, 8) - 4)
-    route = dict(scores=d, scores_type=z.F32, tokens=400, experts=8, slots=2, expert=ctx.alloc(3200),
-                 weight=ctx.alloc(3200), count=ctx.alloc(64), prob=ctx.alloc(64), loss=ctx.alloc(64), work=work)
+    work = ctx.alloc(ctx.experts_route_work(1200, 8))
+    short = ctx.alloc(ctx.experts_route_work(1200, 8) - 4)
+    route = dict(scores=d, scores_type=z.F32, tokens=1200, experts=8, slots=2, expert=ctx.alloc(9600),
+                 weight=ctx.alloc(9600), count=ctx.alloc(64), prob=ctx.alloc(64), loss=ctx.alloc(64), work=work)
     balance = {k: x for k, x in route.items() if k != "weight"}
-    grad = dict(scores=d, scores_type=z.F32, tokens=400, experts=8, slots=2, expert=d, grad_scores=ctx.alloc(12800),
+    grad = dict(scores=d, scores_type=z.F32, tokens=1200, experts=8, slots=2, expert=d, grad_scores=ctx.alloc(38400),
                 grad_weight=d, count=d, grad_loss=d)
     shared = [(dict(experts=0), "1024"), (dict(experts=1025), "1024"), (dict(slots=0), "32 slots"),
               (dict(slots=33), "32 slots"), (dict(tokens=1 << 22), "2\\^22"), (dict(tokens=(1 << 22) + 1), "2\\^22"),
