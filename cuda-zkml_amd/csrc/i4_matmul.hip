@@ -27,6 +27,25 @@ struct I4Args : I8Args {
 
 static __host__ __device__ inline size_t i4_row_bytes(size_t n_in) { return (n_in + 127) / 128 * 64; }
 
+// Rows of x behind N positions, -1 for those that hold none, their loads under way
+// together (a chain of branches had them wait for one another).
+template <bool GROUPED, int N>
+__device__ __forceinline__ void source_rows(const I4Args& a, const uint32_t (&p)[N], int (&s)[N]) {
+  if (!GROUPED || !a.order) {
+#pragma unroll
+    for (int i = 0; i < N; i++) s[i] = !GROUPED || p[i] < a.tokens ? (int)p[i] : -1;
+    return;
+  }
+  int o[N];
+#pragma unroll
+  for (int i = 0; i < N; i++) o[i] = a.order[p[i]];
+#pragma unroll
+  for (int i = 0; i < N; i++) {
+    const uint32_t t = (uint32_t)o[i] / a.slots;
+    s[i] = o[i] >= 0 && t < a.tokens ? (int)t : -1;
+  }
+}
+
 // sx sum + b in one rounding; what is below zero becomes zero, a NaN stays.
 __device__ __forceinline__ float i4_finish(float sum, float sx, float b, int relu) {
   const float f = fmaf(sum, sx, b);
@@ -146,25 +165,33 @@ __global__ __launch_bounds__(64 * KW) void k_i4_wave(I4Args a, uint32_t tiles_t,
     const uint32_t row = i * 16 + (lane >> 2), n = n0 + row < a.n_out ? n0 + row : a.n_out - 1;
     wp[i] = a.w + (ch + n) * a.ld_w + ((lane & 3) ^ (row >> 2 & 3)) * 16;
   }
+  // rows of x that the lane fetches, and of the results that it will finish
+  constexpr int DONE = (FN * FT * NI + KW - 1) / KW;
+  uint32_t place[XP + DONE];
+  int from[XP + DONE];
 #pragma unroll
   for (int p = 0; p < XP; p++) {
     const uint32_t row = (p * 8 + (lane >> 3)) % XROWS;
-    const uint32_t t = r0 + (NI < 4 ? row : row / 16 * 16 + (row & 3) * 4 + (row % 16 >> 2)), r = t < r1 ? t : r1 - 1;
-    const int64_t s = GROUPED ? source_row(a, r) : (int64_t)r;
-    xp[p] = a.x + (size_t)(s < 0 ? 0 : s) * a.ld_x;
+    const uint32_t t = r0 + (NI < 4 ? row : row / 16 * 16 + (row & 3) * 4 + (row % 16 >> 2));
+    place[p] = t < r1 ? t : r1 - 1;
   }
-  // the results that the thread will finish: their factors
-  constexpr int DONE = (FN * FT * NI + KW - 1) / KW;
-  float fx[DONE], fb[DONE];
   bool has[DONE];
 #pragma unroll
   for (int d = 0; d < DONE; d++) {
     const uint32_t r = wave + d * KW, sq = r / NI, t = r0 + sq % FT * 16 + 4 * (r % NI) + c, n = n0 + sq / FT * 16 + fr;
-    const bool in = r < FN * FT * NI && t < r1 && t < r0 + BT && n < a.n_out;
-    int64_t s = -1;
-    if (in && !none) s = GROUPED ? source_row(a, t) : (int64_t)t;
-    has[d] = s >= 0;
-    fx[d] = has[d] && a.sx ? a.sx[s] : 1.0f;
+    has[d] = r < FN * FT * NI && t < r1 && t < r0 + BT && n < a.n_out && !none;
+    place[XP + d] = has[d] ? t : r1 - 1;
+  }
+  source_rows<GROUPED>(a, place, from);
+#pragma unroll
+  for (int p = 0; p < XP; p++) xp[p] = a.x + (size_t)(from[p] < 0 ? 0 : from[p]) * a.ld_x;
+  // the results' factors
+  float fx[DONE], fb[DONE];
+#pragma unroll
+  for (int d = 0; d < DONE; d++) {
+    const uint32_t n = n0 + (wave + d * KW) / NI / FT * 16 + fr;
+    has[d] = has[d] && from[XP + d] >= 0;
+    fx[d] = has[d] && a.sx ? a.sx[from[XP + d]] : 1.0f;
     fb[d] = has[d] && a.bias ? a.bias[ch + n] : 0.0f;
   }
   int8_t* own = lds + wave * OWN;
@@ -453,12 +480,24 @@ __global__ __launch_bounds__(64 * WT * WN, 2) void k_i4_ring(I4Args a, uint32_t 
     if constexpr (ODD) wp[i] = wbase + off;
     else wp[i] = (uint32_t)off;
   }
+  // rows of x: those that the lane fetches, and of the tokens whose scale it loads
+  constexpr int TOKENS = (2 * BT + THREADS - 1) / THREADS;
+  uint32_t place[XR + TOKENS];
+  int from[XR + TOKENS];
 #pragma unroll
   for (uint32_t i = 0; i < XR; i++) {
-    const uint32_t row = (wave * XR + i) * 8 + (lane >> 3), r = r0 + row < r1 ? r0 + row : r1 - 1;
-    int64_t s = GROUPED ? source_row(a, r) : (int64_t)(r - r0);
-    if (s < 0) s = 0;
-    const size_t off = (size_t)s * a.ld_x;
+    const uint32_t r = r0 + (wave * XR + i) * 8 + (lane >> 3);
+    place[i] = r < r1 ? r : r1 - 1;
+  }
+#pragma unroll
+  for (uint32_t i = 0; i < TOKENS; i++) {
+    const uint32_t r = r0 + (tid + i * THREADS) % BT;
+    place[XR + i] = r < r1 ? r : r1 - 1;
+  }
+  source_rows<GROUPED>(a, place, from);
+#pragma unroll
+  for (uint32_t i = 0; i < XR; i++) {
+    const size_t off = (size_t)(from[i] < 0 ? 0 : GROUPED ? (uint32_t)from[i] : from[i] - r0) * a.ld_x;
     if constexpr (ODD) xp[i] = xbase + off;
     else xp[i] = (uint32_t)off + x_chunk(i);
   }
@@ -533,10 +572,9 @@ __global__ __launch_bounds__(64 * WT * WN, 2) void k_i4_ring(I4Args a, uint32_t 
     const uint32_t k = tid + i * THREADS;
     factor[i] = 0.0f;
     if (k < 2 * BT) {  // tokens' scales, and whether they are there
-      const uint32_t t = r0 + k % BT;
-      int64_t s = -1;
-      if (t < r1 && !none) s = GROUPED ? source_row(a, t) : (int64_t)t;
-      factor[i] = s < 0 ? 0.0f : k < BT && a.sx ? a.sx[s] : 1.0f;
+      const int from_k = from[XR + (i < TOKENS ? i : 0)];
+      const bool in = r0 + k % BT < r1 && !none && from_k >= 0;
+      factor[i] = !in ? 0.0f : k < BT && a.sx ? a.sx[from_k] : 1.0f;
     } else if (k < 2 * BT + BN) {
       const uint32_t n = n0 + k - 2 * BT;
       factor[i] = a.bias && n < a.n_out ? a.bias[ch + n] : 0.0f;
