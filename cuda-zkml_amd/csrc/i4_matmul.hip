@@ -754,6 +754,12 @@ static bool near_rows(const I4Args& a, bool grouped) {
   return !(a.ld_w >> 23) && !(a.ld_x >> 23) && (!grouped || !((uint64_t)a.tokens * a.ld_x >> 32));
 }
 
+// Row tiles.  Of the grouped form: whole ones, and a part of one for each expert and for
+// the rows without an expert.
+static uint32_t row_tiles(const I4Args& a, uint32_t bt, bool grouped) {
+  return grouped ? a.rows / bt + (a.experts + 1 < a.rows ? a.experts + 1 : a.rows) : cdiv(a.rows, bt);
+}
+
 static I4Kernel choose_i4(const I4Args& a, bool grouped) {
   const bool whole = whole_rows(a), near = near_rows(a, grouped);
   const uint64_t steps = (a.n_in + 127) / 128, groups = grouped ? (a.experts < a.rows ? a.experts : a.rows) : 0;
@@ -762,7 +768,7 @@ static I4Kernel choose_i4(const I4Args& a, bool grouped) {
   for (int i = 0; i < I4_COUNT; i++) {
     const I4Tile& t = I4_TILES[i];
     const I4Cost& c = grouped ? t.grouped : whole && (near || i < I4_32x128) ? t.whole : t.odd;
-    if (!c.first) continue;
+    if (!c.first || (uint64_t)row_tiles(a, t.bt, grouped) * cdiv(a.n_out, t.bn) > I8_MAX_TILES) continue;
     // an expert's last row tile is half full, or it has only one
     uint64_t tt = cdiv(a.rows, t.bt);
     if (grouped && (tt += groups / 2) < groups) tt = groups;
@@ -777,10 +783,7 @@ static I4Kernel choose_i4(const I4Args& a, bool grouped) {
 template <int G, bool GROUPED, bool ODD>
 static int launch_i4_as(zk_context* ctx, const I4Args& a, I4Kernel k, hipStream_t st) {
   auto go = [&](auto kernel, uint32_t threads) -> int {
-    // row tiles of the grouped form: whole ones, and a part of one for each expert and
-    // for the rows without an expert
-    const uint32_t bt = I4_TILES[k].bt, groups = a.experts + 1 < a.rows ? a.experts + 1 : a.rows;
-    const uint32_t tiles_t = GROUPED ? a.rows / bt + groups : cdiv(a.rows, bt);
+    const uint32_t tiles_t = row_tiles(a, I4_TILES[k].bt, GROUPED);
     const uint32_t tiles_n = cdiv(a.n_out, I4_TILES[k].bn);
     const size_t tiles = (size_t)tiles_t * tiles_n;
     if (tiles > I8_MAX_TILES) return ctx->fail(ZK_ERR_SIZE, "i4 product: rows and n_out make too many tiles");

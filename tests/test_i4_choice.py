@@ -42,6 +42,18 @@ def test_odd_rows_leave_the_largest_tiles():
     assert kernel(2049, 7535, 673) != "stages 256x256"
 
 
+def test_a_launch_holds_the_tiles():
+    """At most 2^22 blocks a launch: the widest layers leave the smallest tiles."""
+    for n_in in (64, 4096):
+        for rows in (1, 4, 5, 16):
+            sizes = [int(s) for s in kernel(rows, 1 << 26, n_in).split()[-1].split("x")]
+            assert -(-rows // sizes[0]) * (2**26 // sizes[1]) <= 1 << 22
+    # grouped: one tile for each expert beside the whole ones
+    for experts, rows, n_out in ((2, 14, 53232046), (1000, 1000, 1 << 16), (60000, 60000, 2048), (8, 64, 1 << 24)):
+        sizes = [int(s) for s in kernel(rows, n_out, 11296, experts, 64).split()[-1].split("x")]
+        assert (rows // sizes[0] + min(experts + 1, rows)) * -(-n_out // sizes[1]) <= 1 << 22
+
+
 def test_sizes_out_of_range():
     assert kernel(1 << 31, 4, 4) is None and kernel(4, (1 << 26) + 1, 4) is None and kernel(4, 4, (1 << 24) + 1) is None
     assert kernel(4, 4, 4, experts=-1) is None and kernel(0, 4, 4) is None
