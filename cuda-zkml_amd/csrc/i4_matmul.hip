@@ -350,7 +350,7 @@ __global__ __launch_bounds__(512) void k_i4_few(I4Args a, const X* __restrict__ 
   };
   if (first < last) begin(first);
   for (uint32_t i = threadIdx.x; i < a.rows * 128; i += 512) {  // behind the rows' ends
-    const uint32_t k = a.n_in / 128 * 128 + i % 128;
+    const uint32_t k = (a.n_in - 1) / 128 * 128 + i % 128;
     if (k >= a.n_in) q[i / 128 * ld + k] = 0;
   }
   quantize_rows<X, KW>(x, ld_x, a.rows, a.n_in, q, ld, part, sx);
