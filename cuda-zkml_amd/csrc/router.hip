@@ -277,7 +277,7 @@ __global__ __launch_bounds__(BALANCE ? balance_threads(L) : ROUTE_THREADS) void 
     if (!CHOOSE) {
 #pragma unroll
       for (int k = 0; k < KEPT; k++)
-        if ((uint32_t)given[k] < a.experts) atomicAdd(&count[given[k]], 1u);
+        if (!empty && (uint32_t)given[k] < a.experts) atomicAdd(&count[given[k]], 1u);
       continue;
     }
     int kept_e[KEPT];

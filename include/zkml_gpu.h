@@ -433,7 +433,7 @@ int zk_experts_combine_grad(zk_context* ctx, const void* d_grad, size_t ld_grad,
  * d_work: zk_experts_route_work(tokens, experts) bytes (0: none needed, may be
  * NULL), 8-byte aligned, used only with these outputs.
  * zk_experts_balance: the same three for given routes (tokens x slots); a route
- * outside [0, experts) names none.
+ * outside [0, experts) names none, nor does one of a masked row, whatever it holds.
  * zk_experts_route_grad: the gradient with regard to the scores of what depends
  * on the weights by grad_weight (tokens x slots; NULL: nothing does) and on the
  * loss by grad_loss[0] (d_count NULL: nothing does; else the counts of

@@ -1,0 +1,62 @@
+"""GPU tests of the experts' router (cuda-zkml_amd/csrc/router.hip) where its inputs end:
+padding that carries routes."""
+import numpy as np
+import pytest
+
+import router_forms as forms
+import zkml_amd as z
+from i8_helpers import TYPES, words
+from test_gpu_router import outputs, say, scores, within, work_of
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def ctx():
+    return z.Context(0)
+
+
+def balance(s, scale, expert):
+    """forms.balance over the tokens that have a score, within the sums as they are made:
+    a lane adds its tokens one after the other, 16 or those of one group of lanes in 256
+    blocks (of 64, 16 or 8 groups); then at most 2 sums over lanes, 15 over waves, and a
+    product and two roundings on the way; the blocks' are added in 64 bits."""
+    on = (s > -np.inf).any(axis=1)
+    tokens, experts, n = len(s), s.shape[1], int(on.sum())
+    groups = 64 if experts <= 256 else 16 if experts <= 512 else 8
+    depth = max(16, -(-tokens // (256 * groups))) + 20
+    p, R = forms.softmax(s, scale)
+    count = np.array([(expert[on] == e).sum() for e in range(experts)] + [n])
+    prob = p.sum(axis=0) / max(n, 1)
+    lim = (p * R).sum(axis=0) / max(n, 1) + depth * 2.0**-24 * prob + 2.0**-126
+    f = count[:-1] / max(1, n * expert.shape[1])
+    loss = experts * (f * prob).sum()
+    return count, prob, loss, lim, experts * (f * lim).sum() + 2.0**-23 * loss
+
+
+def check_balance(o, want):
+    count, prob, loss, prob_lim, loss_lim = want
+    assert np.array_equal(o["count"].read()[0], count)
+    within(o["prob"].read()[0], prob, prob_lim)
+    within(o["loss"].read(), np.array([[loss]]), loss_lim)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16", "i32"])
+@pytest.mark.parametrize("tokens,experts,slots", [(1, 4, 1), (50, 20, 2), (300, 1024, 3), (3000, 24, 20), (700, 400, 2)])
+def test_padding_that_names_experts(ctx, kind, tokens, experts, slots):
+    """Tokens without a score count for nothing, whatever their routes hold; one block's
+    batches and larger ones."""
+    rng = np.random.default_rng([tokens, experts])
+    s, v = scores(rng, tokens, experts, kind)
+    none = rng.random(tokens) < 0.4
+    none[-1] = True
+    s[none] = -2**31 if kind == "i32" else words(np.array([-np.inf]), kind)[0]
+    v[none] = -np.inf
+    expert = rng.integers(0, experts, (tokens, slots)).astype(np.int32)
+    expert[none, 0] = 0
+    scale = 2.0**-12 if kind == "i32" else 1.25
+    say("[balance with padding]", kind, tokens, experts, slots)
+    o = outputs(ctx, tokens, experts, slots, True)
+    ctx.experts_balance(ctx.upload(s), TYPES[kind], tokens, experts, slots, ctx.upload(expert), o["count"].at,
+                        o["prob"].at, o["loss"].at, work_of(ctx, tokens, experts), scale=scale)
+    check_balance(o, balance(v, scale, expert))
