@@ -506,9 +506,8 @@ __global__ __launch_bounds__(ROUTE_THREADS) void k_route_grad(RouteGradArgs a) {
     }
     const float inv = 1.0f / sum_over<L>(z);
     dot = sum_over<L>(dot) * inv;
-    const float by = inv * a.scale;
 #pragma unroll
-    for (int i = 0; i < V; i++) d[i] = ez[i] * by * ((NORMAL ? f[i] : f[i] + g[i]) - dot);
+    for (int i = 0; i < V; i++) d[i] = ez[i] * inv * ((NORMAL ? f[i] : f[i] + g[i]) - dot);
     if constexpr (NORMAL) {
       // softmax over the chosen alone: their own maximum, sum and mean
       float mc = S::none(), zc = 0.0f, gc = 0.0f;
@@ -522,15 +521,16 @@ __global__ __launch_bounds__(ROUTE_THREADS) void k_route_grad(RouteGradArgs a) {
         gc = fmaf(g[i], ez[i], gc);
       }
       zc = sum_over<L>(zc), gc = sum_over<L>(gc);
-      const float ic = zc > 0.0f ? 1.0f / zc : 0.0f, byc = ic * a.scale;
+      const float ic = zc > 0.0f ? 1.0f / zc : 0.0f;
       gc *= ic;
 #pragma unroll
-      for (int i = 0; i < V; i++) d[i] = fmaf(ez[i] * byc, fmaf(-times[i], gc, g[i]), d[i]);
+      for (int i = 0; i < V; i++) d[i] = fmaf(ez[i] * ic, fmaf(-times[i], gc, g[i]), d[i]);
     }
     T out[V];
-    // a masked row's sums are of nothing, an impossible one's are NaN
+    // a masked row's sums are of nothing, an impossible one's are NaN; the scale comes last
+    // (a small one and a probability may have no product in 32 bits)
 #pragma unroll
-    for (int i = 0; i < V; i++) out[i] = (T)(empty ? 0.0f : bad ? NAN : d[i]);
+    for (int i = 0; i < V; i++) out[i] = (T)(empty ? 0.0f : bad ? NAN : d[i] * a.scale);
     T* row = (T*)a.grad + (size_t)t * a.ld_grad;
 #pragma unroll
     for (int k = 0; k < V; k += P::C) {

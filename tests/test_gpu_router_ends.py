@@ -1,11 +1,11 @@
 """GPU tests of the experts' router (cuda-zkml_amd/csrc/router.hip) where its inputs end:
-padding that carries routes."""
+padding that carries routes, scores and scales at the ends of the range."""
 import numpy as np
 import pytest
 
 import router_forms as forms
 import zkml_amd as z
-from i8_helpers import TYPES, words
+from i8_helpers import TYPES, Result, words
 from test_gpu_router import outputs, say, scores, within, work_of
 
 pytestmark = pytest.mark.gpu
@@ -60,3 +60,33 @@ def test_padding_that_names_experts(ctx, kind, tokens, experts, slots):
     ctx.experts_balance(ctx.upload(s), TYPES[kind], tokens, experts, slots, ctx.upload(expert), o["count"].at,
                         o["prob"].at, o["loss"].at, work_of(ctx, tokens, experts), scale=scale)
     check_balance(o, balance(v, scale, expert))
+
+
+def pass_through(ctx, s, v, kind, scale, slots, renormalize, gw, gl):
+    """Routes with balance and the gradient of these scores, against the 64-bit forms."""
+    tokens, experts = v.shape
+    want = forms.chosen(v, slots)
+    d, o = ctx.upload(s), outputs(ctx, tokens, experts, slots, True)
+    ctx.experts_route(d, TYPES[kind], tokens, experts, slots, scale=scale, renormalize=renormalize,
+                      work=work_of(ctx, tokens, experts), **{k: r.at for k, r in o.items()})
+    assert np.array_equal(o["expert"].read(), want)
+    within(o["weight"].read(), *forms.weights(v, scale, want, renormalize))
+    check_balance(o, balance(v, scale, want))
+    if kind == "i32":
+        return
+    out = Result(ctx, tokens, experts, kind)
+    ctx.experts_route_grad(d, TYPES[kind], tokens, experts, slots, o["expert"].at, out.at, scale=scale,
+                           renormalize=renormalize, grad_weight=ctx.upload(gw), count=o["count"].at,
+                           grad_loss=ctx.upload(np.array([gl], np.float32)))
+    count = o["count"].read()[0]
+    within(out.read(), *forms.gradient(v, scale, want, renormalize, gw, count, np.float32(gl)), kind)
+
+
+@pytest.mark.parametrize("renormalize", [True, False])
+def test_the_smallest_scales(ctx, renormalize):
+    """A scale below the normal numbers costs the gradient nothing of its precision."""
+    rng = np.random.default_rng(12)
+    v = words(rng.uniform(-1, 1, (100, 6)) * 2.0**127, "f32")
+    say("[small scale]", renormalize)
+    pass_through(ctx, v, v.astype(np.float64), "f32", 2.0**-140, 3, renormalize,
+                 (rng.normal(0, 1, (100, 3)) * 2.0**110).astype(np.float32), 2.0**110)
