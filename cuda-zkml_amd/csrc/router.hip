@@ -49,16 +49,18 @@ struct RouteArgs {
   float* weight;     // tokens x slots
 };
 
-// exp(scale x) for x <= 0: the hardware's 2^y of y = x scale log2(e).  EXACT: y's own
-// rounding is made good, so that what is left of an error is that of the hardware
-// (1 ulp), of the factor (2^-26 |y|) and of x scale; else y is off by two roundings,
-// which 16-bit results do not show.  Below 2^-126 it gives zero.
+// exp(2 scale x) for x <= 0, half of a difference of scores, so that none is out of range:
+// the hardware's 2^y of y = 2 x scale log2(e), the scale first, since its product with a
+// constant may be out of range.  EXACT: y's own rounding is made good, so that what is left
+// of an error is that of the hardware (1 ulp), of the factor (2^-26 |y|) and of x scale;
+// else y is off by two roundings and the factor, which 16-bit results do not show.  Below
+// 2^-126 it gives zero.
 template <bool EXACT>
 __device__ __forceinline__ float exp_down(float x, float scale) {
-  constexpr float LOG2E = 1.44269504f, LN2 = 0.693147181f;
-  if constexpr (!EXACT) return __builtin_amdgcn_exp2f(x * (scale * LOG2E));
-  const float a = fmaxf(x * scale, -200.0f);
-  const float y = a * LOG2E, lost = fmaf(a, LOG2E, -y), p = __builtin_amdgcn_exp2f(y);
+  constexpr float TWO_LOG2E = 2.88539008f, LN2 = 0.693147181f;
+  if constexpr (!EXACT) return __builtin_amdgcn_exp2f(x * scale * TWO_LOG2E);
+  const float a = fmaxf(x * scale, -100.0f);
+  const float y = a * TWO_LOG2E, lost = fmaf(a, TWO_LOG2E, -y), p = __builtin_amdgcn_exp2f(y);
   return fmaf(p, lost * LN2, p);
 }
 
@@ -76,7 +78,9 @@ struct Score {
   static __device__ __forceinline__ bool bad(float m) { return !(m < INFINITY); }
   // exp(scale (v - m)); v <= m, m a score
   template <bool EXACT>
-  static __device__ __forceinline__ float ex(float v, float m, float scale) { return exp_down<EXACT>(v - m, scale); }
+  static __device__ __forceinline__ float ex(float v, float m, float scale) {
+    return exp_down<EXACT>(fmaf(v, 0.5f, -0.5f * m), scale);
+  }
   // 0: masked, else the score's rank among all of the type above, the expert below
   static __device__ __forceinline__ uint32_t key(float v, uint32_t e) {
     uint16_t b;
@@ -103,7 +107,7 @@ struct Score<int> {
   static __device__ __forceinline__ bool bad(int) { return false; }
   template <bool EXACT>
   static __device__ __forceinline__ float ex(int v, int m, float scale) {
-    return v == none() ? 0.0f : exp_down<EXACT>(-(float)((uint32_t)m - (uint32_t)v), scale);
+    return v == none() ? 0.0f : exp_down<EXACT>(-0.5f * (float)((uint32_t)m - (uint32_t)v), scale);
   }
 };
 

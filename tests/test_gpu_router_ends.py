@@ -83,6 +83,34 @@ def pass_through(ctx, s, v, kind, scale, slots, renormalize, gw, gl):
 
 
 @pytest.mark.parametrize("renormalize", [True, False])
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16", "i32"])
+@pytest.mark.parametrize("tokens,experts", [(200, 12), (60, 300)])
+def test_the_largest_scales(ctx, kind, renormalize, tokens, experts):
+    """Scales up to the end of the range: a softmax of zeros and equal parts."""
+    rng = np.random.default_rng([tokens, experts, 3])
+    s, v = scores(rng, tokens, experts, kind, 0.2, ties=True)
+    for scale in (2.0**127, float(np.finfo(np.float32).max)):
+        say("[large scale]", kind, renormalize, tokens, experts)
+        # gradients that the scores' type holds
+        g = 2.0**-116 if kind == "f16" else 2.0**-20
+        pass_through(ctx, s, v, kind, scale, 3, renormalize, (rng.normal(0, 1, (tokens, 3)) * g).astype(np.float32), g)
+
+
+@pytest.mark.parametrize("renormalize", [True, False])
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_differences_beyond_the_range(ctx, kind, renormalize):
+    """Scores whose difference no 32-bit float holds, at a scale where it matters."""
+    rng = np.random.default_rng(11)
+    big = 2.0**127 * 1.75
+    v = rng.choice([-big, -big / 2, 0.0, big / 4, big], (100, 6))
+    v[0], v[1] = [big, -big, -big, -big, -big, -big], [-np.inf, -big, big, -np.inf, big, 0]
+    s = words(v, kind)
+    say("[far scores]", kind, renormalize)
+    pass_through(ctx, s, v, kind, 2.0**-124, 3, renormalize,
+                 (rng.normal(0, 1, (100, 3)) * 2.0**100).astype(np.float32), 2.0**100)
+
+
+@pytest.mark.parametrize("renormalize", [True, False])
 def test_the_smallest_scales(ctx, renormalize):
     """A scale below the normal numbers costs the gradient nothing of its precision."""
     rng = np.random.default_rng(12)
