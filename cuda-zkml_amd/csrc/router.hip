@@ -482,7 +482,7 @@ __global__ __launch_bounds__(ROUTE_THREADS) void k_route_grad(RouteGradArgs a) {
 #pragma unroll
     for (int i = 0; i < V; i++) top = S::larger(top, v[i]);
     const float m = over_lanes<L>(top, S::larger);
-    const bool bad = S::bad(m), empty = m == S::none();
+    const bool bad = S::bad(m);
     // g: gradients of the experts' weights; times: routes that name them
     float g[V] = {}, times[V] = {};
     if (a.grad_weight)
@@ -531,10 +531,11 @@ __global__ __launch_bounds__(ROUTE_THREADS) void k_route_grad(RouteGradArgs a) {
       for (int i = 0; i < V; i++) d[i] = fmaf(ez[i] * ic, fmaf(-times[i], gc, g[i]), d[i]);
     }
     T out[V];
-    // a masked row's sums are of nothing, an impossible one's are NaN; the scale comes last
-    // (a small one and a probability may have no product in 32 bits)
+    // an impossible row's are NaN, else a masked score's is zero (a masked row's sums are of
+    // nothing, and an infinity or a NaN that came in is one times zero too); the scale comes
+    // last (a small one and a probability may have no product in 32 bits)
 #pragma unroll
-    for (int i = 0; i < V; i++) out[i] = (T)(empty ? 0.0f : bad ? NAN : d[i] * a.scale);
+    for (int i = 0; i < V; i++) out[i] = (T)(bad ? NAN : v[i] == S::none() ? 0.0f : d[i] * a.scale);
     T* row = (T*)a.grad + (size_t)t * a.ld_grad;
 #pragma unroll
     for (int k = 0; k < V; k += P::C) {

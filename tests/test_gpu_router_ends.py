@@ -1,11 +1,12 @@
 """GPU tests of the experts' router (cuda-zkml_amd/csrc/router.hip) where its inputs end:
-padding that carries routes, scores and scales at the ends of the range."""
+padding that carries routes, scores and scales at the ends of the range, gradients that
+are no numbers."""
 import numpy as np
 import pytest
 
 import router_forms as forms
 import zkml_amd as z
-from i8_helpers import TYPES, Result, words
+from i8_helpers import TYPES, Result, values, words
 from test_gpu_router import outputs, say, scores, within, work_of
 
 pytestmark = pytest.mark.gpu
@@ -118,3 +119,32 @@ def test_the_smallest_scales(ctx, renormalize):
     say("[small scale]", renormalize)
     pass_through(ctx, v, v.astype(np.float64), "f32", 2.0**-140, 3, renormalize,
                  (rng.normal(0, 1, (100, 3)) * 2.0**110).astype(np.float32), 2.0**110)
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("renormalize", [True, False])
+@pytest.mark.parametrize("tokens,experts,slots", [(40, 13, 3), (30, 300, 20)])
+def test_masked_scores_of_any_gradient(ctx, kind, renormalize, tokens, experts, slots):
+    """Incoming gradients that overflowed, or are no numbers, leave masked scores' at zero;
+    the weights' stay with their token."""
+    rng = np.random.default_rng([tokens, experts, 5])
+    s, v = scores(rng, tokens, experts, kind, 0.4)
+    v[2] = -np.inf
+    s[2] = words(v[2], kind)
+    expert = forms.chosen(v, slots).astype(np.int32)
+    gw = rng.normal(0, 1, (tokens, slots)).astype(np.float32)
+    lost = [5, 9, 11]
+    gw[5, 0], gw[9, 1], gw[11, 0], gw[11, 1] = np.inf, np.nan, -np.inf, np.inf
+    count = forms.balance(v, 1.0, expert)[0]
+    say("[masked gradients]", kind, renormalize, tokens, experts, slots)
+    for gl in (0.5, np.inf, np.nan):
+        out = Result(ctx, tokens, experts, kind)
+        ctx.experts_route_grad(ctx.upload(s), TYPES[kind], tokens, experts, slots, ctx.upload(expert), out.at,
+                               renormalize=renormalize, grad_weight=ctx.upload(gw),
+                               count=ctx.upload(count.astype(np.int32)),
+                               grad_loss=ctx.upload(np.array([gl], np.float32)))
+        got = out.read()
+        assert not values(got, kind)[v == -np.inf].any()
+        if gl == 0.5:
+            fine = [t for t in range(tokens) if t not in lost]
+            within(got[fine], *forms.gradient(v[fine], 1.0, expert[fine], renormalize, gw[fine], count, gl), kind)
