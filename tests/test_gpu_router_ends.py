@@ -1,6 +1,6 @@
 """GPU tests of the experts' router (cuda-zkml_amd/csrc/router.hip) where its inputs end:
 padding that carries routes, scores and scales at the ends of the range, gradients that
-are no numbers."""
+are no numbers, and the sums over many tokens."""
 import numpy as np
 import pytest
 
@@ -148,3 +148,21 @@ def test_masked_scores_of_any_gradient(ctx, kind, renormalize, tokens, experts, 
         if gl == 0.5:
             fine = [t for t in range(tokens) if t not in lost]
             within(got[fine], *forms.gradient(v[fine], 1.0, expert[fine], renormalize, gw[fine], count, gl), kind)
+
+
+@pytest.mark.parametrize("tokens,experts,kind", [(1 << 20, 7, "bf16"), (200000, 60, "f32"), (30000, 300, "f16"),
+                                                 (20000, 700, "i32")])
+def test_sums_over_many_tokens(ctx, tokens, experts, kind):
+    """Bounds of the sums as they are made: no wave's, block's or pass's part can be missing."""
+    rng = np.random.default_rng([tokens, experts])
+    s, v = scores(rng, tokens, experts, kind)
+    scale = 2.0**-12 if kind == "i32" else 1.0
+    expert = rng.integers(0, experts, (tokens, 2)).astype(np.int32)
+    say("[many tokens]", tokens, experts, kind)
+    o = outputs(ctx, tokens, experts, 2, True)
+    ctx.experts_balance(ctx.upload(s), TYPES[kind], tokens, experts, 2, ctx.upload(expert), o["count"].at,
+                        o["prob"].at, o["loss"].at, work_of(ctx, tokens, experts), scale=scale)
+    want = balance(v, scale, expert)
+    check_balance(o, want)
+    prob, lim = want[1], want[3]
+    assert (lim <= 1e-4 * prob).all() and abs(o["prob"].read().sum(dtype=np.float64) - 1) <= lim.sum()
