@@ -1,0 +1,30 @@
+"""Host tests: the sizes of i4_forms take the kernels that they are meant for, and the
+rule (cuda-zkml_amd/csrc/i4_matmul.hip: choose_i4) names no form that has none."""
+import numpy as np
+import pytest
+
+import zkml_amd as z
+from i4_forms import FORMS, GROUPS
+
+
+def kernel(rows, n_out, n_in, odd, group, experts):
+    name = z.lib().zk_debug_i4_kernel(rows, n_out, n_in, n_in + odd, odd, group, experts)
+    return name and name.decode()
+
+
+@pytest.mark.parametrize("name,odd,group,rows,n_out,n_in,experts", FORMS)
+def test_sizes_reach_their_kernel(name, odd, group, rows, n_out, n_in, experts):
+    assert kernel(rows, n_out, n_in, odd, group, experts) == name
+
+
+def test_every_form_has_a_size():
+    listed = {(name, odd, group, experts > 0) for name, odd, group, _, _, _, experts in FORMS}
+    rng, named = np.random.default_rng(2), set()
+    for _ in range(30000):
+        rows, n_out, n_in = (int(2 ** rng.uniform(0, 13.5)) for _ in range(3))
+        experts = int(2 ** rng.uniform(0, 7)) if rng.random() < 0.5 else 0
+        odd = int(rng.integers(0, 2))
+        if not odd:
+            n_in = max(16, n_in // 16 * 16)
+        named |= {(kernel(rows, n_out, n_in, odd, g, experts), odd, g, experts > 0) for g in GROUPS}
+    assert named <= listed
