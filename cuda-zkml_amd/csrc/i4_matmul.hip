@@ -90,17 +90,20 @@ __device__ __forceinline__ void i4_put(const I4Args& a, uint32_t t, uint32_t n, 
   else ((__bf16*)a.y)[at] = (__bf16)v;
 }
 
-// A scale's bits, and what they are worth (apart, so that a load waits for nothing).
+// A scale's bits, and a sixteenth of what they are worth (apart, so that a load waits for
+// nothing): the products are of 16 times the weights, and sums of scaled groups that were
+// too, until the end, left the range of 32 bits 16 times early.  Only f32 and bf16 scales
+// below 2^-122 lose bits by it, down to a multiple of 2^-145.
 __device__ __forceinline__ uint32_t scale_bits(const I4Args& a, size_t at) {
   return a.scale_type == ZK_F32 ? ((const uint32_t*)a.scale)[at] : ((const uint16_t*)a.scale)[at];
 }
 __device__ __forceinline__ float scale_of(const I4Args& a, uint32_t bits) {
-  if (a.scale_type == ZK_F32) return __uint_as_float(bits);
-  if (a.scale_type == ZK_BF16) return __uint_as_float(bits << 16);
+  if (a.scale_type == ZK_F32) return __uint_as_float(bits) * 0.0625f;
+  if (a.scale_type == ZK_BF16) return __uint_as_float(bits << 16) * 0.0625f;
   const uint16_t b = (uint16_t)bits;
   _Float16 h;
   __builtin_memcpy(&h, &b, 2);
-  return (float)h;
+  return (float)h * 0.0625f;
 }
 
 // A step's products of 16 tokens and 16 channels, a sum for each of its groups, 16 times
@@ -130,7 +133,7 @@ __device__ __forceinline__ void i4_multiply(const v4i (&x)[2], const v4i& p, uin
 // 8192, took 20 us that way), so that waves wait for nobody until the end.
 // The matrix instruction takes 16 tokens (D's rows) and 16 channels (its columns): a lane
 // holds four tokens of one channel, and needs one scale.  16 packed bytes of a lane are its
-// operands of two instructions, 16 times the weights, which the results take back.  G: 128
+// operands of two instructions, 16 times the weights, which the scales take back.  G: 128
 // for groups of whole steps, 64 or 32.  D's row 4 c + i is token 4 i + c of the 16, so
 // that up to four tokens (NI = 1) are one register of each lane.  ODD: x's rows start at
 // any byte or end inside a chunk of 16; they come through registers, masked.
@@ -295,7 +298,7 @@ __global__ __launch_bounds__(64 * KW) void k_i4_wave(I4Args a, uint32_t tiles_t,
     float sum = sums[0][r][lane];
 #pragma unroll
     for (int k = 1; k < KW; k++) sum += sums[k][r][lane];
-    i4_put(a, t, n, has[d] ? i4_finish(sum * 0.0625f, fx[d], fb[d], a.relu) : 0.0f);
+    i4_put(a, t, n, has[d] ? i4_finish(sum, fx[d], fb[d], a.relu) : 0.0f);
   }
 }
 
@@ -399,7 +402,7 @@ __global__ __launch_bounds__(512) void k_i4_few(I4Args a, const X* __restrict__ 
   float sum = sums[0][wave][lane];
 #pragma unroll
   for (uint32_t k = 1; k < KW; k++) sum += sums[k][wave][lane];
-  i4_put(a, t, n, i4_finish(sum * 0.0625f, sx[t], a.bias ? a.bias[n] : 0.0f, a.relu));
+  i4_put(a, t, n, i4_finish(sum, sx[t], a.bias ? a.bias[n] : 0.0f, a.relu));
 }
 
 static bool i4_few(size_t rows, size_t n_out, size_t n_in) {
@@ -711,7 +714,7 @@ __global__ __launch_bounds__(64 * WT * WN, 2) void k_i4_ring(I4Args a, uint32_t 
         const float sx = f[tt], has = f[BT + tt];
 #pragma unroll
         for (int k = 0; k < 8; k++)
-          v[k] = has != 0.0f ? i4_finish(own[row * LD + c + k] * 0.0625f, sx, bias[k], a.relu) : 0.0f;
+          v[k] = has != 0.0f ? i4_finish(own[row * LD + c + k], sx, bias[k], a.relu) : 0.0f;
         const size_t at = (size_t)t * a.ld_y + n;
         if (a.y_type == ZK_F32) put8((float*)a.y + at, a.n_out - n, v);
         else if (a.y_type == ZK_F16) put8((_Float16*)a.y + at, a.n_out - n, v);

@@ -340,7 +340,8 @@ const char* zk_debug_i8_kernel(size_t rows, size_t n_out, size_t n_in, size_t ld
  * depends on the sizes alone; the token's scale and the bias follow in one fused
  * operation, then one rounding to y_type (ZK_F32, ZK_F16, ZK_BF16).  relu,
  * strides, NULL scales and biases and rows of x at any byte as in zk_i8_matmul
- * (d_w_scale may not be NULL); at most 2^26 channels.
+ * (d_w_scale may not be NULL); at most 2^26 channels.  Scales of weights below
+ * 2^-122 count to a multiple of 2^-145.
  * zk_i4_linear: zk_i8_quantize of x's rows, then zk_i4_matmul.  d_work:
  * zk_i4_linear_work(rows, n_in) bytes (0: sizes out of range), 16-byte aligned,
  * free again when the call's work on the stream is done.

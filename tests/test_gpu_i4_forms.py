@@ -1,11 +1,12 @@
 """GPU tests of every form of the 4-bit product's kernels (i4_forms) against the 64-bit
-form, within the bounds of i4_helpers.near."""
+form, within the bounds of i4_helpers.near: ordinary values, and both ends of a
+32-bit float's range."""
 import numpy as np
 import pytest
 
 import zkml_amd as z
 from i4_forms import FORMS
-from i4_helpers import inputs, near, packed, wide_product
+from i4_helpers import inputs, near, packed, product, wide_product
 from i8_helpers import Result, matrix, values
 from test_gpu_i4 import routes
 
@@ -52,3 +53,59 @@ def test_every_form(ctx, form):
     b = rng.normal(0, 1, (max(1, experts), n_out)).astype(np.float32)
     say("[i4 form]", *form)
     near(*run(ctx, form, x, sx, q, s, b, rng), n_in, "f32")
+
+
+def positive(form):
+    """Inputs of a form whose terms are all positive and within a factor of 2, 2 and 4 of the
+    largest; what a result can be at the most."""
+    _, _, group, rows, n_out, n_in, experts = form
+    rng = np.random.default_rng([rows, n_out, n_in, group, 1])
+    x = rng.integers(64, 128, (rows, n_in)).astype(np.int8)
+    q = rng.integers(4, 8, (max(1, experts) * n_out, n_in)).astype(np.int8)
+    s = rng.uniform(1, 2, (max(1, experts), -(-n_in // group), n_out)).astype(np.float32)
+    return rng, x, q, s, 127.0 * 7 * 2 * n_in
+
+
+@pytest.mark.parametrize("form", FORMS, ids=lambda f: "-".join(map(str, f)))
+def test_results_up_to_the_end_of_the_range(ctx, form):
+    """Sums of scaled groups that a 32-bit float holds are not lost on the way."""
+    rng, x, q, s, most = positive(form)
+    s = s * np.float32(2.0 ** (128 - np.ceil(np.log2(most))))
+    say("[i4 large]", *form)
+    got, want, size = run(ctx, form, x, None, q, s, None, rng)
+    assert 2.0**124 < want.max() < 2.0**128
+    near(got, want, size, form[5], "f32")
+
+
+@pytest.mark.parametrize("form", FORMS, ids=lambda f: "-".join(map(str, f)))
+def test_scales_at_the_low_end_of_the_range(ctx, form):
+    """Scales down to 2^-122 count in full."""
+    rng, x, q, s, _ = positive(form)
+    s = s * np.float32(2.0 ** (-122 - np.floor(np.log2(s.min()))))
+    assert 2.0**-122 <= s.min() < 2.0**-121
+    say("[i4 small]", *form)
+    near(*run(ctx, form, x, np.full(form[3], 2.0**100, np.float32), q, s, None, rng), form[5], "f32")
+
+
+def test_scales_below_the_normal_numbers(ctx):
+    """They count to a multiple of 2^-145."""
+    s = np.array([[2.0**-145 * k for k in range(40)]], np.float32)
+    for rows in (1, 300):
+        y = Result(ctx, rows, 40, "f32")
+        ctx.i4_matmul(ctx.upload(np.full((rows, 64), 3, np.int8)), ctx.upload(packed(np.full((40, 64), 5, np.int8))),
+                      ctx.upload(s), rows, 40, 64, 64, y.at, x_scale=ctx.upload(np.full(rows, 2.0**127, np.float32)))
+        assert np.array_equal(y.read(), np.tile(np.arange(40) * np.float32(960 * 2.0**-18), (rows, 1)))
+
+
+@pytest.mark.parametrize("rows,n_out,n_in,group", [(1, 64, 256, 32), (4, 50, 333, 64), (9, 100, 640, 128)])
+def test_linear_up_to_the_end_of_the_range(ctx, rows, n_out, n_in, group):
+    """The few rows that are quantized on the way."""
+    rng, x, q, s, most = positive((None, 0, group, rows, n_out, n_in, 0))
+    x[:, 0] = 127  # a row's scale is 1, its values are the quantized ones
+    s = s * np.float32(2.0 ** (128 - np.ceil(np.log2(most))))
+    y = Result(ctx, rows, n_out, "f32")
+    ctx.i4_linear(ctx.upload(x.astype(np.float32)), z.F32, ctx.upload(packed(q, rng)), ctx.upload(s), rows, n_out, n_in,
+                  group, y.at, z.F32, ctx.alloc(ctx.i4_linear_work(rows, n_in)))
+    want, size = product(x, q, values(s, "f32")[0], group, None, None, False)
+    assert 2.0**124 < want.max() < 2.0**128
+    near(y.read(), want, size, n_in, "f32")
