@@ -105,6 +105,12 @@ __device__ __forceinline__ float scale_of(const I4Args& a, uint32_t bits) {
   __builtin_memcpy(&h, &b, 2);
   return (float)h * 0.0625f;
 }
+// Zero for a group behind the row's end, whose sums are zero: the last one's scale may be
+// an infinity.  (Groups of whole steps have none.)
+template <int NS>
+__device__ __forceinline__ float scale_of_group(const I4Args& a, uint32_t bits, uint32_t g) {
+  return NS == 1 || g < a.groups ? scale_of(a, bits) : 0.0f;
+}
 
 // A step's products of 16 tokens and 16 channels, a sum for each of its groups, 16 times
 // too large: p a lane's packed weights, x its two fragments.  Groups of 32: an instruction's
@@ -234,13 +240,16 @@ __global__ __launch_bounds__(64 * KW) void k_i4_wave(I4Args a, uint32_t tiles_t,
       const uint32_t k = lane + i * 64, n = n0 + k % BN < a.n_out ? n0 + k % BN : a.n_out - 1;
       uint32_t g = w0 * NS + k / BN;
       if (G >= 128) g /= whole;
-      if (g >= a.groups) g = a.groups - 1;  // (behind the row's end: x is zero)
+      if (g >= a.groups) g = a.groups - 1;  // (of a step's part behind the row's end, not used)
       sc[i] = scale_bits(a, ch * a.groups + (size_t)g * a.n_out + n);
     }
     fetch(w0, 0);
     if (w0 + U < end) fetch(w0 + U, 1);
 #pragma unroll
-    for (int i = 0; i < 4 * FN; i++) scales[wave][(lane + i * 64) / BN][(lane + i * 64) % BN] = scale_of(a, sc[i]);
+    for (int i = 0; i < 4 * FN; i++) {
+      const uint32_t k = lane + i * 64;
+      scales[wave][k / BN][k % BN] = scale_of_group<NS>(a, sc[i], w0 * NS + k / BN);
+    }
     uint32_t half = 0;
     for (uint32_t s0 = w0; s0 < end; s0 += U) {
       if (s0 + U < end) wait_loads<LOADS>();
@@ -345,7 +354,7 @@ __global__ __launch_bounds__(512) void k_i4_few(I4Args a, const X* __restrict__ 
       const uint32_t k = lane + i * 64, n = n0 + k % BN < a.n_out ? n0 + k % BN : a.n_out - 1;
       uint32_t g = w0 * NS + k / BN;
       if (G >= 128) g /= whole;
-      if (g >= a.groups) g = a.groups - 1;  // (behind the row's end: x is zero)
+      if (g >= a.groups) g = a.groups - 1;  // (of a step's part behind the row's end, not used)
       sc[i] = scale_bits(a, (size_t)g * a.n_out + n);
     }
     fetch(w0, 0);
@@ -364,7 +373,10 @@ __global__ __launch_bounds__(512) void k_i4_few(I4Args a, const X* __restrict__ 
   for (uint32_t w0 = first; w0 < last; w0 += W) {
     if (w0 != first) begin(w0);
 #pragma unroll
-    for (int i = 0; i < 4; i++) scales[wave][(lane + i * 64) / BN][(lane + i * 64) % BN] = scale_of(a, sc[i]);
+    for (int i = 0; i < 4; i++) {
+      const uint32_t k = lane + i * 64;
+      scales[wave][k / BN][k % BN] = scale_of_group<NS>(a, sc[i], w0 * NS + k / BN);
+    }
     uint32_t half = 0;
     for (uint32_t s0 = w0; s0 < end; s0 += U) {
       if (s0 + U < end) wait_loads<U>();
@@ -559,7 +571,7 @@ __global__ __launch_bounds__(64 * WT * WN, 2) void k_i4_ring(I4Args a, uint32_t 
       const uint32_t k = tid + i * THREADS, n = n0 + k % BN < a.n_out ? n0 + k % BN : a.n_out - 1;
       uint32_t g = window * ROWS + k / BN;
       if (G >= 128) g /= whole;
-      if (g >= a.groups) g = a.groups - 1;  // (behind the row's end: x is zero)
+      if (g >= a.groups) g = a.groups - 1;  // (of a step's part behind the row's end, not used)
       sc[i] = scale_bits(a, ch * a.groups + (size_t)g * a.n_out + n);
     }
   };
@@ -567,7 +579,7 @@ __global__ __launch_bounds__(64 * WT * WN, 2) void k_i4_ring(I4Args a, uint32_t 
 #pragma unroll
     for (uint32_t i = 0; i < SR; i++) {
       const uint32_t k = tid + i * THREADS;
-      scales[window & 1][k / BN][k % BN] = scale_of(a, sc[i]);
+      scales[window & 1][k / BN][k % BN] = scale_of_group<NS>(a, sc[i], window * ROWS + k / BN);
     }
   };
   // the results' factors, a few for each thread, there when they are needed

@@ -109,3 +109,33 @@ def test_linear_up_to_the_end_of_the_range(ctx, rows, n_out, n_in, group):
     want, size = product(x, q, values(s, "f32")[0], group, None, None, False)
     assert 2.0**124 < want.max() < 2.0**128
     near(y.read(), want, size, n_in, "f32")
+
+
+# the last group ends inside the last step
+@pytest.mark.parametrize("odd", [0, 1])
+@pytest.mark.parametrize("rows,n_out,n_in,group", [(1, 64, 160, 32), (4, 40, 200, 64), (20, 40, 208, 32),
+                                                   (60, 100, 336, 64), (300, 300, 160, 32), (700, 260, 304, 64)])
+def test_infinite_scale_of_a_last_group(ctx, rows, n_out, n_in, group, odd):
+    """What lies behind a row's end has no part in an infinite scale of its last group."""
+    x, q = np.full((rows, n_in), 5, dtype=np.int8), np.full((n_out, n_in), -3, dtype=np.int8)
+    groups = -(-n_in // group)
+    s = np.ones((groups, n_out), dtype=np.float32)
+    s[-1, 3], s[-1, 7], s[-1, 11] = np.inf, -np.inf, np.nan
+    want = np.full((rows, n_out), -15.0 * n_in, dtype=np.float32)
+    want[:, 3], want[:, 7], want[:, 11] = -np.inf, np.inf, np.nan
+    w, sd = ctx.upload(packed(q)), ctx.upload(s)
+    say("[i4 last group]", rows, n_out, n_in, group, odd)
+    y = Result(ctx, rows, n_out, "f32")
+    ctx.i4_matmul(matrix(ctx, x, n_in + odd, odd), w, sd, rows, n_out, n_in, group, y.at, ld_x=n_in + odd)
+    assert np.array_equal(y.read(), want, equal_nan=True)
+    # rows of 127: a scale of 1
+    y = Result(ctx, rows, n_out, "f32")
+    ctx.i4_linear(ctx.upload(np.full((rows, n_in), 127, dtype=np.float32)), z.F32, w, sd, rows, n_out, n_in, group, y.at,
+                  z.F32, ctx.alloc(ctx.i4_linear_work(rows, n_in)))
+    want[np.isfinite(want)] = -381.0 * n_in
+    assert np.array_equal(y.read(), want, equal_nan=True)
+    y = Result(ctx, rows, n_out, "f32")
+    ctx.i4_matmul_experts(matrix(ctx, x, n_in + odd, odd), w, sd, ctx.upload(np.array([0, rows], np.int32)), rows, 1,
+                          n_out, n_in, group, y.at, ld_x=n_in + odd)
+    want[np.isfinite(want)] = -15.0 * n_in
+    assert np.array_equal(y.read(), want, equal_nan=True)
