@@ -915,8 +915,10 @@ __global__ __launch_bounds__(256) void k_i4_quantize(const T* __restrict__ w, si
 }
 
 // ------------------------------------------------------------ arguments
+static bool group_size(int group) { return group == 32 || group == 64 || (group >= 128 && group % 128 == 0); }
+
 static int check_group(zk_context* ctx, size_t n_in, int group) {
-  if (group != 32 && group != 64 && (group < 128 || group % 128))
+  if (!group_size(group))
     return ctx->fail(ZK_ERR_INVALID, "i4: a group is 32, 64 or a multiple of 128 weights");
   if (n_in > I4_MAX_IN) return ctx->fail(ZK_ERR_SIZE, "i4: rows longer than 2^24");
   return ZK_OK;
@@ -1022,7 +1024,9 @@ int zk_i4_matmul(zk_context* ctx, const int8_t* d_x, size_t ld_x, const float* d
 const char* zk_debug_i4_kernel(size_t rows, size_t n_out, size_t n_in, size_t ld_x, size_t address, int group,
                                int experts) {
   using namespace zk;
-  if (!rows || !n_out || rows > 0x7fffffffu || n_out > 16 * I8_MAX_TILES || n_in > I4_MAX_IN || experts < 0) return nullptr;
+  if (!rows || !n_out || rows > 0x7fffffffu || n_out > 16 * I8_MAX_TILES || n_in > I4_MAX_IN || experts < 0 ||
+      !group_size(group))
+    return nullptr;
   I4Args a = {};
   a.x = (const int8_t*)address, a.ld_x = ld_x, a.ld_w = i4_row_bytes(n_in);
   set_sizes(a, rows, n_out, n_in, group, 0, ZK_F32, ZK_F32);

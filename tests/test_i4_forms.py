@@ -1,5 +1,8 @@
 """Host tests: the sizes of i4_forms take the kernels that they are meant for, and the
 rule (cuda-zkml_amd/csrc/i4_matmul.hip: choose_i4) names no form that has none."""
+import subprocess
+import sys
+
 import numpy as np
 import pytest
 
@@ -28,3 +31,11 @@ def test_every_form_has_a_size():
             n_in = max(16, n_in // 16 * 16)
         named |= {(kernel(rows, n_out, n_in, odd, g, experts), odd, g, experts > 0) for g in GROUPS}
     assert named <= listed
+
+
+def test_groups_out_of_range():
+    """A group that no product takes has no kernel, and ends no process."""
+    code = ("import sys; sys.path[:0] = sys.argv[1:]; import zkml_amd as z; "
+            "assert all(z.lib().zk_debug_i4_kernel(4, 4, 64, 64, 0, g, e) is None "
+            "for g in (0, -1, -128, 1, 96, 129) for e in (0, 3))")
+    assert subprocess.run([sys.executable, "-c", code, *sys.path]).returncode == 0
