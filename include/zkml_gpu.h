@@ -332,13 +332,14 @@ const char* zk_debug_i8_kernel(size_t rows, size_t n_out, size_t n_in, size_t ld
  * zk_i4_quantize: a matrix of rows x cols to this layout.  scale = max |w| of the
  * group / 7, rounded to scale_type; q = the integer nearest to w / scale (ties to
  * even), between -8 and 7.  A group of zeros, or whose scale rounds to zero, has
- * scale 0 and zeros, one that holds an infinity or a NaN scale NaN and zeros.
- * Padding becomes zero.
+ * scale 0 and zeros, one whose scale rounds to infinity that scale and zeros, one that
+ * holds an infinity or a NaN scale NaN and zeros.  Padding becomes zero.
  * zk_i4_matmul: y[t][n] = x_scale[t] * sum_g w_scale[g][n] acc[t][n][g] + bias[n]
  * with acc[t][n][g] = sum_k x[t][k] q[n][k] over group g.  Sums within 128
- * weights are exact; the groups' terms are added in 32-bit floats, in an order that
- * depends on the sizes alone; the token's scale and the bias follow in one fused
- * operation, then one rounding to y_type (ZK_F32, ZK_F16, ZK_BF16).  relu,
+ * weights are exact; the groups' terms, of a longer one those of each 128 weights, are
+ * added in 32-bit floats, in an order that depends on the sizes, the strides and
+ * x's address, never on the order of execution; the token's scale and the bias follow in one
+ * fused operation, then one rounding to y_type (ZK_F32, ZK_F16, ZK_BF16).  relu,
  * strides, NULL scales and biases and rows of x at any byte as in zk_i8_matmul
  * (d_w_scale may not be NULL); at most 2^26 channels.  Scales of weights below
  * 2^-122 count to a multiple of 2^-145.
@@ -443,7 +444,7 @@ int zk_experts_combine_grad(zk_context* ctx, const void* d_grad, size_t ld_grad,
  * twice.  Masked scores get 0, a row with a NaN or an infinity above NaN.
  * At most 1024 experts and 2^22 pairs.  No result depends on the order of
  * execution.  None of these allocates, waits or uses memory of the context; calls
- * that overlap need a workspace each. */
+ * that overlap need a workspace each.  Outputs may not overlap an input. */
 enum { ZK_MAX_SLOTS = 32 };
 size_t zk_experts_route_work(size_t tokens, int experts);
 int zk_experts_route(zk_context* ctx, const void* d_scores, int type, size_t ld, size_t tokens, int experts, int slots,

@@ -205,6 +205,22 @@ def test_quantize_of_what_has_no_scale(ctx):
     assert np.array_equal(got, want)
 
 
+@pytest.mark.parametrize("rows,n_in,group", [(1, 256, 128), (40, 200, 32), (300, 300, 64)])
+def test_quantize_beyond_the_scales_type(ctx, rows, n_in, group):
+    """A scale that rounds to infinity has zeros, and what is made of it shows it."""
+    rng = np.random.default_rng(group)
+    w = rng.normal(0, 1, (5, n_in)).astype(np.float32)
+    w[2, :group] *= 1e8
+    groups = -(-n_in // group)
+    q, s = Result(ctx, 5, -(-n_in // 128) * 64, "i8"), Result(ctx, groups, 5, "f16")
+    ctx.i4_quantize(ctx.upload(w), z.F32, 5, n_in, group, q.at, s.at, z.F16)
+    sc, got = s.read(), unpacked(q.read().view(np.uint8), n_in)
+    assert sc[0, 2] == np.inf and np.isinf(sc).sum() == 1 and not got[2, :group].any()
+    y = Result(ctx, rows, 5, "f32")
+    ctx.i4_matmul(ctx.upload(np.ones((rows, n_in), np.int8)), q.at, s.at, rows, 5, n_in, group, y.at, scale_type=z.F16)
+    assert np.isnan(y.read()[:, 2]).all() and np.isfinite(np.delete(y.read(), 2, axis=1)).all()
+
+
 LINEAR = [(1, 100, 64, 32), (1, 1024, 8192, 128), (3, 70, 1001, 64), (16, 33, 500, 128), (17, 200, 1024, 128),
           (40, 129, 2100, 64), (300, 257, 640, 128), (8, 100, 20000, 128), (2, 20, 7, 32), (5, 40, 16, 64), (4, 50, 33, 128),
           (16, 300, 2200, 256), (1, 8200, 256, 128), (2, 8192, 130, 32), (13, 31, 1500, 64), (1, 70, 36000, 128)]
