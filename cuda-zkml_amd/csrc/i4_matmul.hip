@@ -105,11 +105,15 @@ __device__ __forceinline__ float scale_of(const I4Args& a, uint32_t bits) {
   __builtin_memcpy(&h, &b, 2);
   return (float)h * 0.0625f;
 }
-// Zero for a group behind the row's end, whose sums are zero: the last one's scale may be
-// an infinity.  (Groups of whole steps have none.)
+// Groups behind the row's end (of a last step, if a group is less than one) have scales of
+// zero: their sums are zero, but the last group's scale may be an infinity.  Of one scale
+// on its way to LDS, and of a wave's window in LDS, from `from` to `to`.
 template <int NS>
 __device__ __forceinline__ float scale_of_group(const I4Args& a, uint32_t bits, uint32_t g) {
   return NS == 1 || g < a.groups ? scale_of(a, bits) : 0.0f;
+}
+__device__ __forceinline__ void zero_scales(float* scales, uint32_t from, uint32_t to, uint32_t lane) {
+  for (uint32_t k = from + lane; k < to; k += 64) scales[k] = 0.0f;
 }
 
 // A step's products of 16 tokens and 16 channels, a sum for each of its groups, 16 times
@@ -248,8 +252,9 @@ __global__ __launch_bounds__(64 * KW) void k_i4_wave(I4Args a, uint32_t tiles_t,
 #pragma unroll
     for (int i = 0; i < 4 * FN; i++) {
       const uint32_t k = lane + i * 64;
-      scales[wave][k / BN][k % BN] = scale_of_group<NS>(a, sc[i], w0 * NS + k / BN);
+      scales[wave][k / BN][k % BN] = scale_of(a, sc[i]);
     }
+    if (NS > 1 && end * NS > a.groups) zero_scales(&scales[wave][0][0], (a.groups - w0 * NS) * BN, ROWS * BN, lane);
     uint32_t half = 0;
     for (uint32_t s0 = w0; s0 < end; s0 += U) {
       if (s0 + U < end) wait_loads<LOADS>();
@@ -375,8 +380,9 @@ __global__ __launch_bounds__(512) void k_i4_few(I4Args a, const X* __restrict__ 
 #pragma unroll
     for (int i = 0; i < 4; i++) {
       const uint32_t k = lane + i * 64;
-      scales[wave][k / BN][k % BN] = scale_of_group<NS>(a, sc[i], w0 * NS + k / BN);
+      scales[wave][k / BN][k % BN] = scale_of(a, sc[i]);
     }
+    if (NS > 1 && end * NS > a.groups) zero_scales(&scales[wave][0][0], (a.groups - w0 * NS) * BN, ROWS * BN, lane);
     uint32_t half = 0;
     for (uint32_t s0 = w0; s0 < end; s0 += U) {
       if (s0 + U < end) wait_loads<U>();
@@ -475,6 +481,7 @@ __global__ __launch_bounds__(64 * WT * WN, 2) void k_i4_ring(I4Args a, uint32_t 
   constexpr uint32_t LD = FN * 32 + 4, OWN = 32 * LD * 4;        // a wave's results of 32 tokens
   static_assert(WAVES * OWN + 4 * (2 * BT + BN) <= STAGES * STAGE, "the results' LDS is the stages'");
   static_assert(XR * 8 * WAVES == BT && WR * 16 * WAVES == BN && SR * THREADS == ROWS * BN, "whole pieces");
+  static_assert(BN % 64 == 0, "a wave's scales are of one row");
   __shared__ __align__(16) int8_t lds[STAGES * STAGE];
   __shared__ float scales[2][ROWS][BN];
   const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -575,11 +582,15 @@ __global__ __launch_bounds__(64 * WT * WN, 2) void k_i4_ring(I4Args a, uint32_t 
       sc[i] = scale_bits(a, ch * a.groups + (size_t)g * a.n_out + n);
     }
   };
-  auto put_scales = [&](uint32_t window) {
+  // INSIDE: all its steps are whole.
+  auto put_scales = [&](auto is_inside, uint32_t window) {
+    constexpr bool INSIDE = decltype(is_inside)::value;
 #pragma unroll
     for (uint32_t i = 0; i < SR; i++) {
       const uint32_t k = tid + i * THREADS;
-      scales[window & 1][k / BN][k % BN] = scale_of_group<NS>(a, sc[i], window * ROWS + k / BN);
+      // (a wave's are of one row)
+      const uint32_t g = window * ROWS + __builtin_amdgcn_readfirstlane(k / BN);
+      scales[window & 1][k / BN][k % BN] = scale_of_group<INSIDE ? 1 : NS>(a, sc[i], g);
     }
   };
   // the results' factors, a few for each thread, there when they are needed
@@ -625,7 +636,7 @@ __global__ __launch_bounds__(64 * WT * WN, 2) void k_i4_ring(I4Args a, uint32_t 
   auto turn = [&](auto is_long, uint32_t s, uint32_t slot) {
     constexpr bool LONG = decltype(is_long)::value;
     if (LONG || s + 1 < steps) put_held(up(slot));
-    if (s % W == 0) put_scales(s / W);
+    if (s % W == 0) put_scales(std::bool_constant<LONG && W <= 2>(), s / W);  // (LONG: s + 2 is whole)
     if (LONG || s + 1 < steps) wait_loads<LOADS>();
     else wait_loads<0>();
     if (!LONG && s >= full) clear_end(s, slot);
