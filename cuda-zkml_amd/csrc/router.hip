@@ -435,6 +435,7 @@ struct RouteGradArgs {
   size_t ld, ld_grad;
   uint32_t tokens, experts, slots;
   float scale;
+  float in, out;             // factors of what comes in and of the gradient; their product is the scale
   const int32_t* expert;
   const float* grad_weight;  // or null
   const int32_t* count;      // or null
@@ -456,7 +457,7 @@ __global__ __launch_bounds__(ROUTE_THREADS) void k_route_grad(RouteGradArgs a) {
   float f[V] = {};
   if (a.count) {
     __shared__ float shared[L * V];
-    const float n = (float)a.count[a.experts], g = *a.grad_loss;
+    const float n = (float)a.count[a.experts], g = *a.grad_loss * a.in;
     const float per = n > 0.0f ? g * ((float)a.experts / (n * n * (float)a.slots)) : 0.0f;
     for (uint32_t e = tid; e < L * V; e += ROUTE_THREADS) shared[e] = e < a.experts ? (float)a.count[e] * per : 0.0f;
     __syncthreads();
@@ -475,7 +476,7 @@ __global__ __launch_bounds__(ROUTE_THREADS) void k_route_grad(RouteGradArgs a) {
       const bool on = a.grad_weight && l + k * L < a.slots;
       const size_t at = (size_t)t * a.slots + l + k * L;
       named[k] = on ? a.expert[at] : -1;
-      gw[k] = on ? a.grad_weight[at] : 0.0f;
+      gw[k] = on ? a.grad_weight[at] * a.in : 0.0f;
     }
     load_scores<T, L, V>((const T*)a.scores + (size_t)t * a.ld, l, a.experts, v);
     float top = S::none();
@@ -510,8 +511,9 @@ __global__ __launch_bounds__(ROUTE_THREADS) void k_route_grad(RouteGradArgs a) {
     }
     const float inv = 1.0f / sum_over<L>(z);
     dot = sum_over<L>(dot) * inv;
+    const float by = bad ? NAN : inv * a.out;
 #pragma unroll
-    for (int i = 0; i < V; i++) d[i] = ez[i] * inv * ((NORMAL ? f[i] : f[i] + g[i]) - dot);
+    for (int i = 0; i < V; i++) d[i] = ez[i] * ((NORMAL ? f[i] : f[i] + g[i]) - dot) * by;
     if constexpr (NORMAL) {
       // softmax over the chosen alone: their own maximum, sum and mean
       float mc = S::none(), zc = 0.0f, gc = 0.0f;
@@ -525,17 +527,17 @@ __global__ __launch_bounds__(ROUTE_THREADS) void k_route_grad(RouteGradArgs a) {
         gc = fmaf(g[i], ez[i], gc);
       }
       zc = sum_over<L>(zc), gc = sum_over<L>(gc);
-      const float ic = zc > 0.0f ? 1.0f / zc : 0.0f;
+      const float ic = zc > 0.0f ? 1.0f / zc : 0.0f, byc = ic * a.out;
       gc *= ic;
 #pragma unroll
-      for (int i = 0; i < V; i++) d[i] = fmaf(ez[i] * ic, fmaf(-times[i], gc, g[i]), d[i]);
+      for (int i = 0; i < V; i++) d[i] = fmaf(ez[i] * fmaf(-times[i], gc, g[i]), byc, d[i]);
     }
     T out[V];
     // an impossible row's are NaN, else a masked score's is zero (a masked row's sums are of
-    // nothing, and an infinity or a NaN that came in is one times zero too); the scale comes
-    // last (a small one and a probability may have no product in 32 bits)
+    // nothing, and an infinity or a NaN that came in is one times zero too)
+    const float gone = bad ? NAN : S::none();
 #pragma unroll
-    for (int i = 0; i < V; i++) out[i] = (T)(bad ? NAN : v[i] == S::none() ? 0.0f : d[i] * a.scale);
+    for (int i = 0; i < V; i++) out[i] = (T)(v[i] == gone ? 0.0f : d[i]);
     T* row = (T*)a.grad + (size_t)t * a.ld_grad;
 #pragma unroll
     for (int k = 0; k < V; k += P::C) {
@@ -717,8 +719,11 @@ int zk_experts_route_grad(zk_context* ctx, const void* d_scores, int type, size_
     if (!aligned(d_grad_scores, type_bytes(type)))
       return ctx->fail(ZK_ERR_INVALID, "experts' route: a pointer is not aligned to its type");
     OnDevice on(ctx);
-    const RouteGradArgs a = {d_scores, ld, ld_grad, (uint32_t)tokens, (uint32_t)experts, (uint32_t)slots, scale,
-                             d_expert, d_grad_weight, d_count, d_grad_loss, d_grad_scores};
+    // a small scale has its product with a probability's sum in 32 bits' normal numbers
+    // only if what comes in gives up 64 of the powers of two
+    const float in = scale < 0x1p-100f ? 0x1p-64f : 1.0f;
+    const RouteGradArgs a = {d_scores, ld, ld_grad, (uint32_t)tokens, (uint32_t)experts, (uint32_t)slots, scale, in,
+                             scale / in, d_expert, d_grad_weight, d_count, d_grad_loss, d_grad_scores};
     hipStream_t st = ctx->s(stream);
     return by_type(type, [&](auto zero) -> int {
       typedef decltype(zero) T;
