@@ -320,10 +320,14 @@ __global__ __launch_bounds__(64 * KW) void k_i4_wave(I4Args a, uint32_t tiles_t,
 // The linear layer of at most 16 rows in one launch: each block asks for its first weights,
 // quantizes all of x's rows into LDS while they come, and goes on as k_i4_wave with its x
 // fragments from there.  Bound by the chain of x's maximum, its bytes and the product.
-// That every block quantizes x again pays as long as all blocks run at once (two a CU) and
-// x is small; in turn, a call this way and in two launches: one row, 8192 to 1024 f16,
-// 8.9 and 12.4 us.
-constexpr uint32_t I4_FEW_OUT = 2 * 256 * 16;
+// That every block quantizes x again pays as long as all blocks run at once (two a CU) and x
+// is small: at most 64 KB, 48 above 4096 channels, where a CU has two blocks.  One launch and
+// two, bf16, on the GPU: 1 x 8192 to 1024 6.8 and 8.0 us, 8 x 4096 to 4096 9.6 and 7.6, 4 x 8192
+// to 8192 14.5 and 10.5; a call from Python, to which a second launch is about 2.7 us: 9.7 and
+// 12.6, 10.1 and 12.4, 14.6 and 12.2.  Over 312 sizes the rule's calls take 1% longer than the
+// shorter of the two on the average, 21% at the most, their kernels 4 and 59% (16 x 2048 to
+// 256), always one launch 3 and 81%, 13 and 117%.
+constexpr uint32_t I4_FEW_OUT = 2 * 256 * 16, I4_FEW_X = 64 * 1024, I4_FEW_X_WIDE = 48 * 1024;
 
 template <class X, int G, int NI>
 __global__ __launch_bounds__(512) void k_i4_few(I4Args a, const X* __restrict__ x, size_t ld_x) {
@@ -423,8 +427,9 @@ __global__ __launch_bounds__(512) void k_i4_few(I4Args a, const X* __restrict__ 
   i4_put(a, t, n, i4_finish(sum, sx[t], a.bias ? a.bias[n] : 0.0f, a.relu));
 }
 
-static bool i4_few(size_t rows, size_t n_out, size_t n_in) {
-  return rows <= FEW_ROWS && n_in >= 16 && n_out <= I4_FEW_OUT && rows * few_ld((uint32_t)n_in) <= FEW_BYTES;
+static bool i4_few(size_t rows, size_t n_out, size_t n_in, int x_type) {
+  return rows <= FEW_ROWS && n_in >= 16 && n_out <= I4_FEW_OUT && rows * few_ld((uint32_t)n_in) <= FEW_BYTES &&
+         rows * n_in * type_bytes(x_type) <= (n_out > I4_FEW_OUT / 2 ? I4_FEW_X_WIDE : I4_FEW_X);
 }
 
 template <int G>
@@ -1071,7 +1076,7 @@ int zk_i4_linear(zk_context* ctx, const void* d_x, int x_type, size_t ld_x, cons
     set_sizes(a, rows, n_out, n_in, group, relu, scale_type, y_type);
     OnDevice on(ctx);
     hipStream_t st = ctx->s(stream);
-    if (i4_few(rows, n_out, n_in)) {
+    if (i4_few(rows, n_out, n_in, x_type)) {
       if (group == 32) return i4_launch_few<32>(ctx, a, d_x, x_type, ld_x, st);
       if (group == 64) return i4_launch_few<64>(ctx, a, d_x, x_type, ld_x, st);
       return i4_launch_few<128>(ctx, a, d_x, x_type, ld_x, st);

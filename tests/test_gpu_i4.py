@@ -247,6 +247,27 @@ def test_linear(ctx, kind, rows, n_out, n_in, group):
     near(y.read(), *product(q8.read(), q, sv[0], group, s8.read()[0], b, False), n_in, kind)
 
 
+@pytest.mark.parametrize("kind,rows,n_out,n_in", [
+    ("bf16", 16, 60, 2048), ("bf16", 16, 60, 2049), ("f32", 1, 50, 16384), ("f32", 1, 50, 16385),
+    ("f16", 1, 40, 32768), ("f16", 1, 40, 32769), ("f32", 8, 4096, 2048), ("f32", 8, 4112, 2048),
+    ("bf16", 12, 4112, 2048), ("bf16", 13, 4112, 2048), ("f16", 4, 30, 8189), ("f32", 17, 30, 64)])
+@pytest.mark.parametrize("group", [64, 128])
+def test_linear_beside_its_limits(ctx, kind, rows, n_out, n_in, group):
+    """Sizes on both sides of where the rows are quantized on the way."""
+    rng = np.random.default_rng([rows, n_out, n_in, group])
+    x = words(rng.normal(0, 1, (rows, n_in)), kind)
+    _, _, q, s, _ = inputs(rng, rows, n_out, n_in, group, "f32")
+    s = s / np.float32(64)
+    sv = values(s, "f32")
+    say("[i4 linear limits]", kind, rows, n_out, n_in, group)
+    xd, y = ctx.upload(x), Result(ctx, rows, n_out, "f32")
+    ctx.i4_linear(xd, TYPES[kind], ctx.upload(packed(q, rng)), ctx.upload(s), rows, n_out, n_in, group, y.at, z.F32,
+                  ctx.alloc(ctx.i4_linear_work(rows, n_in)))
+    q8, s8 = Result(ctx, rows, n_in, "i8"), Result(ctx, 1, rows, "f32")
+    ctx.i8_quantize(xd, TYPES[kind], rows, n_in, q8.at, s8.at)
+    near(y.read(), *wide_product(q8.read(), q, sv[0], group, s8.read()[0], None, False), n_in, "f32")
+
+
 def test_linear_rows_without_a_scale(ctx):
     x = np.ones((4, 200), dtype=np.float32)
     x[1, 7], x[2] = np.inf, 0.0
