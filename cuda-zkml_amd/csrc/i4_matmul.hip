@@ -147,8 +147,8 @@ __device__ __forceinline__ void i4_multiply(const v4i (&x)[2], const v4i& p, uin
 // for groups of whole steps, 64 or 32.  D's row 4 c + i is token 4 i + c of the 16, so
 // that up to four tokens (NI = 1) are one register of each lane.  ODD: x's rows start at
 // any byte or end inside a chunk of 16; they come through registers, masked.
-// 1 row, 4096 to 4096: 4.8 us, a launch and one chain of loads (8 MB of weights: 1.4 us);
-// 48 rows, 8192 to 8192: 12.2 us (34 MB: 5.9 us).
+// Traced: 1 row, 4096 to 4096 4.6 us, a launch and one chain of loads (8 MB of weights:
+// 1.4 us); 48 rows, 8192 to 8192 13.2 us, 12.3 in a graph (34 MB: 5.9 us).
 template <int G, bool GROUPED, bool ODD, int FT, int FN, int NI, int KW, int U>
 __global__ __launch_bounds__(64 * KW) void k_i4_wave(I4Args a, uint32_t tiles_t, uint32_t tiles_n) {
   constexpr uint32_t BT = NI < 4 ? 4 * NI : 16 * FT, BN = 16 * FN;
@@ -472,8 +472,10 @@ __device__ __forceinline__ void put8(T* y, uint32_t left, const float (&v)[8]) {
 // which is what bounds this kernel beside the matrix cores: 32 operations a square and
 // group for four matrix instructions of a step.  Scales come through registers to LDS, four
 // groups' at a time.  ODD: x's rows start at any byte or end inside a chunk; they come
-// through registers, masked.  4096 rows, 8192 to 8192: 298 us, 1.84 POPS; 777 rows, 4096 to
-// 4096, groups of 64: 38 us; 2048 tokens x 4 of 64 experts, 2048 to 1024: 46 us.
+// through registers, masked.  A call among others: 4096 rows, 8192 to 8192 293 us, 1.88 POPS
+// (320 traced); 2048 tokens x 4 of 64 experts, 2048 to 1024 45 us (53).  777 rows, 4096 to
+// 4096, groups of 64: 39 us traced.  The largest tiles have no register left: 4 of a lane's go
+// to memory with groups of 128, 15 with 64, 22 with 32.
 template <int G, bool GROUPED, bool ODD, int WT, int WN, int FT, int FN>
 __global__ __launch_bounds__(64 * WT * WN, 2) void k_i4_ring(I4Args a, uint32_t tiles_t, uint32_t tiles_n) {
   constexpr uint32_t WAVES = WT * WN, THREADS = 64 * WAVES, BT = WT * FT * 32, BN = WN * FN * 32;
@@ -758,7 +760,9 @@ __global__ __launch_bounds__(64 * WT * WN, 2) void k_i4_ring(I4Args a, uint32_t 
 // part for every step of 128 of k (fitted to products of 1 to 4096 rows, 128 to 8192 long,
 // and to 2 to 6400 rows of 8 to 64 experts; the rule's choices took 2, 2.5 and 3% longer
 // than the best of all on the average, 27% at the most).  Rows of x of whole chunks, at any
-// byte, and grouped by expert; 0: not a choice.  Smaller groups lengthen a step.
+// byte, and grouped by expert; 0: not a choice.  Those forms were measured too, and won little:
+// 4 x 32 not grouped at one size in 72, by 7%; grouped, the 16 x 16, 32 x 32 and 48 x 32 at none
+// of 40, 256 x 256 at one, by 8%.  Smaller groups lengthen a step.
 struct I4Cost {
   uint32_t first, step, more, more_step;
 };

@@ -33,10 +33,11 @@ constexpr int balance_threads(int lanes) { return lanes == 16 ? 1024 : 512; }
 
 constexpr uint32_t ROUTE_BLOCKS = 2048;   // of a launch at the most (then a block has several tokens a group)
 constexpr uint32_t BALANCE_BLOCKS = 256;  // one a CU
-// Tokens times (experts + 64) that one block takes alone: a second launch costs the host
-// 3.7 us and the GPU 2.5 to 4, by which time it has done 256 tokens' choice of 60 experts
-// (14.3 us with the gradient on the GPU, 12.0 in two launches; a call 14.2 and 17.9), or
-// counted 500 tokens' (12.6 and 10.2; 13.8 and 17.8).
+// Tokens times (experts + 64) that one block takes alone, by the time of a call from Python, to
+// which a second launch is about 2.8 us: f32, 2 slots, one block and several, 256 tokens' choice of 60 experts 10.7 and 11.6 us, 500 tokens' given routes 9.7
+// and 11.3.  The GPU alone would take several blocks earlier, from about 200 tokens of a
+// choice on and 300 of given routes: these two are 10.5 and 8.1, 9.5 and 7.1 there, 256 of 8
+// 8.1 and 6.3, 128 of 60 6.8 and 8.2.
 constexpr size_t BALANCE_ONE_CHOICE = (size_t)1 << 15, BALANCE_ONE = (size_t)1 << 16;
 
 struct RouteArgs {
@@ -227,7 +228,8 @@ struct BalanceOut {
 // CHOOSE: a token's experts and weights are found; else given.  BALANCE: counts
 // and sums of p are made; one block alone makes the caller's results of them.
 // Bound by the launch and the chain of a token's maxima: 16384 tokens, 8 of 128 experts,
-// bf16, with the balance 8.5 us (4 MB); 32768 x 256, routes given, 9.0 us (17 MB: 1.9 TB/s).
+// bf16, with the balance 9.6 us (4 MB); 32768 x 256, routes given, 9.2 us (17 MB: 1.8 TB/s),
+// traced.
 template <class T, int L, int V, bool CHOOSE, bool BALANCE>
 __global__ __launch_bounds__(BALANCE ? balance_threads(L) : ROUTE_THREADS) void k_route(RouteArgs a, BalanceOut out) {
   typedef Score<T> S;
@@ -374,7 +376,7 @@ __global__ __launch_bounds__(BALANCE ? balance_threads(L) : ROUTE_THREADS) void 
 // The blocks' counts and sums to the caller's: a block has 32 experts and shares the
 // blocks' rows among eight threads each, in a fixed order; the loss is put together by
 // the block that is done last, from all blocks' parts in their order.  256 blocks of 256
-// experts: 5.6 us, two chains of loads behind a launch.
+// experts: 5.7 us traced, two chains of loads behind a launch.
 constexpr uint32_t FINISH_EXPERTS = 32;
 __global__ __launch_bounds__(256) void k_balance_finish(BalanceOut out, uint32_t blocks, uint32_t experts,
                                                         uint32_t slots) {
@@ -429,7 +431,7 @@ __global__ __launch_bounds__(256) void k_balance_finish(BalanceOut out, uint32_t
 }
 
 // ------------------------------------------------------------ gradient
-// One pass as k_route's: 32768 x 256, bf16, 9.9 us (34 MB: 3.4 TB/s).
+// One pass as k_route's: 32768 x 256, bf16, 10.4 us traced (34 MB: 3.3 TB/s).
 struct RouteGradArgs {
   const void* scores;
   size_t ld, ld_grad;
