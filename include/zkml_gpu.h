@@ -343,9 +343,9 @@ const char* zk_debug_i8_kernel(size_t rows, size_t n_out, size_t n_in, size_t ld
  * strides, NULL scales and biases and rows of x at any byte as in zk_i8_matmul
  * (d_w_scale may not be NULL); at most 2^26 channels.  Scales of weights below
  * 2^-122 count to a multiple of 2^-145.
- * zk_i4_linear: zk_i8_quantize of x's rows, then zk_i4_matmul.  d_work:
- * zk_i4_linear_work(rows, n_in) bytes (0: sizes out of range), 16-byte aligned,
- * free again when the call's work on the stream is done.
+ * zk_i4_linear: zk_i8_quantize of x's rows, then zk_i4_matmul, few rows in an order of
+ * sums of their own.  d_work: zk_i4_linear_work(rows, n_in) bytes (0: sizes out of
+ * range), 16-byte aligned, free again when the call's work on the stream is done.
  * zk_i4_matmul_experts: as zk_i8_matmul_experts; expert e's weights begin at
  * d_w + e * n_out * ld_w bytes, its scales at d_w_scale[e * groups * n_out], its
  * biases at d_bias[e * n_out].

@@ -94,7 +94,8 @@ def test_many_rows(ctx, rows, n_out, n_in, group):
     near(y.read(), *product(x, q, sv[0], group, sx, b, True), n_in, "bf16")
 
 
-# every kernel, with rows of whole chunks and with odd ones, in every size of group
+# the sizes of each kernel for whole chunks and groups of 128, with odd rows and other groups
+# too, which may take another one (each form at its own sizes: test_gpu_i4_forms.py)
 @pytest.mark.parametrize("group", [32, 64, 128, 384])
 @pytest.mark.parametrize("odd", [0, 1])
 @pytest.mark.parametrize("name,rows,n_out,n_in", listed(PLAIN))
