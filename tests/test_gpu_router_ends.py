@@ -166,3 +166,25 @@ def test_sums_over_many_tokens(ctx, tokens, experts, kind):
     check_balance(o, want)
     prob, lim = want[1], want[3]
     assert (lim <= 1e-4 * prob).all() and abs(o["prob"].read().sum(dtype=np.float64) - 1) <= lim.sum()
+
+
+@pytest.mark.parametrize("renormalize", [True, False])
+@pytest.mark.parametrize("tokens,experts,slots,kind", [(100001, 24, 2, "f32"), (33000, 70, 20, "bf16"),
+                                                       (9000, 600, 3, "f16")])
+def test_several_tokens_a_group_of_lanes(ctx, tokens, experts, slots, kind, renormalize):
+    """Routes without the balance, and gradients, of more tokens than a launch has groups."""
+    rng = np.random.default_rng(tokens)
+    s, v = scores(rng, tokens, experts, kind, 0.1)
+    gw = rng.normal(0, 1, (tokens, slots)).astype(np.float32)
+    say("[several tokens]", tokens, experts, slots, kind, renormalize)
+    d, o = ctx.upload(s), outputs(ctx, tokens, experts, slots, False)
+    ctx.experts_route(d, TYPES[kind], tokens, experts, slots, renormalize=renormalize, **{k: r.at for k, r in o.items()})
+    want = forms.chosen(v, slots)
+    assert np.array_equal(o["expert"].read(), want)
+    within(o["weight"].read(), *forms.weights(v, 1.0, want, renormalize))
+    count = balance(v, 1.0, want)[0]
+    out = Result(ctx, tokens, experts, kind)
+    ctx.experts_route_grad(d, TYPES[kind], tokens, experts, slots, o["expert"].at, out.at, renormalize=renormalize,
+                           grad_weight=ctx.upload(gw), count=ctx.upload(count.astype(np.int32)),
+                           grad_loss=ctx.upload(np.array([0.3], np.float32)))
+    within(out.read(), *forms.gradient(v, 1.0, want, renormalize, gw, count, np.float32(0.3)), kind)
